@@ -59,6 +59,30 @@ class ah_gemm_desc(C.Structure):
                 ("tile", C.c_int32), ("variant", C.c_int32)]
 
 
+class ah_linear_ce_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("grad_dtype", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("V", C.c_int32),
+                ("mean", C.c_int32), ("X", C.c_void_p), ("ldx", C.c_int64), ("W", C.c_void_p), ("ldw", C.c_int64),
+                ("bias", C.c_void_p), ("labels", C.c_void_p), ("loss", C.c_void_p), ("rowloss", C.c_void_p), ("lse", C.c_void_p),
+                ("dX", C.c_void_p), ("lddx", C.c_int64), ("dW", C.c_void_p), ("lddw", C.c_int64), ("dbias", C.c_void_p),
+                ("grad_scale", C.c_float), ("reserved", C.c_int32), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class ah_orthogonalize_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("out_dtype", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32), ("batch", C.c_int32),
+                ("steps", C.c_int32), ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float),
+                ("G", C.c_void_p), ("ldg", C.c_int64), ("stride_g", C.c_int64), ("O", C.c_void_p), ("ldo", C.c_int64),
+                ("stride_o", C.c_int64), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class ah_muon_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32), ("batch", C.c_int32), ("steps", C.c_int32),
+                ("nesterov", C.c_int32), ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float),
+                ("G", C.c_void_p), ("ldg", C.c_int64), ("stride_g", C.c_int64), ("M", C.c_void_p), ("M_out", C.c_void_p),
+                ("W", C.c_void_p), ("W_out", C.c_void_p), ("W16_out", C.c_void_p), ("ldw", C.c_int64), ("stride_w", C.c_int64),
+                ("lr", C.c_float), ("momentum", C.c_float), ("decay", C.c_float), ("scale", C.c_float),
+                ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
 class ah_opt(C.Structure):
     _fields_ = [("kind", C.c_int32), ("axis", C.c_int32), ("arg", C.c_int32)]
 
@@ -131,6 +155,12 @@ SIGNATURES = {
     "ah_softmax_ce": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, _P, _P]),
     "ah_chain_step": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, _P, _P, _P]),
     "ah_chain_step_noalloc": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, _P, _P, _P]),
+    "ah_linear_ce_workspace": (C.c_int, [_P, C.POINTER(ah_linear_ce_desc), C.POINTER(C.c_int64)]),
+    "ah_linear_ce": (C.c_int, [_P, C.POINTER(ah_linear_ce_desc)]),
+    "ah_orthogonalize_workspace": (C.c_int, [_P, C.POINTER(ah_orthogonalize_desc), C.POINTER(C.c_int64)]),
+    "ah_orthogonalize": (C.c_int, [_P, C.POINTER(ah_orthogonalize_desc)]),
+    "ah_muon_workspace": (C.c_int, [_P, C.POINTER(ah_muon_desc), C.POINTER(C.c_int64)]),
+    "ah_muon_step": (C.c_int, [_P, C.POINTER(ah_muon_desc)]),
     "ah_trainer_create": (C.c_int, [_P, C.c_int32, C.POINTER(C.c_int64), C.c_int32, C.c_float, C.POINTER(_P)]),
     "ah_trainer_destroy": (None, [_P]),
     "ah_trainer_set": (C.c_int, [_P, C.c_int32, _P, C.c_int64]),

@@ -116,6 +116,73 @@ class Device:
         """chain_step with the workspace in the library's per-GPU static array (enqueues only)."""
         L.check(self.lib.ah_chain_step_noalloc(self.h, X.ptr, g.ptr, R, Cc, dX.ptr, dg.ptr, loss.ptr))
 
+    def _sized(self, fn, d) -> int:
+        n = C.c_int64()
+        L.check(fn(self.h, C.byref(d), C.byref(n)))
+        return n.value
+
+    @staticmethod
+    def _linear_ce_desc(dtype, N, D, V, X, W, labels, loss, grad_dtype=L.AH_F32, bias=None, rowloss=None, lse=None, dX=None, dW=None,
+                        dbias=None, grad_scale=1.0, mean=True, ldx=None, ldw=None, lddx=None, lddw=None, ws=None, ws_bytes=None):
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        ld = lambda v: D if v is None else v        # noqa: E731
+        return L.ah_linear_ce_desc(dtype=dtype, grad_dtype=grad_dtype, N=N, D=D, V=V, mean=1 if mean else 0, X=p(X), ldx=ld(ldx), W=p(W),
+                                   ldw=ld(ldw), bias=p(bias), labels=p(labels), loss=p(loss), rowloss=p(rowloss), lse=p(lse), dX=p(dX),
+                                   lddx=ld(lddx), dW=p(dW), lddw=ld(lddw), dbias=p(dbias), grad_scale=grad_scale, ws=p(ws),
+                                   ws_bytes=ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
+
+    def linear_ce(self, **kw) -> None:
+        """Softmax cross-entropy of the linear head X W^T + bias, without keeping the logits; with dX, dW or dbias given also
+        those gradients (keyword arguments mirror ah_linear_ce_desc; strides default to contiguous rows, ws_bytes to ws.nbytes)."""
+        L.check(self.lib.ah_linear_ce(self.h, C.byref(self._linear_ce_desc(**kw))))
+
+    def linear_ce_workspace(self, **kw) -> int:
+        """Bytes of workspace that linear_ce needs for the same arguments (ws left out)."""
+        return self._sized(self.lib.ah_linear_ce_workspace, self._linear_ce_desc(**kw))
+
+    #: Coefficients (a, b, c) of the quintic that raises small singular values fastest while it keeps all of them below 1.3.
+    NS_COEF = (3.4445, -4.7750, 2.0315)
+
+    @classmethod
+    def _orthogonalize_desc(cls, dtype, rows, cols, G, O, out_dtype=L.AH_F32, batch=1, steps=5, coef=None, eps=1e-7, ldg=None, stride_g=None,
+                            ldo=None, stride_o=None, ws=None, ws_bytes=None):
+        a, b, c = cls.NS_COEF if coef is None else coef
+        ldg, ldo = cols if ldg is None else ldg, cols if ldo is None else ldo
+        return L.ah_orthogonalize_desc(dtype=dtype, out_dtype=out_dtype, rows=rows, cols=cols, batch=batch, steps=steps, a=a, b=b, c=c, eps=eps,
+                                       G=G.ptr, ldg=ldg, stride_g=rows * ldg if stride_g is None else stride_g, O=O.ptr, ldo=ldo,
+                                       stride_o=rows * ldo if stride_o is None else stride_o, ws=None if ws is None else ws.ptr,
+                                       ws_bytes=ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
+
+    def orthogonalize(self, **kw) -> None:
+        """O = the steps-th Newton-Schulz iterate of G / (|G| + eps), for one matrix or a batch (keyword arguments mirror
+        ah_orthogonalize_desc; coef is (a, b, c), strides default to contiguous matrices, ws_bytes to ws.nbytes)."""
+        L.check(self.lib.ah_orthogonalize(self.h, C.byref(self._orthogonalize_desc(**kw))))
+
+    def orthogonalize_workspace(self, **kw) -> int:
+        """Bytes of workspace that orthogonalize needs for the same arguments (ws left out)."""
+        return self._sized(self.lib.ah_orthogonalize_workspace, self._orthogonalize_desc(**kw))
+
+    @classmethod
+    def _muon_desc(cls, dtype, rows, cols, G, M, W, lr, M_out=None, W_out=None, W16_out=None, batch=1, steps=5, coef=None, eps=1e-7, momentum=0.95,
+                   nesterov=True, decay=0.0, scale=1.0, ldg=None, stride_g=None, ldw=None, stride_w=None, ws=None, ws_bytes=None):
+        a, b, c = cls.NS_COEF if coef is None else coef
+        ldg, ldw = cols if ldg is None else ldg, cols if ldw is None else ldw
+        return L.ah_muon_desc(dtype=dtype, rows=rows, cols=cols, batch=batch, steps=steps, nesterov=1 if nesterov else 0, a=a, b=b, c=c, eps=eps,
+                              G=G.ptr, ldg=ldg, stride_g=rows * ldg if stride_g is None else stride_g, M=M.ptr,
+                              M_out=M.ptr if M_out is None else M_out.ptr, W=W.ptr, W_out=W.ptr if W_out is None else W_out.ptr,
+                              W16_out=None if W16_out is None else W16_out.ptr, ldw=ldw, stride_w=rows * ldw if stride_w is None else stride_w,
+                              lr=lr, momentum=momentum, decay=decay, scale=scale, ws=None if ws is None else ws.ptr,
+                              ws_bytes=ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
+
+    def muon_step(self, **kw) -> None:
+        """One weight update by orthogonalised momentum (keyword arguments mirror ah_muon_desc; M and W are updated in place
+        unless M_out and W_out are given, strides default to contiguous matrices, ws_bytes to ws.nbytes)."""
+        L.check(self.lib.ah_muon_step(self.h, C.byref(self._muon_desc(**kw))))
+
+    def muon_step_workspace(self, **kw) -> int:
+        """Bytes of workspace that muon_step needs for the same arguments (ws left out)."""
+        return self._sized(self.lib.ah_muon_workspace, self._muon_desc(**kw))
+
     def close(self) -> None:
         if self.h:
             self.lib.ah_close(self.h)

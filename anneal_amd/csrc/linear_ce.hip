@@ -1,0 +1,692 @@
+// linear_ce.hip — loss and gradients of softmax cross-entropy over a linear head's logits, which are never whole in memory.
+//
+//   z = X W^T + b,  lse_n = log sum_v exp z_nv,  l_n = lse_n - z_n,y(n),  P = exp(z - lse) - onehot(y)
+//   dX = s P W,  dW = s P^T X,  db = s sum_n P        (s: the gradient's scale, divided by the number of counted rows for a mean)
+//
+// The counted rows of X are gathered first (rows whose label is outside [0, V) cost nothing after that, and whatever they hold
+// stays out of the products), then worked on in pieces of rows. Per piece: the logits' product, whose epilogue keeps each row's
+// maximum and sum of exponentials per wave tile of the vocabulary and writes only exp(z - tile maximum) (f16 gradients) or z
+// (f32 gradients) of the piece; one pass that joins the statistics of a row; one pass that turns the piece into P in place; the
+// two gradient products. Keeping one piece costs 2 or 4 bytes of traffic five times per logit; computing it again would cost a
+// third product, 2 D operations per logit: at D = 1024 and 1 PFLOP/s that is 2 ps against 2 ps at 5 TB/s, and the gap widens
+// with D.
+//
+// Precision. f16 operands are exact in the products; f32 operands are carried as two f16 planes scaled by a power of two taken
+// from their largest magnitude (plane_gemm.h). P goes into the gradient products as 2^15 P in one f16 plane for f16 gradients
+// (relative 2^-12 for |P| above 2^-29, and a floor of 2^-40) and in two for f32 gradients (2^-23 above 2^-17, floor 2^-40).
+// Statistics, losses and sums are f32; sums over rows and pieces run in a fixed order, so results repeat bit for bit.
+#include "linear_ce.h"
+
+#include <algorithm>
+
+#include "plane_gemm.h"
+
+namespace ah {
+namespace {
+
+using pg::h4;
+using pg::h8;
+typedef half_t h2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kPScale = 15;   // P is carried as 2^15 P: |P| <= 1, so the largest value is 2^15
+
+// Device scalars at the workspace's start.
+struct Scalars {
+    int count;                // counted rows
+    unsigned xmax, wmax;      // bits of the largest magnitudes (f32 operands)
+    int pad;
+};
+
+// Power of two that brings the largest magnitude into [2^14, 2^15); 0 for all-zero or non-finite operands.
+__device__ __forceinline__ int plane_exp(unsigned maxbits) {
+    const float m = __uint_as_float(maxbits);
+    if (!(m > 0.0f) || maxbits >= 0x7f800000u) return 0;
+    return min(14 - ilogbf(m), 120);
+}
+
+__device__ __forceinline__ int chunk_rows(const int *count, int row0, int rows) { return max(0, min(rows, *count - row0)); }
+
+// ── rows that count ────────────────────────────────────────────────────────────
+
+// One workgroup: the counted rows in order (rowmap), each row's place among them or -1 (pos), their labels.
+__global__ __launch_bounds__(1024) void lce_index_kernel(const int *labels, int N, int V, int *rowmap, int *pos, int *lab, Scalars *sc) {
+    __shared__ int sums[16];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int per = (N + 1023) / 1024, a = min(N, t * per), b = min(N, a + per);
+    int c = 0;
+    for (int i = a; i < b; i++) c += (unsigned)labels[i] < (unsigned)V;
+    int inc = c;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += u;
+    }
+    if (lane == 63) sums[wave] = inc;
+    __syncthreads();
+    int base = 0, total = 0;
+    for (int w = 0; w < 16; w++) {
+        if (w < wave) base += sums[w];
+        total += sums[w];
+    }
+    int at = base + inc - c;
+    for (int i = a; i < b; i++) {
+        const int y = labels[i];
+        const bool ok = (unsigned)y < (unsigned)V;
+        pos[i] = ok ? at : -1;
+        if (ok) {
+            rowmap[at] = i;
+            lab[at++] = y;
+        }
+    }
+    if (t == 0) {
+        sc->count = total;
+        sc->xmax = sc->wmax = 0;
+    }
+}
+
+// Largest magnitudes of W and of the counted rows of X (f32): one workgroup per row of either. The bits of non-negative floats
+// order as integers, so the atomic's result does not depend on the order.
+__global__ __launch_bounds__(256) void lce_absmax_kernel(const float *X, long ldx, int N, const float *W, long ldw, int V, int D, const int *pos,
+                                                         Scalars *sc) {
+    __shared__ unsigned red[4];
+    unsigned mx = 0, mw = 0;
+    for (long r = blockIdx.x; r < (long)N + V; r += gridDim.x) {
+        const bool x = r < N;
+        if (x && pos[r] < 0) continue;
+        const float *p = x ? X + r * ldx : W + (r - N) * ldw;
+        unsigned m = 0;
+        for (int i = threadIdx.x; i < D; i += 256) m = max(m, __float_as_uint(p[i]) & 0x7fffffffu);
+        if (x) mx = max(mx, m);
+        else mw = max(mw, m);
+    }
+    for (int k = 0; k < 2; k++) {
+        unsigned m = k ? mw : mx;
+        for (int o = 32; o >= 1; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            m = max(max(red[0], red[1]), max(red[2], red[3]));
+            if (m) atomicMax(k ? &sc->wmax : &sc->xmax, m);
+        }
+    }
+}
+
+// One stored row of the packed operand: Dp columns, zeros past D. f32 values go to two planes, f16 ones stay.
+template <int P>
+__device__ __forceinline__ void pack_row(half_t *out, const void *in, int D, int Dp, int e) {
+    const int t = threadIdx.x;
+    if constexpr (P == 1) {
+        const half_t *p = (const half_t *)in;
+        if (((uintptr_t)p & 15) == 0 && D % 8 == 0) {
+            for (int i = t * 8; i < Dp; i += 256 * 8) *(h8 *)(out + i) = i < D ? *(const h8 *)(p + i) : (h8){};
+        } else {
+            for (int i = t; i < Dp; i += 256) out[i] = i < D ? p[i] : (half_t)0.0f;
+        }
+    } else {
+        const float *p = (const float *)in;
+        const bool vec = ((uintptr_t)p & 15) == 0 && D % 4 == 0;
+        for (int i = t * 4; i < Dp; i += 256 * 4) {
+            floatx4 v = {};
+            if (vec) {
+                if (i < D) v = *(const floatx4 *)(p + i);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = i + k < D ? p[i + k] : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = ldexpf(v[k], e);
+            pg::plane_store(out + pg::plane_col<2>(i), v);
+        }
+    }
+}
+
+// Block r of the first N + 64: row r of X goes to its place among the counted rows, or its dX and outputs are cleared; the last
+// 64 clear the packed rows that fill up the last stage of the dW product. Further blocks pack W, one row each.
+template <int P>
+__global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, half_t *Wp, int Dp, const int *pos, const Scalars *sc) {
+    const long r = blockIdx.x;
+    const int esz = P == 1 ? 2 : 4;
+    if (r < d.N) {
+        const int q = pos[r];
+        if (q >= 0) {
+            pack_row<P>(Xp + (long)q * Dp * P, (const char *)d.X + r * d.ldx * esz, d.D, Dp, P == 2 ? plane_exp(sc->xmax) : 0);
+            return;
+        }
+        if (d.dX) {
+            if (d.g16) for (int i = threadIdx.x; i < d.D; i += 256) ((half_t *)d.dX)[r * d.lddx + i] = (half_t)0.0f;
+            else for (int i = threadIdx.x; i < d.D; i += 256) ((float *)d.dX)[r * d.lddx + i] = 0.0f;
+        }
+        if (threadIdx.x == 0) {
+            if (d.rowloss) d.rowloss[r] = 0.0f;
+            if (d.lse) d.lse[r] = 0.0f;
+        }
+    } else if (r < d.N + 64) {
+        const long q = sc->count + (r - d.N);
+        if (q < ((sc->count + 63) & ~63)) pack_row<1>(Xp + q * Dp * P, nullptr, 0, Dp * P, 0);
+    } else {
+        const long v = r - d.N - 64;
+        pack_row<P>(Wp + v * Dp * P, (const char *)d.W + v * d.ldw * esz, d.D, Dp, P == 2 ? plane_exp(sc->wmax) : 0);
+    }
+}
+
+// ── the logits' product ────────────────────────────────────────────────────────
+
+enum { KEEP_NONE = 0, KEEP_EXP = 1, KEEP_Z = 2 };
+
+struct LogitArgs {
+    pg::Operand X, W;
+    int V, nk, tiles_m, tiles_n;
+    const Scalars *sc;
+    int row0, rows;       // the piece
+    int planes;           // operands are scaled planes
+    const void *bias;
+    int bias16;
+    const int *lab;       // of the piece's rows
+    float *zt;            // each row's logit of its label
+    float2 *stats;        // [rows][T]: maximum and sum of exponentials of each wave tile's columns
+    int T;
+    char *E;              // the piece: [rows][Vp] of exp(z - tile maximum) 2^15 in f16, or of z in f32
+    int Vp;
+};
+
+// Tiles are walked down the rows first: the tiles of one run share their columns of W, the larger operand.
+template <class C, int KEEP>
+__global__ __launch_bounds__(C::NT) void lce_logits_kernel(LogitArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    const int L = pg::xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n);
+    const int m0 = (L % a.tiles_m) * C::BM, n0 = (L / a.tiles_m) * C::BN;
+    if (m0 >= M) return;
+    floatx4 acc[C::FA][C::FB];
+    pg::contract<C>(a.X, a.W, m0, n0, 0, a.nk, smem, acc);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int mb = m0 + (wave / C::WVN) * C::WM + (lane & 15), nb = n0 + (wave % C::WVN) * C::WN + 4 * (lane >> 4);
+    const int tcol = (n0 / C::BN) * C::WVN + wave % C::WVN;
+    const int e = a.planes ? -(plane_exp(a.sc->xmax) + plane_exp(a.sc->wmax)) : 0;
+    const float ninf = -__builtin_inff();
+    floatx4 bias[C::FB];
+#pragma unroll
+    for (int j = 0; j < C::FB; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int n = nb + 16 * j + r;
+            bias[j][r] = n >= a.V ? ninf : !a.bias ? 0.0f : a.bias16 ? (float)((const half_t *)a.bias)[n] : ((const float *)a.bias)[n];
+        }
+#pragma unroll
+    for (int i = 0; i < C::FA; i++) {
+        const int m = mb + 16 * i;
+        const int y = m < M ? a.lab[m] : -1;
+        float mx = ninf;
+#pragma unroll
+        for (int j = 0; j < C::FB; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int n = nb + 16 * j + r;
+                float z = a.planes ? ldexpf(acc[i][j][r], e) : acc[i][j][r];
+                z = n < a.V ? z + bias[j][r] : ninf;
+                acc[i][j][r] = z;
+                mx = fmaxf(mx, z);
+                if (n == y) a.zt[m] = z;
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float ref = mx == ninf ? 0.0f : mx;   // columns that are all -inf (a bias that rules them out) add nothing
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < C::FB; j++) {
+            const int n = nb + 16 * j;
+            floatx4 ex;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                ex[r] = __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
+                sum += ex[r];
+            }
+            if (KEEP != KEEP_NONE && m < M && n < a.Vp) {
+                if constexpr (KEEP == KEEP_EXP) {
+                    h4 h;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) h[r] = (half_t)(ex[r] * (float)(1 << kPScale));
+                    *(h4 *)(a.E + ((long)m * a.Vp + n) * 2) = h;
+                } else {
+                    *(floatx4 *)(a.E + ((long)m * a.Vp + n) * 4) = acc[i][j];
+                }
+            }
+        }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lane < 16 && m < M) a.stats[(long)m * a.T + tcol] = make_float2(mx, sum);
+    }
+}
+
+// ── a row's statistics ─────────────────────────────────────────────────────────
+
+// One wave per row joins the T tiles' (maximum, sum) pairs.
+__global__ __launch_bounds__(256) void lce_rows_kernel(const Scalars *sc, int row0, int rows, const float2 *stats, int T, const float *zt,
+                                                       const int *rowmap, float *lse_c, float *loss_c, float *rowloss, float *lse_out) {
+    const int M = chunk_rows(&sc->count, row0, rows), lane = threadIdx.x & 63;
+    const int m = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (m >= M) return;
+    const float2 *p = stats + (long)m * T;
+    float mx = -__builtin_inff();
+    bool nan = false;
+    for (int t = lane; t < T; t += 64) {
+        mx = fmaxf(mx, p[t].x);
+        nan |= p[t].y != p[t].y;
+    }
+    mx = wave_max(mx);
+    const float ref = mx == -__builtin_inff() ? 0.0f : mx;
+    float s = 0.0f;
+    for (int t = lane; t < T; t += 64) {
+        const float2 v = p[t];
+        if (v.y > 0.0f) s += v.y * __builtin_amdgcn_exp2f((v.x - ref) * kLog2e);
+    }
+    s = wave_sum(s);
+    if (__ballot(nan)) s = __builtin_nanf("");   // a NaN logit, which the maximum passes over
+    if (lane == 0) {
+        const float lse = mx + logf(s), l = lse - zt[m];
+        lse_c[m] = lse;
+        loss_c[m] = l;
+        const int r = rowmap[m];
+        if (rowloss) rowloss[r] = l;
+        if (lse_out) lse_out[r] = lse;
+    }
+}
+
+// One workgroup: the loss, in f64.
+__global__ __launch_bounds__(1024) void lce_loss_kernel(const Scalars *sc, const float *loss_c, int mean, float *loss) {
+    __shared__ double red[16];
+    const int c = sc->count, t = threadIdx.x;
+    double s = 0.0;
+    for (int i = t; i < c; i += 1024) s += (double)loss_c[i];
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((t & 63) == 0) red[t >> 6] = s;
+    __syncthreads();
+    if (t == 0) {
+        double v = 0.0;
+        for (int w = 0; w < 16; w++) v += red[w];
+        *loss = (float)(mean && c > 0 ? v / c : v);
+    }
+}
+
+// ── P, in place of what the product kept ───────────────────────────────────────
+
+struct GradArgs {
+    const Scalars *sc;
+    int row0, rows, V, Vp, T, WN;   // WN: columns of a statistics tile
+    const float2 *stats;
+    const float *lse, *zt;
+    const int *lab;
+    char *E;
+    float *dbpart;                  // [row block][V] column sums of P, or null
+};
+
+constexpr int kGradRows = 64;       // rows of a block; also the k of a one-plane stage, up to which rows are cleared
+
+// A thread owns 8 (f16 kept) or 4 (f32 kept) columns and walks down kGradRows / 4 rows; 64 threads side by side. The in-place
+// change of z to planes is sound because a group of 32 columns belongs to one wave, whose loads return before it stores.
+template <int KEEP>
+__global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
+    constexpr int NC = KEEP == KEEP_EXP ? 8 : 4;
+    __shared__ float red[3][64][NC];
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows), Mp = (M + 63) & ~63;
+    const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * NC, w = threadIdx.x >> 6;
+    const int r0 = blockIdx.y * kGradRows;
+    if (r0 >= Mp) return;
+    float col[NC] = {};
+    if (n < a.Vp) {
+        const int t = min(n / a.WN, a.T - 1);
+        for (int k = w; k < kGradRows; k += 4) {
+            const int m = r0 + k;
+            float p[NC];
+            char *at = a.E + ((long)m * a.Vp + n) * (KEEP == KEEP_EXP ? 2 : 4);
+            if (m < M) {
+                const float lse = a.lse[m];
+                const int y = a.lab[m] - n;
+                if constexpr (KEEP == KEEP_EXP) {
+                    const float mt = a.stats[(long)m * a.T + t].x;
+                    const float f = mt == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mt - lse) * kLog2e);
+                    const h8 v = *(const h8 *)at;
+#pragma unroll
+                    for (int c = 0; c < NC; c++) p[c] = (float)v[c] * f;
+                } else {
+                    const floatx4 z = *(const floatx4 *)at;
+#pragma unroll
+                    for (int c = 0; c < NC; c++) p[c] = __builtin_amdgcn_exp2f((z[c] - lse) * kLog2e) * (float)(1 << kPScale);
+                }
+                if ((unsigned)y < (unsigned)NC) {
+                    const float q = expm1f(a.zt[m] - lse) * (float)(1 << kPScale);
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+                        if (c == y) p[c] = q;
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; c++) p[c] = 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < NC; c++) col[c] += p[c];
+            if constexpr (KEEP == KEEP_EXP) {
+                h8 h;
+#pragma unroll
+                for (int c = 0; c < NC; c++) h[c] = (half_t)p[c];
+                *(h8 *)at = h;
+            } else {
+                floatx4 v = {p[0], p[1], p[2], p[3]};
+                pg::plane_store((half_t *)(a.E + (long)m * a.Vp * 4) + pg::plane_col<2>(n), v);
+            }
+        }
+    }
+    if (!a.dbpart) return;
+    if (w > 0)
+#pragma unroll
+        for (int c = 0; c < NC; c++) red[w - 1][threadIdx.x & 63][c] = col[c];
+    __syncthreads();
+    if (w == 0)
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+            if (n + c < a.V)
+                a.dbpart[((long)(a.row0 + r0) / kGradRows) * a.V + n + c] =
+                    col[c] + red[0][threadIdx.x][c] + red[1][threadIdx.x][c] + red[2][threadIdx.x][c];
+}
+
+__device__ __forceinline__ float grad_mult(const Scalars *sc, float grad_scale, int mean) {
+    return mean ? grad_scale / (float)max(1, sc->count) : grad_scale;
+}
+
+// db: the row blocks' sums in order.
+__global__ __launch_bounds__(256) void lce_dbias_kernel(const Scalars *sc, const float *part, int V, float grad_scale, int mean, float *dbias) {
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= V) return;
+    const int blocks = (sc->count + kGradRows - 1) / kGradRows;
+    float s = 0.0f;
+    for (int b = 0; b < blocks; b++) s += part[(long)b * V + n];
+    dbias[n] = ldexpf(s, -kPScale) * grad_mult(sc, grad_scale, mean);
+}
+
+// ── the gradient products ──────────────────────────────────────────────────────
+
+struct ProductArgs {
+    pg::Operand A, B;
+    int M, N, tiles_m, tiles_n;
+    const Scalars *sc;
+    int row0, rows;
+    int rows_are;          // 0: C's rows are the piece's (dX); 1: k runs over them (dW)
+    int k;                 // k of dX
+    const int *rowmap;     // dX: where C's rows go
+    const unsigned *bmax;  // largest magnitude of the other operand (planes), or null
+    float grad_scale;
+    int mean;
+    void *C;
+    long ldc;
+    int out16, vec;        // C is f16; rows admit vector stores
+    const float *acc_in;   // dW: the earlier pieces' sum, or null
+    float *acc_out;        // dW: the sum goes there in f32 and C is left, or null
+    long ldacc;
+};
+
+template <class C>
+__global__ __launch_bounds__(C::NT) void lce_product_kernel(ProductArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
+    const int rows = chunk_rows(&a.sc->count, a.row0, a.rows);
+    const int M = a.rows_are == 0 ? rows : a.M;
+    const int nk = a.rows_are == 0 ? (a.k + C::BK - 1) / C::BK : ((rows + 63) & ~63) / C::BK;
+    const int L = pg::xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n);
+    const int m0 = (L / a.tiles_n) * C::BM, n0 = (L % a.tiles_n) * C::BN;
+    if (m0 >= M) return;
+    floatx4 acc[C::FA][C::FB];
+    pg::contract<C>(a.A, a.B, m0, n0, 0, nk, smem, acc);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int mb = m0 + (wave / C::WVN) * C::WM + (lane & 15), nb = n0 + (wave % C::WVN) * C::WN + 4 * (lane >> 4);
+    const int e = -kPScale - (a.bmax ? plane_exp(*a.bmax) : 0);
+    const float mult = grad_mult(a.sc, a.grad_scale, a.mean);
+#pragma unroll
+    for (int i = 0; i < C::FA; i++) {
+        const int m = mb + 16 * i;
+        if (m >= M) continue;
+        const long row = a.rowmap ? a.rowmap[m] : m;
+#pragma unroll
+        for (int j = 0; j < C::FB; j++) {
+            const int n = nb + 16 * j;
+            if (n >= a.N) continue;
+            floatx4 v;
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] = ldexpf(acc[i][j][r], e) * mult;
+            const bool vec = a.vec && n + 3 < a.N;
+            if (a.acc_in)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (n + r < a.N) v[r] += a.acc_in[(long)m * a.ldacc + n + r];
+            if (a.acc_out) {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (n + r < a.N) a.acc_out[(long)m * a.ldacc + n + r] = v[r];
+            } else if (a.out16) {
+                half_t *p = (half_t *)a.C + row * a.ldc + n;
+                if (vec) {
+                    h4 h;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) h[r] = (half_t)v[r];
+                    *(h4 *)p = h;
+                } else
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (n + r < a.N) p[r] = (half_t)v[r];
+            } else {
+                float *p = (float *)a.C + row * a.ldc + n;
+                if (vec) *(floatx4 *)p = v;
+                else
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (n + r < a.N) p[r] = v[r];
+            }
+        }
+    }
+}
+
+// ── host ───────────────────────────────────────────────────────────────────────
+
+constexpr int64_t kPieceBytes = 512ll << 20;   // of kept exponentials or logits
+constexpr int kStatCols = 64;                  // the narrowest wave tile: bounds the statistics' columns
+
+struct Layout {
+    int Dp, Vp, P, KE;         // padded widths; planes of X and W; bytes of a kept logit
+    int rows, pieces;          // rows of a piece
+    bool pack_w, grad;
+    int64_t rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, dbpart, dwacc, total;
+};
+
+Layout layout(const LinearCe &d) {
+    Layout l{};
+    l.Dp = (d.D + 63) & ~63;
+    l.Vp = (d.V + 63) & ~63;
+    l.P = d.f16 ? 1 : 2;
+    l.grad = d.dX || d.dW || d.dbias;
+    l.KE = !l.grad ? 0 : d.g16 ? 2 : 4;
+    l.pack_w = !d.f16 || d.D % 64 || d.ldw % 8 || ((uintptr_t)d.W & 15);
+    const int64_t Np = ((int64_t)d.N + 63) & ~63ll;
+    int64_t rows = Np;
+    if (l.KE) rows = std::min(rows, std::max<int64_t>(256, kPieceBytes / ((int64_t)l.Vp * l.KE) / 256 * 256));
+    else rows = std::min<int64_t>(rows, 16384);
+    l.pieces = (int)((Np + rows - 1) / rows);
+    if (l.pieces > 1) rows = ((Np + l.pieces - 1) / l.pieces + 255) / 256 * 256;
+    l.rows = (int)rows;
+    l.pieces = (int)((Np + rows - 1) / rows);
+    int64_t at = sizeof(Scalars);
+    auto take = [&](int64_t bytes) {
+        at = (at + 255) & ~255ll;
+        const int64_t o = at;
+        at += bytes;
+        return o;
+    };
+    l.rowmap = take(Np * 4);
+    l.pos = take(Np * 4);
+    l.lab = take(Np * 4);
+    l.zt = take(Np * 4);
+    l.lse = take(Np * 4);
+    l.loss = take(Np * 4);
+    l.stats = take(rows * ((l.Vp + 255) / 256 * 256 / kStatCols) * 8);
+    l.Xp = take(Np * l.Dp * 2 * l.P);
+    if (l.pack_w) l.Wp = take((int64_t)d.V * l.Dp * 2 * l.P);
+    if (l.KE) l.E = take(rows * l.Vp * l.KE);
+    if (d.dbias) l.dbpart = take(Np / kGradRows * d.V * 4);
+    if (d.dW && d.g16 && l.pieces > 1) l.dwacc = take((int64_t)d.V * d.D * 4);
+    l.total = (at + 255) & ~255ll;
+    return l;
+}
+
+template <int PA, int PB, int TA, int TB>
+using T256 = pg::Tile<256, 256, 4, 2, TA, TB, PA, PB, 2>;
+template <int PA, int PB, int TA, int TB>
+using T128 = pg::Tile<128, 128, 2, 2, TA, TB, PA, PB, 2>;
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+template <class C>
+void launch_logits(LogitArgs a, int keep, int *WN, hipStream_t s) {
+    a.tiles_m = ceil_div(a.rows, C::BM);
+    a.tiles_n = ceil_div(a.V, C::BN);
+    a.T = a.tiles_n * C::WVN;
+    *WN = C::WN;
+    const dim3 grid((unsigned)(a.tiles_m * a.tiles_n));
+    if (keep == KEEP_NONE) hipLaunchKernelGGL((lce_logits_kernel<C, KEEP_NONE>), grid, dim3(C::NT), 0, s, a);
+    else if (keep == KEEP_EXP) hipLaunchKernelGGL((lce_logits_kernel<C, KEEP_EXP>), grid, dim3(C::NT), 0, s, a);
+    else hipLaunchKernelGGL((lce_logits_kernel<C, KEEP_Z>), grid, dim3(C::NT), 0, s, a);
+}
+
+template <class C>
+void launch_product(ProductArgs a, hipStream_t s) {
+    a.tiles_m = ceil_div(a.rows_are == 0 ? a.rows : a.M, C::BM);
+    a.tiles_n = ceil_div(a.N, C::BN);
+    hipLaunchKernelGGL((lce_product_kernel<C>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(C::NT), 0, s, a);
+}
+
+template <int PP, int PO>
+void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Operand &W, const pg::Operand &X, const half_t *P, int piece, char *ws,
+               hipStream_t s) {
+    const Scalars *sc = (const Scalars *)ws;
+    const int *rowmap = (const int *)(ws + l.rowmap) + a.row0;
+    const pg::Operand Prow{(const char *)P, (long)l.Vp * PP, l.rows, l.rows};
+    const pg::Operand Pcol{(const char *)P, (long)l.Vp * PP, l.Vp, l.rows};
+    if (d.dX) {
+        ProductArgs b = a;
+        b.A = Prow;
+        b.B = W;
+        b.B.rows = l.Dp;
+        b.B.k = d.V;
+        b.N = d.D;
+        b.k = d.V;
+        b.rows_are = 0;
+        b.rowmap = rowmap;
+        b.bmax = PO == 2 ? &sc->wmax : nullptr;
+        b.C = d.dX;
+        b.ldc = d.lddx;
+        b.vec = d.lddx % 4 == 0 && ((uintptr_t)d.dX & (d.g16 ? 7 : 15)) == 0;
+        if ((int64_t)a.rows * d.D > 64 * 256 * 256) launch_product<T256<PP, PO, 0, 1>>(b, s);
+        else launch_product<T128<PP, PO, 0, 1>>(b, s);
+    }
+    if (d.dW) {
+        ProductArgs b = a;
+        b.A = Pcol;
+        b.B = X;
+        b.B.rows = l.Dp;
+        b.B.k = l.rows;
+        b.M = d.V;
+        b.N = d.D;
+        b.rows_are = 1;
+        b.bmax = PO == 2 ? &sc->xmax : nullptr;
+        b.C = d.dW;
+        b.ldc = d.lddw;
+        b.vec = d.lddw % 4 == 0 && ((uintptr_t)d.dW & (d.g16 ? 7 : 15)) == 0;
+        if (l.pieces > 1) {
+            float *acc = (float *)(ws + l.dwacc);
+            if (!d.g16) {   // an f32 dW adds up in place
+                b.acc_in = piece ? (const float *)d.dW : nullptr;
+                b.ldacc = d.lddw;
+            } else {
+                b.ldacc = d.D;
+                b.acc_in = piece ? acc : nullptr;
+                b.acc_out = piece + 1 < l.pieces ? acc : nullptr;
+            }
+        }
+        if ((int64_t)d.V * d.D > 64 * 256 * 256) launch_product<T256<PP, PO, 1, 1>>(b, s);
+        else launch_product<T128<PP, PO, 1, 1>>(b, s);
+    }
+}
+
+}  // namespace
+
+int64_t linear_ce_workspace(const LinearCe &d) { return layout(d).total; }
+
+hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
+    const Layout l = layout(d);
+    char *ws = (char *)wsp;
+    Scalars *sc = (Scalars *)ws;
+    int *rowmap = (int *)(ws + l.rowmap), *pos = (int *)(ws + l.pos), *lab = (int *)(ws + l.lab);
+    float *zt = (float *)(ws + l.zt), *lse = (float *)(ws + l.lse), *loss = (float *)(ws + l.loss);
+    float2 *stats = (float2 *)(ws + l.stats);
+    half_t *Xp = (half_t *)(ws + l.Xp), *Wp = l.pack_w ? (half_t *)(ws + l.Wp) : nullptr;
+
+    hipLaunchKernelGGL(lce_index_kernel, dim3(1), dim3(1024), 0, s, d.labels, d.N, d.V, rowmap, pos, lab, sc);
+    if (!d.f16)
+        hipLaunchKernelGGL(lce_absmax_kernel, dim3(std::min<int64_t>((int64_t)d.N + d.V, 2048)), dim3(256), 0, s, (const float *)d.X, d.ldx, d.N,
+                           (const float *)d.W, d.ldw, d.V, d.D, pos, sc);
+    const dim3 pgrid((unsigned)(d.N + 64 + (l.pack_w ? d.V : 0)));
+    if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, Xp, Wp, l.Dp, pos, sc);
+    else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, Xp, Wp, l.Dp, pos, sc);
+
+    const int keep = !l.grad ? KEEP_NONE : d.g16 ? KEEP_EXP : KEEP_Z;
+    const pg::Operand W{l.pack_w ? (const char *)Wp : (const char *)d.W, l.pack_w ? (long)l.Dp * l.P : d.ldw, d.V, l.Dp};
+    for (int piece = 0; piece < l.pieces; piece++) {
+        const int row0 = piece * l.rows, rows = (int)std::min<int64_t>(l.rows, (((int64_t)d.N + 63) & ~63ll) - row0);
+        const pg::Operand X{(const char *)(Xp + (long)row0 * l.Dp * l.P), (long)l.Dp * l.P, rows, l.Dp};
+        LogitArgs a{};
+        a.X = X;
+        a.W = W;
+        a.V = d.V;
+        a.sc = sc;
+        a.row0 = row0;
+        a.rows = rows;
+        a.planes = l.P == 2;
+        a.bias = d.bias;
+        a.bias16 = d.f16;
+        a.lab = lab + row0;
+        a.zt = zt + row0;
+        a.stats = stats;
+        a.E = ws + l.E;
+        a.Vp = l.Vp;
+        int WN = 0;
+        a.nk = l.Dp / (l.P == 1 ? 64 : 32);
+        const bool big = (int64_t)rows * d.V > 128 * 256 * 256;
+        if (l.P == 1) big ? launch_logits<T256<1, 1, 0, 0>>(a, keep, &WN, s) : launch_logits<T128<1, 1, 0, 0>>(a, keep, &WN, s);
+        else big ? launch_logits<T256<2, 2, 0, 0>>(a, keep, &WN, s) : launch_logits<T128<2, 2, 0, 0>>(a, keep, &WN, s);
+        const int T = ceil_div(d.V, big ? 256 : 128) * 2;
+        hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, sc, row0, rows, stats, T, zt + row0, rowmap + row0,
+                           lse + row0, loss + row0, d.rowloss, d.lse);
+        if (!l.grad) continue;
+        GradArgs g{sc, row0, rows, d.V, l.Vp, T, WN, stats, lse + row0, zt + row0, lab + row0, ws + l.E, d.dbias ? (float *)(ws + l.dbpart) : nullptr};
+        const dim3 ggrid((unsigned)ceil_div(l.Vp, 64 * (keep == KEEP_EXP ? 8 : 4)), (unsigned)ceil_div(rows, kGradRows));
+        if (keep == KEEP_EXP) hipLaunchKernelGGL(lce_grad_kernel<KEEP_EXP>, ggrid, dim3(256), 0, s, g);
+        else hipLaunchKernelGGL(lce_grad_kernel<KEEP_Z>, ggrid, dim3(256), 0, s, g);
+        ProductArgs p{};
+        p.sc = sc;
+        p.row0 = row0;
+        p.rows = rows;
+        p.grad_scale = d.grad_scale;
+        p.mean = d.mean;
+        p.out16 = d.g16;
+        const half_t *P = (const half_t *)(ws + l.E);
+        if (d.g16 && d.f16) gradients<1, 1>(d, l, p, W, X, P, piece, ws, s);
+        else if (d.f16) gradients<2, 1>(d, l, p, W, X, P, piece, ws, s);
+        else gradients<2, 2>(d, l, p, W, X, P, piece, ws, s);
+    }
+    if (d.dbias)
+        hipLaunchKernelGGL(lce_dbias_kernel, dim3((unsigned)ceil_div(d.V, 256)), dim3(256), 0, s, sc, (const float *)(ws + l.dbpart), d.V, d.grad_scale,
+                           d.mean, d.dbias);
+    hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, s, sc, loss, d.mean, d.loss);
+    return hipGetLastError();
+}
+
+}  // namespace ah

@@ -311,6 +311,97 @@ int ah_chain_step(ah_device *dev, const float *X, const float *g, int32_t R, int
 int ah_chain_step_noalloc(ah_device *dev, const float *X, const float *g, int32_t R, int32_t Cc, float *dX,
                           float *dg, float *loss);
 
+/* ── The ends of a language model's training step ─────────────────────────────
+ * No counterpart in the reference (no softmax, no cross-entropy and no update rule but SGD: tensor/nn/nn.go:69-106). All calls
+ * are asynchronous on the device stream and allocate nothing, so they can be captured by ah_graph_begin; each takes a workspace
+ * of the caller's, whose size the *_workspace call gives for the same descriptor (pointers set or not as in the call). The workspace needs 16-byte
+ * alignment and no particular contents; calls of one device handle may share one. Graphs hold its address.
+ *
+ * Softmax cross-entropy of a linear head, without keeping the logits. X [N,D], W [V,D], bias [V] (may be null), labels [N]:
+ *   z = X W^T + bias, lse_n = log sum_v exp z_nv, rowloss_n = lse_n - z_n,label(n)
+ *   P = exp(z - lse) - onehot(label), s = grad_scale (over the number of counted rows, if mean)
+ *   dX = s P W, dW = s P^T X, dbias = s sum_n P
+ * A row whose label is outside [0, V) does not count: its rowloss, lse and dX are 0, and what X holds there is not used (it
+ * may be NaN). loss is the counted rows' sum, divided by their number if mean (0 when there are none; all gradients are 0 then).
+ * Null dX, dW or dbias are not computed; with all three null the call does the loss alone. A bias of -inf rules a class out.
+ * A non-finite logit makes its row's loss and gradients NaN. dtype (X, W, bias) AH_F32 or AH_F16; grad_dtype
+ * (dX, dW) AH_F32, or AH_F16 where dtype is AH_F16. loss, rowloss, lse and dbias are f32; losses and statistics are computed in
+ * f32 or wider. f32 operands take part in the products with 22 bits of each value (less below 2^-14 of the operand's largest
+ * magnitude), and P with 22 bits for f32 gradients and 11 for f16 ones, down to an absolute 2^-40. Gradients of f16 that would
+ * underflow take a loss scale as grad_scale. Results repeat bit for bit. Row strides ldx, ldw, lddx, lddw are in elements.
+ * Outputs may not overlap inputs or one another. */
+typedef struct {
+    int32_t dtype, grad_dtype;
+    int32_t N, D, V;
+    int32_t mean;
+    const void *X;
+    int64_t ldx;
+    const void *W;
+    int64_t ldw;
+    const void *bias;
+    const int32_t *labels;
+    float *loss;           /* [1] */
+    float *rowloss;        /* [N] or null */
+    float *lse;            /* [N] or null */
+    void *dX;
+    int64_t lddx;
+    void *dW;
+    int64_t lddw;
+    float *dbias;
+    float grad_scale;
+    int32_t reserved;      /* 0 */
+    void *ws;
+    int64_t ws_bytes;
+} ah_linear_ce_desc;
+int ah_linear_ce_workspace(ah_device *dev, const ah_linear_ce_desc *d, int64_t *bytes);
+int ah_linear_ce(ah_device *dev, const ah_linear_ce_desc *d);
+
+/* Newton-Schulz orthogonalisation of a matrix G [rows, cols], or of `batch` of them:
+ *   X = G / (|G|_F + eps); steps times: A = X X^T (X^T X if rows > cols), X <- (a I + b A + c A A) X (X (..)); O = X
+ * dtype (of G) and out_dtype AH_F32 or AH_F16. The norm is summed in f64; products keep 22 bits of their operands and sum in
+ * f32. The iteration has to keep the singular values below 4 (a = 3.4445, b = -4.7750, c = 2.0315 keeps them below 1.3);
+ * |a| + |b| + |c| may be at most 15 and steps 1 to 64. A zero matrix gives zeros, a non-finite one NaN. O may be G. ldg, ldo: row
+ * strides; stride_g, stride_o: from matrix to matrix, in elements (read only for batch > 1). */
+typedef struct {
+    int32_t dtype, out_dtype;
+    int32_t rows, cols, batch;
+    int32_t steps;
+    float a, b, c, eps;
+    const void *G;
+    int64_t ldg, stride_g;
+    void *O;
+    int64_t ldo, stride_o;
+    void *ws;
+    int64_t ws_bytes;
+} ah_orthogonalize_desc;
+int ah_orthogonalize_workspace(ah_device *dev, const ah_orthogonalize_desc *d, int64_t *bytes);
+int ah_orthogonalize(ah_device *dev, const ah_orthogonalize_desc *d);
+
+/* One weight update by an orthogonalised momentum (the place of AH_EPI_SGD in a training step):
+ *   M_out = momentum M + G;  U = nesterov ? G + momentum M_out : M_out;  O = U orthogonalised as above
+ *   W_out = (1 - lr decay) W - lr scale O;  W16_out = f16(W_out) (may be null)
+ * G is of dtype AH_F32 or AH_F16; M, W and their outputs are f32. M_out may be M and W_out may be W; outputs may not overlap
+ * anything else. M, W and the outputs share the row stride ldw and the matrix stride stride_w. */
+typedef struct {
+    int32_t dtype;
+    int32_t rows, cols, batch;
+    int32_t steps, nesterov;
+    float a, b, c, eps;
+    const void *G;
+    int64_t ldg, stride_g;
+    const float *M;
+    float *M_out;
+    const float *W;
+    float *W_out;
+    void *W16_out;
+    int64_t ldw, stride_w;
+    float lr, momentum, decay, scale;
+    void *ws;
+    int64_t ws_bytes;
+} ah_muon_desc;
+int ah_muon_workspace(ah_device *dev, const ah_muon_desc *d, int64_t *bytes);
+int ah_muon_step(ah_device *dev, const ah_muon_desc *d);
+
 /* ── Device-resident training steps (one BASELINE config each) ───────────────
  * Replaces the reference step pattern: graph build -> tensor.Backward -> one tensor.Realize per gradient
  * -> host SGD (examples/mlp.go:112-142, tensor/nn/nn.go:69-106). Parameters stay resident as f32 masters

@@ -112,16 +112,16 @@ __global__ __launch_bounds__(256) void lce_absmax_kernel(const float *X, long ld
     }
 }
 
-// One stored row of the packed operand: Dp columns, zeros past D. f32 values go to two planes, f16 ones stay.
+// Row r of the packed operand (panels of `rows` rows): Dp columns, zeros past D. f32 values go to two planes, f16 ones stay.
 template <int P>
-__device__ __forceinline__ void pack_row(half_t *out, const void *in, int D, int Dp, int e) {
+__device__ __forceinline__ void pack_row(half_t *out, long rows, long r, const void *in, int D, int Dp, int e) {
     const int t = threadIdx.x;
     if constexpr (P == 1) {
         const half_t *p = (const half_t *)in;
         if (((uintptr_t)p & 15) == 0 && D % 8 == 0) {
-            for (int i = t * 8; i < Dp; i += 256 * 8) *(h8 *)(out + i) = i < D ? *(const h8 *)(p + i) : (h8){};
+            for (int i = t * 8; i < Dp; i += 256 * 8) *(h8 *)(out + pg::panel_at<1>(rows, r, i)) = i < D ? *(const h8 *)(p + i) : (h8){};
         } else {
-            for (int i = t; i < Dp; i += 256) out[i] = i < D ? p[i] : (half_t)0.0f;
+            for (int i = t; i < Dp; i += 256) out[pg::panel_at<1>(rows, r, i)] = i < D ? p[i] : (half_t)0.0f;
         }
     } else {
         const float *p = (const float *)in;
@@ -136,7 +136,7 @@ __device__ __forceinline__ void pack_row(half_t *out, const void *in, int D, int
             }
 #pragma unroll
             for (int k = 0; k < 4; k++) v[k] = ldexpf(v[k], e);
-            pg::plane_store(out + pg::plane_col<2>(i), v);
+            pg::plane_store(out + pg::panel_at<2>(rows, r, i), v);
         }
     }
 }
@@ -144,13 +144,13 @@ __device__ __forceinline__ void pack_row(half_t *out, const void *in, int D, int
 // Block r of the first N + 64: row r of X goes to its place among the counted rows, or its dX and outputs are cleared; the last
 // 64 clear the packed rows that fill up the last stage of the dW product. Further blocks pack W, one row each.
 template <int P>
-__global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, half_t *Wp, int Dp, const int *pos, const Scalars *sc) {
+__global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, int Np, half_t *Wp, int Dp, const int *pos, const Scalars *sc) {
     const long r = blockIdx.x;
     const int esz = P == 1 ? 2 : 4;
     if (r < d.N) {
         const int q = pos[r];
         if (q >= 0) {
-            pack_row<P>(Xp + (long)q * Dp * P, (const char *)d.X + r * d.ldx * esz, d.D, Dp, P == 2 ? plane_exp(sc->xmax) : 0);
+            pack_row<P>(Xp, Np, q, (const char *)d.X + r * d.ldx * esz, d.D, Dp, P == 2 ? plane_exp(sc->xmax) : 0);
             return;
         }
         if (d.dX) {
@@ -163,10 +163,10 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, h
         }
     } else if (r < d.N + 64) {
         const long q = sc->count + (r - d.N);
-        if (q < ((sc->count + 63) & ~63)) pack_row<1>(Xp + q * Dp * P, nullptr, 0, Dp * P, 0);
+        if (q < ((sc->count + 63) & ~63)) pack_row<1>(Xp, Np, q, nullptr, 0, Dp * P, 0);
     } else {
         const long v = r - d.N - 64;
-        pack_row<P>(Wp + v * Dp * P, (const char *)d.W + v * d.ldw * esz, d.D, Dp, P == 2 ? plane_exp(sc->wmax) : 0);
+        pack_row<P>(Wp, d.V, v, (const char *)d.W + v * d.ldw * esz, d.D, Dp, P == 2 ? plane_exp(sc->wmax) : 0);
     }
 }
 
@@ -186,9 +186,12 @@ struct LogitArgs {
     float *zt;            // each row's logit of its label
     float2 *stats;        // [rows][T]: maximum and sum of exponentials of each wave tile's columns
     int T;
-    char *E;              // the piece: [rows][Vp] of exp(z - tile maximum) 2^15 in f16, or of z in f32
+    char *E;              // the piece in panels of 128 bytes: exp(z - tile maximum) 2^15 in f16, or z in f32
     int Vp;
 };
+
+// Bytes to an f32 logit of the piece: 32 columns fill a panel's row, as the planes that replace them do.
+__device__ __forceinline__ long z_at(long rows, long r, long c) { return ((c >> 5) * rows + r) * 128 + (c & 31) * 4; }
 
 // Tiles are walked down the rows first: the tiles of one run share their columns of W, the larger operand.
 template <class C, int KEEP>
@@ -248,9 +251,9 @@ __global__ __launch_bounds__(C::NT) void lce_logits_kernel(LogitArgs a) {
                     h4 h;
 #pragma unroll
                     for (int r = 0; r < 4; r++) h[r] = (half_t)(ex[r] * (float)(1 << kPScale));
-                    *(h4 *)(a.E + ((long)m * a.Vp + n) * 2) = h;
+                    *(h4 *)(a.E + pg::panel_at<1>(a.rows, m, n) * 2) = h;
                 } else {
-                    *(floatx4 *)(a.E + ((long)m * a.Vp + n) * 4) = acc[i][j];
+                    *(floatx4 *)(a.E + z_at(a.rows, m, n)) = acc[i][j];
                 }
             }
         }
@@ -322,10 +325,17 @@ struct GradArgs {
     float *dbpart;                  // [row block][V] column sums of P, or null
 };
 
+// e^x for f32 gradients: the product with log2 e carries what its rounding loses, which at x = -10 is 3e-7 of the result.
+__device__ __forceinline__ float exp_of(float x) {
+    const float t = x * kLog2e, low = fmaf(x, kLog2e, -t) + x * 1.925963033500e-8f;   // log2 e less its f32 value
+    const float r = __builtin_amdgcn_exp2f(t);
+    return t > -126.0f ? fmaf(r, low * 0.69314718f, r) : r;   // -inf stays away from the correction
+}
+
 constexpr int kGradRows = 64;       // rows of a block; also the k of a one-plane stage, up to which rows are cleared
 
-// A thread owns 8 (f16 kept) or 4 (f32 kept) columns and walks down kGradRows / 4 rows; 64 threads side by side. The in-place
-// change of z to planes is sound because a group of 32 columns belongs to one wave, whose loads return before it stores.
+// A thread owns 8 (f16 kept) or 4 (f32 kept) columns, 8 threads a panel's 128 bytes of a row, and walks down kGradRows / 4 rows.
+// The in-place change of z to planes is sound because those 128 bytes belong to one wave, whose loads return before it stores.
 template <int KEEP>
 __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
     constexpr int NC = KEEP == KEEP_EXP ? 8 : 4;
@@ -340,7 +350,7 @@ __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
         for (int k = w; k < kGradRows; k += 4) {
             const int m = r0 + k;
             float p[NC];
-            char *at = a.E + ((long)m * a.Vp + n) * (KEEP == KEEP_EXP ? 2 : 4);
+            char *at = a.E + (KEEP == KEEP_EXP ? pg::panel_at<1>(a.rows, m, n) * 2 : z_at(a.rows, m, n));
             if (m < M) {
                 const float lse = a.lse[m];
                 const int y = a.lab[m] - n;
@@ -353,7 +363,7 @@ __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
                 } else {
                     const floatx4 z = *(const floatx4 *)at;
 #pragma unroll
-                    for (int c = 0; c < NC; c++) p[c] = __builtin_amdgcn_exp2f((z[c] - lse) * kLog2e) * (float)(1 << kPScale);
+                    for (int c = 0; c < NC; c++) p[c] = exp_of(z[c] - lse) * (float)(1 << kPScale);
                 }
                 if ((unsigned)y < (unsigned)NC) {
                     const float q = expm1f(a.zt[m] - lse) * (float)(1 << kPScale);
@@ -374,7 +384,7 @@ __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
                 *(h8 *)at = h;
             } else {
                 floatx4 v = {p[0], p[1], p[2], p[3]};
-                pg::plane_store((half_t *)(a.E + (long)m * a.Vp * 4) + pg::plane_col<2>(n), v);
+                pg::plane_store((half_t *)a.E + pg::panel_at<2>(a.rows, m, n), v);
             }
         }
     }
@@ -433,7 +443,9 @@ __global__ __launch_bounds__(C::NT) void lce_product_kernel(ProductArgs a) {
     const int M = a.rows_are == 0 ? rows : a.M;
     const int nk = a.rows_are == 0 ? (a.k + C::BK - 1) / C::BK : ((rows + 63) & ~63) / C::BK;
     const int L = pg::xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n);
-    const int m0 = (L / a.tiles_n) * C::BM, n0 = (L % a.tiles_n) * C::BN;
+    int tr, tc;
+    pg::grouped_tile(L, a.tiles_m, a.tiles_n, tr, tc);
+    const int m0 = tr * C::BM, n0 = tc * C::BN;
     if (m0 >= M) return;
     floatx4 acc[C::FA][C::FB];
     pg::contract<C>(a.A, a.B, m0, n0, 0, nk, smem, acc);
@@ -455,14 +467,22 @@ __global__ __launch_bounds__(C::NT) void lce_product_kernel(ProductArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; r++) v[r] = ldexpf(acc[i][j][r], e) * mult;
             const bool vec = a.vec && n + 3 < a.N;
-            if (a.acc_in)
+            const bool vacc = a.ldacc % 4 == 0 && n + 3 < a.N;
+            if (a.acc_in) {
+                const float *p = a.acc_in + (long)m * a.ldacc + n;
+                if (vacc && ((uintptr_t)p & 15) == 0) v += *(const floatx4 *)p;
+                else
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (n + r < a.N) v[r] += a.acc_in[(long)m * a.ldacc + n + r];
+                    for (int r = 0; r < 4; r++)
+                        if (n + r < a.N) v[r] += p[r];
+            }
             if (a.acc_out) {
+                float *p = a.acc_out + (long)m * a.ldacc + n;
+                if (vacc) *(floatx4 *)p = v;
+                else
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (n + r < a.N) a.acc_out[(long)m * a.ldacc + n + r] = v[r];
+                    for (int r = 0; r < 4; r++)
+                        if (n + r < a.N) p[r] = v[r];
             } else if (a.out16) {
                 half_t *p = (half_t *)a.C + row * a.ldc + n;
                 if (vec) {
@@ -488,7 +508,8 @@ __global__ __launch_bounds__(C::NT) void lce_product_kernel(ProductArgs a) {
 
 // ── host ───────────────────────────────────────────────────────────────────────
 
-constexpr int64_t kPieceBytes = 512ll << 20;   // of kept exponentials or logits
+constexpr int64_t kPieceBytes = 2048ll << 20;   // of kept exponentials or logits
+constexpr int kMaxPieceRows = 1 << 20;          // a panel's offsets stay within 32 bits
 constexpr int kStatCols = 64;                  // the narrowest wave tile: bounds the statistics' columns
 
 struct Layout {
@@ -505,10 +526,10 @@ Layout layout(const LinearCe &d) {
     l.P = d.f16 ? 1 : 2;
     l.grad = d.dX || d.dW || d.dbias;
     l.KE = !l.grad ? 0 : d.g16 ? 2 : 4;
-    l.pack_w = !d.f16 || d.D % 64 || d.ldw % 8 || ((uintptr_t)d.W & 15);
+    l.pack_w = !d.f16 || d.D % 64 || d.ldw % 8 || ((uintptr_t)d.W & 15) || d.ldw > 1 << 22;
     const int64_t Np = ((int64_t)d.N + 63) & ~63ll;
     int64_t rows = Np;
-    if (l.KE) rows = std::min(rows, std::max<int64_t>(256, kPieceBytes / ((int64_t)l.Vp * l.KE) / 256 * 256));
+    if (l.KE) rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, kPieceBytes / ((int64_t)l.Vp * l.KE) / 256 * 256)});
     else rows = std::min<int64_t>(rows, 16384);
     l.pieces = (int)((Np + rows - 1) / rows);
     if (l.pieces > 1) rows = ((Np + l.pieces - 1) / l.pieces + 255) / 256 * 256;
@@ -568,8 +589,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
                hipStream_t s) {
     const Scalars *sc = (const Scalars *)ws;
     const int *rowmap = (const int *)(ws + l.rowmap) + a.row0;
-    const pg::Operand Prow{(const char *)P, (long)l.Vp * PP, l.rows, l.rows};
-    const pg::Operand Pcol{(const char *)P, (long)l.Vp * PP, l.Vp, l.rows};
+    const pg::Operand Prow = pg::panels(P, a.rows, a.rows, a.rows), Pcol = pg::panels(P, a.rows, l.Vp, a.rows);
     if (d.dX) {
         ProductArgs b = a;
         b.A = Prow;
@@ -592,7 +612,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
         b.A = Pcol;
         b.B = X;
         b.B.rows = l.Dp;
-        b.B.k = l.rows;
+        b.B.k = a.rows;
         b.M = d.V;
         b.N = d.D;
         b.rows_are = 1;
@@ -634,14 +654,15 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         hipLaunchKernelGGL(lce_absmax_kernel, dim3(std::min<int64_t>((int64_t)d.N + d.V, 2048)), dim3(256), 0, s, (const float *)d.X, d.ldx, d.N,
                            (const float *)d.W, d.ldw, d.V, d.D, pos, sc);
     const dim3 pgrid((unsigned)(d.N + 64 + (l.pack_w ? d.V : 0)));
-    if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, Xp, Wp, l.Dp, pos, sc);
-    else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, Xp, Wp, l.Dp, pos, sc);
+    const int Np = (d.N + 63) & ~63;
+    if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc);
+    else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc);
 
     const int keep = !l.grad ? KEEP_NONE : d.g16 ? KEEP_EXP : KEEP_Z;
-    const pg::Operand W{l.pack_w ? (const char *)Wp : (const char *)d.W, l.pack_w ? (long)l.Dp * l.P : d.ldw, d.V, l.Dp};
+    const pg::Operand W = l.pack_w ? pg::panels(Wp, d.V, d.V, l.Dp) : pg::row_major(d.W, d.ldw, d.V, l.Dp);
     for (int piece = 0; piece < l.pieces; piece++) {
-        const int row0 = piece * l.rows, rows = (int)std::min<int64_t>(l.rows, (((int64_t)d.N + 63) & ~63ll) - row0);
-        const pg::Operand X{(const char *)(Xp + (long)row0 * l.Dp * l.P), (long)l.Dp * l.P, rows, l.Dp};
+        const int row0 = piece * l.rows, rows = std::min(l.rows, Np - row0);
+        const pg::Operand X = pg::panels(Xp + (long)row0 * 64, Np, rows, l.Dp);
         LogitArgs a{};
         a.X = X;
         a.W = W;

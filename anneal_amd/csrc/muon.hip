@@ -23,61 +23,113 @@ namespace {
 using pg::h4;
 
 constexpr int kSX = 12, kSA = 13, kSB = 11;   // powers of two of the planes
-constexpr int kParts = 256;                   // blocks that sum a matrix's squares, at most
+constexpr int kBlocks = 1024;                 // blocks of an elementwise pass over a matrix, at most
 
-__device__ __forceinline__ float load_g(const Muon &d, long i) {
-    return d.f16 ? (float)((const half_t *)d.G)[i] : ((const float *)d.G)[i];
+// Four values from column c of a row of `cols`, zeros past its end; vec: rows start at multiples of four elements.
+template <class T>
+__device__ __forceinline__ floatx4 load4(const T *row, int c, int cols, bool vec) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    floatx4 v = {};
+    if (vec && c + 3 < cols) {
+        const t4 x = *(const t4 *)(row + c);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = (float)x[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (c + k < cols) v[k] = (float)row[c + k];
+    }
+    return v;
 }
 
-// U at (r, c) of matrix z, from G and the new momentum.
-__device__ __forceinline__ float update_of(const Muon &d, float g, float m) { return d.nesterov ? g + d.momentum * m : m; }
+template <class T>
+__device__ __forceinline__ void store4(T *row, int c, int cols, bool vec, floatx4 v) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 x;
+#pragma unroll
+    for (int k = 0; k < 4; k++) x[k] = (T)v[k];
+    if (vec && c + 3 < cols) *(t4 *)(row + c) = x;
+    else
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (c + k < cols) row[c + k] = x[k];
+}
+
+__device__ __forceinline__ floatx4 load_g(const Muon &d, long z, int r, int c) {
+    const long at = z * d.sg + r * d.ldg;
+    return d.f16 ? load4((const half_t *)d.G + at, c, d.cols, d.vec_g) : load4((const float *)d.G + at, c, d.cols, d.vec_g);
+}
+
+// U from G and the new momentum.
+__device__ __forceinline__ floatx4 update_of(const Muon &d, floatx4 g, floatx4 m) {
+    const float mu = d.momentum;
+    if (!d.nesterov) return m;
+#pragma unroll
+    for (int k = 0; k < 4; k++) g[k] += mu * m[k];
+    return g;
+}
+
+// The elementwise passes give a wave one segment of a row at a time.
+constexpr int kSegment = 1024;
 
 // Sums of squares of U per block in f64 (f32 squares of small gradients would vanish); with momentum also M_out.
 __global__ __launch_bounds__(256) void muon_norm_kernel(Muon d, double *part) {
     __shared__ double red[4];
-    const long z = blockIdx.y, n = (long)d.rows * d.cols;
+    const long z = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (d.cols + kSegment - 1) / kSegment;
+    const float mu = d.momentum;
     double s = 0.0;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
-        const long r = i / d.cols, c = i - r * d.cols;
-        float u = load_g(d, z * d.sg + r * d.ldg + c);
-        if (d.W) {
-            const long k = z * d.sw + r * d.ldw + c;
-            const float m = d.momentum * d.M[k] + u;
-            d.M_out[k] = m;
-            u = update_of(d, u, m);
+    for (long q = (long)blockIdx.x * 4 + wave; q < (long)d.rows * segs; q += (long)gridDim.x * 4) {
+        const int r = (int)(q / segs), c0 = (int)(q - (long)r * segs) * kSegment + lane * 4;
+#pragma unroll
+        for (int i = 0; i < kSegment; i += 256) {
+            const int c = c0 + i;
+            if (c >= d.cols) continue;
+            floatx4 u = load_g(d, z, r, c);
+            if (d.W) {
+                const long at = z * d.sw + r * d.ldw;
+                floatx4 m = load4(d.M + at, c, d.cols, d.vec_w);
+#pragma unroll
+                for (int k = 0; k < 4; k++) m[k] = mu * m[k] + u[k];
+                store4(d.M_out + at, c, d.cols, d.vec_w, m);
+                u = update_of(d, u, m);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) s += (double)u[k] * (double)u[k];
         }
-        s += (double)u * (double)u;
     }
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if (lane == 0) red[wave] = s;
     __syncthreads();
     if (threadIdx.x == 0) part[z * gridDim.x + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
-// X's planes: U / (|U| + eps), zeros past the matrix. A block takes whole stored rows.
+// X's planes: U / (|U| + eps), zeros past the matrix.
 __global__ __launch_bounds__(256) void muon_pack_kernel(Muon d, const double *part, int parts, half_t *X, int Rp, int Cp) {
-    __shared__ float inv_s;
+    __shared__ double red[4];
     const long z = blockIdx.y;
-    if (threadIdx.x < 64) {
-        double s = 0.0;
-        for (int i = threadIdx.x; i < parts; i += 64) s += part[z * parts + i];
-        for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-        if (threadIdx.x == 0) inv_s = (float)((double)(1 << kSX) / (sqrt(s) + (double)d.eps));
-    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (Cp + kSegment - 1) / kSegment;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < parts; i += 256) s += part[z * parts + i];
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) red[wave] = s;
     __syncthreads();
-    const float inv = inv_s;
-    for (int r = blockIdx.x; r < Rp; r += gridDim.x) {
-        half_t *out = X + (z * Rp + r) * (long)Cp * 2;
-        for (int c = threadIdx.x * 4; c < Cp; c += 1024) {
-            floatx4 v = {};
-            if (r < d.rows)
+    const float inv = (float)((double)(1 << kSX) / (sqrt(red[0] + red[1] + red[2] + red[3]) + (double)d.eps));
+    half_t *out = X + z * (long)Rp * Cp * 2;
+    for (long q = (long)blockIdx.x * 4 + wave; q < (long)Rp * segs; q += (long)gridDim.x * 4) {
+        const int r = (int)(q / segs), c0 = (int)(q - (long)r * segs) * kSegment + lane * 4;
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (c + k < d.cols) {
-                        const float g = load_g(d, z * d.sg + r * d.ldg + c + k);
-                        v[k] = (d.W ? update_of(d, g, d.M_out[z * d.sw + r * d.ldw + c + k]) : g) * inv;
-                    }
-            pg::plane_store(out + pg::plane_col<2>(c), v);
+        for (int i = 0; i < kSegment; i += 256) {
+            const int c = c0 + i;
+            if (c >= Cp) continue;
+            floatx4 v = {};
+            if (r < d.rows && c < d.cols) {
+                v = load_g(d, z, r, c);
+                if (d.W) v = update_of(d, v, load4(d.M_out + z * d.sw + r * d.ldw, c, d.cols, d.vec_w));
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] *= inv;
+            }
+            pg::plane_store(out + pg::panel_at<2>(Rp, r, c), v);
         }
     }
 }
@@ -93,7 +145,8 @@ struct NsArgs {
     int tiles_m, tiles_n;
     const half_t *Q;        // NS_POLY: the Gram matrix's planes
     half_t *out;            // planes
-    long sQ, so, ldo;       // halves
+    long sQ, so;            // halves
+    int rows;               // of out's panels
 };
 
 template <class C, int WHAT>
@@ -104,10 +157,7 @@ __global__ __launch_bounds__(C::NT) void ns_product_kernel(NsArgs p, Muon d) {
     int tr, tc;
     const int L = pg::xcd_tile(blockIdx.x, gridDim.x);
     if constexpr (SYM) pg::tri_tile(L, tr, tc);
-    else {
-        tr = L / p.tiles_n;
-        tc = L % p.tiles_n;
-    }
+    else pg::grouped_tile(L, p.tiles_m, p.tiles_n, tr, tc);
     const int m0 = tr * C::BM, n0 = tc * C::BN;
     pg::Operand A = p.A, B = p.B;
     A.p += z * p.sA;
@@ -131,7 +181,7 @@ __global__ __launch_bounds__(C::NT) void ns_product_kernel(NsArgs p, Muon d) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) v[r] *= 1.0f / (1 << (2 * kSX - kSA));
             } else if constexpr (WHAT == NS_POLY) {
-                const half_t *q = p.Q + z * p.sQ + (long)m * p.ldo + pg::plane_col<2>(n);
+                const half_t *q = p.Q + z * p.sQ + pg::panel_at<2>(p.rows, m, n);
                 const h4 hi = *(const h4 *)q, lo = *(const h4 *)(q + 32);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
@@ -145,32 +195,31 @@ __global__ __launch_bounds__(C::NT) void ns_product_kernel(NsArgs p, Muon d) {
             }
             if constexpr (WHAT != NS_LAST) {
                 half_t *o = p.out + z * p.so;
-                pg::plane_store(o + (long)m * p.ldo + pg::plane_col<2>(n), v);
+                pg::plane_store(o + pg::panel_at<2>(p.rows, m, n), v);
                 if (SYM && m0 != n0) {
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const half_t hi = (half_t)v[r];
-                        half_t *t = o + (long)(n + r) * p.ldo + pg::plane_col<2>(m);
+                        half_t *t = o + pg::panel_at<2>(p.rows, n + r, m);
                         t[0] = hi;
                         t[32] = (half_t)(v[r] - (float)hi);
                     }
                 }
             } else {
-                if (m >= d.rows) continue;
+                if (m >= d.rows || n >= d.cols) continue;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    if (n + r >= d.cols) continue;
-                    const float x = v[r] * (1.0f / (1 << (kSB + kSX)));
-                    if (d.W) {
-                        const long k = z * d.sw + (long)m * d.ldw + n + r;
-                        const float w = keep * d.W[k] - step * x;
-                        d.W_out[k] = w;
-                        if (d.W16_out) ((half_t *)d.W16_out)[k] = (half_t)w;
-                    } else {
-                        const long k = z * d.so + (long)m * d.ldo + n + r;
-                        if (d.out16) ((half_t *)d.O)[k] = (half_t)x;
-                        else ((float *)d.O)[k] = x;
-                    }
+                for (int r = 0; r < 4; r++) v[r] *= 1.0f / (1 << (kSB + kSX));
+                if (d.W) {
+                    const long at = z * d.sw + (long)m * d.ldw;
+                    const floatx4 w = load4(d.W + at, n, d.cols, d.vec_w);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) v[r] = keep * w[r] - step * v[r];
+                    store4(d.W_out + at, n, d.cols, d.vec_w, v);
+                    if (d.W16_out) store4((half_t *)d.W16_out + at, n, d.cols, d.vec_o, v);
+                } else {
+                    const long at = z * d.so + (long)m * d.ldo;
+                    if (d.out16) store4((half_t *)d.O + at, n, d.cols, d.vec_o, v);
+                    else store4((float *)d.O + at, n, d.cols, d.vec_o, v);
                 }
             }
         }
@@ -178,6 +227,8 @@ __global__ __launch_bounds__(C::NT) void ns_product_kernel(NsArgs p, Muon d) {
 }
 
 // ── host ───────────────────────────────────────────────────────────────────────
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 struct Layout {
     int Rp, Cp, S;   // padded sides, the short one
@@ -190,7 +241,7 @@ Layout layout(const Muon &d) {
     l.Rp = (d.rows + 63) & ~63;
     l.Cp = (d.cols + 63) & ~63;
     l.S = d.rows <= d.cols ? l.Rp : l.Cp;
-    l.parts = (int)std::min<int64_t>(kParts, ((int64_t)d.rows * d.cols + 4095) / 4096);
+    l.parts = (int)std::min<int64_t>(kBlocks, ((int64_t)d.rows * ceil_div(d.cols, kSegment) + 3) / 4);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         at = (at + 255) & ~255ll;
@@ -206,8 +257,6 @@ Layout layout(const Muon &d) {
     l.total = (at + 255) & ~255ll;
     return l;
 }
-
-int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 template <class C, int WHAT>
 void launch(NsArgs p, const Muon &d, hipStream_t s) {
@@ -228,23 +277,31 @@ void product(const NsArgs &p, const Muon &d, hipStream_t s) {
 
 int64_t muon_workspace(const Muon &d) { return layout(d).total; }
 
-hipError_t muon(const Muon &d, void *wsp, hipStream_t s) {
+hipError_t muon(const Muon &in, void *wsp, hipStream_t s) {
+    Muon d = in;
+    const auto vec = [&](const void *p, long ld, long stride, int esz) {
+        return !p || (((uintptr_t)p % (4 * esz)) == 0 && ld % 4 == 0 && (d.batch == 1 || stride % 4 == 0));
+    };
+    d.vec_g = vec(d.G, d.ldg, d.sg, d.f16 ? 2 : 4);
+    d.vec_w = vec(d.M, d.ldw, d.sw, 4) && vec(d.M_out, d.ldw, d.sw, 4) && vec(d.W, d.ldw, d.sw, 4) && vec(d.W_out, d.ldw, d.sw, 4);
+    d.vec_o = d.W ? vec(d.W16_out, d.ldw, d.sw, 2) : vec(d.O, d.ldo, d.so, d.out16 ? 2 : 4);
     const Layout l = layout(d);
     char *ws = (char *)wsp;
     double *part = (double *)(ws + l.part);
     half_t *X = (half_t *)(ws + l.X0), *Xn = (half_t *)(ws + l.X1), *A = (half_t *)(ws + l.A), *B = (half_t *)(ws + l.B);
     const bool wide = d.rows <= d.cols;
     hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)l.parts, (unsigned)d.batch), dim3(256), 0, s, d, part);
-    hipLaunchKernelGGL(muon_pack_kernel, dim3((unsigned)std::min(l.Rp, 2048), (unsigned)d.batch), dim3(256), 0, s, d, part, l.parts, X, l.Rp, l.Cp);
-    const long ldx = 2l * l.Cp, lds = 2l * l.S, sx = (long)l.Rp * l.Cp * 4, ss = (long)l.S * l.S * 4;
+    hipLaunchKernelGGL(muon_pack_kernel, dim3((unsigned)std::min<int64_t>(kBlocks, (int64_t)l.Rp / 4 * ceil_div(l.Cp, kSegment)), (unsigned)d.batch),
+                       dim3(256), 0, s, d, part, l.parts, X, l.Rp, l.Cp);
+    const long sx = (long)l.Rp * l.Cp * 4, ss = (long)l.S * l.S * 4;
     for (int k = 0; k < d.steps; k++) {
         NsArgs g{};   // A = X X^T or X^T X
         g.M = g.N = l.S;
         g.out = A;
         g.so = ss / 2;
-        g.ldo = lds;
+        g.rows = l.S;
         g.sA = g.sB = sx;
-        g.A = g.B = pg::Operand{(const char *)X, ldx, l.S, wide ? l.Cp : l.Rp};
+        g.A = g.B = pg::panels(X, l.Rp, l.S, wide ? l.Cp : l.Rp);
         g.nk = (wide ? l.Cp : l.Rp) / 32;
         if (wide) product<0, 0, NS_GRAM>(g, d, s);
         else product<1, 1, NS_GRAM>(g, d, s);
@@ -254,7 +311,7 @@ hipError_t muon(const Muon &d, void *wsp, hipStream_t s) {
         q.sQ = ss / 2;
         q.out = B;
         q.sA = q.sB = ss;
-        q.A = q.B = pg::Operand{(const char *)A, lds, l.S, l.S};
+        q.A = q.B = pg::panels(A, l.S, l.S, l.S);
         q.nk = l.S / 32;
         product<0, 0, NS_POLY>(q, d, s);
 
@@ -263,15 +320,15 @@ hipError_t muon(const Muon &d, void *wsp, hipStream_t s) {
         n.N = l.Cp;
         n.out = Xn;
         n.so = sx / 2;
-        n.ldo = ldx;
-        const pg::Operand b{(const char *)B, lds, l.S, l.S};
+        n.rows = l.Rp;
+        const pg::Operand b = pg::panels(B, l.S, l.S, l.S);
         if (wide) {
             n.A = b;
             n.sA = ss;
-            n.B = pg::Operand{(const char *)X, ldx, l.Cp, l.Rp};
+            n.B = pg::panels(X, l.Rp, l.Cp, l.Rp);
             n.sB = sx;
         } else {
-            n.A = pg::Operand{(const char *)X, ldx, l.Rp, l.Cp};
+            n.A = pg::panels(X, l.Rp, l.Rp, l.Cp);
             n.sA = sx;
             n.B = b;
             n.sB = ss;

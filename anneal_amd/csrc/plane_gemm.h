@@ -12,6 +12,8 @@
 // line). To the staging code it is an f16 matrix of twice the width, so both planes of a tile arrive with the one set of
 // global->LDS loads, and a stage of 32 k in two planes has the LDS image of a stage of 64 k in one.
 //   T = 0: rows of the operand are stored rows, k runs along them;  T = 1: stored rows are k, the operand's rows run along them.
+// Matrices that only these kernels read are stored in panels of 128-byte columns: all rows' first 128 bytes, then all rows' next.
+// A stage of 256 rows is then one run of 32 KiB, whatever the matrix's width.
 //
 // Per stage a wave reads each fragment once: hi*hi and lo*hi share B's hi, hi*hi and hi*lo share A's hi. So two planes take 2/3
 // of the LDS reads per MFMA that one plane takes, and a 256x256 tile of 8 waves is bound by MFMA issue, not by LDS.
@@ -28,10 +30,10 @@ using g16::s4;
 
 typedef half_t h4 __attribute__((ext_vector_type(4)));
 
-// Halves from the start of a stored row to the hi value of column c (lo: 32 further) in a matrix of P planes.
+// Halves from the start of a matrix of P planes in panels of `rows` rows to the (hi) value of row r, column c (lo: 32 further).
 template <int P>
-__host__ __device__ __forceinline__ long plane_col(long c) {
-    return P == 1 ? c : (c >> 5) * 64 + (c & 31);
+__host__ __device__ __forceinline__ long panel_at(long rows, long r, long c) {
+    return P == 1 ? ((c >> 6) * rows + r) * 64 + (c & 63) : ((c >> 5) * rows + r) * 64 + (c & 31);
 }
 
 // Splits 4 values into the two planes at p (hi) and p + 32 (lo).
@@ -56,7 +58,7 @@ struct PFetch {
     static_assert(T == 0 || W >= 128, "the T = 1 swizzle spans eight 16-column segments");
     uint32_t off[PER];
     // rmax: rows of the operand (a multiple of 8 for T = 1); a row past it reads the last one
-    __device__ __forceinline__ void init(long ld, int r0, int rmax, int wave, int lane) {
+    __device__ __forceinline__ void init(long ld, long ps, int r0, int rmax, int wave, int lane) {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int b = wave * PER + j;
@@ -68,7 +70,7 @@ struct PFetch {
             } else {
                 const int kk = b * ROWS + (16 * lane) / (2 * W), pos = (16 * lane) % (2 * W) / 16;
                 const int m = min(((pos >> 1) ^ g16::mn_swz(kk)) * 16 + (pos & 1) * 8, (rmax - r0) * P - 8);
-                off[j] = (uint32_t)((long)kk * ld * 2 + m * 2);
+                off[j] = (uint32_t)((long)kk * ld * 2 + (m >> 6) * ps + (m & 63) * 2);
             }
         }
     }
@@ -83,22 +85,35 @@ struct PFetch {
     }
 };
 
-// Fragment of 16 operand rows from row r, 32 k: lane l holds row r + l%16, k 8*(l/16) .. +7. s: the k-step of a one-plane stage
-// of 64 k, or the plane of a two-plane one.
+// Fragments of 16 operand rows and 32 k: lane l holds row l%16, k 8*(l/16) .. +7. s: the k-step of a one-plane stage of 64 k, or
+// the plane of a two-plane one. A fragment's LDS address is the wave's first one with a constant xored into bits 5 to 7 (the
+// swizzle) and a constant added, so one register per operand addresses all of them; a stage's base is added per stage.
 template <int R, int T, int P, int BK>
-__device__ __forceinline__ h8 pfrag(const char *tile, int r, int s, int lane) {
-    if constexpr (T == 0) {
-        return *(const h8 *)(tile + g16::koff<BK * P>(r + (lane & 15), 4 * s + (lane >> 4)));
-    } else {
+struct PFrag {
+    static constexpr int W = T == 0 ? BK * P : R * P;
+    static_assert(T == 1 || W == 64, "stored rows of 128 bytes");
+    uint32_t first;
+    __device__ __forceinline__ void init(uint32_t lds, int r, int lane) {   // lds: of the operand in buffer 0; r: the wave's first row
         const int g = lane >> 4, j = lane & 15;
-        const int c = P == 2 ? (r >> 5) * 64 + s * 32 + (r & 31) : r;
-        const int m = c + 4 * (j & 3), k = (P == 2 ? 0 : 32 * s) + 8 * g + (j >> 2);
-        s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(tile + g16::mnoff<R * P>(k, m)));
-        s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(tile + g16::mnoff<R * P>(k + 4, m)));
-        typedef short s8 __attribute__((ext_vector_type(8)));
-        return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        if constexpr (T == 0) first = lds + g16::koff<W>(r + j, g);
+        else first = lds + g16::mnoff<W>(8 * g + (j >> 2), r * P + 4 * (j & 3));
     }
-}
+    // fragment i; stage = first + the buffer's offset, opaque to the compiler, which would otherwise keep every address it finds
+    static __device__ __forceinline__ h8 read(uint32_t stage, int i, int s) {
+        typedef const __attribute__((address_space(3))) char *ptr;
+        if constexpr (T == 0) {
+            return *(const __attribute__((address_space(3))) h8 *)((ptr)(stage ^ (uint32_t)(((i & 1) << 7) | (s << 6))) + 2048 * i);
+        } else {
+            // 16-column segments: a plane's 32 columns are two, the planes of 32 columns four
+            const int seg = P == 2 ? (i >> 1) * 4 + s * 2 + (i & 1) : i, k = P == 2 ? 0 : 32 * s;
+            const ptr p = (ptr)(stage ^ (uint32_t)((seg & 7) << 5)) + (seg >> 3) * 256 + k * (W * 2);
+            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
+            const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 4 * (W * 2)));
+            typedef short s8 __attribute__((ext_vector_type(8)));
+            return __builtin_bit_cast(h8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
 
 // BM x BN tile shared by WVM x WVN waves; NS stages of BK k in LDS.
 template <int BM_, int BN_, int WVM_, int WVN_, int TA_, int TB_, int PA_, int PB_, int NS_>
@@ -109,6 +124,10 @@ struct Tile {
     static constexpr int ABYTES = BM * BK * PA * 2, STAGE = ABYTES + BN * BK * PB * 2, SMEM = NS * STAGE;
     using FetchA = PFetch<BM, TA, PA, BK, NW>;
     using FetchB = PFetch<BN, TB, PB, BK, NW>;
+    using FragA = PFrag<BM, TA, PA, BK>;
+    using FragB = PFrag<BN, TB, PB, BK>;
+    static_assert((TA == 0 || WM * PA == 64 || WM * PA % 128 == 0) && (TB == 0 || WN * PB == 64 || WN * PB % 128 == 0),
+                  "a fragment's segment is the wave's first one xor a constant");
     static_assert(PA >= PB, "a two-plane B takes a two-plane A");
     static_assert(SMEM <= 160 * 1024, "stages exceed the LDS");
 };
@@ -116,9 +135,15 @@ struct Tile {
 struct Operand {
     const char *p;   // the array
     long ld;         // halves from a stored row to the next
+    long ps;         // bytes from 64 halves of a row to the next 64
     int rows;        // operand rows
     int k;           // T = 1: stored rows that exist (stages past them read the last one)
 };
+
+// `stored` rows in panels; rows of the operand, k as above.
+inline Operand panels(const void *p, long stored, int rows, int k) { return {(const char *)p, 64, stored * 128, rows, k}; }
+// Rows one after the other.
+inline Operand row_major(const void *p, long ld, int rows, int k) { return {(const char *)p, ld, 128, rows, k}; }
 
 // acc[i][j] += the tile's products over stages kt0 .. kt0 + nk - 1. The first MFMA operand is B's fragment, so a lane ends up
 // with one row m = 16 i + lane%16 of C and four neighbouring columns n = 16 j + 4 (lane/16) + r: rows leave as 16-byte stores and
@@ -142,32 +167,51 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
 
     typename C::FetchA fa;
     typename C::FetchB fb;
-    fa.init(A.ld, m0, A.rows, wave, lane);
-    fb.init(B.ld, n0, B.rows, wave, lane);
-    const char *Ab = A.p + (C::TA == 0 ? (long)m0 * A.ld * 2 : (long)m0 * C::PA * 2);
-    const char *Bb = B.p + (C::TB == 0 ? (long)n0 * B.ld * 2 : (long)n0 * C::PB * 2);
+    // a tile's rows start a multiple of 64 halves into a stored row (T = 1), and a stage of k fills 64 halves (T = 0)
+    static_assert(C::TA == 1 || BK * C::PA == 64, "a stage of A is one panel");
+    static_assert(C::TB == 1 || BK * C::PB == 64, "a stage of B is one panel");
+    fa.init(A.ld, A.ps, m0, A.rows, wave, lane);
+    fb.init(B.ld, B.ps, n0, B.rows, wave, lane);
+    const char *Ab = A.p + (C::TA == 0 ? (long)m0 * A.ld * 2 : (long)(m0 * C::PA / 64) * A.ps);
+    const char *Bb = B.p + (C::TB == 0 ? (long)n0 * B.ld * 2 : (long)(n0 * C::PB / 64) * B.ps);
+    const long da = C::TA == 0 ? A.ps : (long)BK * A.ld * 2, db = C::TB == 0 ? B.ps : (long)BK * B.ld * 2;   // bytes a stage
     auto issue_one = [&](int f, int t, int buf) {   // load f of stage t into buffer buf
-        const long k = (long)(kt0 + t) * BK;
-        if (f < PERA) fa.issue(f, Ab + (C::TA == 0 ? k * C::PA * 2 : k * A.ld * 2), A.ld, BK, lds + buf * STAGE, wave_u, lane);
-        else fb.issue(f - PERA, Bb + (C::TB == 0 ? k * C::PB * 2 : k * B.ld * 2), B.ld, C::TB == 1 ? (int)(B.k - k) : BK,
-                      lds + buf * STAGE + ABYTES, wave_u, lane);
+        if (f < PERA) fa.issue(f, Ab + (kt0 + t) * da, A.ld, BK, lds + buf * STAGE, wave_u, lane);
+        else fb.issue(f - PERA, Bb + (kt0 + t) * db, B.ld, C::TB == 1 ? B.k - (kt0 + t) * BK : BK, lds + buf * STAGE + ABYTES, wave_u, lane);
     };
+    typename C::FragA ra;
+    typename C::FragB rb;
+    ra.init(lds, wm0, lane);
+    rb.init(lds + ABYTES, wn0, lane);
     auto fragA = [&](h8 (&v)[FA], int buf, int s) {
+        uint32_t at = ra.first + buf * STAGE;
+        asm volatile("" : "+v"(at));
 #pragma unroll
-        for (int i = 0; i < FA; i++) v[i] = pfrag<C::BM, C::TA, C::PA, BK>(smem + buf * STAGE, wm0 + 16 * i, s, lane);
+        for (int i = 0; i < FA; i++) v[i] = C::FragA::read(at, i, s);
     };
     auto fragB = [&](h8 (&v)[FB], int buf, int s) {
+        uint32_t at = rb.first + buf * STAGE;
+        asm volatile("" : "+v"(at));
 #pragma unroll
-        for (int j = 0; j < FB; j++) v[j] = pfrag<C::BN, C::TB, C::PB, BK>(smem + buf * STAGE + ABYTES, wn0 + 16 * j, s, lane);
+        for (int j = 0; j < FB; j++) v[j] = C::FragB::read(at, j, s);
     };
-    auto mma = [&](h8 (&a)[FA], h8 (&b)[FB]) {
-        __builtin_amdgcn_sched_barrier(0);
+    // a group of MFMAs, with the NR LDS reads that stand before it spread between them
+    auto mma = [&](h8 (&a)[FA], h8 (&b)[FB], auto nr) {
+        constexpr int NM = FA * FB, NR = decltype(nr)::value, PER = NM >= NR ? NM / NR : 1, EACH = NM >= NR ? 1 : (NR + NM - 1) / NM;
 #pragma unroll
         for (int i = 0; i < FA; i++)
 #pragma unroll
             for (int j = 0; j < FB; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[j], a[i], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < NR / EACH; q++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);    // MFMAs
+            __builtin_amdgcn_sched_group_barrier(0x100, EACH, 0);   // LDS reads
+        }
         __builtin_amdgcn_sched_barrier(0);
     };
+    constexpr std::integral_constant<int, FA *(C::TA ? 2 : 1)> NRA{};                                // LDS reads of A's fragments,
+    constexpr std::integral_constant<int, FB *(C::TB ? 2 : 1)> NRB{};                                // of B's,
+    constexpr std::integral_constant<int, decltype(NRA)::value + decltype(NRB)::value> NRAB{};       // of both
     // the last group of stage t, with the refill of its buffer spread between the MFMAs (the tail re-fetches the last stage into
     // idle buffers, so that the number of loads in flight stays the same)
     auto mma_refill = [&](h8 (&a)[FA], h8 (&b)[FB], int t, int buf) {
@@ -212,9 +256,9 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
         auto stage = [&](int t, int buf, h8 (&a)[FA], h8 (&an)[FA]) {
             const int nbuf = buf + 1 == NS ? 0 : buf + 1;
             fragA(an, buf, 1);   // lo
-            mma(a, b0);
+            mma(a, b0, NRA);
             fragB(b1, buf, 1);   // lo
-            mma(an, b0);
+            mma(an, b0, NRB);
             open_next();
             fragA(an, nbuf, 0);
             fragB(b0, nbuf, 0);
@@ -233,7 +277,7 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
         auto stage = [&](int t, int buf, h8 (&b)[FB], h8 (&bn)[FB]) {
             const int nbuf = buf + 1 == NS ? 0 : buf + 1;
             fragA(a1, buf, 1);   // lo
-            mma(a0, b);
+            mma(a0, b, NRA);
             open_next();
             fragA(a0, nbuf, 0);
             fragB(bn, nbuf, 0);
@@ -254,7 +298,7 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
             const int nbuf = buf + 1 == NS ? 0 : buf + 1;
             fragA(a1, buf, 1);   // second k-step
             fragB(b1, buf, 1);
-            mma(a0, b0);
+            mma(a0, b0, NRAB);
             open_next();
             fragA(a0, nbuf, 0);
             fragB(b0, nbuf, 0);
@@ -269,6 +313,14 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
 __device__ __forceinline__ int xcd_tile(int L, int n) {
     const int x = L & 7, i = L >> 3, q = n >> 3, r = n & 7;
     return x * q + min(x, r) + i;
+}
+
+// Tile t of tiles_m x tiles_n: rows in groups of 4, walked by columns within a group, so that the tiles at work on one XCD
+// share operand panels in its L2.
+__device__ __forceinline__ void grouped_tile(int t, int tiles_m, int tiles_n, int &row, int &col) {
+    const int g = t / (4 * tiles_n) * 4, rem = t - g * tiles_n, size = min(4, tiles_m - g);
+    row = g + rem % size;
+    col = rem / size;
 }
 
 // Tile t of the upper triangle (row <= column) of a square of n tiles a side, walked by columns.

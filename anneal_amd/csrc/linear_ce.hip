@@ -176,7 +176,8 @@ enum { KEEP_NONE = 0, KEEP_EXP = 1, KEEP_Z = 2 };
 
 struct LogitArgs {
     pg::Operand X, W;
-    int V, nk, tiles_m, tiles_n;
+    int V, nk, tiles_m;
+    pg::Work w;
     const Scalars *sc;
     int row0, rows;       // the piece
     int planes;           // operands are scaled planes
@@ -194,73 +195,89 @@ struct LogitArgs {
 __device__ __forceinline__ long z_at(long rows, long r, long c) { return ((c >> 5) * rows + r) * 128 + (c & 31) * 4; }
 
 // Tiles are walked down the rows first: the tiles of one run share their columns of W, the larger operand.
-template <class C, int KEEP>
-__global__ __launch_bounds__(C::NT) void lce_logits_kernel(LogitArgs a) {
-    __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
-    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
-    const int L = pg::xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n);
-    const int m0 = (L % a.tiles_m) * C::BM, n0 = (L / a.tiles_m) * C::BN;
-    if (m0 >= M) return;
-    floatx4 acc[C::FA][C::FB];
-    pg::contract<C>(a.X, a.W, m0, n0, 0, a.nk, smem, acc);
+template <class C>
+__device__ __forceinline__ void logits_tile(const LogitArgs &a, int tile, int &m0, int &n0) {
+    m0 = tile % a.tiles_m * C::BM;
+    n0 = tile / a.tiles_m * C::BN;
+}
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int mb = m0 + (wave / C::WVN) * C::WM + (lane & 15), nb = n0 + (wave % C::WVN) * C::WN + 4 * (lane >> 4);
-    const int tcol = (n0 / C::BN) * C::WVN + wave % C::WVN;
+// What follows the product, for accumulator row i.
+template <class C, int KEEP>
+__device__ __forceinline__ void logits_row(const LogitArgs &a, int M, int m0, int n0, int i, floatx4 (&z)[C::FB]) {
+    const pg::Place<C> at(m0, n0);
+    const int m = at.m + 16 * i, tcol = n0 / C::WN + at.wave % C::WVN;
     const int e = a.planes ? -(plane_exp(a.sc->xmax) + plane_exp(a.sc->wmax)) : 0;
+    const int y = m < M ? a.lab[m] : -1;
     const float ninf = -__builtin_inff();
-    floatx4 bias[C::FB];
+    float mx = ninf;
 #pragma unroll
     for (int j = 0; j < C::FB; j++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const int n = nb + 16 * j + r;
-            bias[j][r] = n >= a.V ? ninf : !a.bias ? 0.0f : a.bias16 ? (float)((const half_t *)a.bias)[n] : ((const float *)a.bias)[n];
+            const int n = at.n + 16 * j + r;
+            float v = a.planes ? ldexpf(z[j][r], e) : z[j][r];
+            if (n >= a.V) v = ninf;
+            else if (a.bias) v += a.bias16 ? (float)((const half_t *)a.bias)[n] : ((const float *)a.bias)[n];
+            z[j][r] = v;
+            mx = fmaxf(mx, v);
+            if (n == y) a.zt[m] = v;
         }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float ref = mx == ninf ? 0.0f : mx;   // columns that are all -inf (a bias that rules them out) add nothing
+    float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < C::FA; i++) {
-        const int m = mb + 16 * i;
-        const int y = m < M ? a.lab[m] : -1;
-        float mx = ninf;
+    for (int j = 0; j < C::FB; j++) {
+        const int n = at.n + 16 * j;
+        floatx4 ex;
 #pragma unroll
-        for (int j = 0; j < C::FB; j++)
+        for (int r = 0; r < 4; r++) {
+            ex[r] = __builtin_amdgcn_exp2f((z[j][r] - ref) * kLog2e);
+            sum += ex[r];
+        }
+        if (KEEP != KEEP_NONE && m < M && n < a.Vp) {
+            if constexpr (KEEP == KEEP_EXP) {
+                h4 h;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int n = nb + 16 * j + r;
-                float z = a.planes ? ldexpf(acc[i][j][r], e) : acc[i][j][r];
-                z = n < a.V ? z + bias[j][r] : ninf;
-                acc[i][j][r] = z;
-                mx = fmaxf(mx, z);
-                if (n == y) a.zt[m] = z;
-            }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float ref = mx == ninf ? 0.0f : mx;   // columns that are all -inf (a bias that rules them out) add nothing
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < C::FB; j++) {
-            const int n = nb + 16 * j;
-            floatx4 ex;
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                ex[r] = __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
-                sum += ex[r];
-            }
-            if (KEEP != KEEP_NONE && m < M && n < a.Vp) {
-                if constexpr (KEEP == KEEP_EXP) {
-                    h4 h;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) h[r] = (half_t)(ex[r] * (float)(1 << kPScale));
-                    *(h4 *)(a.E + pg::panel_at<1>(a.rows, m, n) * 2) = h;
-                } else {
-                    *(floatx4 *)(a.E + z_at(a.rows, m, n)) = acc[i][j];
-                }
+                for (int r = 0; r < 4; r++) h[r] = (half_t)(ex[r] * (float)(1 << kPScale));
+                *(h4 *)(a.E + pg::panel_at<1>(a.rows, m, n) * 2) = h;
+            } else {
+                *(floatx4 *)(a.E + z_at(a.rows, m, n)) = z[j];
             }
         }
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (lane < 16 && m < M) a.stats[(long)m * a.T + tcol] = make_float2(mx, sum);
     }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (at.lane < 16 && m < M) a.stats[(long)m * a.T + tcol] = make_float2(mx, sum);
+}
+
+template <class C, int KEEP>
+__global__ __launch_bounds__(C::NT) void lce_logits_kernel(LogitArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    int tile, slot, first, count, m0, n0;
+    pg::pick(a.w, blockIdx.x, a.nk, tile, slot, first, count);
+    logits_tile<C>(a, tile, m0, n0);
+    if (m0 >= M) return;
+    floatx4 acc[C::FA][C::FB];
+    pg::contract<C>(a.X, a.W, m0, n0, first, count, smem, acc);
+    if (slot >= 0) {
+        pg::store_partials<C>(a.w.part, slot, acc);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < C::FA; i++) logits_row<C, KEEP>(a, M, m0, n0, i, acc[i]);
+}
+
+template <class C, int KEEP>
+__global__ __launch_bounds__(C::NT) void lce_logits_join_kernel(LogitArgs a) {
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    int m0, n0;
+    logits_tile<C>(a, a.w.whole + blockIdx.x, m0, n0);
+    if (m0 >= M) return;
+    floatx4 z[C::FB];
+    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, z);
+    logits_row<C, KEEP>(a, M, m0, n0, blockIdx.y, z);
 }
 
 // ── a row's statistics ─────────────────────────────────────────────────────────
@@ -321,7 +338,7 @@ struct GradArgs {
     const float2 *stats;
     const float *lse, *zt;
     const int *lab;
-    char *E;
+    char *E, *P;                    // what the product kept; P: E itself, or where one plane made of z goes
     float *dbpart;                  // [row block][V] column sums of P, or null
 };
 
@@ -336,7 +353,7 @@ constexpr int kGradRows = 64;       // rows of a block; also the k of a one-plan
 
 // A thread owns 8 (f16 kept) or 4 (f32 kept) columns, 8 threads a panel's 128 bytes of a row, and walks down kGradRows / 4 rows.
 // The in-place change of z to planes is sound because those 128 bytes belong to one wave, whose loads return before it stores.
-template <int KEEP>
+template <int KEEP, int PLANES>
 __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
     constexpr int NC = KEEP == KEEP_EXP ? 8 : 4;
     __shared__ float red[3][64][NC];
@@ -382,9 +399,14 @@ __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
 #pragma unroll
                 for (int c = 0; c < NC; c++) h[c] = (half_t)p[c];
                 *(h8 *)at = h;
+            } else if constexpr (PLANES == 1) {
+                h4 h;
+#pragma unroll
+                for (int c = 0; c < NC; c++) h[c] = (half_t)p[c];
+                *(h4 *)((half_t *)a.P + pg::panel_at<1>(a.rows, m, n)) = h;
             } else {
                 floatx4 v = {p[0], p[1], p[2], p[3]};
-                pg::plane_store((half_t *)a.E + pg::panel_at<2>(a.rows, m, n), v);
+                pg::plane_store((half_t *)a.P + pg::panel_at<2>(a.rows, m, n), v);
             }
         }
     }
@@ -420,6 +442,7 @@ __global__ __launch_bounds__(256) void lce_dbias_kernel(const Scalars *sc, const
 struct ProductArgs {
     pg::Operand A, B;
     int M, N, tiles_m, tiles_n;
+    pg::Work w;
     const Scalars *sc;
     int row0, rows;
     int rows_are;          // 0: C's rows are the piece's (dX); 1: k runs over them (dW)
@@ -436,74 +459,101 @@ struct ProductArgs {
     long ldacc;
 };
 
+__device__ __forceinline__ int product_rows(const ProductArgs &a, int &nk, int BK) {
+    const int rows = chunk_rows(&a.sc->count, a.row0, a.rows);
+    nk = ((a.rows_are == 0 ? a.k : (rows + 63) & ~63) + BK - 1) / BK;
+    return a.rows_are == 0 ? rows : a.M;
+}
+
+template <class C>
+__device__ __forceinline__ void product_tile(const ProductArgs &a, int tile, int &m0, int &n0) {
+    int tr, tc;
+    pg::grouped_tile(tile, a.tiles_m, a.tiles_n, tr, tc);
+    m0 = tr * C::BM;
+    n0 = tc * C::BN;
+}
+
+// What follows the product, for accumulator row i.
+template <class C>
+__device__ __forceinline__ void product_row(const ProductArgs &a, int M, int m0, int n0, int i, const floatx4 (&acc)[C::FB]) {
+    const pg::Place<C> at(m0, n0);
+    const int m = at.m + 16 * i, e = -kPScale - (a.bmax ? plane_exp(*a.bmax) : 0);
+    if (m >= M) return;
+    const float mult = grad_mult(a.sc, a.grad_scale, a.mean);
+    const long row = a.rowmap ? a.rowmap[m] : m;
+#pragma unroll
+    for (int j = 0; j < C::FB; j++) {
+        const int n = at.n + 16 * j;
+        if (n >= a.N) continue;
+        floatx4 v;
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] = ldexpf(acc[j][r], e) * mult;
+        const bool vec = a.vec && n + 3 < a.N;
+        const bool vacc = a.ldacc % 4 == 0 && n + 3 < a.N;
+        if (a.acc_in) {
+            const float *p = a.acc_in + (long)m * a.ldacc + n;
+            if (vacc && ((uintptr_t)p & 15) == 0) v += *(const floatx4 *)p;
+            else
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (n + r < a.N) v[r] += p[r];
+        }
+        if (a.acc_out) {
+            float *p = a.acc_out + (long)m * a.ldacc + n;
+            if (vacc) *(floatx4 *)p = v;
+            else
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (n + r < a.N) p[r] = v[r];
+        } else if (a.out16) {
+            half_t *p = (half_t *)a.C + row * a.ldc + n;
+            if (vec) {
+                h4 h;
+#pragma unroll
+                for (int r = 0; r < 4; r++) h[r] = (half_t)v[r];
+                *(h4 *)p = h;
+            } else
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (n + r < a.N) p[r] = (half_t)v[r];
+        } else {
+            float *p = (float *)a.C + row * a.ldc + n;
+            if (vec) *(floatx4 *)p = v;
+            else
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (n + r < a.N) p[r] = v[r];
+        }
+    }
+}
+
 template <class C>
 __global__ __launch_bounds__(C::NT) void lce_product_kernel(ProductArgs a) {
     __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
-    const int rows = chunk_rows(&a.sc->count, a.row0, a.rows);
-    const int M = a.rows_are == 0 ? rows : a.M;
-    const int nk = a.rows_are == 0 ? (a.k + C::BK - 1) / C::BK : ((rows + 63) & ~63) / C::BK;
-    const int L = pg::xcd_tile(blockIdx.x, a.tiles_m * a.tiles_n);
-    int tr, tc;
-    pg::grouped_tile(L, a.tiles_m, a.tiles_n, tr, tc);
-    const int m0 = tr * C::BM, n0 = tc * C::BN;
+    int nk, tile, slot, first, count, m0, n0;
+    const int M = product_rows(a, nk, C::BK);
+    pg::pick(a.w, blockIdx.x, nk, tile, slot, first, count);
+    product_tile<C>(a, tile, m0, n0);
     if (m0 >= M) return;
     floatx4 acc[C::FA][C::FB];
-    pg::contract<C>(a.A, a.B, m0, n0, 0, nk, smem, acc);
-
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int mb = m0 + (wave / C::WVN) * C::WM + (lane & 15), nb = n0 + (wave % C::WVN) * C::WN + 4 * (lane >> 4);
-    const int e = -kPScale - (a.bmax ? plane_exp(*a.bmax) : 0);
-    const float mult = grad_mult(a.sc, a.grad_scale, a.mean);
-#pragma unroll
-    for (int i = 0; i < C::FA; i++) {
-        const int m = mb + 16 * i;
-        if (m >= M) continue;
-        const long row = a.rowmap ? a.rowmap[m] : m;
-#pragma unroll
-        for (int j = 0; j < C::FB; j++) {
-            const int n = nb + 16 * j;
-            if (n >= a.N) continue;
-            floatx4 v;
-#pragma unroll
-            for (int r = 0; r < 4; r++) v[r] = ldexpf(acc[i][j][r], e) * mult;
-            const bool vec = a.vec && n + 3 < a.N;
-            const bool vacc = a.ldacc % 4 == 0 && n + 3 < a.N;
-            if (a.acc_in) {
-                const float *p = a.acc_in + (long)m * a.ldacc + n;
-                if (vacc && ((uintptr_t)p & 15) == 0) v += *(const floatx4 *)p;
-                else
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (n + r < a.N) v[r] += p[r];
-            }
-            if (a.acc_out) {
-                float *p = a.acc_out + (long)m * a.ldacc + n;
-                if (vacc) *(floatx4 *)p = v;
-                else
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (n + r < a.N) p[r] = v[r];
-            } else if (a.out16) {
-                half_t *p = (half_t *)a.C + row * a.ldc + n;
-                if (vec) {
-                    h4 h;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) h[r] = (half_t)v[r];
-                    *(h4 *)p = h;
-                } else
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (n + r < a.N) p[r] = (half_t)v[r];
-            } else {
-                float *p = (float *)a.C + row * a.ldc + n;
-                if (vec) *(floatx4 *)p = v;
-                else
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (n + r < a.N) p[r] = v[r];
-            }
-        }
+    pg::contract<C>(a.A, a.B, m0, n0, first, count, smem, acc);
+    if (slot >= 0) {
+        pg::store_partials<C>(a.w.part, slot, acc);
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < C::FA; i++) product_row<C>(a, M, m0, n0, i, acc[i]);
+}
+
+template <class C>
+__global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) {
+    int nk, m0, n0;
+    const int M = product_rows(a, nk, C::BK);
+    product_tile<C>(a, a.w.whole + blockIdx.x, m0, n0);
+    if (m0 >= M) return;
+    floatx4 v[C::FB];
+    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, v);
+    product_row<C>(a, M, m0, n0, blockIdx.y, v);
 }
 
 // ── host ───────────────────────────────────────────────────────────────────────
@@ -513,11 +563,21 @@ constexpr int kMaxPieceRows = 1 << 20;          // a panel's offsets stay within
 constexpr int kStatCols = 64;                  // the narrowest wave tile: bounds the statistics' columns
 
 struct Layout {
-    int Dp, Vp, P, KE;         // padded widths; planes of X and W; bytes of a kept logit
+    int Dp, Vp, P, KE;         // padded widths; planes of X and W; bytes of a kept logit (and of the P that takes its place)
+    int keep, PP;              // what the logits' product keeps; planes of P
     int rows, pieces;          // rows of a piece
     bool pack_w, grad;
-    int64_t rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, dbpart, dwacc, total;
+    int64_t rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, Pp, dbpart, dwacc, sums, total;
 };
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+pg::Plan plan_of(int64_t M, int64_t N, int64_t k, int pa, int pb) {
+    return pg::plan((long)ceil_div(M, 256) * ceil_div(N, 256), (long)ceil_div(M, 128) * ceil_div(N, 128), k, pa, pb);
+}
+pg::Plan logits_plan(const Layout &l, int V, int rows) { return plan_of(rows, V, l.Dp, l.P, l.P); }
+pg::Plan dx_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(rows, d.D, d.V, l.PP, l.P); }
+pg::Plan dw_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(d.V, d.D, rows, l.PP, l.P); }
 
 Layout layout(const LinearCe &d) {
     Layout l{};
@@ -525,7 +585,10 @@ Layout layout(const LinearCe &d) {
     l.Vp = (d.V + 63) & ~63;
     l.P = d.f16 ? 1 : 2;
     l.grad = d.dX || d.dW || d.dbias;
-    l.KE = !l.grad ? 0 : d.g16 ? 2 : 4;
+    // f16 gradients make do with exp(z - maximum) in f16; db, which is f32, takes the logits themselves
+    l.keep = !l.grad ? KEEP_NONE : d.g16 && !d.dbias ? KEEP_EXP : KEEP_Z;
+    l.PP = d.g16 ? 1 : 2;
+    l.KE = l.keep == KEEP_NONE ? 0 : l.keep == KEEP_EXP ? 2 : d.g16 ? 6 : 4;
     l.pack_w = !d.f16 || d.D % 64 || d.ldw % 8 || ((uintptr_t)d.W & 15) || d.ldw > 1 << 22;
     const int64_t Np = ((int64_t)d.N + 63) & ~63ll;
     int64_t rows = Np;
@@ -551,9 +614,17 @@ Layout layout(const LinearCe &d) {
     l.stats = take(rows * ((l.Vp + 255) / 256 * 256 / kStatCols) * 8);
     l.Xp = take(Np * l.Dp * 2 * l.P);
     if (l.pack_w) l.Wp = take((int64_t)d.V * l.Dp * 2 * l.P);
-    if (l.KE) l.E = take(rows * l.Vp * l.KE);
+    if (l.KE) l.E = l.Pp = take(rows * l.Vp * std::min(l.KE, 4));
+    if (l.KE == 6) l.Pp = take(rows * l.Vp * 2);
     if (d.dbias) l.dbpart = take(Np / kGradRows * d.V * 4);
     if (d.dW && d.g16 && l.pieces > 1) l.dwacc = take((int64_t)d.V * d.D * 4);
+    int64_t sums = 0;
+    for (const int64_t r : {rows, Np - (l.pieces - 1) * rows}) {   // the last piece has fewer rows, and its own plan
+        sums = std::max(sums, (int64_t)logits_plan(l, d.V, (int)r).part_bytes());
+        if (d.dX) sums = std::max(sums, (int64_t)dx_plan(l, d, (int)r).part_bytes());
+        if (d.dW) sums = std::max(sums, (int64_t)dw_plan(l, d, (int)r).part_bytes());
+    }
+    l.sums = take(sums);
     l.total = (at + 255) & ~255ll;
     return l;
 }
@@ -563,53 +634,60 @@ using T256 = pg::Tile<256, 256, 4, 2, TA, TB, PA, PB, 2>;
 template <int PA, int PB, int TA, int TB>
 using T128 = pg::Tile<128, 128, 2, 2, TA, TB, PA, PB, 2>;
 
-int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
-
-template <class C>
-void launch_logits(LogitArgs a, int keep, int *WN, hipStream_t s) {
+template <class C, int KEEP>
+void launch_logits(LogitArgs a, hipStream_t s) {
     a.tiles_m = ceil_div(a.rows, C::BM);
-    a.tiles_n = ceil_div(a.V, C::BN);
-    a.T = a.tiles_n * C::WVN;
-    *WN = C::WN;
-    const dim3 grid((unsigned)(a.tiles_m * a.tiles_n));
-    if (keep == KEEP_NONE) hipLaunchKernelGGL((lce_logits_kernel<C, KEEP_NONE>), grid, dim3(C::NT), 0, s, a);
-    else if (keep == KEEP_EXP) hipLaunchKernelGGL((lce_logits_kernel<C, KEEP_EXP>), grid, dim3(C::NT), 0, s, a);
-    else hipLaunchKernelGGL((lce_logits_kernel<C, KEEP_Z>), grid, dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((lce_logits_kernel<C, KEEP>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a);
+    if (a.w.splits > 1) hipLaunchKernelGGL((lce_logits_join_kernel<C, KEEP>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
+}
+
+template <int P>
+void logits(const LogitArgs &a, bool big, int keep, hipStream_t s) {
+    using B = T256<P, P, 0, 0>;
+    using S = T128<P, P, 0, 0>;
+    if (keep == KEEP_NONE) big ? launch_logits<B, KEEP_NONE>(a, s) : launch_logits<S, KEEP_NONE>(a, s);
+    else if (keep == KEEP_Z) big ? launch_logits<B, KEEP_Z>(a, s) : launch_logits<S, KEEP_Z>(a, s);
+    else if constexpr (P == 1) big ? launch_logits<B, KEEP_EXP>(a, s) : launch_logits<S, KEEP_EXP>(a, s);
 }
 
 template <class C>
 void launch_product(ProductArgs a, hipStream_t s) {
     a.tiles_m = ceil_div(a.rows_are == 0 ? a.rows : a.M, C::BM);
     a.tiles_n = ceil_div(a.N, C::BN);
-    hipLaunchKernelGGL((lce_product_kernel<C>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((lce_product_kernel<C>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a);
+    if (a.w.splits > 1) hipLaunchKernelGGL((lce_product_join_kernel<C>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
 }
 
 template <int PP, int PO>
-void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Operand &W, const pg::Operand &X, const half_t *P, int piece, char *ws,
-               hipStream_t s) {
+void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Operand &W, const pg::Operand &X, int piece, char *ws, hipStream_t s) {
     const Scalars *sc = (const Scalars *)ws;
-    const int *rowmap = (const int *)(ws + l.rowmap) + a.row0;
-    const pg::Operand Prow = pg::panels(P, a.rows, a.rows, a.rows), Pcol = pg::panels(P, a.rows, l.Vp, a.rows);
+    const char *P = ws + l.Pp;
     if (d.dX) {
         ProductArgs b = a;
-        b.A = Prow;
+        const pg::Plan plan = dx_plan(l, d, a.rows);
+        b.w = plan.w;
+        b.w.part = (float *)(ws + l.sums);
+        b.A = pg::panels(P, a.rows, a.rows, a.rows);
         b.B = W;
         b.B.rows = l.Dp;
         b.B.k = d.V;
         b.N = d.D;
         b.k = d.V;
         b.rows_are = 0;
-        b.rowmap = rowmap;
+        b.rowmap = (const int *)(ws + l.rowmap) + a.row0;
         b.bmax = PO == 2 ? &sc->wmax : nullptr;
         b.C = d.dX;
         b.ldc = d.lddx;
         b.vec = d.lddx % 4 == 0 && ((uintptr_t)d.dX & (d.g16 ? 7 : 15)) == 0;
-        if ((int64_t)a.rows * d.D > 64 * 256 * 256) launch_product<T256<PP, PO, 0, 1>>(b, s);
+        if (plan.big) launch_product<T256<PP, PO, 0, 1>>(b, s);
         else launch_product<T128<PP, PO, 0, 1>>(b, s);
     }
     if (d.dW) {
         ProductArgs b = a;
-        b.A = Pcol;
+        const pg::Plan plan = dw_plan(l, d, a.rows);
+        b.w = plan.w;
+        b.w.part = (float *)(ws + l.sums);
+        b.A = pg::panels(P, a.rows, l.Vp, a.rows);
         b.B = X;
         b.B.rows = l.Dp;
         b.B.k = a.rows;
@@ -631,7 +709,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
                 b.acc_out = piece + 1 < l.pieces ? acc : nullptr;
             }
         }
-        if ((int64_t)d.V * d.D > 64 * 256 * 256) launch_product<T256<PP, PO, 1, 1>>(b, s);
+        if (plan.big) launch_product<T256<PP, PO, 1, 1>>(b, s);
         else launch_product<T128<PP, PO, 1, 1>>(b, s);
     }
 }
@@ -658,15 +736,18 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
     if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc);
     else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc);
 
-    const int keep = !l.grad ? KEEP_NONE : d.g16 ? KEEP_EXP : KEEP_Z;
     const pg::Operand W = l.pack_w ? pg::panels(Wp, d.V, d.V, l.Dp) : pg::row_major(d.W, d.ldw, d.V, l.Dp);
     for (int piece = 0; piece < l.pieces; piece++) {
         const int row0 = piece * l.rows, rows = std::min(l.rows, Np - row0);
         const pg::Operand X = pg::panels(Xp + (long)row0 * 64, Np, rows, l.Dp);
+        const pg::Plan plan = logits_plan(l, d.V, rows);
         LogitArgs a{};
         a.X = X;
         a.W = W;
         a.V = d.V;
+        a.nk = l.Dp / (l.P == 1 ? 64 : 32);
+        a.w = plan.w;
+        a.w.part = (float *)(ws + l.sums);
         a.sc = sc;
         a.row0 = row0;
         a.rows = rows;
@@ -676,21 +757,20 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         a.lab = lab + row0;
         a.zt = zt + row0;
         a.stats = stats;
+        a.T = 2 * ceil_div(d.V, plan.big ? 256 : 128);   // two waves side by side in either tile
         a.E = ws + l.E;
         a.Vp = l.Vp;
-        int WN = 0;
-        a.nk = l.Dp / (l.P == 1 ? 64 : 32);
-        const bool big = (int64_t)rows * d.V > 128 * 256 * 256;
-        if (l.P == 1) big ? launch_logits<T256<1, 1, 0, 0>>(a, keep, &WN, s) : launch_logits<T128<1, 1, 0, 0>>(a, keep, &WN, s);
-        else big ? launch_logits<T256<2, 2, 0, 0>>(a, keep, &WN, s) : launch_logits<T128<2, 2, 0, 0>>(a, keep, &WN, s);
-        const int T = ceil_div(d.V, big ? 256 : 128) * 2;
-        hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, sc, row0, rows, stats, T, zt + row0, rowmap + row0,
+        if (l.P == 1) logits<1>(a, plan.big, l.keep, s);
+        else logits<2>(a, plan.big, l.keep, s);
+        hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, sc, row0, rows, stats, a.T, zt + row0, rowmap + row0,
                            lse + row0, loss + row0, d.rowloss, d.lse);
         if (!l.grad) continue;
-        GradArgs g{sc, row0, rows, d.V, l.Vp, T, WN, stats, lse + row0, zt + row0, lab + row0, ws + l.E, d.dbias ? (float *)(ws + l.dbpart) : nullptr};
-        const dim3 ggrid((unsigned)ceil_div(l.Vp, 64 * (keep == KEEP_EXP ? 8 : 4)), (unsigned)ceil_div(rows, kGradRows));
-        if (keep == KEEP_EXP) hipLaunchKernelGGL(lce_grad_kernel<KEEP_EXP>, ggrid, dim3(256), 0, s, g);
-        else hipLaunchKernelGGL(lce_grad_kernel<KEEP_Z>, ggrid, dim3(256), 0, s, g);
+        const GradArgs g{sc, row0, rows, d.V, l.Vp, a.T, plan.big ? 128 : 64, stats, lse + row0, zt + row0, lab + row0, ws + l.E, ws + l.Pp,
+                         d.dbias ? (float *)(ws + l.dbpart) : nullptr};
+        const dim3 ggrid((unsigned)ceil_div(l.Vp, 64 * (l.keep == KEEP_EXP ? 8 : 4)), (unsigned)ceil_div(rows, kGradRows));
+        if (l.keep == KEEP_EXP) hipLaunchKernelGGL((lce_grad_kernel<KEEP_EXP, 1>), ggrid, dim3(256), 0, s, g);
+        else if (l.PP == 1) hipLaunchKernelGGL((lce_grad_kernel<KEEP_Z, 1>), ggrid, dim3(256), 0, s, g);
+        else hipLaunchKernelGGL((lce_grad_kernel<KEEP_Z, 2>), ggrid, dim3(256), 0, s, g);
         ProductArgs p{};
         p.sc = sc;
         p.row0 = row0;
@@ -698,10 +778,9 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         p.grad_scale = d.grad_scale;
         p.mean = d.mean;
         p.out16 = d.g16;
-        const half_t *P = (const half_t *)(ws + l.E);
-        if (d.g16 && d.f16) gradients<1, 1>(d, l, p, W, X, P, piece, ws, s);
-        else if (d.f16) gradients<2, 1>(d, l, p, W, X, P, piece, ws, s);
-        else gradients<2, 2>(d, l, p, W, X, P, piece, ws, s);
+        if (l.PP == 1) gradients<1, 1>(d, l, p, W, X, piece, ws, s);
+        else if (d.f16) gradients<2, 1>(d, l, p, W, X, piece, ws, s);
+        else gradients<2, 2>(d, l, p, W, X, piece, ws, s);
     }
     if (d.dbias)
         hipLaunchKernelGGL(lce_dbias_kernel, dim3((unsigned)ceil_div(d.V, 256)), dim3(256), 0, s, sc, (const float *)(ws + l.dbpart), d.V, d.grad_scale,

@@ -22,7 +22,7 @@ struct OnDevice {
     }
 };
 
-constexpr int64_t kMaxSide = 1 << 20, kMaxRows = 1 << 27, kMaxStride = 1ll << 40;
+constexpr int64_t kMaxSide = 1 << 20, kMaxRows = 1 << 27, kMaxStride = 1ll << 40, kMaxElems = 1ll << 40;
 
 // A block of device memory: rows of `width` bytes, `ld` bytes apart.
 struct Span {
@@ -66,6 +66,7 @@ int linear_ce_args(ah_device *dev, const ah_linear_ce_desc *d, LinearCe *o) {
     if (d->N < 1 || d->D < 1 || d->V < 1 || d->N > kMaxRows || d->V > kMaxRows || d->D > kMaxSide)
         return set_error(AH_ERR_INVALID, "%s: N=%d D=%d V=%d (1 to %lld rows and classes, 1 to %lld features)", fn, d->N, d->D, d->V,
                          (long long)kMaxRows, (long long)kMaxSide);
+    if ((int64_t)d->N * d->D > kMaxElems || (int64_t)d->V * d->D > kMaxElems) return set_error(AH_ERR_INVALID, "%s: more than 2^40 elements", fn);
     if (!d->X || !d->W || !d->labels || !d->loss) return set_error(AH_ERR_INVALID, "%s: null X, W, labels or loss", fn);
     if (d->ldx < d->D || d->ldw < d->D || (d->dX && d->lddx < d->D) || (d->dW && d->lddw < d->D) || d->ldx > kMaxStride || d->ldw > kMaxStride ||
         (d->dX && d->lddx > kMaxStride) || (d->dW && d->lddw > kMaxStride))
@@ -97,6 +98,7 @@ int ns_common(const char *fn, ah_device *dev, int32_t dtype, int32_t rows, int32
     if (dtype != AH_F32 && dtype != AH_F16) return set_error(AH_ERR_UNSUPPORTED, "%s: dtype %d", fn, dtype);
     if (rows < 1 || cols < 1 || batch < 1 || rows > kMaxSide || cols > kMaxSide || batch > 65535)
         return set_error(AH_ERR_INVALID, "%s: %d matrices of %d x %d (sides 1 to %lld, 1 to 65535 matrices)", fn, batch, rows, cols, (long long)kMaxSide);
+    if ((int64_t)(rows + 63) * (cols + 63) * batch > kMaxElems) return set_error(AH_ERR_INVALID, "%s: more than 2^40 elements", fn);
     if (steps < 1 || steps > 64) return set_error(AH_ERR_INVALID, "%s: %d steps (1 to 64)", fn, steps);
     if (!(fabsf(a) + fabsf(b) + fabsf(c) <= 15.0f)) return set_error(AH_ERR_INVALID, "%s: |a| + |b| + |c| is over 15", fn);
     if (!(eps >= 0.0f) || !std::isfinite(eps)) return set_error(AH_ERR_INVALID, "%s: eps is negative or not finite", fn);

@@ -1,7 +1,7 @@
 // muon.hip — Newton-Schulz orthogonalisation, and the momentum step whose update it orthogonalises.
 //
-//   X = U / (|U|_F + eps);  steps times:  A = X X^T,  B = a I + b A + c A A,  X <- B X      (U wide)
-//                                         A = X^T X,                          X <- X B      (U tall)
+//   X = U / (|U|_F + eps);  steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X      (U wide)
+//                                         A = X^T X,                    X <- a X + X B      (U tall)
 //
 // The iteration raises small singular values by a = 3.4 a step, 480-fold in five: what is lost of X to rounding grows as much. So X, A
 // and B are carried as two f16 planes (22 bits, plane_gemm.h) and every product is three f16 products in an f32 accumulator;
@@ -9,8 +9,9 @@
 // The planes hold 2^12 X, 2^13 A and 2^11 B: with the singular values of X at most 1.2, as the iteration keeps them, entries
 // stay far below f16's largest value, and entries down to 2^-22 of the matrix's norm keep 22 bits less what they are below 2^-14.
 //
-// A and B are symmetric: only tiles on and above the diagonal are computed and each is stored twice. a I is folded into B, so X
-// is read by the last product alone. X, A and B stay padded with zeros to multiples of 64, where no product needs a bound.
+// A and B are symmetric: only tiles on and above the diagonal are computed and each is stored twice. a X is added in the last
+// product's epilogue: folded into B as a I it would be rounded with B, and where singular values are small a X is all there is.
+// X, A and B stay padded with zeros to multiples of 64, where no product needs a bound.
 #include "muon.h"
 
 #include <algorithm>
@@ -143,87 +144,109 @@ struct NsArgs {
     long sA, sB;            // bytes from matrix to matrix
     int M, N, nk;           // padded sizes
     int tiles_m, tiles_n;
-    const half_t *Q;        // NS_POLY: the Gram matrix's planes
+    int tiles;              // of one matrix
+    pg::Work w;
+    const half_t *Q;        // planes added in the epilogue: the Gram matrix (NS_POLY), X (NS_NEXT, NS_LAST)
     half_t *out;            // planes
     long sQ, so;            // halves
-    int rows;               // of out's panels
+    int rows;               // of Q's and out's panels
 };
+
+template <class C, int WHAT>
+__device__ __forceinline__ void ns_tile(const NsArgs &p, int tile, long &z, int &m0, int &n0) {
+    z = tile / p.tiles;
+    int tr, tc;
+    if constexpr (WHAT == NS_GRAM || WHAT == NS_POLY) pg::tri_tile(tile - (int)z * p.tiles, p.tiles_m, tr, tc);
+    else pg::grouped_tile(tile - (int)z * p.tiles, p.tiles_m, p.tiles_n, tr, tc);
+    m0 = tr * C::BM;
+    n0 = tc * C::BN;
+}
+
+// What follows a product, for accumulator row i.
+template <class C, int WHAT>
+__device__ __forceinline__ void ns_row(const NsArgs &p, const Muon &d, long z, int m0, int n0, int i, const floatx4 (&acc)[C::FB]) {
+    constexpr bool SYM = WHAT == NS_GRAM || WHAT == NS_POLY;
+    const pg::Place<C> at(m0, n0);
+    const int m = at.m + 16 * i;
+    if (m >= p.M) return;
+    const float ca = d.a, cb = d.b, cc = d.c, keep = 1.0f - d.lr * d.decay, step = d.lr * d.scale;
+#pragma unroll
+    for (int j = 0; j < C::FB; j++) {
+        const int n = at.n + 16 * j;
+        if (n >= p.N) continue;
+        floatx4 v = acc[j], q = {};
+        if constexpr (WHAT != NS_GRAM) {
+            const half_t *s = p.Q + z * p.sQ + pg::panel_at<2>(p.rows, m, n);
+            const h4 hi = *(const h4 *)s, lo = *(const h4 *)(s + 32);
+#pragma unroll
+            for (int r = 0; r < 4; r++) q[r] = (float)hi[r] + (float)lo[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if constexpr (WHAT == NS_GRAM) v[r] *= 1.0f / (1 << (2 * kSX - kSA));
+            else if constexpr (WHAT == NS_POLY) v[r] = cc * (v[r] * (1.0f / (1 << (2 * kSA - kSB)))) + cb * (q[r] * (1.0f / (1 << (kSA - kSB))));
+            else v[r] = ca * q[r] + v[r] * (1.0f / (1 << kSB));
+        }
+        if constexpr (WHAT != NS_LAST) {
+            half_t *o = p.out + z * p.so;
+            pg::plane_store(o + pg::panel_at<2>(p.rows, m, n), v);
+            if (SYM && m0 != n0) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const half_t hi = (half_t)v[r];
+                    half_t *t = o + pg::panel_at<2>(p.rows, n + r, m);
+                    t[0] = hi;
+                    t[32] = (half_t)(v[r] - (float)hi);
+                }
+            }
+        } else {
+            if (m >= d.rows || n >= d.cols) continue;
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] *= 1.0f / (1 << kSX);
+            if (d.W) {
+                const long w0 = z * d.sw + (long)m * d.ldw;
+                const floatx4 w = load4(d.W + w0, n, d.cols, d.vec_w);
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[r] = keep * w[r] - step * v[r];
+                store4(d.W_out + w0, n, d.cols, d.vec_w, v);
+                if (d.W16_out) store4((half_t *)d.W16_out + w0, n, d.cols, d.vec_o, v);
+            } else {
+                const long o0 = z * d.so + (long)m * d.ldo;
+                if (d.out16) store4((half_t *)d.O + o0, n, d.cols, d.vec_o, v);
+                else store4((float *)d.O + o0, n, d.cols, d.vec_o, v);
+            }
+        }
+    }
+}
 
 template <class C, int WHAT>
 __global__ __launch_bounds__(C::NT) void ns_product_kernel(NsArgs p, Muon d) {
     __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
-    constexpr bool SYM = WHAT == NS_GRAM || WHAT == NS_POLY;
-    const long z = blockIdx.y;
-    int tr, tc;
-    const int L = pg::xcd_tile(blockIdx.x, gridDim.x);
-    if constexpr (SYM) pg::tri_tile(L, tr, tc);
-    else pg::grouped_tile(L, p.tiles_m, p.tiles_n, tr, tc);
-    const int m0 = tr * C::BM, n0 = tc * C::BN;
+    int tile, slot, first, count, m0, n0;
+    long z;
+    pg::pick(p.w, blockIdx.x, p.nk, tile, slot, first, count);
+    ns_tile<C, WHAT>(p, tile, z, m0, n0);
     pg::Operand A = p.A, B = p.B;
     A.p += z * p.sA;
     B.p += z * p.sB;
     floatx4 acc[C::FA][C::FB];
-    pg::contract<C>(A, B, m0, n0, 0, p.nk, smem, acc);
-
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int mb = m0 + (wave / C::WVN) * C::WM + (lane & 15), nb = n0 + (wave % C::WVN) * C::WN + 4 * (lane >> 4);
-    const float ca = d.a, cb = d.b, cc = d.c, keep = 1.0f - d.lr * d.decay, step = d.lr * d.scale;
-#pragma unroll
-    for (int i = 0; i < C::FA; i++) {
-        const int m = mb + 16 * i;
-        if (m >= p.M) continue;
-#pragma unroll
-        for (int j = 0; j < C::FB; j++) {
-            const int n = nb + 16 * j;
-            if (n >= p.N) continue;
-            floatx4 v = acc[i][j];
-            if constexpr (WHAT == NS_GRAM) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) v[r] *= 1.0f / (1 << (2 * kSX - kSA));
-            } else if constexpr (WHAT == NS_POLY) {
-                const half_t *q = p.Q + z * p.sQ + pg::panel_at<2>(p.rows, m, n);
-                const h4 hi = *(const h4 *)q, lo = *(const h4 *)(q + 32);
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float g = (float)hi[r] + (float)lo[r];
-                    v[r] = cc * (v[r] * (1.0f / (1 << (2 * kSA - kSB)))) + cb * (g * (1.0f / (1 << (kSA - kSB))));
-                    if (n + r == m) v[r] += ca * (float)(1 << kSB);
-                }
-            } else if constexpr (WHAT == NS_NEXT) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) v[r] *= 1.0f / (1 << kSB);
-            }
-            if constexpr (WHAT != NS_LAST) {
-                half_t *o = p.out + z * p.so;
-                pg::plane_store(o + pg::panel_at<2>(p.rows, m, n), v);
-                if (SYM && m0 != n0) {
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const half_t hi = (half_t)v[r];
-                        half_t *t = o + pg::panel_at<2>(p.rows, n + r, m);
-                        t[0] = hi;
-                        t[32] = (half_t)(v[r] - (float)hi);
-                    }
-                }
-            } else {
-                if (m >= d.rows || n >= d.cols) continue;
-#pragma unroll
-                for (int r = 0; r < 4; r++) v[r] *= 1.0f / (1 << (kSB + kSX));
-                if (d.W) {
-                    const long at = z * d.sw + (long)m * d.ldw;
-                    const floatx4 w = load4(d.W + at, n, d.cols, d.vec_w);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) v[r] = keep * w[r] - step * v[r];
-                    store4(d.W_out + at, n, d.cols, d.vec_w, v);
-                    if (d.W16_out) store4((half_t *)d.W16_out + at, n, d.cols, d.vec_o, v);
-                } else {
-                    const long at = z * d.so + (long)m * d.ldo;
-                    if (d.out16) store4((half_t *)d.O + at, n, d.cols, d.vec_o, v);
-                    else store4((float *)d.O + at, n, d.cols, d.vec_o, v);
-                }
-            }
-        }
+    pg::contract<C>(A, B, m0, n0, first, count, smem, acc);
+    if (slot >= 0) {
+        pg::store_partials<C>(p.w.part, slot, acc);
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < C::FA; i++) ns_row<C, WHAT>(p, d, z, m0, n0, i, acc[i]);
+}
+
+template <class C, int WHAT>
+__global__ __launch_bounds__(C::NT) void ns_join_kernel(NsArgs p, Muon d) {
+    int m0, n0;
+    long z;
+    ns_tile<C, WHAT>(p, p.w.whole + blockIdx.x, z, m0, n0);
+    floatx4 v[C::FB];
+    pg::sum_partials<C>(p.w, blockIdx.x, blockIdx.y, v);
+    ns_row<C, WHAT>(p, d, z, m0, n0, blockIdx.y, v);
 }
 
 // ── host ───────────────────────────────────────────────────────────────────────
@@ -233,8 +256,19 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 struct Layout {
     int Rp, Cp, S;   // padded sides, the short one
     int parts;
-    int64_t part, X0, X1, A, B, total;
+    int64_t part, X0, X1, A, B, sums, total;
 };
+
+bool symmetric(int what) { return what == NS_GRAM || what == NS_POLY; }
+
+// Tiles of one product over the batch and how they are split, for M x N results summed over k.
+pg::Plan ns_plan(int what, int batch, int M, int N, int k) {
+    const auto tiles = [&](int w) -> long {
+        const long m = ceil_div(M, w), n = ceil_div(N, w);
+        return batch * (symmetric(what) ? m * (m + 1) / 2 : m * n);
+    };
+    return pg::plan(tiles(256), tiles(128), k, 2, 2);
+}
 
 Layout layout(const Muon &d) {
     Layout l{};
@@ -254,6 +288,9 @@ Layout layout(const Muon &d) {
     l.X1 = take((int64_t)d.batch * l.Rp * l.Cp * 4);
     l.A = take((int64_t)d.batch * l.S * l.S * 4);
     l.B = take((int64_t)d.batch * l.S * l.S * 4);
+    const int K = d.rows <= d.cols ? l.Cp : l.Rp;
+    l.sums = take(std::max({ns_plan(NS_GRAM, d.batch, l.S, l.S, K).part_bytes(), ns_plan(NS_POLY, d.batch, l.S, l.S, l.S).part_bytes(),
+                            ns_plan(NS_NEXT, d.batch, l.Rp, l.Cp, l.S).part_bytes()}));
     l.total = (at + 255) & ~255ll;
     return l;
 }
@@ -262,14 +299,17 @@ template <class C, int WHAT>
 void launch(NsArgs p, const Muon &d, hipStream_t s) {
     p.tiles_m = ceil_div(p.M, C::BM);
     p.tiles_n = ceil_div(p.N, C::BN);
-    const int tiles = WHAT == NS_GRAM || WHAT == NS_POLY ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
-    hipLaunchKernelGGL((ns_product_kernel<C, WHAT>), dim3((unsigned)tiles, (unsigned)d.batch), dim3(C::NT), 0, s, p, d);
+    p.tiles = symmetric(WHAT) ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+    hipLaunchKernelGGL((ns_product_kernel<C, WHAT>), dim3((unsigned)p.w.blocks()), dim3(C::NT), 0, s, p, d);
+    if (p.w.splits > 1) hipLaunchKernelGGL((ns_join_kernel<C, WHAT>), dim3((unsigned)p.w.rest, C::FA), dim3(C::NT), 0, s, p, d);
 }
 
 template <int TA, int TB, int WHAT>
-void product(const NsArgs &p, const Muon &d, hipStream_t s) {
-    const int64_t tiles = (int64_t)ceil_div(p.M, 256) * ceil_div(p.N, 256) * d.batch;
-    if (tiles >= 128) launch<pg::Tile<256, 256, 4, 2, TA, TB, 2, 2, 2>, WHAT>(p, d, s);
+void product(NsArgs p, const Muon &d, float *part, hipStream_t s) {
+    const pg::Plan plan = ns_plan(WHAT, d.batch, p.M, p.N, p.nk * 32);
+    p.w = plan.w;
+    p.w.part = part;
+    if (plan.big) launch<pg::Tile<256, 256, 4, 2, TA, TB, 2, 2, 2>, WHAT>(p, d, s);
     else launch<pg::Tile<128, 128, 2, 2, TA, TB, 2, 2, 2>, WHAT>(p, d, s);
 }
 
@@ -288,6 +328,7 @@ hipError_t muon(const Muon &in, void *wsp, hipStream_t s) {
     const Layout l = layout(d);
     char *ws = (char *)wsp;
     double *part = (double *)(ws + l.part);
+    float *sums = (float *)(ws + l.sums);
     half_t *X = (half_t *)(ws + l.X0), *Xn = (half_t *)(ws + l.X1), *A = (half_t *)(ws + l.A), *B = (half_t *)(ws + l.B);
     const bool wide = d.rows <= d.cols;
     hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)l.parts, (unsigned)d.batch), dim3(256), 0, s, d, part);
@@ -303,19 +344,21 @@ hipError_t muon(const Muon &in, void *wsp, hipStream_t s) {
         g.sA = g.sB = sx;
         g.A = g.B = pg::panels(X, l.Rp, l.S, wide ? l.Cp : l.Rp);
         g.nk = (wide ? l.Cp : l.Rp) / 32;
-        if (wide) product<0, 0, NS_GRAM>(g, d, s);
-        else product<1, 1, NS_GRAM>(g, d, s);
+        if (wide) product<0, 0, NS_GRAM>(g, d, sums, s);
+        else product<1, 1, NS_GRAM>(g, d, sums, s);
 
-        NsArgs q = g;   // B = a I + b A + c A A
+        NsArgs q = g;   // B = b A + c A A
         q.Q = A;
         q.sQ = ss / 2;
         q.out = B;
         q.sA = q.sB = ss;
         q.A = q.B = pg::panels(A, l.S, l.S, l.S);
         q.nk = l.S / 32;
-        product<0, 0, NS_POLY>(q, d, s);
+        product<0, 0, NS_POLY>(q, d, sums, s);
 
-        NsArgs n{};   // B X or X B (B is symmetric: its rows serve as columns)
+        NsArgs n{};   // a X + B X or a X + X B (B is symmetric: its rows serve as columns)
+        n.Q = X;
+        n.sQ = sx / 2;
         n.M = l.Rp;
         n.N = l.Cp;
         n.out = Xn;
@@ -335,8 +378,8 @@ hipError_t muon(const Muon &in, void *wsp, hipStream_t s) {
         }
         n.nk = l.S / 32;
         const bool last = k + 1 == d.steps;
-        if (wide) last ? product<0, 1, NS_LAST>(n, d, s) : product<0, 1, NS_NEXT>(n, d, s);
-        else last ? product<0, 0, NS_LAST>(n, d, s) : product<0, 0, NS_NEXT>(n, d, s);
+        if (wide) last ? product<0, 1, NS_LAST>(n, d, sums, s) : product<0, 1, NS_NEXT>(n, d, sums, s);
+        else last ? product<0, 0, NS_LAST>(n, d, sums, s) : product<0, 0, NS_NEXT>(n, d, sums, s);
         std::swap(X, Xn);
     }
     return hipGetLastError();

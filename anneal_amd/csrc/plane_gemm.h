@@ -323,12 +323,143 @@ __device__ __forceinline__ void grouped_tile(int t, int tiles_m, int tiles_n, in
     col = rem / size;
 }
 
-// Tile t of the upper triangle (row <= column) of a square of n tiles a side, walked by columns.
-__device__ __forceinline__ void tri_tile(int t, int &row, int &col) {
-    col = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
-    while ((col + 1) * (col + 2) / 2 <= t) col++;
-    while (col * (col + 1) / 2 > t) col--;
-    row = t - col * (col + 1) / 2;
+// Tile t of the upper triangle (row <= column) of a square of n tiles a side: rows in groups of 4, walked by columns within a
+// group, as above.
+__device__ __forceinline__ void tri_tile(int t, int n, int &row, int &col) {
+    int g = 0;
+    for (;; g += 4) {   // a group's four rows hold n - g, n - g - 1, ... tiles
+        const int rows = min(4, n - g), count = rows * (n - g) - rows * (rows - 1) / 2;
+        if (t < count) break;
+        t -= count;
+    }
+    const int rows = min(4, n - g);
+    // the columns of the group's corner hold 1, 2, .. tiles, the others `rows`
+    int c = 0;
+    while (c < rows - 1 && t > c) t -= ++c;
+    if (c == rows - 1) {
+        c += t / rows;
+        t %= rows;
+    }
+    row = g + t;
+    col = g + c;
+}
+
+// ── tiles, and K split over workgroups ─────────────────────────────────────────
+// Tiles are worked on in rounds of as many as the chip takes at once. What is left for the last round (all of them, where there
+// are few) is split over K: `splits` workgroups share a tile's stages and leave their accumulators in the workspace, and a second
+// kernel adds them in order (results repeat bit for bit) and runs the epilogue, one workgroup for each 16 rows of a tile's waves.
+struct Work {
+    int whole, rest, splits;   // tiles 0 .. whole-1 in one piece each, then `rest` tiles of `splits` pieces
+    float *part;               // [split][rest] partial tiles
+    __host__ __device__ int tiles() const { return whole + rest; }
+    __host__ __device__ int blocks() const { return whole + rest * splits; }
+};
+
+// Workgroup b's tile and its stages [first, first + count) of nk; slot: where its partial sums go, -1 for a whole tile.
+__device__ __forceinline__ void pick(const Work &w, int b, int nk, int &tile, int &slot, int &first, int &count) {
+    slot = -1;
+    first = 0;
+    count = nk;
+    if (b < w.whole) {
+        tile = xcd_tile(b, w.whole);
+        return;
+    }
+    const int r = xcd_tile(b - w.whole, w.rest * w.splits), split = r / w.rest;
+    tile = w.whole + r - split * w.rest;
+    if (w.splits == 1) return;
+    const int q = (nk + w.splits - 1) / w.splits;
+    first = min(nk, split * q);
+    count = min(nk, first + q) - first;
+    slot = r;
+}
+
+// Partial sums of accumulator row i: [slot][i][j][thread] of four floats.
+template <class C>
+__device__ __forceinline__ floatx4 *partial(float *part, long slot, int i) {
+    return (floatx4 *)part + (slot * C::FA + i) * C::FB * C::NT + threadIdx.x;
+}
+template <class C>
+__device__ __forceinline__ void store_partials(float *part, long slot, const floatx4 (&acc)[C::FA][C::FB]) {
+#pragma unroll
+    for (int i = 0; i < C::FA; i++)
+#pragma unroll
+        for (int j = 0; j < C::FB; j++) partial<C>(part, slot, i)[j * C::NT] = acc[i][j];
+}
+template <class C>
+__device__ __forceinline__ void sum_partials(const Work &w, int r, int i, floatx4 (&v)[C::FB]) {
+#pragma unroll
+    for (int j = 0; j < C::FB; j++) v[j] = (floatx4){};
+    constexpr int B = 32 / C::FB;   // splits whose loads are in flight together
+    int s = 0;
+    for (; s + B <= w.splits; s += B) {
+        floatx4 x[B][C::FB];
+#pragma unroll
+        for (int b = 0; b < B; b++)
+#pragma unroll
+            for (int j = 0; j < C::FB; j++) x[b][j] = partial<C>(w.part, (long)(s + b) * w.rest + r, i)[j * C::NT];
+#pragma unroll
+        for (int b = 0; b < B; b++)
+#pragma unroll
+            for (int j = 0; j < C::FB; j++) v[j] += x[b][j];
+    }
+    for (; s < w.splits; s++)
+#pragma unroll
+        for (int j = 0; j < C::FB; j++) v[j] += partial<C>(w.part, (long)s * w.rest + r, i)[j * C::NT];
+}
+
+// A wave's place in a tile: the row of C that this lane holds of accumulator row 0, and its first column.
+template <class C>
+struct Place {
+    int m, n, lane, wave;
+    // Opaque, so that an epilogue that runs row after row forms its addresses anew for each: kept for all rows, they spill.
+    __device__ __forceinline__ Place(int m0, int n0) {
+        lane = threadIdx.x & 63;
+        wave = threadIdx.x >> 6;
+        m = m0 + (wave / C::WVN) * C::WM + (lane & 15);
+        n = n0 + (wave % C::WVN) * C::WN + 4 * (lane >> 4);
+        asm volatile("" : "+v"(m), "+v"(n)::"memory");
+    }
+};
+
+// Tile width and splits of a product, by a model of the time it takes.
+struct Plan {
+    bool big;   // 256 x 256 tiles (8 waves, one workgroup a CU), else 128 x 128 (4 waves, two a CU)
+    Work w;
+    long part_bytes() const { return w.splits > 1 ? (long)w.rest * w.splits * (big ? 65536 : 16384) * 4 : 0; }
+};
+
+// tiles256, tiles128: tiles at either width; k: the summed length; pa, pb: planes. Microseconds a stage of the tile loops on this
+// chip, measured over k = 4096 with operands in panels (a stage is 64 k of one plane, 32 of two):
+//                    256 x 256: 32 / 256 workgroups    128 x 128: up to 256 / 512
+//   planes 1 x 1               1.28 / 1.77                    0.75 / 1.15
+//   planes 2 x 1               1.23 / 1.58                    0.64 / 0.97
+//   planes 2 x 2               1.62 / 2.30                    0.74 / 1.33
+// (many CUs at once run slower than few: the clock gives way). Splitting adds a launch and the partial sums' way to memory and back.
+inline Plan plan(long tiles256, long tiles128, long k, int pa, int pb) {
+    const int row = pa == 1 ? 0 : pb == 1 ? 1 : 2;
+    constexpr double kFew[3] = {1.25, 1.2, 1.55}, kMore[3] = {0.52, 0.38, 0.75};
+    constexpr double kOne[3] = {0.75, 0.64, 0.74}, kTwo[3] = {1.15, 0.97, 1.33};
+    const long nk = (k + (row == 0 ? 63 : 31)) / (row == 0 ? 64 : 32);
+    Plan best{};
+    double best_us = 1e30;
+    for (int big = 0; big < 2; big++) {
+        const long tiles = big ? tiles256 : tiles128, slots = big ? 256 : 512;
+        const auto stage = [&](long wg) { return big ? kFew[row] + kMore[row] * (double)wg / 256 : wg <= 256 ? kOne[row] : kTwo[row]; };
+        const double fixed = big ? 5.0 : 3.5;   // first loads and the epilogue
+        const long rest = tiles % slots, rounds = tiles / slots;
+        for (int s = 1; s <= 32 && (s == 1 || (rest * s <= slots && nk >= 2 * s)); s++) {
+            const double joined = (double)rest * s * (big ? 262144 : 65536) * 2 / 4e6;   // us at 4 TB/s
+            const double us = rounds * (nk * stage(slots) + fixed) + (rest ? (double)((nk + s - 1) / s) * stage(rest * s) + fixed : 0) +
+                              (s > 1 ? 4.0 + joined : 0);
+            if (us < best_us) {
+                best_us = us;
+                best.big = big != 0;
+                best.w = s == 1 ? Work{(int)tiles, 0, 1, nullptr} : Work{(int)(rounds * slots), (int)rest, s, nullptr};
+            }
+            if (!rest) break;
+        }
+    }
+    return best;
 }
 
 }  // namespace pg

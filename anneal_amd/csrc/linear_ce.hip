@@ -84,31 +84,53 @@ __global__ __launch_bounds__(1024) void lce_index_kernel(const int *labels, int 
     }
 }
 
-// Largest magnitudes of W and of the counted rows of X (f32): one workgroup per row of either. The bits of non-negative floats
-// order as integers, so the atomic's result does not depend on the order.
+// Largest magnitudes of W and of the counted rows of X (f32), a wave per stretch of 2048 values of a row. The bits of
+// non-negative floats order as integers, so the atomic's result does not depend on the order.
 __global__ __launch_bounds__(256) void lce_absmax_kernel(const float *X, long ldx, int N, const float *W, long ldw, int V, int D, const int *pos,
                                                          Scalars *sc) {
-    __shared__ unsigned red[4];
+    __shared__ unsigned red[2][4];
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (D + 2047) / 2048;
+    const bool vx = ldx % 4 == 0 && ((uintptr_t)X & 15) == 0, vw = ldw % 4 == 0 && ((uintptr_t)W & 15) == 0;
     unsigned mx = 0, mw = 0;
-    for (long r = blockIdx.x; r < (long)N + V; r += gridDim.x) {
+    for (long q = (long)blockIdx.x * 4 + wave; q < ((long)N + V) * segs; q += (long)gridDim.x * 4) {
+        const long r = q / segs;
+        const int c0 = (int)(q - r * segs) * 2048 + lane * 4, end = min(D, c0 - lane * 4 + 2048);
         const bool x = r < N;
         if (x && pos[r] < 0) continue;
-        const float *p = x ? X + r * ldx : W + (r - N) * ldw;
+        const uint32_t *p = (const uint32_t *)(x ? X + r * ldx : W + (r - N) * ldw);
         unsigned m = 0;
-        for (int i = threadIdx.x; i < D; i += 256) m = max(m, __float_as_uint(p[i]) & 0x7fffffffu);
+        if (x ? vx : vw) {
+#pragma unroll
+            for (int k = 0; k < 2048; k += 256) {
+                const int c = c0 + k;
+                if (c + 3 < end) {
+                    const u4 v = *(const u4 *)(p + c) & 0x7fffffffu;
+                    m = max(m, max(max(v[0], v[1]), max(v[2], v[3])));
+                } else {
+                    for (int u = c; u < end; u++) m = max(m, p[u] & 0x7fffffffu);
+                }
+            }
+        } else {
+            for (int c = c0 - lane * 3; c < end; c += 64) m = max(m, p[c] & 0x7fffffffu);
+        }
         if (x) mx = max(mx, m);
         else mw = max(mw, m);
     }
-    for (int k = 0; k < 2; k++) {
-        unsigned m = k ? mw : mx;
-        for (int o = 32; o >= 1; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            m = max(max(red[0], red[1]), max(red[2], red[3]));
-            if (m) atomicMax(k ? &sc->wmax : &sc->xmax, m);
-        }
+    for (int o = 32; o >= 1; o >>= 1) {
+        mx = max(mx, (unsigned)__shfl_xor((int)mx, o, 64));
+        mw = max(mw, (unsigned)__shfl_xor((int)mw, o, 64));
+    }
+    if (lane == 0) {
+        red[0][wave] = mx;
+        red[1][wave] = mw;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const unsigned *p = red[threadIdx.x];
+        const unsigned m = max(max(p[0], p[1]), max(p[2], p[3]));
+        unsigned *to = threadIdx.x ? &sc->wmax : &sc->xmax;
+        if (m > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(to, m);
     }
 }
 
@@ -201,58 +223,84 @@ __device__ __forceinline__ void logits_tile(const LogitArgs &a, int tile, int &m
     n0 = tile / a.tiles_m * C::BN;
 }
 
-// What follows the product, for accumulator row i.
-template <class C, int KEEP>
-__device__ __forceinline__ void logits_row(const LogitArgs &a, int M, int m0, int n0, int i, floatx4 (&z)[C::FB]) {
+// What follows the product, for NR accumulator rows from row i0. What the rows share (biases, where the columns lie in E) is
+// formed once; their labels are loaded together.
+template <class C, int KEEP, int NR>
+__device__ __forceinline__ void logits_rows(const LogitArgs &a, int M, int m0, int n0, int i0, floatx4 (&z)[NR][C::FB]) {
     const pg::Place<C> at(m0, n0);
-    const int m = at.m + 16 * i, tcol = n0 / C::WN + at.wave % C::WVN;
+    const int tcol = n0 / C::WN + at.wave % C::WVN, m1 = at.m + 16 * i0;
     const int e = a.planes ? -(plane_exp(a.sc->xmax) + plane_exp(a.sc->wmax)) : 0;
-    const int y = m < M ? a.lab[m] : -1;
     const float ninf = -__builtin_inff();
-    float mx = ninf;
+    const bool whole = n0 + C::BN <= a.V;
+    int y[NR];
+#pragma unroll
+    for (int i = 0; i < NR; i++) y[i] = m1 + 16 * i < M ? a.lab[m1 + 16 * i] - at.n : -1;
+    floatx4 bias[C::FB];   // -inf past the last class
 #pragma unroll
     for (int j = 0; j < C::FB; j++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int n = at.n + 16 * j + r;
-            float v = a.planes ? ldexpf(z[j][r], e) : z[j][r];
-            if (n >= a.V) v = ninf;
-            else if (a.bias) v += a.bias16 ? (float)((const half_t *)a.bias)[n] : ((const float *)a.bias)[n];
-            z[j][r] = v;
-            mx = fmaxf(mx, v);
-            if (n == y) a.zt[m] = v;
+            bias[j][r] = n >= a.V ? ninf : !a.bias ? 0.0f : a.bias16 ? (float)((const half_t *)a.bias)[n] : ((const float *)a.bias)[n];
         }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float ref = mx == ninf ? 0.0f : mx;   // columns that are all -inf (a bias that rules them out) add nothing
-    float sum = 0.0f;
+    // this lane's first column in E; 16 j columns on are (j & pm) further in the panel and j / (pm + 1) panels on
+    constexpr int LOG = KEEP == KEEP_EXP ? 6 : 5, PM = (1 << (LOG - 4)) - 1, SZ = KEEP == KEEP_EXP ? 2 : 4;
+    char *const tile = KEEP == KEEP_NONE ? nullptr : a.E + (long)((n0 + (at.wave % C::WVN) * C::WN) >> LOG) * a.rows * 128 + (long)m0 * 128;
+    const uint32_t panel = (uint32_t)a.rows * 128;
 #pragma unroll
-    for (int j = 0; j < C::FB; j++) {
-        const int n = at.n + 16 * j;
-        floatx4 ex;
+    for (int i = 0; i < NR; i++) {
+        __builtin_amdgcn_sched_barrier(0);   // one row at a time: together they spill
+        int m = m1 + 16 * i;
+        asm volatile("" : "+v"(m));
+        float mx = ninf;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            ex[r] = __builtin_amdgcn_exp2f((z[j][r] - ref) * kLog2e);
-            sum += ex[r];
+        for (int j = 0; j < C::FB; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                z[i][j][r] = ldexpf(z[i][j][r], e) + bias[j][r];
+                mx = fmaxf(mx, z[i][j][r]);
+            }
+        if ((unsigned)y[i] < (unsigned)(16 * C::FB) && (y[i] & 15) < 4) {   // the label's column is this lane's
+            float zt = 0.0f;
+#pragma unroll
+            for (int j = 0; j < C::FB; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) zt = y[i] == 16 * j + r ? z[i][j][r] : zt;
+            a.zt[m] = zt;
         }
-        if (KEEP != KEEP_NONE && m < M && n < a.Vp) {
-            if constexpr (KEEP == KEEP_EXP) {
-                h4 h;
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float ref = mx == ninf ? 0.0f : mx;   // columns that are all -inf (a bias that rules them out) add nothing
+        float sum = 0.0f;
+        const uint32_t off = (uint32_t)(m - m0) * 128 + 4 * (at.lane >> 4) * SZ;
 #pragma unroll
-                for (int r = 0; r < 4; r++) h[r] = (half_t)(ex[r] * (float)(1 << kPScale));
-                *(h4 *)(a.E + pg::panel_at<1>(a.rows, m, n) * 2) = h;
-            } else {
-                *(floatx4 *)(a.E + z_at(a.rows, m, n)) = z[j];
+        for (int j = 0; j < C::FB; j++) {
+            floatx4 ex;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                ex[r] = __builtin_amdgcn_exp2f((z[i][j][r] - ref) * kLog2e);
+                sum += ex[r];
+            }
+            if (KEEP != KEEP_NONE && m < M && (whole || at.n + 16 * j < a.Vp)) {
+                char *p = tile + (off + (uint32_t)(j / (PM + 1)) * panel) + (j & PM) * 16 * SZ;
+                if constexpr (KEEP == KEEP_EXP) {
+                    h4 h;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) h[r] = (half_t)(ex[r] * (float)(1 << kPScale));
+                    *(h4 *)p = h;
+                } else {
+                    *(floatx4 *)p = z[i][j];
+                }
             }
         }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (at.lane < 16 && m < M) a.stats[(long)m * a.T + tcol] = make_float2(mx, sum);
     }
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
-    if (at.lane < 16 && m < M) a.stats[(long)m * a.T + tcol] = make_float2(mx, sum);
 }
 
 template <class C, int KEEP>
-__global__ __launch_bounds__(C::NT) void lce_logits_kernel(LogitArgs a) {
+__global__ __launch_bounds__(C::NT, 2) void lce_logits_kernel(LogitArgs a) {
     __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
     const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
     int tile, slot, first, count, m0, n0;
@@ -265,8 +313,7 @@ __global__ __launch_bounds__(C::NT) void lce_logits_kernel(LogitArgs a) {
         pg::store_partials<C>(a.w.part, slot, acc);
         return;
     }
-#pragma unroll
-    for (int i = 0; i < C::FA; i++) logits_row<C, KEEP>(a, M, m0, n0, i, acc[i]);
+    logits_rows<C, KEEP, C::FA>(a, M, m0, n0, 0, acc);
 }
 
 template <class C, int KEEP>
@@ -275,9 +322,9 @@ __global__ __launch_bounds__(C::NT) void lce_logits_join_kernel(LogitArgs a) {
     int m0, n0;
     logits_tile<C>(a, a.w.whole + blockIdx.x, m0, n0);
     if (m0 >= M) return;
-    floatx4 z[C::FB];
-    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, z);
-    logits_row<C, KEEP>(a, M, m0, n0, blockIdx.y, z);
+    floatx4 z[1][C::FB];
+    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, z[0]);
+    logits_rows<C, KEEP, 1>(a, M, m0, n0, blockIdx.y, z);
 }
 
 // ── a row's statistics ─────────────────────────────────────────────────────────
@@ -459,7 +506,7 @@ struct ProductArgs {
     long ldacc;
 };
 
-__device__ __forceinline__ int product_rows(const ProductArgs &a, int &nk, int BK) {
+__device__ __forceinline__ int product_size(const ProductArgs &a, int &nk, int BK) {
     const int rows = chunk_rows(&a.sc->count, a.row0, a.rows);
     nk = ((a.rows_are == 0 ? a.k : (rows + 63) & ~63) + BK - 1) / BK;
     return a.rows_are == 0 ? rows : a.M;
@@ -473,14 +520,10 @@ __device__ __forceinline__ void product_tile(const ProductArgs &a, int tile, int
     n0 = tc * C::BN;
 }
 
-// What follows the product, for accumulator row i.
+// What follows the product, for accumulator row i: row m of C, which is row `row` of the output.
 template <class C>
-__device__ __forceinline__ void product_row(const ProductArgs &a, int M, int m0, int n0, int i, const floatx4 (&acc)[C::FB]) {
-    const pg::Place<C> at(m0, n0);
-    const int m = at.m + 16 * i, e = -kPScale - (a.bmax ? plane_exp(*a.bmax) : 0);
-    if (m >= M) return;
-    const float mult = grad_mult(a.sc, a.grad_scale, a.mean);
-    const long row = a.rowmap ? a.rowmap[m] : m;
+__device__ __forceinline__ void product_row(const ProductArgs &a, int m, long row, int n0, float mult, int e, const floatx4 (&acc)[C::FB]) {
+    const pg::Place<C> at(0, n0);
 #pragma unroll
     for (int j = 0; j < C::FB; j++) {
         const int n = at.n + 16 * j;
@@ -527,11 +570,25 @@ __device__ __forceinline__ void product_row(const ProductArgs &a, int M, int m0,
     }
 }
 
+// NR accumulator rows from row i0; their places are loaded together.
+template <class C, int NR>
+__device__ __forceinline__ void product_rows(const ProductArgs &a, int M, int m0, int n0, int i0, const floatx4 (&acc)[NR][C::FB]) {
+    const pg::Place<C> at(m0, n0);
+    const int m1 = at.m + 16 * i0, e = -kPScale - (a.bmax ? plane_exp(*a.bmax) : 0);
+    const float mult = grad_mult(a.sc, a.grad_scale, a.mean);
+    int row[NR];
+#pragma unroll
+    for (int i = 0; i < NR; i++) row[i] = m1 + 16 * i >= M ? -1 : a.rowmap ? a.rowmap[m1 + 16 * i] : m1 + 16 * i;
+#pragma unroll
+    for (int i = 0; i < NR; i++)
+        if (row[i] >= 0) product_row<C>(a, m1 + 16 * i, row[i], n0, mult, e, acc[i]);
+}
+
 template <class C>
-__global__ __launch_bounds__(C::NT) void lce_product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
     __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
     int nk, tile, slot, first, count, m0, n0;
-    const int M = product_rows(a, nk, C::BK);
+    const int M = product_size(a, nk, C::BK);
     pg::pick(a.w, blockIdx.x, nk, tile, slot, first, count);
     product_tile<C>(a, tile, m0, n0);
     if (m0 >= M) return;
@@ -541,19 +598,18 @@ __global__ __launch_bounds__(C::NT) void lce_product_kernel(ProductArgs a) {
         pg::store_partials<C>(a.w.part, slot, acc);
         return;
     }
-#pragma unroll
-    for (int i = 0; i < C::FA; i++) product_row<C>(a, M, m0, n0, i, acc[i]);
+    product_rows<C, C::FA>(a, M, m0, n0, 0, acc);
 }
 
 template <class C>
 __global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) {
     int nk, m0, n0;
-    const int M = product_rows(a, nk, C::BK);
+    const int M = product_size(a, nk, C::BK);
     product_tile<C>(a, a.w.whole + blockIdx.x, m0, n0);
     if (m0 >= M) return;
-    floatx4 v[C::FB];
-    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, v);
-    product_row<C>(a, M, m0, n0, blockIdx.y, v);
+    floatx4 v[1][C::FB];
+    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, v[0]);
+    product_rows<C, 1>(a, M, m0, n0, blockIdx.y, v);
 }
 
 // ── host ───────────────────────────────────────────────────────────────────────
@@ -729,7 +785,7 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
 
     hipLaunchKernelGGL(lce_index_kernel, dim3(1), dim3(1024), 0, s, d.labels, d.N, d.V, rowmap, pos, lab, sc);
     if (!d.f16)
-        hipLaunchKernelGGL(lce_absmax_kernel, dim3(std::min<int64_t>((int64_t)d.N + d.V, 2048)), dim3(256), 0, s, (const float *)d.X, d.ldx, d.N,
+        hipLaunchKernelGGL(lce_absmax_kernel, dim3((unsigned)std::min<int64_t>(((int64_t)d.N + d.V) * ceil_div(d.D, 2048) / 4 + 1, 1024)), dim3(256), 0, s, (const float *)d.X, d.ldx, d.N,
                            (const float *)d.W, d.ldw, d.V, d.D, pos, sc);
     const dim3 pgrid((unsigned)(d.N + 64 + (l.pack_w ? d.V : 0)));
     const int Np = (d.N + 63) & ~63;

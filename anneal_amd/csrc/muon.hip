@@ -162,35 +162,43 @@ __device__ __forceinline__ void ns_tile(const NsArgs &p, int tile, long &z, int 
     n0 = tc * C::BN;
 }
 
-// What follows a product, for accumulator row i.
+// The planes that row m's epilogue adds, summed.
+template <class C>
+__device__ __forceinline__ void ns_load(const NsArgs &p, long z, int m, int n0, floatx4 (&q)[C::FB]) {
+    const half_t *base = p.Q + z * p.sQ;
+#pragma unroll
+    for (int j = 0; j < C::FB; j++) {
+        const int n = n0 + 16 * j;
+        if (m >= p.M || n >= p.N) continue;
+        const half_t *s = base + pg::panel_at<2>(p.rows, m, n);
+        const h4 hi = *(const h4 *)s, lo = *(const h4 *)(s + 32);
+#pragma unroll
+        for (int r = 0; r < 4; r++) q[j][r] = (float)hi[r] + (float)lo[r];
+    }
+}
+
+// What follows a product, for row m of it.
 template <class C, int WHAT>
-__device__ __forceinline__ void ns_row(const NsArgs &p, const Muon &d, long z, int m0, int n0, int i, const floatx4 (&acc)[C::FB]) {
+__device__ __forceinline__ void ns_row(const NsArgs &p, const Muon &d, long z, int m, int n0, bool mirror, const floatx4 (&acc)[C::FB],
+                                       const floatx4 (&q)[C::FB]) {
     constexpr bool SYM = WHAT == NS_GRAM || WHAT == NS_POLY;
-    const pg::Place<C> at(m0, n0);
-    const int m = at.m + 16 * i;
     if (m >= p.M) return;
     const float ca = d.a, cb = d.b, cc = d.c, keep = 1.0f - d.lr * d.decay, step = d.lr * d.scale;
 #pragma unroll
     for (int j = 0; j < C::FB; j++) {
-        const int n = at.n + 16 * j;
+        const int n = n0 + 16 * j;
         if (n >= p.N) continue;
-        floatx4 v = acc[j], q = {};
-        if constexpr (WHAT != NS_GRAM) {
-            const half_t *s = p.Q + z * p.sQ + pg::panel_at<2>(p.rows, m, n);
-            const h4 hi = *(const h4 *)s, lo = *(const h4 *)(s + 32);
-#pragma unroll
-            for (int r = 0; r < 4; r++) q[r] = (float)hi[r] + (float)lo[r];
-        }
+        floatx4 v = acc[j];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             if constexpr (WHAT == NS_GRAM) v[r] *= 1.0f / (1 << (2 * kSX - kSA));
-            else if constexpr (WHAT == NS_POLY) v[r] = cc * (v[r] * (1.0f / (1 << (2 * kSA - kSB)))) + cb * (q[r] * (1.0f / (1 << (kSA - kSB))));
-            else v[r] = ca * q[r] + v[r] * (1.0f / (1 << kSB));
+            else if constexpr (WHAT == NS_POLY) v[r] = cc * (v[r] * (1.0f / (1 << (2 * kSA - kSB)))) + cb * (q[j][r] * (1.0f / (1 << (kSA - kSB))));
+            else v[r] = ca * q[j][r] + v[r] * (1.0f / (1 << kSB));
         }
         if constexpr (WHAT != NS_LAST) {
             half_t *o = p.out + z * p.so;
             pg::plane_store(o + pg::panel_at<2>(p.rows, m, n), v);
-            if (SYM && m0 != n0) {
+            if (SYM && mirror) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const half_t hi = (half_t)v[r];
@@ -219,8 +227,24 @@ __device__ __forceinline__ void ns_row(const NsArgs &p, const Muon &d, long z, i
     }
 }
 
+// NR accumulator rows from row i0; what a row adds is loaded while the one before it is worked on.
+template <class C, int WHAT, int NR>
+__device__ __forceinline__ void ns_rows(const NsArgs &p, const Muon &d, long z, int m0, int n0, int i0, const floatx4 (&acc)[NR][C::FB]) {
+    const pg::Place<C> at(m0, n0);
+    const int m1 = at.m + 16 * i0;
+    floatx4 q[2][C::FB] = {};
+    if constexpr (WHAT != NS_GRAM) ns_load<C>(p, z, m1, at.n, q[0]);
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const pg::Place<C> row(m0, n0);   // fresh addresses for each row
+        if constexpr (WHAT != NS_GRAM)
+            if (i + 1 < NR) ns_load<C>(p, z, m1 + 16 * (i + 1), row.n, q[(i + 1) & 1]);
+        ns_row<C, WHAT>(p, d, z, m1 + 16 * i, row.n, m0 != n0, acc[i], q[i & 1]);
+    }
+}
+
 template <class C, int WHAT>
-__global__ __launch_bounds__(C::NT) void ns_product_kernel(NsArgs p, Muon d) {
+__global__ __launch_bounds__(C::NT, 2) void ns_product_kernel(NsArgs p, Muon d) {
     __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
     int tile, slot, first, count, m0, n0;
     long z;
@@ -235,8 +259,7 @@ __global__ __launch_bounds__(C::NT) void ns_product_kernel(NsArgs p, Muon d) {
         pg::store_partials<C>(p.w.part, slot, acc);
         return;
     }
-#pragma unroll
-    for (int i = 0; i < C::FA; i++) ns_row<C, WHAT>(p, d, z, m0, n0, i, acc[i]);
+    ns_rows<C, WHAT, C::FA>(p, d, z, m0, n0, 0, acc);
 }
 
 template <class C, int WHAT>
@@ -244,9 +267,9 @@ __global__ __launch_bounds__(C::NT) void ns_join_kernel(NsArgs p, Muon d) {
     int m0, n0;
     long z;
     ns_tile<C, WHAT>(p, p.w.whole + blockIdx.x, z, m0, n0);
-    floatx4 v[C::FB];
-    pg::sum_partials<C>(p.w, blockIdx.x, blockIdx.y, v);
-    ns_row<C, WHAT>(p, d, z, m0, n0, blockIdx.y, v);
+    floatx4 v[1][C::FB];
+    pg::sum_partials<C>(p.w, blockIdx.x, blockIdx.y, v[0]);
+    ns_rows<C, WHAT, 1>(p, d, z, m0, n0, blockIdx.y, v);
 }
 
 // ── host ───────────────────────────────────────────────────────────────────────

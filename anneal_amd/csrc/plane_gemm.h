@@ -417,7 +417,7 @@ struct Place {
         wave = threadIdx.x >> 6;
         m = m0 + (wave / C::WVN) * C::WM + (lane & 15);
         n = n0 + (wave % C::WVN) * C::WN + 4 * (lane >> 4);
-        asm volatile("" : "+v"(m), "+v"(n)::"memory");
+        asm volatile("" : "+v"(m), "+v"(n));
     }
 };
 

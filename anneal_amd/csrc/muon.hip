@@ -3,18 +3,26 @@
 //   X = U / (|U|_F + eps);  steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X      (U wide)
 //                                         A = X^T X,                    X <- a X + X B      (U tall)
 //
-// The iteration raises small singular values by a = 3.4 a step, 480-fold in five: what is lost of X to rounding grows as much. So X, A
-// and B are carried as two f16 planes (22 bits, plane_gemm.h) and every product is three f16 products in an f32 accumulator;
-// against 64 bits the result is as far off as 32-bit products leave it (2e-6 to 4e-6), and takes 3/16 of the f32 MFMAs' time.
-// The planes hold 2^12 X, 2^13 A and 2^11 B: with the singular values of X at most 1.2, as the iteration keeps them, entries
-// stay far below f16's largest value, and entries down to 2^-22 of the matrix's norm keep 22 bits less what they are below 2^-14.
+// The iteration raises small singular values by a = 3.4 a step, 480-fold in five: what is lost of X to rounding grows as much. So
+// all matrices are carried as two f16 planes (22 bits, plane_gemm.h) and every product is three f16 products in an f32
+// accumulator; against 64 bits the result is about as far off as 32-bit products leave it, in 3/16 of the f32 MFMAs' time. Each
+// matrix is scaled by a power of two (kSX ..): with the singular values of X at most 1.2, as the iteration keeps them, entries stay
+// far below f16's largest value, and entries down to 2^-22 of the matrix's norm keep 22 bits less what they are below 2^-14.
 //
-// A and B are symmetric: only tiles on and above the diagonal are computed and each is stored twice. a X is added in the last
-// product's epilogue: folded into B as a I it would be rounded with B, and where singular values are small a X is all there is.
-// X, A and B stay padded with zeros to multiples of 64, where no product needs a bound.
+// Several steps in one. A + (a I + B) A (a I + B) = the next step's A: all are polynomials of one symmetric matrix and commute. So a
+// group of g steps can be run on the s x s side (s the short side, l the long one) and applied to X once:
+//   Q = a I + B;  then g - 1 times:  A <- (a I + B) A (a I + B),  B = b A + c A A,  Q <- (a I + B) Q;      X <- Q X
+// All products but X's own are symmetric, half the tiles: a group costs s^2 l + (4 g - 3) s^3 + 2 s^2 l multiply-adds against
+// g (3 s^2 l + s^3) step by step. Every A after a group's first carries the rounding of the one before, a^2-fold, so groups have at
+// most 3 steps (2 where a is over 3.5). Which way is faster goes by the modelled time of the products (plan).
+//
+// A, B, Q are symmetric: only tiles on and above the diagonal are computed and each is stored twice. Multiples of I stay outside
+// the planes (a X is added in the last product's epilogue): folded in they would be rounded with the rest, and where singular
+// values are small they are all there is. Matrices stay padded with zeros to multiples of 64, where no product needs a bound.
 #include "muon.h"
 
 #include <algorithm>
+#include <cmath>
 
 #include "plane_gemm.h"
 
@@ -23,7 +31,7 @@ namespace {
 
 using pg::h4;
 
-constexpr int kSX = 12, kSA = 13, kSB = 11;   // powers of two of the planes
+constexpr int kSX = 12, kSA = 13, kSB = 11, kSBA = 12;   // powers of two of the planes: X, A, B, (a I + B) A
 constexpr int kBlocks = 1024;                 // blocks of an elementwise pass over a matrix, at most
 
 // Four values from column c of a row of `cols`, zeros past its end; vec: rows start at multiples of four elements.
@@ -137,7 +145,8 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(Muon d, const double *pa
 
 // ── the products ───────────────────────────────────────────────────────────────
 
-enum { NS_GRAM = 0, NS_POLY = 1, NS_NEXT = 2, NS_LAST = 3 };
+// NS_SYM: a symmetric matrix, stored on both sides of the diagonal. NS_NEXT: planes. NS_LAST: the caller's output.
+enum { NS_SYM = 0, NS_NEXT = 1, NS_LAST = 2 };
 
 struct NsArgs {
     pg::Operand A, B;
@@ -146,26 +155,27 @@ struct NsArgs {
     int tiles_m, tiles_n;
     int tiles;              // of one matrix
     pg::Work w;
-    const half_t *Q;        // planes added in the epilogue: the Gram matrix (NS_POLY), X (NS_NEXT, NS_LAST)
+    const half_t *P1, *P2;  // planes added in the epilogue, or null
     half_t *out;            // planes
-    long sQ, so;            // halves
-    int rows;               // of Q's and out's panels
+    long sp, so;            // halves from matrix to matrix of P1 and P2, of out
+    int rows;               // of their panels
+    float k0, k1, k2;       // out = k0 (the product) + k1 P1 + k2 P2
 };
 
 template <class C, int WHAT>
 __device__ __forceinline__ void ns_tile(const NsArgs &p, int tile, long &z, int &m0, int &n0) {
     z = tile / p.tiles;
     int tr, tc;
-    if constexpr (WHAT == NS_GRAM || WHAT == NS_POLY) pg::tri_tile(tile - (int)z * p.tiles, p.tiles_m, tr, tc);
+    if constexpr (WHAT == NS_SYM) pg::tri_tile(tile - (int)z * p.tiles, p.tiles_m, tr, tc);
     else pg::grouped_tile(tile - (int)z * p.tiles, p.tiles_m, p.tiles_n, tr, tc);
     m0 = tr * C::BM;
     n0 = tc * C::BN;
 }
 
-// The planes that row m's epilogue adds, summed.
+// q += k P at row m.
 template <class C>
-__device__ __forceinline__ void ns_load(const NsArgs &p, long z, int m, int n0, floatx4 (&q)[C::FB]) {
-    const half_t *base = p.Q + z * p.sQ;
+__device__ __forceinline__ void ns_add(const NsArgs &p, const half_t *P, float k, long z, int m, int n0, floatx4 (&q)[C::FB]) {
+    const half_t *base = P + z * p.sp;
 #pragma unroll
     for (int j = 0; j < C::FB; j++) {
         const int n = n0 + 16 * j;
@@ -173,32 +183,36 @@ __device__ __forceinline__ void ns_load(const NsArgs &p, long z, int m, int n0, 
         const half_t *s = base + pg::panel_at<2>(p.rows, m, n);
         const h4 hi = *(const h4 *)s, lo = *(const h4 *)(s + 32);
 #pragma unroll
-        for (int r = 0; r < 4; r++) q[j][r] = (float)hi[r] + (float)lo[r];
+        for (int r = 0; r < 4; r++) q[j][r] += k * ((float)hi[r] + (float)lo[r]);
     }
+}
+
+// What row m's epilogue adds to k0 times the product.
+template <class C>
+__device__ __forceinline__ void ns_load(const NsArgs &p, long z, int m, int n0, floatx4 (&q)[C::FB]) {
+#pragma unroll
+    for (int j = 0; j < C::FB; j++) q[j] = (floatx4){};
+    if (p.P1) ns_add<C>(p, p.P1, p.k1, z, m, n0, q);
+    if (p.P2) ns_add<C>(p, p.P2, p.k2, z, m, n0, q);
 }
 
 // What follows a product, for row m of it.
 template <class C, int WHAT>
 __device__ __forceinline__ void ns_row(const NsArgs &p, const Muon &d, long z, int m, int n0, bool mirror, const floatx4 (&acc)[C::FB],
                                        const floatx4 (&q)[C::FB]) {
-    constexpr bool SYM = WHAT == NS_GRAM || WHAT == NS_POLY;
     if (m >= p.M) return;
-    const float ca = d.a, cb = d.b, cc = d.c, keep = 1.0f - d.lr * d.decay, step = d.lr * d.scale;
+    const float k0 = p.k0, keep = 1.0f - d.lr * d.decay, step = d.lr * d.scale;
 #pragma unroll
     for (int j = 0; j < C::FB; j++) {
         const int n = n0 + 16 * j;
         if (n >= p.N) continue;
         floatx4 v = acc[j];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            if constexpr (WHAT == NS_GRAM) v[r] *= 1.0f / (1 << (2 * kSX - kSA));
-            else if constexpr (WHAT == NS_POLY) v[r] = cc * (v[r] * (1.0f / (1 << (2 * kSA - kSB)))) + cb * (q[j][r] * (1.0f / (1 << (kSA - kSB))));
-            else v[r] = ca * q[j][r] + v[r] * (1.0f / (1 << kSB));
-        }
+        for (int r = 0; r < 4; r++) v[r] = k0 * v[r] + q[j][r];
         if constexpr (WHAT != NS_LAST) {
             half_t *o = p.out + z * p.so;
             pg::plane_store(o + pg::panel_at<2>(p.rows, m, n), v);
-            if (SYM && mirror) {
+            if (WHAT == NS_SYM && mirror) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const half_t hi = (half_t)v[r];
@@ -232,13 +246,12 @@ template <class C, int WHAT, int NR>
 __device__ __forceinline__ void ns_rows(const NsArgs &p, const Muon &d, long z, int m0, int n0, int i0, const floatx4 (&acc)[NR][C::FB]) {
     const pg::Place<C> at(m0, n0);
     const int m1 = at.m + 16 * i0;
-    floatx4 q[2][C::FB] = {};
-    if constexpr (WHAT != NS_GRAM) ns_load<C>(p, z, m1, at.n, q[0]);
+    floatx4 q[2][C::FB];
+    ns_load<C>(p, z, m1, at.n, q[0]);
 #pragma unroll
     for (int i = 0; i < NR; i++) {
         const pg::Place<C> row(m0, n0);   // fresh addresses for each row
-        if constexpr (WHAT != NS_GRAM)
-            if (i + 1 < NR) ns_load<C>(p, z, m1 + 16 * (i + 1), row.n, q[(i + 1) & 1]);
+        if (i + 1 < NR) ns_load<C>(p, z, m1 + 16 * (i + 1), row.n, q[(i + 1) & 1]);
         ns_row<C, WHAT>(p, d, z, m1 + 16 * i, row.n, m0 != n0, acc[i], q[i & 1]);
     }
 }
@@ -276,28 +289,57 @@ __global__ __launch_bounds__(C::NT) void ns_join_kernel(NsArgs p, Muon d) {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-struct Layout {
-    int Rp, Cp, S;   // padded sides, the short one
-    int parts;
-    int64_t part, X0, X1, A, B, sums, total;
-};
-
-bool symmetric(int what) { return what == NS_GRAM || what == NS_POLY; }
-
 // Tiles of one product over the batch and how they are split, for M x N results summed over k.
-pg::Plan ns_plan(int what, int batch, int M, int N, int k) {
+pg::Plan ns_plan(bool symmetric, int batch, int M, int N, int k) {
     const auto tiles = [&](int w) -> long {
         const long m = ceil_div(M, w), n = ceil_div(N, w);
-        return batch * (symmetric(what) ? m * (m + 1) / 2 : m * n);
+        return batch * (symmetric ? m * (m + 1) / 2 : m * n);
     };
     return pg::plan(tiles(256), tiles(128), k, 2, 2);
+}
+
+constexpr int kMaxGroup = 3;
+
+struct Layout {
+    int Rp, Cp, S, K;   // padded sides; the short one, the long one
+    bool wide;
+    int group;          // steps of a group, at most
+    int parts;
+    pg::Plan gram, square, apply;
+    int64_t part, X0, X1, square_at[6], sums, total;
+};
+
+// Sizes of the groups that `steps` steps are run in: as many as can be of `group`, the larger ones first (a group's own rounding
+// grows with what the steps after it raise), none of one step where two of two do.
+int group_size(int group, int left) {
+    if (group == 3 && left == 4) return 2;
+    return std::min(group, left);
 }
 
 Layout layout(const Muon &d) {
     Layout l{};
     l.Rp = (d.rows + 63) & ~63;
     l.Cp = (d.cols + 63) & ~63;
-    l.S = d.rows <= d.cols ? l.Rp : l.Cp;
+    l.wide = d.rows <= d.cols;
+    l.S = l.wide ? l.Rp : l.Cp;
+    l.K = l.wide ? l.Cp : l.Rp;
+    l.gram = ns_plan(true, d.batch, l.S, l.S, l.K);
+    l.square = ns_plan(true, d.batch, l.S, l.S, l.S);
+    l.apply = ns_plan(false, d.batch, l.Rp, l.Cp, l.S);
+    // |a + b x + c x^2| over what the squared singular values reach bounds a step's growth; the planes of Q hold its cube up to 43
+    double grow = 0;
+    for (int i = 0; i <= 60; i++) {
+        const double x = i * 0.025;
+        grow = std::max(grow, std::fabs(d.a + d.b * x + d.c * x * x));
+    }
+    const int most = grow <= 3.5 ? kMaxGroup : grow <= 5.0 ? 2 : 1;
+    double single = d.steps * (l.gram.us + l.square.us + l.apply.us), grouped = 0;
+    for (int left = d.steps; left > 0;) {
+        const int g = group_size(most, left);
+        grouped += l.gram.us + (4 * g - 3) * l.square.us + l.apply.us;
+        left -= g;
+    }
+    l.group = grouped < single ? most : 1;
     l.parts = (int)std::min<int64_t>(kBlocks, ((int64_t)d.rows * ceil_div(d.cols, kSegment) + 3) / 4);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -309,11 +351,8 @@ Layout layout(const Muon &d) {
     l.part = take((int64_t)d.batch * l.parts * 8);
     l.X0 = take((int64_t)d.batch * l.Rp * l.Cp * 4);
     l.X1 = take((int64_t)d.batch * l.Rp * l.Cp * 4);
-    l.A = take((int64_t)d.batch * l.S * l.S * 4);
-    l.B = take((int64_t)d.batch * l.S * l.S * 4);
-    const int K = d.rows <= d.cols ? l.Cp : l.Rp;
-    l.sums = take(std::max({ns_plan(NS_GRAM, d.batch, l.S, l.S, K).part_bytes(), ns_plan(NS_POLY, d.batch, l.S, l.S, l.S).part_bytes(),
-                            ns_plan(NS_NEXT, d.batch, l.Rp, l.Cp, l.S).part_bytes()}));
+    for (int i = 0; i < (l.group > 1 ? 6 : 2); i++) l.square_at[i] = take((int64_t)d.batch * l.S * l.S * 4);
+    l.sums = take(std::max({l.gram.part_bytes(), l.square.part_bytes(), l.apply.part_bytes()}));
     l.total = (at + 255) & ~255ll;
     return l;
 }
@@ -322,19 +361,24 @@ template <class C, int WHAT>
 void launch(NsArgs p, const Muon &d, hipStream_t s) {
     p.tiles_m = ceil_div(p.M, C::BM);
     p.tiles_n = ceil_div(p.N, C::BN);
-    p.tiles = symmetric(WHAT) ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+    p.tiles = WHAT == NS_SYM ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
     hipLaunchKernelGGL((ns_product_kernel<C, WHAT>), dim3((unsigned)p.w.blocks()), dim3(C::NT), 0, s, p, d);
     if (p.w.splits > 1) hipLaunchKernelGGL((ns_join_kernel<C, WHAT>), dim3((unsigned)p.w.rest, C::FA), dim3(C::NT), 0, s, p, d);
 }
 
 template <int TA, int TB, int WHAT>
-void product(NsArgs p, const Muon &d, float *part, hipStream_t s) {
-    const pg::Plan plan = ns_plan(WHAT, d.batch, p.M, p.N, p.nk * 32);
+void product(NsArgs p, const pg::Plan &plan, const Muon &d, float *sums, hipStream_t s) {
     p.w = plan.w;
-    p.w.part = part;
+    p.w.part = sums;
     if (plan.big) launch<pg::Tile<256, 256, 4, 2, TA, TB, 2, 2, 2>, WHAT>(p, d, s);
     else launch<pg::Tile<128, 128, 2, 2, TA, TB, 2, 2, 2>, WHAT>(p, d, s);
 }
+
+// A symmetric s x s matrix in planes scaled by 2^e.
+struct Square {
+    half_t *p;
+    int e;
+};
 
 }  // namespace
 
@@ -352,57 +396,85 @@ hipError_t muon(const Muon &in, void *wsp, hipStream_t s) {
     char *ws = (char *)wsp;
     double *part = (double *)(ws + l.part);
     float *sums = (float *)(ws + l.sums);
-    half_t *X = (half_t *)(ws + l.X0), *Xn = (half_t *)(ws + l.X1), *A = (half_t *)(ws + l.A), *B = (half_t *)(ws + l.B);
-    const bool wide = d.rows <= d.cols;
+    half_t *X = (half_t *)(ws + l.X0), *Xn = (half_t *)(ws + l.X1);
     hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)l.parts, (unsigned)d.batch), dim3(256), 0, s, d, part);
     hipLaunchKernelGGL(muon_pack_kernel, dim3((unsigned)std::min<int64_t>(kBlocks, (int64_t)l.Rp / 4 * ceil_div(l.Cp, kSegment)), (unsigned)d.batch),
                        dim3(256), 0, s, d, part, l.parts, X, l.Rp, l.Cp);
+
     const long sx = (long)l.Rp * l.Cp * 4, ss = (long)l.S * l.S * 4;
-    for (int k = 0; k < d.steps; k++) {
-        NsArgs g{};   // A = X X^T or X^T X
-        g.M = g.N = l.S;
-        g.out = A;
-        g.so = ss / 2;
-        g.rows = l.S;
-        g.sA = g.sB = sx;
-        g.A = g.B = pg::panels(X, l.Rp, l.S, wide ? l.Cp : l.Rp);
-        g.nk = (wide ? l.Cp : l.Rp) / 32;
-        if (wide) product<0, 0, NS_GRAM>(g, d, sums, s);
-        else product<1, 1, NS_GRAM>(g, d, sums, s);
-
-        NsArgs q = g;   // B = b A + c A A
-        q.Q = A;
-        q.sQ = ss / 2;
-        q.out = B;
-        q.sA = q.sB = ss;
-        q.A = q.B = pg::panels(A, l.S, l.S, l.S);
+    const auto buf = [&](int i) { return (half_t *)(ws + l.square_at[i]); };
+    const auto square = [&](const half_t *p) { return pg::panels(p, l.S, l.S, l.S); };
+    // out = k (left right) + k1 p1 + k2 p2, matrices without their planes' scales
+    const auto symmetric = [&](Square out, Square left, Square right, double k, double k1, Square p1, double k2, Square p2) {
+        NsArgs q{};
+        q.M = q.N = l.S;
         q.nk = l.S / 32;
-        product<0, 0, NS_POLY>(q, d, sums, s);
+        q.A = square(left.p);
+        q.B = square(right.p);
+        q.sA = q.sB = ss;
+        q.out = out.p;
+        q.so = q.sp = ss / 2;
+        q.rows = l.S;
+        q.k0 = (float)std::ldexp(k, out.e - left.e - right.e);
+        q.P1 = p1.p;
+        q.k1 = (float)std::ldexp(k1, out.e - p1.e);
+        q.P2 = p2.p;
+        q.k2 = (float)std::ldexp(k2, out.e - p2.e);
+        product<0, 0, NS_SYM>(q, l.square, d, sums, s);
+    };
+    const Square none{nullptr, 0};
+    for (int left = d.steps; left > 0;) {
+        const int g = group_size(l.group, left);
+        left -= g;
+        Square A{buf(0), kSA}, B{buf(1), kSB};
+        NsArgs q{};   // A = X X^T or X^T X
+        q.M = q.N = l.S;
+        q.nk = l.K / 32;
+        q.A = q.B = pg::panels(X, l.Rp, l.S, l.K);
+        q.sA = q.sB = sx;
+        q.out = A.p;
+        q.so = ss / 2;
+        q.rows = l.S;
+        q.k0 = 1.0f / (1 << (2 * kSX - kSA));
+        if (l.wide) product<0, 0, NS_SYM>(q, l.gram, d, sums, s);
+        else product<1, 1, NS_SYM>(q, l.gram, d, sums, s);
 
-        NsArgs n{};   // a X + B X or a X + X B (B is symmetric: its rows serve as columns)
-        n.Q = X;
-        n.sQ = sx / 2;
+        symmetric(B, A, A, d.c, d.b, A, 0, none);   // B = b A + c A A
+        Square Q = B;                               // the group's polynomial is qi I + Q
+        double qi = d.a;
+        for (int i = 1; i < g; i++) {
+            const Square BA{buf(2), kSBA}, Bn{buf(i == 1 ? 3 : 1), kSB}, Qn{buf(3 + i), i == 1 ? 11 : 9};
+            symmetric(BA, B, A, 1, d.a, A, 0, none);       // (a I + B) A
+            symmetric(A, BA, B, 1, d.a, BA, 0, none);      // (a I + B) A (a I + B)
+            symmetric(Bn, A, A, d.c, d.b, A, 0, none);
+            symmetric(Qn, Bn, Q, 1, d.a, Q, qi, Bn);       // (a I + B) (qi I + Q) - a qi I
+            B = Bn;
+            Q = Qn;
+            qi *= d.a;
+        }
+        NsArgs n{};   // X <- qi X + Q X or qi X + X Q (Q is symmetric: its rows serve as columns)
         n.M = l.Rp;
         n.N = l.Cp;
+        n.nk = l.S / 32;
         n.out = Xn;
-        n.so = sx / 2;
+        n.so = n.sp = sx / 2;
         n.rows = l.Rp;
-        const pg::Operand b = pg::panels(B, l.S, l.S, l.S);
-        if (wide) {
-            n.A = b;
+        n.P1 = X;
+        n.k1 = (float)qi;
+        n.k0 = (float)std::ldexp(1.0, -Q.e);
+        if (l.wide) {
+            n.A = square(Q.p);
             n.sA = ss;
             n.B = pg::panels(X, l.Rp, l.Cp, l.Rp);
             n.sB = sx;
+            left ? product<0, 1, NS_NEXT>(n, l.apply, d, sums, s) : product<0, 1, NS_LAST>(n, l.apply, d, sums, s);
         } else {
             n.A = pg::panels(X, l.Rp, l.Rp, l.Cp);
             n.sA = sx;
-            n.B = b;
+            n.B = square(Q.p);
             n.sB = ss;
+            left ? product<0, 0, NS_NEXT>(n, l.apply, d, sums, s) : product<0, 0, NS_LAST>(n, l.apply, d, sums, s);
         }
-        n.nk = l.S / 32;
-        const bool last = k + 1 == d.steps;
-        if (wide) last ? product<0, 1, NS_LAST>(n, d, sums, s) : product<0, 1, NS_NEXT>(n, d, sums, s);
-        else last ? product<0, 0, NS_LAST>(n, d, sums, s) : product<0, 0, NS_NEXT>(n, d, sums, s);
         std::swap(X, Xn);
     }
     return hipGetLastError();

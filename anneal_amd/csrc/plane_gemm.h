@@ -425,6 +425,7 @@ struct Place {
 struct Plan {
     bool big;   // 256 x 256 tiles (8 waves, one workgroup a CU), else 128 x 128 (4 waves, two a CU)
     Work w;
+    double us;
     long part_bytes() const { return w.splits > 1 ? (long)w.rest * w.splits * (big ? 65536 : 16384) * 4 : 0; }
 };
 
@@ -452,7 +453,7 @@ inline Plan plan(long tiles256, long tiles128, long k, int pa, int pb) {
             const double us = rounds * (nk * stage(slots) + fixed) + (rest ? (double)((nk + s - 1) / s) * stage(rest * s) + fixed : 0) +
                               (s > 1 ? 4.0 + joined : 0);
             if (us < best_us) {
-                best_us = us;
+                best_us = best.us = us;
                 best.big = big != 0;
                 best.w = s == 1 ? Work{(int)tiles, 0, 1, nullptr} : Work{(int)(rounds * slots), (int)rest, s, nullptr};
             }

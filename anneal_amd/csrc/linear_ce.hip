@@ -245,7 +245,8 @@ __device__ __forceinline__ void logits_rows(const LogitArgs &a, int M, int m0, i
         }
     // this lane's first column in E; 16 j columns on are (j & pm) further in the panel and j / (pm + 1) panels on
     constexpr int LOG = KEEP == KEEP_EXP ? 6 : 5, PM = (1 << (LOG - 4)) - 1, SZ = KEEP == KEEP_EXP ? 2 : 4;
-    char *const tile = KEEP == KEEP_NONE ? nullptr : a.E + (long)((n0 + (at.wave % C::WVN) * C::WN) >> LOG) * a.rows * 128 + (long)m0 * 128;
+    const int nw = n0 + (at.wave % C::WVN) * C::WN;
+    char *const tile = KEEP == KEEP_NONE ? nullptr : a.E + ((long)(nw >> LOG) * a.rows + m0) * 128 + (nw & ((1 << LOG) - 1)) * SZ;
     const uint32_t panel = (uint32_t)a.rows * 128;
 #pragma unroll
     for (int i = 0; i < NR; i++) {
@@ -616,7 +617,7 @@ __global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) 
 
 constexpr int64_t kPieceBytes = 2048ll << 20;   // of kept exponentials or logits
 constexpr int kMaxPieceRows = 1 << 20;          // a panel's offsets stay within 32 bits
-constexpr int kStatCols = 64;                  // the narrowest wave tile: bounds the statistics' columns
+constexpr int kStatCols = 32;                  // the narrowest wave tile: bounds the statistics' columns
 
 struct Layout {
     int Dp, Vp, P, KE;         // padded widths; planes of X and W; bytes of a kept logit (and of the P that takes its place)
@@ -628,12 +629,13 @@ struct Layout {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-pg::Plan plan_of(int64_t M, int64_t N, int64_t k, int pa, int pb) {
-    return pg::plan((long)ceil_div(M, 256) * ceil_div(N, 256), (long)ceil_div(M, 128) * ceil_div(N, 128), k, pa, pb);
+pg::Plan plan_of(int64_t M, int64_t N, int64_t k, int pa, int pb, bool narrow) {
+    return pg::plan([&](int w) { return (long)ceil_div(M, w) * ceil_div(N, w); }, k, pa, pb, narrow);
 }
-pg::Plan logits_plan(const Layout &l, int V, int rows) { return plan_of(rows, V, l.Dp, l.P, l.P); }
-pg::Plan dx_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(rows, d.D, d.V, l.PP, l.P); }
-pg::Plan dw_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(d.V, d.D, rows, l.PP, l.P); }
+pg::Plan logits_plan(const Layout &l, int V, int rows) { return plan_of(rows, V, l.Dp, l.P, l.P, true); }
+// (64-wide tiles of one plane have no layout for operands along k)
+pg::Plan dx_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(rows, d.D, d.V, l.PP, l.P, l.P == 2); }
+pg::Plan dw_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(d.V, d.D, rows, l.PP, l.P, l.P == 2); }
 
 Layout layout(const LinearCe &d) {
     Layout l{};
@@ -685,11 +687,6 @@ Layout layout(const LinearCe &d) {
     return l;
 }
 
-template <int PA, int PB, int TA, int TB>
-using T256 = pg::Tile<256, 256, 4, 2, TA, TB, PA, PB, 2>;
-template <int PA, int PB, int TA, int TB>
-using T128 = pg::Tile<128, 128, 2, 2, TA, TB, PA, PB, 2>;
-
 template <class C, int KEEP>
 void launch_logits(LogitArgs a, hipStream_t s) {
     a.tiles_m = ceil_div(a.rows, C::BM);
@@ -697,13 +694,11 @@ void launch_logits(LogitArgs a, hipStream_t s) {
     if (a.w.splits > 1) hipLaunchKernelGGL((lce_logits_join_kernel<C, KEEP>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
 }
 
-template <int P>
-void logits(const LogitArgs &a, bool big, int keep, hipStream_t s) {
-    using B = T256<P, P, 0, 0>;
-    using S = T128<P, P, 0, 0>;
-    if (keep == KEEP_NONE) big ? launch_logits<B, KEEP_NONE>(a, s) : launch_logits<S, KEEP_NONE>(a, s);
-    else if (keep == KEEP_Z) big ? launch_logits<B, KEEP_Z>(a, s) : launch_logits<S, KEEP_Z>(a, s);
-    else if constexpr (P == 1) big ? launch_logits<B, KEEP_EXP>(a, s) : launch_logits<S, KEEP_EXP>(a, s);
+template <class C>
+void logits(const LogitArgs &a, int keep, hipStream_t s) {
+    if (keep == KEEP_NONE) launch_logits<C, KEEP_NONE>(a, s);
+    else if (keep == KEEP_Z) launch_logits<C, KEEP_Z>(a, s);
+    else if constexpr (C::PA == 1) launch_logits<C, KEEP_EXP>(a, s);
 }
 
 template <class C>
@@ -712,6 +707,13 @@ void launch_product(ProductArgs a, hipStream_t s) {
     a.tiles_n = ceil_div(a.N, C::BN);
     hipLaunchKernelGGL((lce_product_kernel<C>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a);
     if (a.w.splits > 1) hipLaunchKernelGGL((lce_product_join_kernel<C>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
+}
+
+template <int TA, int TB, int PA, int PB>
+void launch_product(const ProductArgs &a, int width, hipStream_t s) {
+    if (width == 256) launch_product<pg::Tile256<TA, TB, PA, PB>>(a, s);
+    else if (width == 128) launch_product<pg::Tile128<TA, TB, PA, PB>>(a, s);
+    else if constexpr (PB == 2) launch_product<pg::Tile64<TA, TB, PA, PB>>(a, s);
 }
 
 template <int PP, int PO>
@@ -735,8 +737,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
         b.C = d.dX;
         b.ldc = d.lddx;
         b.vec = d.lddx % 4 == 0 && ((uintptr_t)d.dX & (d.g16 ? 7 : 15)) == 0;
-        if (plan.big) launch_product<T256<PP, PO, 0, 1>>(b, s);
-        else launch_product<T128<PP, PO, 0, 1>>(b, s);
+        launch_product<0, 1, PP, PO>(b, plan.width, s);
     }
     if (d.dW) {
         ProductArgs b = a;
@@ -765,8 +766,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
                 b.acc_out = piece + 1 < l.pieces ? acc : nullptr;
             }
         }
-        if (plan.big) launch_product<T256<PP, PO, 1, 1>>(b, s);
-        else launch_product<T128<PP, PO, 1, 1>>(b, s);
+        launch_product<1, 1, PP, PO>(b, plan.width, s);
     }
 }
 
@@ -813,15 +813,22 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         a.lab = lab + row0;
         a.zt = zt + row0;
         a.stats = stats;
-        a.T = 2 * ceil_div(d.V, plan.big ? 256 : 128);   // two waves side by side in either tile
+        a.T = 2 * ceil_div(d.V, plan.width);   // two waves side by side in every tile
         a.E = ws + l.E;
         a.Vp = l.Vp;
-        if (l.P == 1) logits<1>(a, plan.big, l.keep, s);
-        else logits<2>(a, plan.big, l.keep, s);
+        if (l.P == 1) {
+            if (plan.width == 256) logits<pg::Tile256<0, 0, 1, 1>>(a, l.keep, s);
+            else if (plan.width == 128) logits<pg::Tile128<0, 0, 1, 1>>(a, l.keep, s);
+            else logits<pg::Tile64<0, 0, 1, 1>>(a, l.keep, s);
+        } else {
+            if (plan.width == 256) logits<pg::Tile256<0, 0, 2, 2>>(a, l.keep, s);
+            else if (plan.width == 128) logits<pg::Tile128<0, 0, 2, 2>>(a, l.keep, s);
+            else logits<pg::Tile64<0, 0, 2, 2>>(a, l.keep, s);
+        }
         hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, sc, row0, rows, stats, a.T, zt + row0, rowmap + row0,
                            lse + row0, loss + row0, d.rowloss, d.lse);
         if (!l.grad) continue;
-        const GradArgs g{sc, row0, rows, d.V, l.Vp, a.T, plan.big ? 128 : 64, stats, lse + row0, zt + row0, lab + row0, ws + l.E, ws + l.Pp,
+        const GradArgs g{sc, row0, rows, d.V, l.Vp, a.T, plan.width / 2, stats, lse + row0, zt + row0, lab + row0, ws + l.E, ws + l.Pp,
                          d.dbias ? (float *)(ws + l.dbpart) : nullptr};
         const dim3 ggrid((unsigned)ceil_div(l.Vp, 64 * (l.keep == KEEP_EXP ? 8 : 4)), (unsigned)ceil_div(rows, kGradRows));
         if (l.keep == KEEP_EXP) hipLaunchKernelGGL((lce_grad_kernel<KEEP_EXP, 1>), ggrid, dim3(256), 0, s, g);

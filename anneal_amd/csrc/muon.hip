@@ -295,7 +295,7 @@ pg::Plan ns_plan(bool symmetric, int batch, int M, int N, int k) {
         const long m = ceil_div(M, w), n = ceil_div(N, w);
         return batch * (symmetric ? m * (m + 1) / 2 : m * n);
     };
-    return pg::plan(tiles(256), tiles(128), k, 2, 2);
+    return pg::plan(tiles, k, 2, 2, true);
 }
 
 constexpr int kMaxGroup = 3;
@@ -370,8 +370,9 @@ template <int TA, int TB, int WHAT>
 void product(NsArgs p, const pg::Plan &plan, const Muon &d, float *sums, hipStream_t s) {
     p.w = plan.w;
     p.w.part = sums;
-    if (plan.big) launch<pg::Tile<256, 256, 4, 2, TA, TB, 2, 2, 2>, WHAT>(p, d, s);
-    else launch<pg::Tile<128, 128, 2, 2, TA, TB, 2, 2, 2>, WHAT>(p, d, s);
+    if (plan.width == 256) launch<pg::Tile256<TA, TB, 2, 2>, WHAT>(p, d, s);
+    else if (plan.width == 128) launch<pg::Tile128<TA, TB, 2, 2>, WHAT>(p, d, s);
+    else launch<pg::Tile64<TA, TB, 2, 2>, WHAT>(p, d, s);
 }
 
 // A symmetric s x s matrix in planes scaled by 2^e.

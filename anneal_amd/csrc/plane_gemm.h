@@ -423,39 +423,52 @@ struct Place {
 
 // Tile width and splits of a product, by a model of the time it takes.
 struct Plan {
-    bool big;   // 256 x 256 tiles (8 waves, one workgroup a CU), else 128 x 128 (4 waves, two a CU)
+    int width;   // of the tiles: 256 (8 waves, one workgroup a CU), 128 (4 waves, two a CU) or 64 (4 waves, two a CU, four stages)
     Work w;
     double us;
-    long part_bytes() const { return w.splits > 1 ? (long)w.rest * w.splits * (big ? 65536 : 16384) * 4 : 0; }
+    long part_bytes() const { return w.splits > 1 ? (long)w.rest * w.splits * width * width * 4 : 0; }
 };
+template <int TA, int TB, int PA, int PB>
+using Tile256 = Tile<256, 256, 4, 2, TA, TB, PA, PB, 2>;
+template <int TA, int TB, int PA, int PB>
+using Tile128 = Tile<128, 128, 2, 2, TA, TB, PA, PB, 2>;
+template <int TA, int TB, int PA, int PB>
+using Tile64 = Tile<64, 64, 2, 2, TA, TB, PA, PB, 4>;
 
-// tiles256, tiles128: tiles at either width; k: the summed length; pa, pb: planes. Microseconds a stage of the tile loops on this
-// chip, measured over k = 4096 with operands in panels (a stage is 64 k of one plane, 32 of two):
-//                    256 x 256: 32 / 256 workgroups    128 x 128: up to 256 / 512
-//   planes 1 x 1               1.28 / 1.77                    0.75 / 1.15
-//   planes 2 x 1               1.23 / 1.58                    0.64 / 0.97
-//   planes 2 x 2               1.62 / 2.30                    0.74 / 1.33
-// (many CUs at once run slower than few: the clock gives way). Splitting adds a launch and the partial sums' way to memory and back.
-inline Plan plan(long tiles256, long tiles128, long k, int pa, int pb) {
+// tiles(width): number of tiles at a width; k: the summed length; pa, pb: planes; narrow: 64-wide tiles may be taken. Microseconds
+// a stage of the tile loops on this chip, measured over k = 1024 to 4096 with operands in panels (a stage is 64 k of one plane, 32
+// of two), by workgroups:
+//                  256 wide: 32 / 256      128 wide: to 256 / 512      64 wide: to 256 / 512
+//   planes 1 x 1      1.28 / 1.77             0.72 / 1.15                 0.22 / 0.36
+//   planes 2 x 1      1.23 / 1.58             0.61 / 0.97                   -
+//   planes 2 x 2      1.62 / 2.30             0.68 / 1.33                 0.26 / 0.41
+// (many CUs at once run slower than few: the clock gives way). Splitting adds a launch and the partial sums' way to memory and
+// back. 1024 x 1024 over k = 1024 in two planes, measured: 15 us in 256 tiles of 64, 24 in 64 of 128.
+template <class Tiles>
+Plan plan(Tiles tiles, long k, int pa, int pb, bool narrow) {
     const int row = pa == 1 ? 0 : pb == 1 ? 1 : 2;
-    constexpr double kFew[3] = {1.25, 1.2, 1.55}, kMore[3] = {0.52, 0.38, 0.75};
-    constexpr double kOne[3] = {0.75, 0.64, 0.74}, kTwo[3] = {1.15, 0.97, 1.33};
+    constexpr double kFew[3] = {1.22, 1.18, 1.53}, kMore[3] = {0.55, 0.40, 0.77};
+    constexpr double k128[3][2] = {{0.72, 1.15}, {0.61, 0.97}, {0.68, 1.33}}, k64[3][2] = {{0.22, 0.36}, {0.30, 0.50}, {0.26, 0.41}};
     const long nk = (k + (row == 0 ? 63 : 31)) / (row == 0 ? 64 : 32);
     Plan best{};
     double best_us = 1e30;
-    for (int big = 0; big < 2; big++) {
-        const long tiles = big ? tiles256 : tiles128, slots = big ? 256 : 512;
-        const auto stage = [&](long wg) { return big ? kFew[row] + kMore[row] * (double)wg / 256 : wg <= 256 ? kOne[row] : kTwo[row]; };
-        const double fixed = big ? 5.0 : 3.5;   // first loads and the epilogue
-        const long rest = tiles % slots, rounds = tiles / slots;
+    for (const int width : {256, 128, 64}) {
+        if (width == 64 && !narrow) break;
+        const long n = tiles(width), slots = width == 256 ? 256 : 512;
+        const auto stage = [&](long wg) {
+            return width == 256 ? kFew[row] + kMore[row] * (double)wg / 256 : width == 128 ? k128[row][wg > 256] : k64[row][wg > 256];
+        };
+        const double fixed = width == 256 ? 7.0 : 5.0;   // launch, first loads, the epilogue
+        const long rest = n % slots, rounds = n / slots;
         for (int s = 1; s <= 32 && (s == 1 || (rest * s <= slots && nk >= 2 * s)); s++) {
-            const double joined = (double)rest * s * (big ? 262144 : 65536) * 2 / 4e6;   // us at 4 TB/s
+            const double joined = (double)rest * s * width * width * 8 / 4e6;   // us at 4 TB/s
             const double us = rounds * (nk * stage(slots) + fixed) + (rest ? (double)((nk + s - 1) / s) * stage(rest * s) + fixed : 0) +
                               (s > 1 ? 4.0 + joined : 0);
             if (us < best_us) {
-                best_us = best.us = us;
-                best.big = big != 0;
-                best.w = s == 1 ? Work{(int)tiles, 0, 1, nullptr} : Work{(int)(rounds * slots), (int)rest, s, nullptr};
+                best_us = us;
+                best.us = us;
+                best.width = width;
+                best.w = s == 1 ? Work{(int)n, 0, 1, nullptr} : Work{(int)(rounds * slots), (int)rest, s, nullptr};
             }
             if (!rest) break;
         }

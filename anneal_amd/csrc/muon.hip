@@ -13,8 +13,9 @@
 // group of g steps can be run on the s x s side (s the short side, l the long one) and applied to X once:
 //   Q = a I + B;  then g - 1 times:  A <- (a I + B) A (a I + B),  B = b A + c A A,  Q <- (a I + B) Q;      X <- Q X
 // All products but X's own are symmetric, half the tiles: a group costs s^2 l + (4 g - 3) s^3 + 2 s^2 l multiply-adds against
-// g (3 s^2 l + s^3) step by step. Every A after a group's first carries the rounding of the one before, a^2-fold, so groups have at
-// most 3 steps (2 where a is over 3.5). Which way is faster goes by the modelled time of the products (plan).
+// g (3 s^2 l + s^3) step by step. Every A after a group's first carries the rounding of the one before, a^2-fold, and Q and qi I
+// cancel where singular values are near 1, so groups have at most 3 steps (muon_dev.h). Which way is faster goes by the modelled
+// time of the products (plan).
 //
 // A, B, Q are symmetric: only tiles on and above the diagonal are computed and each is stored twice. Multiples of I stay outside
 // the planes (a X is added in the last product's epilogue): folded in they would be rounded with the rest, and where singular
@@ -24,62 +25,14 @@
 #include <algorithm>
 #include <cmath>
 
-#include "plane_gemm.h"
+#include "muon_dev.h"
 
 namespace ah {
 namespace {
 
-using pg::h4;
+using namespace ns;
 
-constexpr int kSX = 12, kSA = 13, kSB = 11, kSBA = 12;   // powers of two of the planes: X, A, B, (a I + B) A
-constexpr int kBlocks = 1024;                 // blocks of an elementwise pass over a matrix, at most
-
-// Four values from column c of a row of `cols`, zeros past its end; vec: rows start at multiples of four elements.
-template <class T>
-__device__ __forceinline__ floatx4 load4(const T *row, int c, int cols, bool vec) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    floatx4 v = {};
-    if (vec && c + 3 < cols) {
-        const t4 x = *(const t4 *)(row + c);
-#pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = (float)x[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (c + k < cols) v[k] = (float)row[c + k];
-    }
-    return v;
-}
-
-template <class T>
-__device__ __forceinline__ void store4(T *row, int c, int cols, bool vec, floatx4 v) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    t4 x;
-#pragma unroll
-    for (int k = 0; k < 4; k++) x[k] = (T)v[k];
-    if (vec && c + 3 < cols) *(t4 *)(row + c) = x;
-    else
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (c + k < cols) row[c + k] = x[k];
-}
-
-__device__ __forceinline__ floatx4 load_g(const Muon &d, long z, int r, int c) {
-    const long at = z * d.sg + r * d.ldg;
-    return d.f16 ? load4((const half_t *)d.G + at, c, d.cols, d.vec_g) : load4((const float *)d.G + at, c, d.cols, d.vec_g);
-}
-
-// U from G and the new momentum.
-__device__ __forceinline__ floatx4 update_of(const Muon &d, floatx4 g, floatx4 m) {
-    const float mu = d.momentum;
-    if (!d.nesterov) return m;
-#pragma unroll
-    for (int k = 0; k < 4; k++) g[k] += mu * m[k];
-    return g;
-}
-
-// The elementwise passes give a wave one segment of a row at a time.
-constexpr int kSegment = 1024;
+constexpr int kBlocks = 1024;   // blocks of an elementwise pass over a matrix, at most
 
 // Sums of squares of U per block in f64 (f32 squares of small gradients would vanish); with momentum also M_out.
 __global__ __launch_bounds__(256) void muon_norm_kernel(Muon d, double *part) {
@@ -118,12 +71,7 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(Muon d, const double *pa
     __shared__ double red[4];
     const long z = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (Cp + kSegment - 1) / kSegment;
-    double s = 0.0;
-    for (int i = threadIdx.x; i < parts; i += 256) s += part[z * parts + i];
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (lane == 0) red[wave] = s;
-    __syncthreads();
-    const float inv = (float)((double)(1 << kSX) / (sqrt(red[0] + red[1] + red[2] + red[3]) + (double)d.eps));
+    const float inv = inverse_norm<256>(d, part, parts, z, red);
     half_t *out = X + z * (long)Rp * Cp * 2;
     for (long q = (long)blockIdx.x * 4 + wave; q < (long)Rp * segs; q += (long)gridDim.x * 4) {
         const int r = (int)(q / segs), c0 = (int)(q - (long)r * segs) * kSegment + lane * 4;
@@ -131,14 +79,7 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(Muon d, const double *pa
         for (int i = 0; i < kSegment; i += 256) {
             const int c = c0 + i;
             if (c >= Cp) continue;
-            floatx4 v = {};
-            if (r < d.rows && c < d.cols) {
-                v = load_g(d, z, r, c);
-                if (d.W) v = update_of(d, v, load4(d.M_out + z * d.sw + r * d.ldw, c, d.cols, d.vec_w));
-#pragma unroll
-                for (int k = 0; k < 4; k++) v[k] *= inv;
-            }
-            pg::plane_store(out + pg::panel_at<2>(Rp, r, c), v);
+            pg::plane_store(out + pg::panel_at<2>(Rp, r, c), scaled_update(d, z, r, c, inv));
         }
     }
 }
@@ -201,7 +142,7 @@ template <class C, int WHAT>
 __device__ __forceinline__ void ns_row(const NsArgs &p, const Muon &d, long z, int m, int n0, bool mirror, const floatx4 (&acc)[C::FB],
                                        const floatx4 (&q)[C::FB]) {
     if (m >= p.M) return;
-    const float k0 = p.k0, keep = 1.0f - d.lr * d.decay, step = d.lr * d.scale;
+    const float k0 = p.k0;
 #pragma unroll
     for (int j = 0; j < C::FB; j++) {
         const int n = n0 + 16 * j;
@@ -222,21 +163,9 @@ __device__ __forceinline__ void ns_row(const NsArgs &p, const Muon &d, long z, i
                 }
             }
         } else {
-            if (m >= d.rows || n >= d.cols) continue;
 #pragma unroll
             for (int r = 0; r < 4; r++) v[r] *= 1.0f / (1 << kSX);
-            if (d.W) {
-                const long w0 = z * d.sw + (long)m * d.ldw;
-                const floatx4 w = load4(d.W + w0, n, d.cols, d.vec_w);
-#pragma unroll
-                for (int r = 0; r < 4; r++) v[r] = keep * w[r] - step * v[r];
-                store4(d.W_out + w0, n, d.cols, d.vec_w, v);
-                if (d.W16_out) store4((half_t *)d.W16_out + w0, n, d.cols, d.vec_o, v);
-            } else {
-                const long o0 = z * d.so + (long)m * d.ldo;
-                if (d.out16) store4((half_t *)d.O + o0, n, d.cols, d.vec_o, v);
-                else store4((float *)d.O + o0, n, d.cols, d.vec_o, v);
-            }
+            store_result(d, z, m, n, v);
         }
     }
 }
@@ -298,23 +227,14 @@ pg::Plan ns_plan(bool symmetric, int batch, int M, int N, int k) {
     return pg::plan(tiles, k, 2, 2, true);
 }
 
-constexpr int kMaxGroup = 3;
-
 struct Layout {
     int Rp, Cp, S, K;   // padded sides; the short one, the long one
     bool wide;
     int group;          // steps of a group, at most
     int parts;
     pg::Plan gram, square, apply;
-    int64_t part, X0, X1, square_at[6], sums, total;
+    int64_t part, small, X0, X1, square_at[6], sums, total;
 };
-
-// Sizes of the groups that `steps` steps are run in: as many as can be of `group`, the larger ones first (a group's own rounding
-// grows with what the steps after it raise), none of one step where two of two do.
-int group_size(int group, int left) {
-    if (group == 3 && left == 4) return 2;
-    return std::min(group, left);
-}
 
 Layout layout(const Muon &d) {
     Layout l{};
@@ -326,16 +246,10 @@ Layout layout(const Muon &d) {
     l.gram = ns_plan(true, d.batch, l.S, l.S, l.K);
     l.square = ns_plan(true, d.batch, l.S, l.S, l.S);
     l.apply = ns_plan(false, d.batch, l.Rp, l.Cp, l.S);
-    // |a + b x + c x^2| over what the squared singular values reach bounds a step's growth; the planes of Q hold its cube up to 43
-    double grow = 0;
-    for (int i = 0; i <= 60; i++) {
-        const double x = i * 0.025;
-        grow = std::max(grow, std::fabs(d.a + d.b * x + d.c * x * x));
-    }
-    const int most = grow <= 3.5 ? kMaxGroup : grow <= 5.0 ? 2 : 1;
+    const int most = longest_group(d);
     double single = d.steps * (l.gram.us + l.square.us + l.apply.us), grouped = 0;
-    for (int left = d.steps; left > 0;) {
-        const int g = group_size(most, left);
+    for (int left = d.steps, index = 0; left > 0; index++) {
+        const int g = group_size(most, index, left);
         grouped += l.gram.us + (4 * g - 3) * l.square.us + l.apply.us;
         left -= g;
     }
@@ -349,6 +263,11 @@ Layout layout(const Muon &d) {
         return o;
     };
     l.part = take((int64_t)d.batch * l.parts * 8);
+    if (std::min(d.rows, d.cols) <= kSmallSide) {
+        l.small = take(muon_small_workspace(d));
+        l.total = (at + 255) & ~255ll;
+        return l;
+    }
     l.X0 = take((int64_t)d.batch * l.Rp * l.Cp * 4);
     l.X1 = take((int64_t)d.batch * l.Rp * l.Cp * 4);
     for (int i = 0; i < (l.group > 1 ? 6 : 2); i++) l.square_at[i] = take((int64_t)d.batch * l.S * l.S * 4);
@@ -399,6 +318,10 @@ hipError_t muon(const Muon &in, void *wsp, hipStream_t s) {
     float *sums = (float *)(ws + l.sums);
     half_t *X = (half_t *)(ws + l.X0), *Xn = (half_t *)(ws + l.X1);
     hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)l.parts, (unsigned)d.batch), dim3(256), 0, s, d, part);
+    if (std::min(d.rows, d.cols) <= kSmallSide) {
+        muon_small(d, part, l.parts, ws + l.small, s);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL(muon_pack_kernel, dim3((unsigned)std::min<int64_t>(kBlocks, (int64_t)l.Rp / 4 * ceil_div(l.Cp, kSegment)), (unsigned)d.batch),
                        dim3(256), 0, s, d, part, l.parts, X, l.Rp, l.Cp);
 
@@ -424,8 +347,8 @@ hipError_t muon(const Muon &in, void *wsp, hipStream_t s) {
         product<0, 0, NS_SYM>(q, l.square, d, sums, s);
     };
     const Square none{nullptr, 0};
-    for (int left = d.steps; left > 0;) {
-        const int g = group_size(l.group, left);
+    for (int left = d.steps, index = 0; left > 0; index++) {
+        const int g = group_size(l.group, index, left);
         left -= g;
         Square A{buf(0), kSA}, B{buf(1), kSB};
         NsArgs q{};   // A = X X^T or X^T X

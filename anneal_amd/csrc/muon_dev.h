@@ -1,0 +1,130 @@
+// muon_dev.h — device code shared by the two forms of the orthogonalisation (muon.hip, muon_small.hip).
+#pragma once
+#include <algorithm>
+#include <cmath>
+
+#include "muon.h"
+#include "plane_gemm.h"
+
+namespace ah {
+namespace ns {
+
+using pg::h4;
+
+constexpr int kSX = 12, kSA = 13, kSB = 11, kSBA = 12;   // powers of two of the planes: X, A, B, (a I + B) A
+
+// Four values from column c of a row of `cols`, zeros past its end; vec: rows start at multiples of four elements.
+template <class T>
+__device__ __forceinline__ floatx4 load4(const T *row, int c, int cols, bool vec) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    floatx4 v = {};
+    if (vec && c + 3 < cols) {
+        const t4 x = *(const t4 *)(row + c);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = (float)x[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (c + k < cols) v[k] = (float)row[c + k];
+    }
+    return v;
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T *row, int c, int cols, bool vec, floatx4 v) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 x;
+#pragma unroll
+    for (int k = 0; k < 4; k++) x[k] = (T)v[k];
+    if (vec && c + 3 < cols) *(t4 *)(row + c) = x;
+    else
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (c + k < cols) row[c + k] = x[k];
+}
+
+__device__ __forceinline__ floatx4 load_g(const Muon &d, long z, int r, int c) {
+    const long at = z * d.sg + r * d.ldg;
+    return d.f16 ? load4((const half_t *)d.G + at, c, d.cols, d.vec_g) : load4((const float *)d.G + at, c, d.cols, d.vec_g);
+}
+
+// U from G and the new momentum.
+__device__ __forceinline__ floatx4 update_of(const Muon &d, floatx4 g, floatx4 m) {
+    const float mu = d.momentum;
+    if (!d.nesterov) return m;
+#pragma unroll
+    for (int k = 0; k < 4; k++) g[k] += mu * m[k];
+    return g;
+}
+
+// The elementwise passes give a wave one segment of a row at a time.
+constexpr int kSegment = 1024;
+
+// Four values of the update, at column c of row r of matrix z, times inv; zeros past the matrix.
+__device__ __forceinline__ floatx4 scaled_update(const Muon &d, long z, int r, int c, float inv) {
+    floatx4 v = {};
+    if (r < d.rows && c < d.cols) {
+        v = load_g(d, z, r, c);
+        if (d.W) v = update_of(d, v, load4(d.M_out + z * d.sw + r * d.ldw, c, d.cols, d.vec_w));
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] *= inv;
+    }
+    return v;
+}
+
+// 2^kSX / (|U| + eps) from the blocks' sums of squares; red: NT / 64 doubles of LDS. All NT threads of a workgroup.
+template <int NT>
+__device__ __forceinline__ float inverse_norm(const Muon &d, const double *part, int parts, long z, double *red) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < parts; i += NT) s += part[z * parts + i];
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = red[0];
+    for (int w = 1; w < NT / 64; w++) s += red[w];
+    return (float)((double)(1 << kSX) / (sqrt(s) + (double)d.eps));
+}
+
+// Four values of the last iterate (without the planes' scale) at column c of row r: into O, or into the weights.
+__device__ __forceinline__ void store_result(const Muon &d, long z, int r, int c, floatx4 v) {
+    if (r >= d.rows || c >= d.cols) return;
+    const float keep = 1.0f - d.lr * d.decay, step = d.lr * d.scale;
+    if (d.W) {
+        const long w0 = z * d.sw + (long)r * d.ldw;
+        const floatx4 w = load4(d.W + w0, c, d.cols, d.vec_w);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = keep * w[k] - step * v[k];
+        store4(d.W_out + w0, c, d.cols, d.vec_w, v);
+        if (d.W16_out) store4((half_t *)d.W16_out + w0, c, d.cols, d.vec_o, v);
+    } else {
+        const long o0 = z * d.so + (long)r * d.ldo;
+        if (d.out16) store4((half_t *)d.O + o0, c, d.cols, d.vec_o, v);
+        else store4((float *)d.O + o0, c, d.cols, d.vec_o, v);
+    }
+}
+
+}  // namespace ns
+
+// Steps of the longest group: |a + b x + c x^2| over what the squared singular values reach bounds a step's growth, and the planes
+// of three steps' Q hold its cube up to 43. A short side under 256 starts with larger singular values of X and has less to average
+// over: three steps at once cost it more than 32-bit products lose (16 x 64: 7 times the error of step by step).
+inline int longest_group(const Muon &d) {
+    double grow = 0;
+    for (int i = 0; i <= 60; i++) {
+        const double x = i * 0.025;
+        grow = std::max(grow, std::fabs(d.a + d.b * x + d.c * x * x));
+    }
+    return grow <= 3.5 && std::min(d.rows, d.cols) >= 256 ? 3 : grow <= 5.0 ? 2 : 1;
+}
+// Steps of group `index` with `left` to go: 3, 2, 1, 1, .. or 2, 1, 1, .. Of the ways to cut five steps in 32-bit products these
+// stay nearest to step by step over short sides of 8 to 512 and flat and steep spectra (1.1 to 1.7 times its error at 3, 2 from 256
+// on, 1.0 to 1.3 at 2, 1, 1, 1 below; pairs throughout 1.2 to 2.8, other cuts 4 to 40). Step by step in planes has 0.6 (s = 4096) to
+// 1.5 times (s = 8) the error of 32-bit products.
+inline int group_size(int longest, int index, int left) { return std::min(std::max(1, longest - index), left); }
+
+// The form for a short side of at most kSmallSide (muon_small.hip).
+constexpr int kSmallSide = 128;
+int64_t muon_small_workspace(const Muon &d);
+void muon_small(const Muon &d, const double *part, int parts, void *ws, hipStream_t s);
+
+}  // namespace ah

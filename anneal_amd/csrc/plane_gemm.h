@@ -389,22 +389,19 @@ template <class C>
 __device__ __forceinline__ void sum_partials(const Work &w, int r, int i, floatx4 (&v)[C::FB]) {
 #pragma unroll
     for (int j = 0; j < C::FB; j++) v[j] = (floatx4){};
-    constexpr int B = 32 / C::FB;   // splits whose loads are in flight together
-    int s = 0;
-    for (; s + B <= w.splits; s += B) {
+    constexpr int B = C::FB == 8 ? 4 : 8;   // splits whose loads are in flight together
+    for (int s = 0; s < w.splits; s += B) {
         floatx4 x[B][C::FB];
 #pragma unroll
         for (int b = 0; b < B; b++)
 #pragma unroll
-            for (int j = 0; j < C::FB; j++) x[b][j] = partial<C>(w.part, (long)(s + b) * w.rest + r, i)[j * C::NT];
+            for (int j = 0; j < C::FB; j++)
+                x[b][j] = s + b < w.splits ? partial<C>(w.part, (long)(s + b) * w.rest + r, i)[j * C::NT] : (floatx4){};
 #pragma unroll
         for (int b = 0; b < B; b++)
 #pragma unroll
             for (int j = 0; j < C::FB; j++) v[j] += x[b][j];
     }
-    for (; s < w.splits; s++)
-#pragma unroll
-        for (int j = 0; j < C::FB; j++) v[j] += partial<C>(w.part, (long)s * w.rest + r, i)[j * C::NT];
 }
 
 // A wave's place in a tile: the row of C that this lane holds of accumulator row 0, and its first column.

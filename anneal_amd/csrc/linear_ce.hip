@@ -89,9 +89,8 @@ __global__ __launch_bounds__(1024) void lce_index_kernel(const int *labels, int 
 __global__ __launch_bounds__(256) void lce_absmax_kernel(const float *X, long ldx, int N, const float *W, long ldw, int V, int D, const int *pos,
                                                          Scalars *sc) {
     __shared__ unsigned red[2][4];
-    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(4)));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (D + 2047) / 2048;
-    const bool vx = ldx % 4 == 0 && ((uintptr_t)X & 15) == 0, vw = ldw % 4 == 0 && ((uintptr_t)W & 15) == 0;
     unsigned mx = 0, mw = 0;
     for (long q = (long)blockIdx.x * 4 + wave; q < ((long)N + V) * segs; q += (long)gridDim.x * 4) {
         const long r = q / segs;
@@ -100,19 +99,15 @@ __global__ __launch_bounds__(256) void lce_absmax_kernel(const float *X, long ld
         if (x && pos[r] < 0) continue;
         const uint32_t *p = (const uint32_t *)(x ? X + r * ldx : W + (r - N) * ldw);
         unsigned m = 0;
-        if (x ? vx : vw) {
 #pragma unroll
-            for (int k = 0; k < 2048; k += 256) {
-                const int c = c0 + k;
-                if (c + 3 < end) {
-                    const u4 v = *(const u4 *)(p + c) & 0x7fffffffu;
-                    m = max(m, max(max(v[0], v[1]), max(v[2], v[3])));
-                } else {
-                    for (int u = c; u < end; u++) m = max(m, p[u] & 0x7fffffffu);
-                }
+        for (int k = 0; k < 2048; k += 256) {
+            const int c = c0 + k;
+            if (c + 3 < end) {
+                const u4 v = *(const u4 *)(p + c) & 0x7fffffffu;
+                m = max(m, max(max(v[0], v[1]), max(v[2], v[3])));
+            } else {
+                for (int u = c; u < end; u++) m = max(m, p[u] & 0x7fffffffu);
             }
-        } else {
-            for (int c = c0 - lane * 3; c < end; c += 64) m = max(m, p[c] & 0x7fffffffu);
         }
         if (x) mx = max(mx, m);
         else mw = max(mw, m);
@@ -140,22 +135,16 @@ __device__ __forceinline__ void pack_row(half_t *out, long rows, long r, const v
     const int t = threadIdx.x;
     if constexpr (P == 1) {
         const half_t *p = (const half_t *)in;
-        if (((uintptr_t)p & 15) == 0 && D % 8 == 0) {
-            for (int i = t * 8; i < Dp; i += 256 * 8) *(h8 *)(out + pg::panel_at<1>(rows, r, i)) = i < D ? *(const h8 *)(p + i) : (h8){};
-        } else {
-            for (int i = t; i < Dp; i += 256) out[pg::panel_at<1>(rows, r, i)] = i < D ? p[i] : (half_t)0.0f;
+        for (int i = t * 8; i < Dp; i += 256 * 8) {
+            h8 v = {};
+            if (i + 7 < D) v = *(const pg::h8_any *)(p + i);
+            else
+                for (int k = 0; i + k < D; k++) v[k] = p[i + k];
+            *(h8 *)(out + pg::panel_at<1>(rows, r, i)) = v;
         }
     } else {
-        const float *p = (const float *)in;
-        const bool vec = ((uintptr_t)p & 15) == 0 && D % 4 == 0;
         for (int i = t * 4; i < Dp; i += 256 * 4) {
-            floatx4 v = {};
-            if (vec) {
-                if (i < D) v = *(const floatx4 *)(p + i);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; k++) v[k] = i + k < D ? p[i + k] : 0.0f;
-            }
+            floatx4 v = pg::load4((const float *)in, i, D);
 #pragma unroll
             for (int k = 0; k < 4; k++) v[k] = ldexpf(v[k], e);
             pg::plane_store(out + pg::panel_at<2>(rows, r, i), v);
@@ -501,7 +490,7 @@ struct ProductArgs {
     int mean;
     void *C;
     long ldc;
-    int out16, vec;        // C is f16; rows admit vector stores
+    int out16;             // C is f16
     const float *acc_in;   // dW: the earlier pieces' sum, or null
     float *acc_out;        // dW: the sum goes there in f32 and C is left, or null
     long ldacc;
@@ -513,10 +502,24 @@ __device__ __forceinline__ int product_size(const ProductArgs &a, int &nk, int B
     return a.rows_are == 0 ? rows : a.M;
 }
 
+// The work that is there: the host plans for rows that all count; where fewer do, dX has fewer tiles, and the workgroups that share
+// the K of its tiles are dealt to those.
 template <class C>
-__device__ __forceinline__ void product_tile(const ProductArgs &a, int tile, int &m0, int &n0) {
+__device__ __forceinline__ pg::Work product_work(const ProductArgs &a, int M, int nk, int &tiles_m) {
+    pg::Work w = a.w;
+    tiles_m = a.rows_are == 0 ? (M + C::BM - 1) / C::BM : a.tiles_m;
+    const int tiles = tiles_m * a.tiles_n;
+    if (a.rows_are == 0 && tiles < w.tiles()) {
+        if (w.splits == 1 || tiles > w.rest) w = pg::Work{min(tiles, w.whole), max(0, tiles - w.whole), w.splits, w.part};
+        else w = pg::Work{0, tiles, max(1, min(w.rest * w.splits / max(1, tiles), nk / 2)), w.part};
+    }
+    return w;
+}
+
+template <class C>
+__device__ __forceinline__ void product_tile(const ProductArgs &a, int tile, int tiles_m, int &m0, int &n0) {
     int tr, tc;
-    pg::grouped_tile(tile, a.tiles_m, a.tiles_n, tr, tc);
+    pg::grouped_tile(tile, tiles_m, a.tiles_n, tr, tc);
     m0 = tr * C::BM;
     n0 = tc * C::BN;
 }
@@ -532,42 +535,10 @@ __device__ __forceinline__ void product_row(const ProductArgs &a, int m, long ro
         floatx4 v;
 #pragma unroll
         for (int r = 0; r < 4; r++) v[r] = ldexpf(acc[j][r], e) * mult;
-        const bool vec = a.vec && n + 3 < a.N;
-        const bool vacc = a.ldacc % 4 == 0 && n + 3 < a.N;
-        if (a.acc_in) {
-            const float *p = a.acc_in + (long)m * a.ldacc + n;
-            if (vacc && ((uintptr_t)p & 15) == 0) v += *(const floatx4 *)p;
-            else
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (n + r < a.N) v[r] += p[r];
-        }
-        if (a.acc_out) {
-            float *p = a.acc_out + (long)m * a.ldacc + n;
-            if (vacc) *(floatx4 *)p = v;
-            else
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (n + r < a.N) p[r] = v[r];
-        } else if (a.out16) {
-            half_t *p = (half_t *)a.C + row * a.ldc + n;
-            if (vec) {
-                h4 h;
-#pragma unroll
-                for (int r = 0; r < 4; r++) h[r] = (half_t)v[r];
-                *(h4 *)p = h;
-            } else
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (n + r < a.N) p[r] = (half_t)v[r];
-        } else {
-            float *p = (float *)a.C + row * a.ldc + n;
-            if (vec) *(floatx4 *)p = v;
-            else
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (n + r < a.N) p[r] = v[r];
-        }
+        if (a.acc_in) v += pg::load4(a.acc_in + (long)m * a.ldacc, n, a.N);
+        if (a.acc_out) pg::store4(a.acc_out + (long)m * a.ldacc, n, a.N, v);
+        else if (a.out16) pg::store4((half_t *)a.C + row * a.ldc, n, a.N, v);
+        else pg::store4((float *)a.C + row * a.ldc, n, a.N, v);
     }
 }
 
@@ -588,15 +559,16 @@ __device__ __forceinline__ void product_rows(const ProductArgs &a, int M, int m0
 template <class C>
 __global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
     __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
-    int nk, tile, slot, first, count, m0, n0;
+    int nk, tiles_m, tile, slot, first, count, m0, n0;
     const int M = product_size(a, nk, C::BK);
-    pg::pick(a.w, blockIdx.x, nk, tile, slot, first, count);
-    product_tile<C>(a, tile, m0, n0);
-    if (m0 >= M) return;
+    const pg::Work w = product_work<C>(a, M, nk, tiles_m);
+    if ((int)blockIdx.x >= w.blocks()) return;
+    pg::pick(w, blockIdx.x, nk, tile, slot, first, count);
+    product_tile<C>(a, tile, tiles_m, m0, n0);
     floatx4 acc[C::FA][C::FB];
     pg::contract<C>(a.A, a.B, m0, n0, first, count, smem, acc);
     if (slot >= 0) {
-        pg::store_partials<C>(a.w.part, slot, acc);
+        pg::store_partials<C>(w.part, slot, acc);
         return;
     }
     product_rows<C, C::FA>(a, M, m0, n0, 0, acc);
@@ -604,12 +576,13 @@ __global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
 
 template <class C>
 __global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) {
-    int nk, m0, n0;
+    int nk, tiles_m, m0, n0;
     const int M = product_size(a, nk, C::BK);
-    product_tile<C>(a, a.w.whole + blockIdx.x, m0, n0);
-    if (m0 >= M) return;
+    const pg::Work w = product_work<C>(a, M, nk, tiles_m);
+    if ((int)blockIdx.x >= w.rest || w.splits == 1) return;
+    product_tile<C>(a, w.whole + blockIdx.x, tiles_m, m0, n0);
     floatx4 v[1][C::FB];
-    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, v[0]);
+    pg::sum_partials<C>(w, blockIdx.x, blockIdx.y, v[0]);
     product_rows<C, 1>(a, M, m0, n0, blockIdx.y, v);
 }
 
@@ -736,7 +709,6 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
         b.bmax = PO == 2 ? &sc->wmax : nullptr;
         b.C = d.dX;
         b.ldc = d.lddx;
-        b.vec = d.lddx % 4 == 0 && ((uintptr_t)d.dX & (d.g16 ? 7 : 15)) == 0;
         launch_product<0, 1, PP, PO>(b, plan.width, s);
     }
     if (d.dW) {
@@ -754,7 +726,6 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
         b.bmax = PO == 2 ? &sc->xmax : nullptr;
         b.C = d.dW;
         b.ldc = d.lddw;
-        b.vec = d.lddw % 4 == 0 && ((uintptr_t)d.dW & (d.g16 ? 7 : 15)) == 0;
         if (l.pieces > 1) {
             float *acc = (float *)(ws + l.dwacc);
             if (!d.g16) {   // an f32 dW adds up in place

@@ -26,7 +26,6 @@ struct Muon {
     long ldw, sw;               // of M, W and their outputs
     float lr, momentum, decay, scale;
     int nesterov;
-    int vec_g, vec_w, vec_o;    // set by muon(): rows of G, of M and W, of the last output admit accesses of four elements
 };
 
 int64_t muon_workspace(const Muon &d);

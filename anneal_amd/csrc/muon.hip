@@ -50,10 +50,10 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(Muon d, double *part) {
             floatx4 u = load_g(d, z, r, c);
             if (d.W) {
                 const long at = z * d.sw + r * d.ldw;
-                floatx4 m = load4(d.M + at, c, d.cols, d.vec_w);
+                floatx4 m = load4(d.M + at, c, d.cols);
 #pragma unroll
                 for (int k = 0; k < 4; k++) m[k] = mu * m[k] + u[k];
-                store4(d.M_out + at, c, d.cols, d.vec_w, m);
+                store4(d.M_out + at, c, d.cols, m);
                 u = update_of(d, u, m);
             }
 #pragma unroll
@@ -304,14 +304,7 @@ struct Square {
 
 int64_t muon_workspace(const Muon &d) { return layout(d).total; }
 
-hipError_t muon(const Muon &in, void *wsp, hipStream_t s) {
-    Muon d = in;
-    const auto vec = [&](const void *p, long ld, long stride, int esz) {
-        return !p || (((uintptr_t)p % (4 * esz)) == 0 && ld % 4 == 0 && (d.batch == 1 || stride % 4 == 0));
-    };
-    d.vec_g = vec(d.G, d.ldg, d.sg, d.f16 ? 2 : 4);
-    d.vec_w = vec(d.M, d.ldw, d.sw, 4) && vec(d.M_out, d.ldw, d.sw, 4) && vec(d.W, d.ldw, d.sw, 4) && vec(d.W_out, d.ldw, d.sw, 4);
-    d.vec_o = d.W ? vec(d.W16_out, d.ldw, d.sw, 2) : vec(d.O, d.ldo, d.so, d.out16 ? 2 : 4);
+hipError_t muon(const Muon &d, void *wsp, hipStream_t s) {
     const Layout l = layout(d);
     char *ws = (char *)wsp;
     double *part = (double *)(ws + l.part);

@@ -10,42 +10,14 @@ namespace ah {
 namespace ns {
 
 using pg::h4;
+using pg::load4;
+using pg::store4;
 
 constexpr int kSX = 12, kSA = 13, kSB = 11, kSBA = 12;   // powers of two of the planes: X, A, B, (a I + B) A
 
-// Four values from column c of a row of `cols`, zeros past its end; vec: rows start at multiples of four elements.
-template <class T>
-__device__ __forceinline__ floatx4 load4(const T *row, int c, int cols, bool vec) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    floatx4 v = {};
-    if (vec && c + 3 < cols) {
-        const t4 x = *(const t4 *)(row + c);
-#pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = (float)x[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (c + k < cols) v[k] = (float)row[c + k];
-    }
-    return v;
-}
-
-template <class T>
-__device__ __forceinline__ void store4(T *row, int c, int cols, bool vec, floatx4 v) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    t4 x;
-#pragma unroll
-    for (int k = 0; k < 4; k++) x[k] = (T)v[k];
-    if (vec && c + 3 < cols) *(t4 *)(row + c) = x;
-    else
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (c + k < cols) row[c + k] = x[k];
-}
-
 __device__ __forceinline__ floatx4 load_g(const Muon &d, long z, int r, int c) {
     const long at = z * d.sg + r * d.ldg;
-    return d.f16 ? load4((const half_t *)d.G + at, c, d.cols, d.vec_g) : load4((const float *)d.G + at, c, d.cols, d.vec_g);
+    return d.f16 ? load4((const half_t *)d.G + at, c, d.cols) : load4((const float *)d.G + at, c, d.cols);
 }
 
 // U from G and the new momentum.
@@ -65,7 +37,7 @@ __device__ __forceinline__ floatx4 scaled_update(const Muon &d, long z, int r, i
     floatx4 v = {};
     if (r < d.rows && c < d.cols) {
         v = load_g(d, z, r, c);
-        if (d.W) v = update_of(d, v, load4(d.M_out + z * d.sw + r * d.ldw, c, d.cols, d.vec_w));
+        if (d.W) v = update_of(d, v, load4(d.M_out + z * d.sw + r * d.ldw, c, d.cols));
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] *= inv;
     }
@@ -91,15 +63,15 @@ __device__ __forceinline__ void store_result(const Muon &d, long z, int r, int c
     const float keep = 1.0f - d.lr * d.decay, step = d.lr * d.scale;
     if (d.W) {
         const long w0 = z * d.sw + (long)r * d.ldw;
-        const floatx4 w = load4(d.W + w0, c, d.cols, d.vec_w);
+        const floatx4 w = load4(d.W + w0, c, d.cols);
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = keep * w[k] - step * v[k];
-        store4(d.W_out + w0, c, d.cols, d.vec_w, v);
-        if (d.W16_out) store4((half_t *)d.W16_out + w0, c, d.cols, d.vec_o, v);
+        store4(d.W_out + w0, c, d.cols, v);
+        if (d.W16_out) store4((half_t *)d.W16_out + w0, c, d.cols, v);
     } else {
         const long o0 = z * d.so + (long)r * d.ldo;
-        if (d.out16) store4((half_t *)d.O + o0, c, d.cols, d.vec_o, v);
-        else store4((float *)d.O + o0, c, d.cols, d.vec_o, v);
+        if (d.out16) store4((half_t *)d.O + o0, c, d.cols, v);
+        else store4((float *)d.O + o0, c, d.cols, v);
     }
 }
 

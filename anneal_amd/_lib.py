@@ -64,7 +64,7 @@ class ah_linear_ce_desc(C.Structure):
                 ("mean", C.c_int32), ("X", C.c_void_p), ("ldx", C.c_int64), ("W", C.c_void_p), ("ldw", C.c_int64),
                 ("bias", C.c_void_p), ("labels", C.c_void_p), ("loss", C.c_void_p), ("rowloss", C.c_void_p), ("lse", C.c_void_p),
                 ("dX", C.c_void_p), ("lddx", C.c_int64), ("dW", C.c_void_p), ("lddw", C.c_int64), ("dbias", C.c_void_p),
-                ("grad_scale", C.c_float), ("reserved", C.c_int32), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+                ("grad_scale", C.c_float), ("piece_mb", C.c_int32), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
 
 
 class ah_orthogonalize_desc(C.Structure):

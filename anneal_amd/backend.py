@@ -123,12 +123,12 @@ class Device:
 
     @staticmethod
     def _linear_ce_desc(dtype, N, D, V, X, W, labels, loss, grad_dtype=L.AH_F32, bias=None, rowloss=None, lse=None, dX=None, dW=None,
-                        dbias=None, grad_scale=1.0, mean=True, ldx=None, ldw=None, lddx=None, lddw=None, ws=None, ws_bytes=None):
+                        dbias=None, grad_scale=1.0, mean=True, piece_mb=0, ldx=None, ldw=None, lddx=None, lddw=None, ws=None, ws_bytes=None):
         p = lambda b: None if b is None else b.ptr  # noqa: E731
         ld = lambda v: D if v is None else v        # noqa: E731
         return L.ah_linear_ce_desc(dtype=dtype, grad_dtype=grad_dtype, N=N, D=D, V=V, mean=1 if mean else 0, X=p(X), ldx=ld(ldx), W=p(W),
                                    ldw=ld(ldw), bias=p(bias), labels=p(labels), loss=p(loss), rowloss=p(rowloss), lse=p(lse), dX=p(dX),
-                                   lddx=ld(lddx), dW=p(dW), lddw=ld(lddw), dbias=p(dbias), grad_scale=grad_scale, ws=p(ws),
+                                   lddx=ld(lddx), dW=p(dW), lddw=ld(lddw), dbias=p(dbias), grad_scale=grad_scale, piece_mb=piece_mb, ws=p(ws),
                                    ws_bytes=ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
 
     def linear_ce(self, **kw) -> None:

@@ -18,6 +18,7 @@ struct LinearCe {
     long lddx, lddw;
     float *dbias;               // [V] or null
     float grad_scale;
+    int piece_mb;               // MiB of kept logits, at most (0: 2048)
     int mean;                   // divide loss and gradients by the number of counted rows
 };
 

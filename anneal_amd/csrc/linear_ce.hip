@@ -588,7 +588,7 @@ __global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) 
 
 // ── host ───────────────────────────────────────────────────────────────────────
 
-constexpr int64_t kPieceBytes = 2048ll << 20;   // of kept exponentials or logits
+constexpr int kPieceMb = 2048;   // MiB of kept exponentials or logits: one piece holds 8192 rows of 131072 f16 exponentials
 constexpr int kMaxPieceRows = 1 << 20;          // a panel's offsets stay within 32 bits
 constexpr int kStatCols = 32;                  // the narrowest wave tile: bounds the statistics' columns
 
@@ -623,7 +623,7 @@ Layout layout(const LinearCe &d) {
     l.pack_w = !d.f16 || d.D % 64 || d.ldw % 8 || ((uintptr_t)d.W & 15) || d.ldw > 1 << 22;
     const int64_t Np = ((int64_t)d.N + 63) & ~63ll;
     int64_t rows = Np;
-    if (l.KE) rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, kPieceBytes / ((int64_t)l.Vp * l.KE) / 256 * 256)});
+    if (l.KE) rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, ((int64_t)(d.piece_mb ? d.piece_mb : kPieceMb) << 20) / ((int64_t)l.Vp * l.KE) / 256 * 256)});
     else rows = std::min<int64_t>(rows, 16384);
     l.pieces = (int)((Np + rows - 1) / rows);
     if (l.pieces > 1) rows = ((Np + l.pieces - 1) / l.pieces + 255) / 256 * 256;

@@ -72,7 +72,7 @@ int linear_ce_args(ah_device *dev, const ah_linear_ce_desc *d, LinearCe *o) {
         (d->dX && d->lddx > kMaxStride) || (d->dW && d->lddw > kMaxStride))
         return set_error(AH_ERR_INVALID, "%s: a row stride is less than D=%d or past 2^40", fn, d->D);
     if (!std::isfinite(d->grad_scale)) return set_error(AH_ERR_INVALID, "%s: grad_scale is not finite", fn);
-    if (d->reserved) return set_error(AH_ERR_INVALID, "%s: reserved is not 0", fn);
+    if (d->piece_mb < 0) return set_error(AH_ERR_INVALID, "%s: piece_mb=%d", fn, d->piece_mb);
     const int e = esize(d->dtype), g = esize(d->grad_dtype);
     int rc;
     if ((rc = aligned(fn, "X", d->X, e)) || (rc = aligned(fn, "W", d->W, e)) || (rc = aligned(fn, "bias", d->bias, e)) ||
@@ -89,6 +89,7 @@ int linear_ce_args(ah_device *dev, const ah_linear_ce_desc *d, LinearCe *o) {
     o->dX = d->dX; o->dW = d->dW; o->lddx = d->lddx; o->lddw = d->lddw; o->dbias = d->dbias;
     o->grad_scale = d->grad_scale;
     o->mean = d->mean != 0;
+    o->piece_mb = d->piece_mb;
     return AH_OK;
 }
 

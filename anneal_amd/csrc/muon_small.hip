@@ -98,7 +98,7 @@ enum { FIRST = 0, STEP = 1, LAST = 2 };
 
 // S: the padded short side, 64 or 128. WIDE: the matrix has S rows, else S columns. The waves, S / 32 x S / 32 over every product,
 // hold 32 x 32 of a square each: at S = 128 four on a SIMD, which cover each other's LDS reads and conversions (with one of
-// 64 x 64 a step of 128 x 784 took 20 us instead of %s).
+// 64 x 64 a step of 128 x 784 took 20 us, not 16).
 template <int S, bool WIDE, int WHAT>
 __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(SmallArgs p, Muon d) {
     constexpr int WV = S / 32, NT = WV * WV * 64;

@@ -26,17 +26,27 @@
 //   mse_loss    data0 loss [1], data1 per-wave partials [parts]; loss = f16(sum) * scale.
 //   chain       data0 dX [R,Cc], data1 X [R,Cc], data2 g [Cc]; side data3 dg [Cc], data4 loss [1];
 //               spin=n: polls before a workgroup takes other parts' statistics itself (the result does not depend on it).
+//   linear_ce   data0 dX [N,D], data1 X [N,D], data2 W [V,D], data3 labels i32 [N], with bias=1 data4 bias [V];
+//               then the side outputs dW [V,D], loss f32 [1] and with bias=1 dbias f32 [V]. dtype=f32|f16 (X, W, bias),
+//               grad=f32|f16 (dX, dW); mean=0|1 (1), scale (1) of the gradients, N may be sym. See ah_linear_ce.
+//   orthogonalize  data0 O [rows,cols] (out=f32|f16), data1 G [rows,cols] (dtype=f32|f16); steps (5), a, b, c, eps. See
+//               ah_orthogonalize.
+//   muon        data0 W' f32 [rows,cols], data1 W f32, data2 G (dtype=f32|f16), data3 M f32; side data4 M' f32; lr, mu (0.95),
+//               wd (0), scale (1), nesterov=0|1 (1), steps, a, b, c, eps as above. See ah_muon_step.
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <map>
 
 #include "ah_internal.h"
 #include "conv.h"
 #include "gemm.h"
 #include "itemops.h"
+#include "linear_ce.h"
+#include "muon.h"
 #include "rowops.h"
 
 namespace ah {
@@ -571,6 +581,151 @@ int template_chain(const Params &P, TemplateKernel *t) {
     return AH_OK;
 }
 
+// ── the ends of a language model's step ───────────────────────────────────────────────────────────
+bool is_dtype(const std::string &s) { return s == "f32" || s == "f16"; }
+
+int template_linear_ce(const Params &P, TemplateKernel *t) {
+    Dim N, D, V;
+    GET("N", N, true);
+    GET("D", D, false);
+    GET("V", V, false);
+    const std::string dt = P.str("dtype", "f32"), gt = P.str("grad", "f32"), key = t->key;
+    if (!is_dtype(dt) || !is_dtype(gt) || (dt == "f32" && gt == "f16"))
+        return set_error(AH_ERR_UNSUPPORTED, "tmpl linear_ce: dtype=%s grad=%s", dt.c_str(), gt.c_str());
+    if (D.v < 1 || V.v < 1 || D.v > 1 << 20 || V.v > 1 << 27 || (!N.sym && (N.v < 1 || N.v > 1 << 27)) || D.v * V.v > 1l << 40)
+        return set_error(AH_ERR_INVALID, "tmpl linear_ce: N=%ld D=%ld V=%ld", N.v, D.v, V.v);
+    const bool bias = P.integer("bias", 0) == 1;
+    const int e = dt == "f16" ? 2 : 4, g = gt == "f16" ? 2 : 4, first = bias ? 5 : 4;   // first: PARAM of dW
+    LinearCe c{};
+    c.f16 = e == 2;
+    c.g16 = g == 2;
+    c.D = (int)D.v;
+    c.V = (int)V.v;
+    c.ldx = c.ldw = c.lddx = c.lddw = D.v;
+    c.mean = P.integer("mean", 1) != 0;
+    c.grad_scale = P.real("scale", 1.0f);
+    if (!std::isfinite(c.grad_scale)) return set_error(AH_ERR_INVALID, "tmpl linear_ce: scale is not finite");
+    t->side = {{first, false}, {first + 1, false}};
+    if (bias) t->side.push_back({first + 2, false});
+    t->bytes = [=](int64_t sv) -> std::vector<int64_t> {
+        const int64_t n = N.with(sv);
+        std::vector<int64_t> b = {n * D.v * g, n * D.v * e, V.v * D.v * e, n * 4};
+        if (bias) b.push_back(V.v * e);
+        b.push_back(V.v * D.v * g);
+        b.push_back(4);
+        if (bias) b.push_back(V.v * 4);
+        return b;
+    };
+    // the layout goes by which outputs there are and by W's alignment (device allocations are aligned)
+    const auto with = [=](int64_t n, void *const *p) {
+        LinearCe d = c;
+        static char any[64] __attribute__((aligned(64)));
+        void *const none = any;
+        d.N = (int)n;
+        d.dX = p ? p[0] : none;
+        d.X = p ? p[1] : none;
+        d.W = p ? p[2] : none;
+        d.labels = (const int *)(p ? p[3] : none);
+        d.bias = bias ? (p ? p[4] : none) : nullptr;
+        d.dW = p ? p[first] : none;
+        d.loss = (float *)(p ? p[first + 1] : none);
+        d.dbias = bias ? (float *)(p ? p[first + 2] : none) : nullptr;
+        return d;
+    };
+    t->workspace = [=](int64_t sv) -> int64_t {
+        const int64_t n = N.with(sv);
+        return n >= 1 && n <= 1 << 27 && n * D.v <= 1l << 40 ? linear_ce_workspace(with(n, nullptr)) : 0;
+    };
+    t->run = [=](ah_device *d, TemplateKernel *self, void *const *ptrs, int32_t n_ptrs, const int32_t *sc, int32_t ns) -> int {
+        if (int rc = need(key.c_str(), n_ptrs, first + 2 + bias)) return rc;
+        AT(N, n);
+        if (n < 1 || n > 1 << 27 || n * D.v > 1l << 40) return set_error(AH_ERR_INVALID, "%s: N=%ld", key.c_str(), n);
+        const LinearCe a = with(n, ptrs);
+        if (int rc = ensure_ws(self, linear_ce_workspace(a))) return rc;
+        AH_HIP(linear_ce(a, self->ws, d->stream));
+        return AH_OK;
+    };
+    return AH_OK;
+}
+
+// Size, polynomial and gradient type of a key of either kind.
+int newton_schulz_params(const Params &P, Muon *m) {
+    Dim R, C;
+    GET("rows", R, false);
+    GET("cols", C, false);
+    const std::string dt = P.str("dtype", "f32");
+    if (!is_dtype(dt)) return set_error(AH_ERR_UNSUPPORTED, "tmpl %s: dtype=%s", P.name.c_str(), dt.c_str());
+    const long steps = P.integer("steps", 5);
+    *m = Muon{};
+    m->f16 = dt == "f16";
+    m->a = P.real("a", 3.4445f);
+    m->b = P.real("b", -4.7750f);
+    m->c = P.real("c", 2.0315f);
+    m->eps = P.real("eps", 1e-7f);
+    if (R.v < 1 || C.v < 1 || R.v > 1 << 20 || C.v > 1 << 20 || (R.v + 63) * (C.v + 63) > 1l << 40 || steps < 1 || steps > 64 ||
+        !(fabsf(m->a) + fabsf(m->b) + fabsf(m->c) <= 15.0f) || !(m->eps >= 0.0f) || !std::isfinite(m->eps))
+        return set_error(AH_ERR_INVALID, "tmpl %s: rows=%ld cols=%ld steps=%ld a=%g b=%g c=%g eps=%g", P.name.c_str(), R.v, C.v, steps, m->a, m->b,
+                         m->c, m->eps);
+    m->rows = (int)R.v;
+    m->cols = (int)C.v;
+    m->batch = 1;
+    m->steps = (int)steps;
+    m->ldg = m->ldo = m->ldw = C.v;
+    m->sg = m->so = m->sw = R.v * C.v;
+    return AH_OK;
+}
+
+int template_orthogonalize(const Params &P, TemplateKernel *t) {
+    Muon m;
+    if (int rc = newton_schulz_params(P, &m)) return rc;
+    const std::string ot = P.str("out", "f32"), key = t->key;
+    if (!is_dtype(ot)) return set_error(AH_ERR_UNSUPPORTED, "tmpl orthogonalize: out=%s", ot.c_str());
+    m.out16 = ot == "f16";
+    const int64_t n = (int64_t)m.rows * m.cols;
+    t->bytes = [=](int64_t) -> std::vector<int64_t> { return {n * (m.out16 ? 2 : 4), n * (m.f16 ? 2 : 4)}; };
+    t->workspace = [=](int64_t) { return muon_workspace(m); };
+    t->run = [=](ah_device *d, TemplateKernel *self, void *const *ptrs, int32_t n_ptrs, const int32_t *, int32_t) -> int {
+        if (int rc = need(key.c_str(), n_ptrs, 2)) return rc;
+        if (int rc = ensure_ws(self, muon_workspace(m))) return rc;
+        Muon a = m;
+        a.O = ptrs[0];
+        a.G = ptrs[1];
+        AH_HIP(muon(a, self->ws, d->stream));
+        return AH_OK;
+    };
+    return AH_OK;
+}
+
+int template_muon(const Params &P, TemplateKernel *t) {
+    Muon m;
+    if (int rc = newton_schulz_params(P, &m)) return rc;
+    const std::string key = t->key;
+    m.lr = P.real("lr", 0.0f);
+    m.momentum = P.real("mu", 0.95f);
+    m.decay = P.real("wd", 0.0f);
+    m.scale = P.real("scale", 1.0f);
+    m.nesterov = P.integer("nesterov", 1) != 0;
+    if (!P.has("lr") || !std::isfinite(m.lr) || !std::isfinite(m.momentum) || !std::isfinite(m.decay) || !std::isfinite(m.scale))
+        return set_error(AH_ERR_INVALID, "tmpl muon: lr is required; lr, mu, wd and scale are finite");
+    const int64_t n = (int64_t)m.rows * m.cols;
+    t->side = {{4, false}};
+    t->bytes = [=](int64_t) -> std::vector<int64_t> { return {n * 4, n * 4, n * (m.f16 ? 2 : 4), n * 4, n * 4}; };
+    t->workspace = [=](int64_t) { return muon_workspace(m); };
+    t->run = [=](ah_device *d, TemplateKernel *self, void *const *ptrs, int32_t n_ptrs, const int32_t *, int32_t) -> int {
+        if (int rc = need(key.c_str(), n_ptrs, 5)) return rc;
+        if (int rc = ensure_ws(self, muon_workspace(m))) return rc;
+        Muon a = m;
+        a.W_out = (float *)ptrs[0];
+        a.W = (const float *)ptrs[1];
+        a.G = ptrs[2];
+        a.M = (const float *)ptrs[3];
+        a.M_out = (float *)ptrs[4];
+        AH_HIP(muon(a, self->ws, d->stream));
+        return AH_OK;
+    };
+    return AH_OK;
+}
+
 }  // namespace
 
 TemplateKernel::~TemplateKernel() {
@@ -603,6 +758,9 @@ int template_create(const std::string &source, TemplateKernel **out) {
     else if (P.name == "sgd") rc = template_sgd(P, t);
     else if (P.name == "mse_loss") rc = template_mse_loss(P, t);
     else if (P.name == "chain") rc = template_chain(P, t);
+    else if (P.name == "linear_ce") rc = template_linear_ce(P, t);
+    else if (P.name == "orthogonalize") rc = template_orthogonalize(P, t);
+    else if (P.name == "muon") rc = template_muon(P, t);
     else rc = set_error(AH_ERR_UNSUPPORTED, "unknown template '%s'", P.name.c_str());
     if (rc != AH_OK) {
         delete t;

@@ -328,7 +328,7 @@ int ah_chain_step_noalloc(ah_device *dev, const float *X, const float *g, int32_
  * (dX, dW) AH_F32, or AH_F16 where dtype is AH_F16. loss, rowloss, lse and dbias are f32; losses and statistics are computed in
  * f32 or wider. f32 operands take part in the products with 22 bits of each value (less below 2^-14 of the operand's largest
  * magnitude), and P with 22 bits for f32 gradients and 11 for f16 ones, down to an absolute 2^-40. Gradients of f16 that would
- * underflow take a loss scale as grad_scale. Results repeat bit for bit. Row strides ldx, ldw, lddx, lddw are in elements.
+ * underflow take a loss scale as grad_scale. Results repeat bit for bit (for one piece_mb: more pieces round dW more often). Row strides ldx, ldw, lddx, lddw are in elements.
  * Outputs may not overlap inputs or one another. */
 typedef struct {
     int32_t dtype, grad_dtype;
@@ -349,7 +349,7 @@ typedef struct {
     int64_t lddw;
     float *dbias;
     float grad_scale;
-    int32_t reserved;      /* 0 */
+    int32_t piece_mb;      /* MiB of logits that are kept at a time with gradients; 0: 2048. At least 256 rows are */
     void *ws;
     int64_t ws_bytes;
 } ah_linear_ce_desc;

@@ -29,7 +29,7 @@ LCE_BAD = [(dict(dtype=L.AH_BF16), UNSUPPORTED), (dict(grad_dtype=L.AH_I32), UNS
            (dict(N=0), INVALID), (dict(N=-3), INVALID), (dict(D=0), INVALID), (dict(V=0), INVALID), (dict(D=(1 << 20) + 1), INVALID),
            (dict(X=None), INVALID), (dict(W=None), INVALID), (dict(labels=None), INVALID), (dict(loss=None), INVALID),
            (dict(ldx=7), INVALID), (dict(ldw=-8), INVALID), (dict(lddx=7), INVALID), (dict(lddw=0), INVALID), (dict(ldw=1 << 41), INVALID),
-           (dict(grad_scale=float("nan")), INVALID), (dict(grad_scale=float("inf")), INVALID), (dict(reserved=1), INVALID),
+           (dict(grad_scale=float("nan")), INVALID), (dict(grad_scale=float("inf")), INVALID), (dict(piece_mb=-1), INVALID),
            (dict(X=P + 2), INVALID), (dict(dX=8 * P + 1), INVALID), (dict(labels=4 * P + 2), INVALID)]
 LCE_BAD_CALL = [(dict(ws=None), INVALID), (dict(ws=16 * P + 4), INVALID), (dict(ws_bytes=100), INVALID), (dict(dX=P), INVALID),
                 (dict(dX=P + 64), INVALID), (dict(dW=2 * P), INVALID), (dict(dW=8 * P + 96), INVALID), (dict(rowloss=5 * P), INVALID),

@@ -49,55 +49,76 @@ __device__ __forceinline__ int chunk_rows(const int *count, int row0, int rows) 
 
 // ── rows that count ────────────────────────────────────────────────────────────
 
-// One workgroup: the counted rows in order (rowmap), each row's place among them or -1 (pos), their labels.
-__global__ __launch_bounds__(1024) void lce_index_kernel(const int *labels, int N, int V, int *rowmap, int *pos, int *lab, Scalars *sc) {
-    __shared__ int sums[16];
+constexpr int kMaxBlocks = 1024;  // workgroups that look for the largest magnitudes, at most
+
+struct ScanArgs {
+    const int *labels;
+    int N, V, D;
+    int *rowmap, *pos, *lab;
+    Scalars *sc;
+    const float *X, *W;    // f32 operands
+    long ldx, ldw;
+    uint2 *maxes;          // [workgroup] bits of the largest magnitudes of X's counted rows and of W
+};
+
+// Workgroup 0: the counted rows in order (rowmap), each row's place among them or -1 (pos), their labels. 16 rows a thread at a
+// time, so that their labels are loaded together.
+__device__ __forceinline__ void index_rows(const ScanArgs &a) {
+    __shared__ int sums[4];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int per = (N + 1023) / 1024, a = min(N, t * per), b = min(N, a + per);
-    int c = 0;
-    for (int i = a; i < b; i++) c += (unsigned)labels[i] < (unsigned)V;
-    int inc = c;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += u;
-    }
-    if (lane == 63) sums[wave] = inc;
-    __syncthreads();
-    int base = 0, total = 0;
-    for (int w = 0; w < 16; w++) {
-        if (w < wave) base += sums[w];
-        total += sums[w];
-    }
-    int at = base + inc - c;
-    for (int i = a; i < b; i++) {
-        const int y = labels[i];
-        const bool ok = (unsigned)y < (unsigned)V;
-        pos[i] = ok ? at : -1;
-        if (ok) {
-            rowmap[at] = i;
-            lab[at++] = y;
+    int done = 0;
+    for (int r0 = 0; r0 < a.N; r0 += 4096) {
+        int y[16], c = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int r = r0 + t * 16 + i;
+            y[i] = r < a.N ? a.labels[r] : -1;
+            c += (unsigned)y[i] < (unsigned)a.V;
+        }
+        int inc = c;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(inc, o, 64);
+            if (lane >= o) inc += u;
+        }
+        __syncthreads();
+        if (lane == 63) sums[wave] = inc;
+        __syncthreads();
+        int at = done + inc - c;
+        for (int w = 0; w < 4; w++) {
+            if (w < wave) at += sums[w];
+            done += sums[w];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int r = r0 + t * 16 + i;
+            const bool ok = (unsigned)y[i] < (unsigned)a.V;
+            if (r < a.N) a.pos[r] = ok ? at : -1;
+            if (ok) {
+                a.rowmap[at] = r;
+                a.lab[at++] = y[i];
+            }
         }
     }
-    if (t == 0) {
-        sc->count = total;
-        sc->xmax = sc->wmax = 0;
-    }
+    if (t == 0) a.sc->count = done;
 }
 
-// Largest magnitudes of W and of the counted rows of X (f32), a wave per stretch of 2048 values of a row. The bits of
-// non-negative floats order as integers, so the atomic's result does not depend on the order.
-__global__ __launch_bounds__(256) void lce_absmax_kernel(const float *X, long ldx, int N, const float *W, long ldw, int V, int D, const int *pos,
-                                                         Scalars *sc) {
+// Workgroup 0 indexes the rows; the others (f32 operands) find the largest magnitudes of W and of the counted rows of X, a wave per
+// stretch of 2048 values of a row. The bits of non-negative floats order as integers.
+__global__ __launch_bounds__(256) void lce_scan_kernel(ScanArgs a) {
+    if (blockIdx.x == 0) {
+        index_rows(a);
+        return;
+    }
     __shared__ unsigned red[2][4];
     typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(4)));
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (D + 2047) / 2048;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (a.D + 2047) / 2048;
     unsigned mx = 0, mw = 0;
-    for (long q = (long)blockIdx.x * 4 + wave; q < ((long)N + V) * segs; q += (long)gridDim.x * 4) {
+    for (long q = (long)(blockIdx.x - 1) * 4 + wave; q < ((long)a.N + a.V) * segs; q += (long)(gridDim.x - 1) * 4) {
         const long r = q / segs;
-        const int c0 = (int)(q - r * segs) * 2048 + lane * 4, end = min(D, c0 - lane * 4 + 2048);
-        const bool x = r < N;
-        if (x && pos[r] < 0) continue;
-        const uint32_t *p = (const uint32_t *)(x ? X + r * ldx : W + (r - N) * ldw);
+        const int c0 = (int)(q - r * segs) * 2048 + lane * 4, end = min(a.D, c0 - lane * 4 + 2048);
+        const bool x = r < a.N;
+        if (x && (unsigned)a.labels[r] >= (unsigned)a.V) continue;
+        const uint32_t *p = (const uint32_t *)(x ? a.X + r * a.ldx : a.W + (r - a.N) * a.ldw);
         unsigned m = 0;
 #pragma unroll
         for (int k = 0; k < 2048; k += 256) {
@@ -121,21 +142,30 @@ __global__ __launch_bounds__(256) void lce_absmax_kernel(const float *X, long ld
         red[1][wave] = mw;
     }
     __syncthreads();
-    if (threadIdx.x < 2) {
-        const unsigned *p = red[threadIdx.x];
-        const unsigned m = max(max(p[0], p[1]), max(p[2], p[3]));
-        unsigned *to = threadIdx.x ? &sc->wmax : &sc->xmax;
-        if (m > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(to, m);
-    }
+    if (threadIdx.x == 0)
+        a.maxes[blockIdx.x - 1] = make_uint2(max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3])), max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3])));
 }
 
-// Row r of the packed operand (panels of `rows` rows): Dp columns, zeros past D. f32 values go to two planes, f16 ones stay.
+// The workgroups' largest magnitudes joined; all 256 threads of a workgroup.
+__device__ __forceinline__ uint2 join_maxes(const uint2 *maxes, int n) {
+    __shared__ uint2 red[4];
+    uint2 m = make_uint2(0, 0);
+    for (int i = threadIdx.x; i < n; i += 256) m = make_uint2(max(m.x, maxes[i].x), max(m.y, maxes[i].y));
+    for (int o = 32; o >= 1; o >>= 1)
+        m = make_uint2(max(m.x, (unsigned)__shfl_xor((int)m.x, o, 64)), max(m.y, (unsigned)__shfl_xor((int)m.y, o, 64)));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    return make_uint2(max(max(red[0].x, red[1].x), max(red[2].x, red[3].x)), max(max(red[0].y, red[1].y), max(red[2].y, red[3].y)));
+}
+
+// One wave: row r of the packed operand (panels of `rows` rows): Dp columns, zeros past D. f32 values go to two planes, f16 ones stay.
 template <int P>
-__device__ __forceinline__ void pack_row(half_t *out, long rows, long r, const void *in, int D, int Dp, int e) {
-    const int t = threadIdx.x;
+__device__ __forceinline__ void pack_row(half_t *__restrict__ out, long rows, long r, const void *__restrict__ in, int D, int Dp, int e) {
+    const int t = threadIdx.x & 63;
     if constexpr (P == 1) {
         const half_t *p = (const half_t *)in;
-        for (int i = t * 8; i < Dp; i += 256 * 8) {
+#pragma unroll 2
+        for (int i = t * 8; i < Dp; i += 64 * 8) {
             h8 v = {};
             if (i + 7 < D) v = *(const pg::h8_any *)(p + i);
             else
@@ -143,7 +173,8 @@ __device__ __forceinline__ void pack_row(half_t *out, long rows, long r, const v
             *(h8 *)(out + pg::panel_at<1>(rows, r, i)) = v;
         }
     } else {
-        for (int i = t * 4; i < Dp; i += 256 * 4) {
+#pragma unroll 4
+        for (int i = t * 4; i < Dp; i += 64 * 4) {
             floatx4 v = pg::load4((const float *)in, i, D);
 #pragma unroll
             for (int k = 0; k < 4; k++) v[k] = ldexpf(v[k], e);
@@ -152,32 +183,47 @@ __device__ __forceinline__ void pack_row(half_t *out, long rows, long r, const v
     }
 }
 
-// Block r of the first N + 64: row r of X goes to its place among the counted rows, or its dX and outputs are cleared; the last
-// 64 clear the packed rows that fill up the last stage of the dW product. Further blocks pack W, one row each.
+// A wave a row. Of the first N + 64, row r of X goes to its place among the counted rows, or its dX and outputs are cleared; the last
+// 64 clear the packed rows that fill up the last stage of the dW product. The others pack W.
 template <int P>
-__global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, int Np, half_t *Wp, int Dp, const int *pos, const Scalars *sc) {
-    const long r = blockIdx.x;
-    const int esz = P == 1 ? 2 : 4;
-    if (r < d.N) {
-        const int q = pos[r];
-        if (q >= 0) {
-            pack_row<P>(Xp, Np, q, (const char *)d.X + r * d.ldx * esz, d.D, Dp, P == 2 ? plane_exp(sc->xmax) : 0);
-            return;
+__global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, int Np, half_t *Wp, int Dp, const int *pos, Scalars *sc,
+                                                       const uint2 *maxes, int blocks) {
+    int ex = 0, ew = 0;
+    if constexpr (P == 2) {
+        const uint2 top = join_maxes(maxes, blocks);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            sc->xmax = top.x;
+            sc->wmax = top.y;
         }
-        if (d.dX) {
-            if (d.g16) for (int i = threadIdx.x; i < d.D; i += 256) ((half_t *)d.dX)[r * d.lddx + i] = (half_t)0.0f;
-            else for (int i = threadIdx.x; i < d.D; i += 256) ((float *)d.dX)[r * d.lddx + i] = 0.0f;
+        ex = plane_exp(top.x);
+        ew = plane_exp(top.y);
+    }
+    constexpr int ESZ = P == 1 ? 2 : 4;
+    const int lane = threadIdx.x & 63, count = sc->count;
+    const long total = (long)d.N + 64 + (Wp ? d.V : 0);
+    for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < total; r += (long)gridDim.x * 4) {
+        if (r < d.N) {
+            const int q = pos[r];
+            if (q >= 0) {
+                pack_row<P>(Xp, Np, q, (const char *)d.X + r * d.ldx * ESZ, d.D, Dp, ex);
+                continue;
+            }
+            if (d.dX)
+                for (int i = lane * 4; i < d.D; i += 256) {
+                    if (d.g16) pg::store4((half_t *)d.dX + r * d.lddx, i, d.D, (floatx4){});
+                    else pg::store4((float *)d.dX + r * d.lddx, i, d.D, (floatx4){});
+                }
+            if (lane == 0) {
+                if (d.rowloss) d.rowloss[r] = 0.0f;
+                if (d.lse) d.lse[r] = 0.0f;
+            }
+        } else if (r < d.N + 64) {
+            const long q = count + (r - d.N);
+            if (q < ((count + 63) & ~63)) pack_row<1>(Xp, Np, q, nullptr, 0, Dp * P, 0);
+        } else {
+            const long v = r - d.N - 64;
+            pack_row<P>(Wp, d.V, v, (const char *)d.W + v * d.ldw * ESZ, d.D, Dp, ew);
         }
-        if (threadIdx.x == 0) {
-            if (d.rowloss) d.rowloss[r] = 0.0f;
-            if (d.lse) d.lse[r] = 0.0f;
-        }
-    } else if (r < d.N + 64) {
-        const long q = sc->count + (r - d.N);
-        if (q < ((sc->count + 63) & ~63)) pack_row<1>(Xp, Np, q, nullptr, 0, Dp * P, 0);
-    } else {
-        const long v = r - d.N - 64;
-        pack_row<P>(Wp, d.V, v, (const char *)d.W + v * d.ldw * esz, d.D, Dp, P == 2 ? plane_exp(sc->wmax) : 0);
     }
 }
 
@@ -351,22 +397,6 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(const Scalars *sc, int ro
     }
 }
 
-// One workgroup: the loss, in f64.
-__global__ __launch_bounds__(1024) void lce_loss_kernel(const Scalars *sc, const float *loss_c, int mean, float *loss) {
-    __shared__ double red[16];
-    const int c = sc->count, t = threadIdx.x;
-    double s = 0.0;
-    for (int i = t; i < c; i += 1024) s += (double)loss_c[i];
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((t & 63) == 0) red[t >> 6] = s;
-    __syncthreads();
-    if (t == 0) {
-        double v = 0.0;
-        for (int w = 0; w < 16; w++) v += red[w];
-        *loss = (float)(mean && c > 0 ? v / c : v);
-    }
-}
-
 // ── P, in place of what the product kept ───────────────────────────────────────
 
 struct GradArgs {
@@ -464,14 +494,28 @@ __device__ __forceinline__ float grad_mult(const Scalars *sc, float grad_scale, 
     return mean ? grad_scale / (float)max(1, sc->count) : grad_scale;
 }
 
-// db: the row blocks' sums in order.
-__global__ __launch_bounds__(256) void lce_dbias_kernel(const Scalars *sc, const float *part, int V, float grad_scale, int mean, float *dbias) {
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= V) return;
-    const int blocks = (sc->count + kGradRows - 1) / kGradRows;
-    float s = 0.0f;
-    for (int b = 0; b < blocks; b++) s += part[(long)b * V + n];
-    dbias[n] = ldexpf(s, -kPScale) * grad_mult(sc, grad_scale, mean);
+// Workgroup 0: the loss, in f64. The others: db, the row blocks' sums in order.
+__global__ __launch_bounds__(256) void lce_finish_kernel(const Scalars *sc, const float *loss_c, int mean, float *loss, const float *part, int V,
+                                                         float grad_scale, float *dbias) {
+    const int c = sc->count, t = threadIdx.x;
+    if (blockIdx.x > 0) {
+        const int n = (blockIdx.x - 1) * 256 + t, blocks = (c + kGradRows - 1) / kGradRows;
+        if (n >= V) return;
+        float s = 0.0f;
+        for (int b = 0; b < blocks; b++) s += part[(long)b * V + n];
+        dbias[n] = ldexpf(s, -kPScale) * grad_mult(sc, grad_scale, mean);
+        return;
+    }
+    __shared__ double red[4];
+    double s = 0.0;
+    for (int i = t; i < c; i += 256) s += (double)loss_c[i];
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((t & 63) == 0) red[t >> 6] = s;
+    __syncthreads();
+    if (t == 0) {
+        s = red[0] + red[1] + red[2] + red[3];
+        *loss = (float)(mean && c > 0 ? s / c : s);
+    }
 }
 
 // ── the gradient products ──────────────────────────────────────────────────────
@@ -597,7 +641,7 @@ struct Layout {
     int keep, PP;              // what the logits' product keeps; planes of P
     int rows, pieces;          // rows of a piece
     bool pack_w, grad;
-    int64_t rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, Pp, dbpart, dwacc, sums, total;
+    int64_t maxes, rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, Pp, dbpart, dwacc, sums, total;
 };
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -636,6 +680,7 @@ Layout layout(const LinearCe &d) {
         at += bytes;
         return o;
     };
+    l.maxes = take(kMaxBlocks * sizeof(uint2));
     l.rowmap = take(Np * 4);
     l.pos = take(Np * 4);
     l.lab = take(Np * 4);
@@ -754,14 +799,14 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
     float2 *stats = (float2 *)(ws + l.stats);
     half_t *Xp = (half_t *)(ws + l.Xp), *Wp = l.pack_w ? (half_t *)(ws + l.Wp) : nullptr;
 
-    hipLaunchKernelGGL(lce_index_kernel, dim3(1), dim3(1024), 0, s, d.labels, d.N, d.V, rowmap, pos, lab, sc);
-    if (!d.f16)
-        hipLaunchKernelGGL(lce_absmax_kernel, dim3((unsigned)std::min<int64_t>(((int64_t)d.N + d.V) * ceil_div(d.D, 2048) / 4 + 1, 1024)), dim3(256), 0, s, (const float *)d.X, d.ldx, d.N,
-                           (const float *)d.W, d.ldw, d.V, d.D, pos, sc);
-    const dim3 pgrid((unsigned)(d.N + 64 + (l.pack_w ? d.V : 0)));
+    uint2 *maxes = (uint2 *)(ws + l.maxes);
+    const int scans = d.f16 ? 0 : (int)std::min<int64_t>(((int64_t)d.N + d.V) * ceil_div(d.D, 2048) / 4 + 1, kMaxBlocks);
+    const ScanArgs scan{d.labels, d.N, d.V, d.D, rowmap, pos, lab, sc, (const float *)d.X, (const float *)d.W, d.ldx, d.ldw, maxes};
+    hipLaunchKernelGGL(lce_scan_kernel, dim3((unsigned)(1 + scans)), dim3(256), 0, s, scan);
+    const dim3 pgrid((unsigned)std::min<int64_t>(((int64_t)d.N + 64 + (l.pack_w ? d.V : 0) + 3) / 4, 4096));
     const int Np = (d.N + 63) & ~63;
-    if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc);
-    else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc);
+    if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc, maxes, scans);
+    else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc, maxes, scans);
 
     const pg::Operand W = l.pack_w ? pg::panels(Wp, d.V, d.V, l.Dp) : pg::row_major(d.W, d.ldw, d.V, l.Dp);
     for (int piece = 0; piece < l.pieces; piece++) {
@@ -816,10 +861,8 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         else if (d.f16) gradients<2, 1>(d, l, p, W, X, piece, ws, s);
         else gradients<2, 2>(d, l, p, W, X, piece, ws, s);
     }
-    if (d.dbias)
-        hipLaunchKernelGGL(lce_dbias_kernel, dim3((unsigned)ceil_div(d.V, 256)), dim3(256), 0, s, sc, (const float *)(ws + l.dbpart), d.V, d.grad_scale,
-                           d.mean, d.dbias);
-    hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, s, sc, loss, d.mean, d.loss);
+    hipLaunchKernelGGL(lce_finish_kernel, dim3((unsigned)(1 + (d.dbias ? ceil_div(d.V, 256) : 0))), dim3(256), 0, s, sc, loss, d.mean, d.loss,
+                       (const float *)(ws + l.dbpart), d.V, d.grad_scale, d.dbias);
     return hipGetLastError();
 }
 

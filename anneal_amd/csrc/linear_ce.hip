@@ -68,13 +68,22 @@ __device__ __forceinline__ void index_rows(const ScanArgs &a) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     int done = 0;
     for (int r0 = 0; r0 < a.N; r0 += 4096) {
+        typedef int i4 __attribute__((ext_vector_type(4), aligned(4)));
+        const int first = r0 + t * 16;
         int y[16], c = 0;
+        if (first + 15 < a.N) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int r = r0 + t * 16 + i;
-            y[i] = r < a.N ? a.labels[r] : -1;
-            c += (unsigned)y[i] < (unsigned)a.V;
+            for (int i = 0; i < 16; i += 4) {
+                const i4 v = *(const i4 *)(a.labels + first + i);
+#pragma unroll
+                for (int k = 0; k < 4; k++) y[i + k] = v[k];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) y[i] = first + i < a.N ? a.labels[first + i] : -1;
         }
+#pragma unroll
+        for (int i = 0; i < 16; i++) c += (unsigned)y[i] < (unsigned)a.V;
         int inc = c;
         for (int o = 1; o < 64; o <<= 1) {
             const int u = __shfl_up(inc, o, 64);
@@ -90,7 +99,7 @@ __device__ __forceinline__ void index_rows(const ScanArgs &a) {
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const int r = r0 + t * 16 + i;
+            const int r = first + i;
             const bool ok = (unsigned)y[i] < (unsigned)a.V;
             if (r < a.N) a.pos[r] = ok ? at : -1;
             if (ok) {
@@ -524,6 +533,7 @@ struct ProductArgs {
     pg::Operand A, B;
     int M, N, tiles_m, tiles_n;
     pg::Work w;
+    int cap;               // partial tiles that there is room for
     const Scalars *sc;
     int row0, rows;
     int rows_are;          // 0: C's rows are the piece's (dX); 1: k runs over them (dW)
@@ -546,18 +556,14 @@ __device__ __forceinline__ int product_size(const ProductArgs &a, int &nk, int B
     return a.rows_are == 0 ? rows : a.M;
 }
 
-// The work that is there: the host plans for rows that all count; where fewer do, dX has fewer tiles, and the workgroups that share
-// the K of its tiles are dealt to those.
+// The work that is there: the host plans for rows that all count; where fewer do, dX has fewer tiles, and its workgroups are dealt
+// to those (8192 rows of 2048 features over 32000 classes of which three quarters count are 192 tiles of 256: 1.5 ms in one piece
+// each, %s in four).
 template <class C>
 __device__ __forceinline__ pg::Work product_work(const ProductArgs &a, int M, int nk, int &tiles_m) {
-    pg::Work w = a.w;
     tiles_m = a.rows_are == 0 ? (M + C::BM - 1) / C::BM : a.tiles_m;
-    const int tiles = tiles_m * a.tiles_n;
-    if (a.rows_are == 0 && tiles < w.tiles()) {
-        if (w.splits == 1 || tiles > w.rest) w = pg::Work{min(tiles, w.whole), max(0, tiles - w.whole), w.splits, w.part};
-        else w = pg::Work{0, tiles, max(1, min(w.rest * w.splits / max(1, tiles), nk / 2)), w.part};
-    }
-    return w;
+    if (a.rows_are == 1 || tiles_m == a.tiles_m) return a.w;
+    return pg::deal(tiles_m * a.tiles_n, nk, C::BM == 256 ? 256 : 512, a.cap, C::BM == 256 ? 0.07f : C::BM == 128 ? 0.03f : 0.02f, a.w.part);
 }
 
 template <class C>
@@ -652,6 +658,12 @@ pg::Plan plan_of(int64_t M, int64_t N, int64_t k, int pa, int pb, bool narrow) {
 pg::Plan logits_plan(const Layout &l, int V, int rows) { return plan_of(rows, V, l.Dp, l.P, l.P, true); }
 // (64-wide tiles of one plane have no layout for operands along k)
 pg::Plan dx_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(rows, d.D, d.V, l.PP, l.P, l.P == 2); }
+// Room for partial tiles: four rounds of them where half a round to two rounds of tiles may turn out to be fewer (below that, what
+// the plan has fills a round with any number of tiles; above, rounds are short against the whole).
+int dx_cap(const pg::Plan &p) {
+    const int slots = p.width == 256 ? 256 : 512, planned = p.w.splits > 1 ? p.w.rest * p.w.splits : 0;
+    return p.w.tiles() > slots / 2 && p.w.tiles() <= 2 * slots ? std::max(planned, 4 * slots) : planned;
+}
 pg::Plan dw_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(d.V, d.D, rows, l.PP, l.P, l.P == 2); }
 
 Layout layout(const LinearCe &d) {
@@ -697,7 +709,10 @@ Layout layout(const LinearCe &d) {
     int64_t sums = 0;
     for (const int64_t r : {rows, Np - (l.pieces - 1) * rows}) {   // the last piece has fewer rows, and its own plan
         sums = std::max(sums, (int64_t)logits_plan(l, d.V, (int)r).part_bytes());
-        if (d.dX) sums = std::max(sums, (int64_t)dx_plan(l, d, (int)r).part_bytes());
+        if (d.dX) {
+            const pg::Plan p = dx_plan(l, d, (int)r);
+            sums = std::max(sums, (int64_t)dx_cap(p) * p.width * p.width * 4);
+        }
         if (d.dW) sums = std::max(sums, (int64_t)dw_plan(l, d, (int)r).part_bytes());
     }
     l.sums = take(sums);
@@ -723,8 +738,9 @@ template <class C>
 void launch_product(ProductArgs a, hipStream_t s) {
     a.tiles_m = ceil_div(a.rows_are == 0 ? a.rows : a.M, C::BM);
     a.tiles_n = ceil_div(a.N, C::BN);
-    hipLaunchKernelGGL((lce_product_kernel<C>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a);
-    if (a.w.splits > 1) hipLaunchKernelGGL((lce_product_join_kernel<C>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((lce_product_kernel<C>), dim3((unsigned)std::max(a.w.blocks(), a.cap)), dim3(C::NT), 0, s, a);
+    const int joins = std::max(a.w.splits > 1 ? a.w.rest : 0, std::min(a.cap / 2, a.tiles_m * a.tiles_n));
+    if (joins) hipLaunchKernelGGL((lce_product_join_kernel<C>), dim3((unsigned)joins, C::FA), dim3(C::NT), 0, s, a);
 }
 
 template <int TA, int TB, int PA, int PB>
@@ -743,6 +759,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
         const pg::Plan plan = dx_plan(l, d, a.rows);
         b.w = plan.w;
         b.w.part = (float *)(ws + l.sums);
+        b.cap = dx_cap(plan);
         b.A = pg::panels(P, a.rows, a.rows, a.rows);
         b.B = W;
         b.B.rows = l.Dp;

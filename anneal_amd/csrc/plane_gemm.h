@@ -18,6 +18,8 @@
 // Per stage a wave reads each fragment once: hi*hi and lo*hi share B's hi, hi*hi and hi*lo share A's hi. So two planes take 2/3
 // of the LDS reads per MFMA that one plane takes, and a 256x256 tile of 8 waves is bound by MFMA issue, not by LDS.
 #pragma once
+#include <algorithm>
+
 #include "ah_common.h"
 #include "gemm16_kernel.h"
 
@@ -389,9 +391,9 @@ __device__ __forceinline__ void tri_tile(int t, int n, int &row, int &col) {
 }
 
 // ── tiles, and K split over workgroups ─────────────────────────────────────────
-// Tiles are worked on in rounds of as many as the chip takes at once. What is left for the last round (all of them, where there
-// are few) is split over K: `splits` workgroups share a tile's stages and leave their accumulators in the workspace, and a second
-// kernel adds them in order (results repeat bit for bit) and runs the epilogue, one workgroup for each 16 rows of a tile's waves.
+// Tiles are worked on in rounds of as many as the chip takes at once. What does not fill a round (all of them, where there are few)
+// is split over K: `splits` workgroups share a tile's stages and leave their accumulators in the workspace, and a second kernel
+// adds them in order (results repeat bit for bit) and runs the epilogue, one workgroup for each 16 rows of a tile's waves.
 struct Work {
     int whole, rest, splits;   // tiles 0 .. whole-1 in one piece each, then `rest` tiles of `splits` pieces
     float *part;               // [split][rest] partial tiles
@@ -415,6 +417,21 @@ __device__ __forceinline__ void pick(const Work &w, int b, int nk, int &tile, in
     first = min(nk, split * q);
     count = min(nk, first + q) - first;
     slot = r;
+}
+
+// `tiles` tiles of nk stages on a chip that takes `slots` at once, with room for `cap` partial tiles: how a kernel deals out work whose
+// size the host did not know. Costs in stages: three for a round's start and end, `join` for a partial tile's way to memory and back.
+__device__ __forceinline__ Work deal(int tiles, int nk, int slots, int cap, float join, float *part) {
+    int best = 1;
+    float best_cost = 1e30f;
+    for (int s = 1; s <= 16 && (s == 1 || (tiles * s <= cap && nk >= 2 * s)); s++) {
+        const float cost = (float)((tiles * s + slots - 1) / slots * ((nk + s - 1) / s + 3)) + (s > 1 ? 4.0f + join * (float)(tiles * s) : 0.0f);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = s;
+        }
+    }
+    return best == 1 ? Work{tiles, 0, 1, part} : Work{0, tiles, best, part};
 }
 
 // Partial sums of accumulator row i: [slot][i][j][thread] of four floats.
@@ -501,9 +518,10 @@ Plan plan(Tiles tiles, long k, int pa, int pb, bool narrow) {
         };
         const double fixed = width == 256 ? 7.0 : 5.0;   // launch, first loads, the epilogue
         const long rest = n % slots, rounds = n / slots;
-        for (int s = 1; s <= 32 && (s == 1 || (rest * s <= slots && nk >= 2 * s)); s++) {
+        for (int s = 1; s <= 32 && (s == 1 || (rest * s <= 4 * slots && nk >= 2 * s)); s++) {
             const double joined = (double)rest * s * width * width * 8 / 4e6;   // us at 4 TB/s
-            const double us = rounds * (nk * stage(slots) + fixed) + (rest ? (double)((nk + s - 1) / s) * stage(rest * s) + fixed : 0) +
+            const long turns = (rest * s + slots - 1) / slots;
+            const double us = rounds * (nk * stage(slots) + fixed) + turns * ((double)((nk + s - 1) / s) * stage(std::min(slots, rest * s)) + fixed) +
                               (s > 1 ? 4.0 + joined : 0);
             if (us < best_us) {
                 best_us = us;

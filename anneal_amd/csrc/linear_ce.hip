@@ -676,7 +676,7 @@ Layout layout(const LinearCe &d) {
     l.keep = !l.grad ? KEEP_NONE : d.g16 && !d.dbias ? KEEP_EXP : KEEP_Z;
     l.PP = d.g16 ? 1 : 2;
     l.KE = l.keep == KEEP_NONE ? 0 : l.keep == KEEP_EXP ? 2 : d.g16 ? 6 : 4;
-    l.pack_w = !d.f16 || d.D % 64 || d.ldw % 8 || ((uintptr_t)d.W & 15) || d.ldw > 1 << 22;
+    l.pack_w = !d.f16 || d.D % 8 || d.ldw % 8 || ((uintptr_t)d.W & 15) || d.ldw > 1 << 22;
     const int64_t Np = ((int64_t)d.N + 63) & ~63ll;
     int64_t rows = Np;
     if (l.KE) rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, ((int64_t)(d.piece_mb ? d.piece_mb : kPieceMb) << 20) / ((int64_t)l.Vp * l.KE) / 256 * 256)});
@@ -762,7 +762,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
         b.cap = dx_cap(plan);
         b.A = pg::panels(P, a.rows, a.rows, a.rows);
         b.B = W;
-        b.B.rows = l.Dp;
+        b.B.rows = l.pack_w ? l.Dp : d.D;
         b.B.k = d.V;
         b.N = d.D;
         b.k = d.V;
@@ -825,7 +825,7 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
     if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc, maxes, scans);
     else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc, maxes, scans);
 
-    const pg::Operand W = l.pack_w ? pg::panels(Wp, d.V, d.V, l.Dp) : pg::row_major(d.W, d.ldw, d.V, l.Dp);
+    const pg::Operand W = l.pack_w ? pg::panels(Wp, d.V, d.V, l.Dp) : pg::row_major(d.W, d.ldw, d.V, d.D);
     for (int piece = 0; piece < l.pieces; piece++) {
         const int row0 = piece * l.rows, rows = std::min(l.rows, Np - row0);
         const pg::Operand X = pg::panels(Xp + (long)row0 * 64, Np, rows, l.Dp);

@@ -120,12 +120,18 @@ struct PFetch {
             }
         }
     }
-    // krem: k-rows of the operand from the stage's first on; one past them (T = 1) reads the last
+    // krem: k of the operand from the stage's first on. Past them T = 1 reads the last k-row and T = 0 the stage's first chunk of the
+    // row (krem is then a multiple of a chunk's 8): the other operand is 0 there, and nothing behind the array is read.
     __device__ __forceinline__ void issue(int j, const char *base, long ld, int krem, uint32_t lds, int wave_u, int lane) const {
         uint32_t o = off[j];
-        if (T == 1 && krem < BK) {
-            const int kk = (wave_u * PER + j) * ROWS + (16 * lane) / (2 * W);
-            if (kk >= krem) o -= (uint32_t)((long)(kk - (krem - 1)) * ld * 2);
+        if (krem < BK) {
+            if constexpr (T == 1) {
+                const int kk = (wave_u * PER + j) * ROWS + (16 * lane) / (2 * W);
+                if (kk >= krem) o -= (uint32_t)((long)(kk - (krem - 1)) * ld * 2);
+            } else if constexpr (P == 1) {
+                const int q = 4 * (wave_u * PER + j) + (lane >> 4), c = ((lane & 15) ^ (q & 15)) % (W / 8);
+                if (c * 8 >= krem) o -= (uint32_t)(c * 16);
+            }
         }
         g16::dma16(o, base, lds + (uint32_t)((wave_u * PER + j) * 1024));
     }
@@ -183,7 +189,7 @@ struct Operand {
     long ld;         // halves from a stored row to the next
     long ps;         // bytes from 64 halves of a row to the next 64
     int rows;        // operand rows
-    int k;           // T = 1: stored rows that exist (stages past them read the last one)
+    int k;           // k that there are (B's may end inside a stage: PFetch::issue)
 };
 
 // `stored` rows in panels; rows of the operand, k as above.
@@ -223,7 +229,7 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
     const long da = C::TA == 0 ? A.ps : (long)BK * A.ld * 2, db = C::TB == 0 ? B.ps : (long)BK * B.ld * 2;   // bytes a stage
     auto issue_one = [&](int f, int t, int buf) {   // load f of stage t into buffer buf
         if (f < PERA) fa.issue(f, Ab + (kt0 + t) * da, A.ld, BK, lds + buf * STAGE, wave_u, lane);
-        else fb.issue(f - PERA, Bb + (kt0 + t) * db, B.ld, C::TB == 1 ? B.k - (kt0 + t) * BK : BK, lds + buf * STAGE + ABYTES, wave_u, lane);
+        else fb.issue(f - PERA, Bb + (kt0 + t) * db, B.ld, C::TB == 1 || C::PB == 1 ? B.k - (kt0 + t) * BK : BK, lds + buf * STAGE + ABYTES, wave_u, lane);
     };
     typename C::FragA ra;
     typename C::FragB rb;

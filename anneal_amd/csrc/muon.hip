@@ -219,12 +219,12 @@ __global__ __launch_bounds__(C::NT) void ns_join_kernel(NsArgs p, Muon d) {
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Tiles of one product over the batch and how they are split, for M x N results summed over k.
-pg::Plan ns_plan(bool symmetric, int batch, int M, int N, int k) {
+pg::Plan ns_plan(bool symmetric, int batch, int M, int N, int k, long piece = 1l << 40) {
     const auto tiles = [&](int w) -> long {
         const long m = ceil_div(M, w), n = ceil_div(N, w);
         return batch * (symmetric ? m * (m + 1) / 2 : m * n);
     };
-    return pg::plan(tiles, k, 2, 2, true);
+    return pg::plan(tiles, k, 2, 2, true, piece);
 }
 
 struct Layout {
@@ -243,7 +243,9 @@ Layout layout(const Muon &d) {
     l.wide = d.rows <= d.cols;
     l.S = l.wide ? l.Rp : l.Cp;
     l.K = l.wide ? l.Cp : l.Rp;
-    l.gram = ns_plan(true, d.batch, l.S, l.S, l.K);
+    // Sums over the long side in pieces of at most 2048 (or of the short side, which the other products sum over), added in the join:
+    // in one chain of 7384 the diagonal's rounding errors cost the result 3.8e-6 at 9 x 7384 x 704, in pieces 2.2e-6, at no time.
+    l.gram = ns_plan(true, d.batch, l.S, l.S, l.K, std::max(2048, l.S));
     l.square = ns_plan(true, d.batch, l.S, l.S, l.S);
     l.apply = ns_plan(false, d.batch, l.Rp, l.Cp, l.S);
     const int most = longest_group(d);

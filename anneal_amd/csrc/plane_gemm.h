@@ -507,9 +507,9 @@ using Tile64 = Tile<64, 64, 2, 2, TA, TB, PA, PB, 4>;
 //   planes 2 x 1      1.23 / 1.58             0.61 / 0.97                   -
 //   planes 2 x 2      1.62 / 2.30             0.68 / 1.33                 0.26 / 0.41
 // (many CUs at once run slower than few: the clock gives way). Splitting adds a launch and the partial sums' way to memory and
-// back. 1024 x 1024 over k = 1024 in two planes, measured: 15 us in 256 tiles of 64, 24 in 64 of 128.
+// back; no piece is longer than `piece`. 1024 x 1024 over k = 1024 in two planes, measured: 15 us in 256 tiles of 64, 24 in 64 of 128.
 template <class Tiles>
-Plan plan(Tiles tiles, long k, int pa, int pb, bool narrow) {
+Plan plan(Tiles tiles, long k, int pa, int pb, bool narrow, long piece = 1l << 40) {
     const int row = pa == 1 ? 0 : pb == 1 ? 1 : 2;
     constexpr double kFew[3] = {1.22, 1.18, 1.53}, kMore[3] = {0.55, 0.40, 0.77};
     constexpr double k128[3][2] = {{0.72, 1.15}, {0.61, 0.97}, {0.68, 1.33}}, k64[3][2] = {{0.22, 0.36}, {0.30, 0.50}, {0.26, 0.41}};
@@ -523,8 +523,9 @@ Plan plan(Tiles tiles, long k, int pa, int pb, bool narrow) {
             return width == 256 ? kFew[row] + kMore[row] * (double)wg / 256 : width == 128 ? k128[row][wg > 256] : k64[row][wg > 256];
         };
         const double fixed = width == 256 ? 7.0 : 5.0;   // launch, first loads, the epilogue
-        const long rest = n % slots, rounds = n / slots;
-        for (int s = 1; s <= 32 && (s == 1 || (rest * s <= 4 * slots && nk >= 2 * s)); s++) {
+        const long least = (nk * (row == 0 ? 64 : 32) + piece - 1) / piece;
+        const long rest = least > 1 ? n : n % slots, rounds = least > 1 ? 0 : n / slots;
+        for (long s = std::max(1l, least); s <= std::max(32l, least) && (s <= least || (rest * s <= 4 * slots && nk >= 2 * s)); s++) {
             const double joined = (double)rest * s * width * width * 8 / 4e6;   // us at 4 TB/s
             const long turns = (rest * s + slots - 1) / slots;
             const double us = rounds * (nk * stage(slots) + fixed) + turns * ((double)((nk + s - 1) / s) * stage(std::min(slots, rest * s)) + fixed) +
@@ -533,7 +534,7 @@ Plan plan(Tiles tiles, long k, int pa, int pb, bool narrow) {
                 best_us = us;
                 best.us = us;
                 best.width = width;
-                best.w = s == 1 ? Work{(int)n, 0, 1, nullptr} : Work{(int)(rounds * slots), (int)rest, s, nullptr};
+                best.w = s == 1 ? Work{(int)n, 0, 1, nullptr} : Work{(int)(rounds * slots), (int)rest, (int)s, nullptr};
             }
             if (!rest) break;
         }

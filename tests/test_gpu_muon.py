@@ -134,6 +134,21 @@ def test_in_place(dev):
     ws.free()
 
 
+@pytest.mark.parametrize("rows,cols", [(150, 5003), (5003, 150)])
+def test_long_sides_of_a_batch(dev, rows, cols):
+    """More tiles than the chip takes at once, each summed in pieces: every matrix is the one alone to its last bits' rounding."""
+    batch = 60
+    G = gradient(np.random.default_rng(rows), rows, cols, L.AH_F32)
+    want, err = iterate(G.astype(np.float64))
+    g, o = dev.buffer(G), dev.buffer(batch * G.size)
+    args = dict(dtype=L.AH_F32, rows=rows, cols=cols, batch=batch, G=g, O=o, stride_g=0)
+    dev.orthogonalize(ws=dev.buffer(dev.orthogonalize_workspace(**args) // 4 + 4), **args)
+    got = o.read().reshape(batch, rows, cols)
+    for z in range(batch):
+        assert np.array_equal(got[z], got[0])
+    assert np.linalg.norm(got[0] - want) <= min(err + U32 * np.linalg.norm(want), 2e-5 * np.linalg.norm(want))
+
+
 @pytest.mark.parametrize("nesterov", [True, False])
 @pytest.mark.parametrize("dtype", [L.AH_F32, L.AH_F16], ids=["f32", "f16"])
 @pytest.mark.parametrize("batch,rows,cols", [(1, 128, 784), (1, 100, 33), (2, 65, 130)])

@@ -19,6 +19,7 @@
 
 #include <algorithm>
 
+#include "linear_ce_few.h"
 #include "plane_gemm.h"
 
 namespace ah {
@@ -53,7 +54,7 @@ constexpr int kMaxBlocks = 1024;  // workgroups that look for the largest magnit
 
 struct ScanArgs {
     const int *labels;
-    int N, V, D;
+    int N, V, D, Wrows;    // Wrows: V, or 0 where W need not be looked at
     int *rowmap, *pos, *lab;
     Scalars *sc;
     const float *X, *W;    // f32 operands
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(256) void lce_scan_kernel(ScanArgs a) {
     typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(4)));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (a.D + 2047) / 2048;
     unsigned mx = 0, mw = 0;
-    for (long q = (long)(blockIdx.x - 1) * 4 + wave; q < ((long)a.N + a.V) * segs; q += (long)(gridDim.x - 1) * 4) {
+    for (long q = (long)(blockIdx.x - 1) * 4 + wave; q < ((long)a.N + a.Wrows) * segs; q += (long)(gridDim.x - 1) * 4) {
         const long r = q / segs;
         const int c0 = (int)(q - r * segs) * 2048 + lane * 4, end = min(a.D, c0 - lane * 4 + 2048);
         const bool x = r < a.N;
@@ -361,6 +362,30 @@ __global__ __launch_bounds__(C::NT, 2) void lce_logits_kernel(LogitArgs a) {
     logits_rows<C, KEEP, C::FA>(a, M, m0, n0, 0, acc);
 }
 
+// The same from X and W as they lie, for few rows.
+struct FewArgs {
+    const void *X, *W;
+    long ldx, ldw;
+    const int *rowmap;
+    int D, Vp;
+};
+template <class C, int KEEP, bool F16>
+__global__ __launch_bounds__(C::NT, 2) void lce_few_logits_kernel(LogitArgs a, FewArgs f) {
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    if (M == 0) return;
+    int tile, slot, first, count, m0, n0;
+    pg::pick(a.w, blockIdx.x, a.nk, tile, slot, first, count);
+    logits_tile<C>(a, tile, m0, n0);
+    __shared__ __attribute__((aligned(16))) char smem[few::smem_bytes<C>()];
+    floatx4 acc[C::FA][C::FB];
+    few::contract_along<C, F16>(f.X, f.ldx, f.rowmap, M, f.W, f.ldw, a.V, f.D, n0, first, count, smem, acc);
+    if (slot >= 0) {
+        pg::store_partials<C>(a.w.part, slot, acc);
+        return;
+    }
+    logits_rows<C, KEEP, C::FA>(a, M, m0, n0, 0, acc);
+}
+
 template <class C, int KEEP>
 __global__ __launch_bounds__(C::NT) void lce_logits_join_kernel(LogitArgs a) {
     const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
@@ -383,6 +408,7 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(const Scalars *sc, int ro
     const float2 *p = stats + (long)m * T;
     float mx = -__builtin_inff();
     bool nan = false;
+#pragma unroll 8
     for (int t = lane; t < T; t += 64) {
         mx = fmaxf(mx, p[t].x);
         nan |= p[t].y != p[t].y;
@@ -390,6 +416,7 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(const Scalars *sc, int ro
     mx = wave_max(mx);
     const float ref = mx == -__builtin_inff() ? 0.0f : mx;
     float s = 0.0f;
+#pragma unroll 8
     for (int t = lane; t < T; t += 64) {
         const float2 v = p[t];
         if (v.y > 0.0f) s += v.y * __builtin_amdgcn_exp2f((v.x - ref) * kLog2e);
@@ -558,7 +585,7 @@ __device__ __forceinline__ int product_size(const ProductArgs &a, int &nk, int B
 
 // The work that is there: the host plans for rows that all count; where fewer do, dX has fewer tiles, and its workgroups are dealt
 // to those (8192 rows of 2048 features over 32000 classes of which three quarters count are 192 tiles of 256: 1.5 ms in one piece
-// each, %s in four).
+// each, 1.25 in four, and 0.05 for the join).
 template <class C>
 __device__ __forceinline__ pg::Work product_work(const ProductArgs &a, int M, int nk, int &tiles_m) {
     tiles_m = a.rows_are == 0 ? (M + C::BM - 1) / C::BM : a.tiles_m;
@@ -624,6 +651,31 @@ __global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
     product_rows<C, C::FA>(a, M, m0, n0, 0, acc);
 }
 
+// dX from W as it lies, for few rows: one row of tiles.
+template <class C, int PP, bool F16>
+__global__ __launch_bounds__(C::NT, 2) void lce_few_dx_kernel(ProductArgs a, FewArgs f, const char *P) {
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    if (M == 0) return;
+    int tile, slot, first, count;
+    pg::pick(a.w, blockIdx.x, (a.k + few::across_v(PP) - 1) / few::across_v(PP), tile, slot, first, count);
+    __shared__ __attribute__((aligned(16))) char smem[few::smem_bytes<C>()];
+    floatx4 acc[C::FA][C::FB];
+    few::contract_across<C, PP, F16>(P, a.rows, f.Vp, f.W, f.ldw, a.k, a.N, tile * C::BN, first, count, smem, acc);
+    if (slot >= 0) {
+        pg::store_partials<C>(a.w.part, slot, acc);
+        return;
+    }
+    product_rows<C, C::FA>(a, M, 0, tile * C::BN, 0, acc);
+}
+template <class C>
+__global__ __launch_bounds__(C::NT) void lce_few_dx_join_kernel(ProductArgs a) {
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    if (16 * (int)blockIdx.y >= M) return;
+    floatx4 v[1][C::FB];
+    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, v[0]);
+    product_rows<C, 1>(a, M, 0, (a.w.whole + blockIdx.x) * C::BN, blockIdx.y, v);
+}
+
 template <class C>
 __global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) {
     int nk, tiles_m, m0, n0;
@@ -640,6 +692,9 @@ __global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) 
 
 constexpr int kPieceMb = 2048;   // MiB of kept exponentials or logits: one piece holds 8192 rows of 131072 f16 exponentials
 constexpr int kMaxPieceRows = 1 << 20;          // a panel's offsets stay within 32 bits
+// Rows up to which a W that would have to be packed is read as it lies. 4096 features, 32000 classes in f32, with gradients, packed and as
+// it lies: 16 rows 731 and 438 us, 128 rows 823 and 850; the loss alone 433 and 139 us at 16 rows, 545 and 367 at 121 (2944 x 51416).
+constexpr int kFewRows = 128;
 constexpr int kStatCols = 32;                  // the narrowest wave tile: bounds the statistics' columns
 
 struct Layout {
@@ -647,6 +702,7 @@ struct Layout {
     int keep, PP;              // what the logits' product keeps; planes of P
     int rows, pieces;          // rows of a piece
     bool pack_w, grad;
+    int few;                   // 16-row tiles of the form for few rows, or 0
     int64_t maxes, rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, Pp, dbpart, dwacc, sums, total;
 };
 
@@ -664,6 +720,16 @@ int dx_cap(const pg::Plan &p) {
     const int slots = p.width == 256 ? 256 : 512, planned = p.w.splits > 1 ? p.w.rest * p.w.splits : 0;
     return p.w.tiles() > slots / 2 && p.w.tiles() <= 2 * slots ? std::max(planned, 4 * slots) : planned;
 }
+// The form for few rows: tiles of 128 classes, 1.75 us a stage at the rate of memory, 3.4 at the f32 matrix rate for 128 rows; tiles of
+// 256 features, twice that.
+double few_stage(const Layout &l, const LinearCe &d) { return std::max(1.75, d.f16 ? 0.0 : 0.43 * l.few); }
+pg::Work few_logits_work(const Layout &l, const LinearCe &d) {
+    return few::work(ceil_div(d.V, 128), ceil_div(d.D, few::along_k(d.f16)), few_stage(l, d), l.few * 16l * 128 * 4);
+}
+pg::Work few_dx_work(const Layout &l, const LinearCe &d) {
+    return few::work(ceil_div(d.D, 256), ceil_div(d.V, few::across_v(l.PP)), 2 * few_stage(l, d), l.few * 16l * 256 * 4);
+}
+int64_t few_part_bytes(const Layout &l, const pg::Work &w, int columns) { return w.splits > 1 ? (int64_t)w.rest * w.splits * l.few * 16 * columns * 4 : 0; }
 pg::Plan dw_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(d.V, d.D, rows, l.PP, l.P, l.P == 2); }
 
 Layout layout(const LinearCe &d) {
@@ -677,6 +743,10 @@ Layout layout(const LinearCe &d) {
     l.PP = d.g16 ? 1 : 2;
     l.KE = l.keep == KEEP_NONE ? 0 : l.keep == KEEP_EXP ? 2 : d.g16 ? 6 : 4;
     l.pack_w = !d.f16 || d.D % 8 || d.ldw % 8 || ((uintptr_t)d.W & 15) || d.ldw > 1 << 22;
+    if (l.pack_w && d.N <= kFewRows && d.D >= 8) {
+        l.pack_w = false;
+        l.few = d.N <= 16 ? 1 : d.N <= 64 ? 4 : 8;
+    }
     const int64_t Np = ((int64_t)d.N + 63) & ~63ll;
     int64_t rows = Np;
     if (l.KE) rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, ((int64_t)(d.piece_mb ? d.piece_mb : kPieceMb) << 20) / ((int64_t)l.Vp * l.KE) / 256 * 256)});
@@ -708,8 +778,9 @@ Layout layout(const LinearCe &d) {
     if (d.dW && d.g16 && l.pieces > 1) l.dwacc = take((int64_t)d.V * d.D * 4);
     int64_t sums = 0;
     for (const int64_t r : {rows, Np - (l.pieces - 1) * rows}) {   // the last piece has fewer rows, and its own plan
-        sums = std::max(sums, (int64_t)logits_plan(l, d.V, (int)r).part_bytes());
-        if (d.dX) {
+        sums = std::max(sums, l.few ? few_part_bytes(l, few_logits_work(l, d), 128) : (int64_t)logits_plan(l, d.V, (int)r).part_bytes());
+        if (d.dX && l.few) sums = std::max(sums, few_part_bytes(l, few_dx_work(l, d), 256));
+        else if (d.dX) {
             const pg::Plan p = dx_plan(l, d, (int)r);
             sums = std::max(sums, (int64_t)dx_cap(p) * p.width * p.width * 4);
         }
@@ -734,6 +805,28 @@ void logits(const LogitArgs &a, int keep, hipStream_t s) {
     else if constexpr (C::PA == 1) launch_logits<C, KEEP_EXP>(a, s);
 }
 
+template <int FA, bool F16, int KEEP>
+void launch_few_logits(LogitArgs a, const FewArgs &f, hipStream_t s) {
+    typedef few::Tile<FA, 2> C;
+    a.tiles_m = 1;
+    hipLaunchKernelGGL((lce_few_logits_kernel<C, KEEP, F16>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a, f);
+    if (a.w.splits > 1) hipLaunchKernelGGL((lce_logits_join_kernel<C, KEEP>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
+}
+template <int FA>
+void few_logits(const LogitArgs &a, const FewArgs &f, const LinearCe &d, int keep, hipStream_t s) {
+    if (!d.f16) keep == KEEP_NONE ? launch_few_logits<FA, false, KEEP_NONE>(a, f, s) : launch_few_logits<FA, false, KEEP_Z>(a, f, s);
+    else if (keep == KEEP_NONE) launch_few_logits<FA, true, KEEP_NONE>(a, f, s);
+    else if (keep == KEEP_EXP) launch_few_logits<FA, true, KEEP_EXP>(a, f, s);
+    else launch_few_logits<FA, true, KEEP_Z>(a, f, s);
+}
+
+template <int PP, bool F16, int FA>
+void launch_few_dx(const ProductArgs &a, const FewArgs &f, const char *P, hipStream_t s) {
+    typedef few::Tile<FA, 4> C;
+    hipLaunchKernelGGL((lce_few_dx_kernel<C, PP, F16>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a, f, P);
+    if (a.w.splits > 1) hipLaunchKernelGGL((lce_few_dx_join_kernel<C>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
+}
+
 template <class C>
 void launch_product(ProductArgs a, hipStream_t s) {
     a.tiles_m = ceil_div(a.rows_are == 0 ? a.rows : a.M, C::BM);
@@ -756,22 +849,31 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
     const char *P = ws + l.Pp;
     if (d.dX) {
         ProductArgs b = a;
-        const pg::Plan plan = dx_plan(l, d, a.rows);
-        b.w = plan.w;
-        b.w.part = (float *)(ws + l.sums);
-        b.cap = dx_cap(plan);
-        b.A = pg::panels(P, a.rows, a.rows, a.rows);
-        b.B = W;
-        b.B.rows = l.pack_w ? l.Dp : d.D;
-        b.B.k = d.V;
         b.N = d.D;
         b.k = d.V;
         b.rows_are = 0;
         b.rowmap = (const int *)(ws + l.rowmap) + a.row0;
-        b.bmax = PO == 2 ? &sc->wmax : nullptr;
         b.C = d.dX;
         b.ldc = d.lddx;
-        launch_product<0, 1, PP, PO>(b, plan.width, s);
+        if (l.few) {
+            const FewArgs f{d.X, d.W, d.ldx, d.ldw, b.rowmap, d.D, l.Vp};
+            b.w = few_dx_work(l, d);
+            b.w.part = (float *)(ws + l.sums);
+            if (l.few == 1) launch_few_dx<PP, PO == 1, 1>(b, f, P, s);
+            else if (l.few == 4) launch_few_dx<PP, PO == 1, 4>(b, f, P, s);
+            else launch_few_dx<PP, PO == 1, 8>(b, f, P, s);
+        } else {
+            const pg::Plan plan = dx_plan(l, d, a.rows);
+            b.w = plan.w;
+            b.w.part = (float *)(ws + l.sums);
+            b.cap = dx_cap(plan);
+            b.A = pg::panels(P, a.rows, a.rows, a.rows);
+            b.B = W;
+            b.B.rows = l.pack_w ? l.Dp : d.D;
+            b.B.k = d.V;
+            b.bmax = PO == 2 ? &sc->wmax : nullptr;
+            launch_product<0, 1, PP, PO>(b, plan.width, s);
+        }
     }
     if (d.dW) {
         ProductArgs b = a;
@@ -817,8 +919,8 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
     half_t *Xp = (half_t *)(ws + l.Xp), *Wp = l.pack_w ? (half_t *)(ws + l.Wp) : nullptr;
 
     uint2 *maxes = (uint2 *)(ws + l.maxes);
-    const int scans = d.f16 ? 0 : (int)std::min<int64_t>(((int64_t)d.N + d.V) * ceil_div(d.D, 2048) / 4 + 1, kMaxBlocks);
-    const ScanArgs scan{d.labels, d.N, d.V, d.D, rowmap, pos, lab, sc, (const float *)d.X, (const float *)d.W, d.ldx, d.ldw, maxes};
+    const int Wrows = l.few ? 0 : d.V, scans = d.f16 ? 0 : (int)std::min<int64_t>(((int64_t)d.N + Wrows) * ceil_div(d.D, 2048) / 4 + 1, kMaxBlocks);
+    const ScanArgs scan{d.labels, d.N, d.V, d.D, Wrows, rowmap, pos, lab, sc, (const float *)d.X, (const float *)d.W, d.ldx, d.ldw, maxes};
     hipLaunchKernelGGL(lce_scan_kernel, dim3((unsigned)(1 + scans)), dim3(256), 0, s, scan);
     const dim3 pgrid((unsigned)std::min<int64_t>(((int64_t)d.N + 64 + (l.pack_w ? d.V : 0) + 3) / 4, 4096));
     const int Np = (d.N + 63) & ~63;
@@ -834,22 +936,28 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         a.X = X;
         a.W = W;
         a.V = d.V;
-        a.nk = l.Dp / (l.P == 1 ? 64 : 32);
-        a.w = plan.w;
+        a.nk = l.few ? ceil_div(d.D, few::along_k(d.f16)) : l.Dp / (l.P == 1 ? 64 : 32);
+        a.w = l.few ? few_logits_work(l, d) : plan.w;
         a.w.part = (float *)(ws + l.sums);
         a.sc = sc;
         a.row0 = row0;
         a.rows = rows;
-        a.planes = l.P == 2;
+        a.planes = l.P == 2 && !l.few;
         a.bias = d.bias;
         a.bias16 = d.f16;
         a.lab = lab + row0;
         a.zt = zt + row0;
         a.stats = stats;
-        a.T = 2 * ceil_div(d.V, plan.width);   // two waves side by side in every tile
+        const int wave = l.few ? 32 : plan.width / 2;   // columns of a wave
+        a.T = ceil_div(d.V, l.few ? 128 : plan.width) * (l.few ? 4 : 2);
         a.E = ws + l.E;
         a.Vp = l.Vp;
-        if (l.P == 1) {
+        if (l.few) {
+            const FewArgs f{d.X, d.W, d.ldx, d.ldw, rowmap, d.D, l.Vp};
+            if (l.few == 1) few_logits<1>(a, f, d, l.keep, s);
+            else if (l.few == 4) few_logits<4>(a, f, d, l.keep, s);
+            else few_logits<8>(a, f, d, l.keep, s);
+        } else if (l.P == 1) {
             if (plan.width == 256) logits<pg::Tile256<0, 0, 1, 1>>(a, l.keep, s);
             else if (plan.width == 128) logits<pg::Tile128<0, 0, 1, 1>>(a, l.keep, s);
             else logits<pg::Tile64<0, 0, 1, 1>>(a, l.keep, s);
@@ -861,7 +969,7 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, sc, row0, rows, stats, a.T, zt + row0, rowmap + row0,
                            lse + row0, loss + row0, d.rowloss, d.lse);
         if (!l.grad) continue;
-        const GradArgs g{sc, row0, rows, d.V, l.Vp, a.T, plan.width / 2, stats, lse + row0, zt + row0, lab + row0, ws + l.E, ws + l.Pp,
+        const GradArgs g{sc, row0, rows, d.V, l.Vp, a.T, wave, stats, lse + row0, zt + row0, lab + row0, ws + l.E, ws + l.Pp,
                          d.dbias ? (float *)(ws + l.dbpart) : nullptr};
         const dim3 ggrid((unsigned)ceil_div(l.Vp, 64 * (l.keep == KEEP_EXP ? 8 : 4)), (unsigned)ceil_div(rows, kGradRows));
         if (l.keep == KEEP_EXP) hipLaunchKernelGGL((lce_grad_kernel<KEEP_EXP, 1>), ggrid, dim3(256), 0, s, g);

@@ -224,6 +224,41 @@ def test_strides(dev, dtype, pad):
         v.free()
 
 
+# Around the forms' limits (16, 64, 128 rows; 8 features) and a stage's and a tile's (64 or 128 of either sum, 128 classes, 256 features);
+# long sums are split.
+FEW = [(1, 8, 3), (5, 7, 40), (16, 70, 300), (17, 65, 129), (64, 131, 260), (65, 261, 97), (128, 333, 1030), (129, 333, 1030), (33, 4099, 70), (9, 41, 20011)]
+
+
+@pytest.mark.parametrize("types", TYPES, ids=["f32", "f16", "f16_f32grad"])
+@pytest.mark.parametrize("shape", FEW, ids=lambda s: "%dx%dx%d" % s)
+@pytest.mark.parametrize("pad", [3, 8])
+def test_few_rows_of_any_stride(dev, types, shape, pad):
+    """Few rows and W as it lies: rows that end anywhere, NaN between them and behind the last."""
+    dtype, gdtype = types
+    c = Case(*shape, dtype=dtype, grad_dtype=gdtype, labels=np.where(np.arange(shape[0]) % 5 == 3, -1, np.arange(shape[0]) * 7 % shape[2]))
+    t, ld = NP[gdtype], c.D + pad
+    wide = lambda a: np.concatenate([np.pad(a, ((0, 0), (0, pad)), constant_values=np.nan).ravel(), np.full(64, np.nan, a.dtype)])   # noqa: E731
+    b = {"X": dev.buffer(wide(c.X), dtype), "W": dev.buffer(wide(c.W), dtype), "labels": dev.buffer(c.labels, L.AH_I32), "bias": dev.buffer(c.b, dtype),
+         "loss": dev.buffer(1), "rowloss": dev.buffer(c.N), "dX": dev.buffer(np.full((c.N, ld), 777, t), gdtype),
+         "dW": dev.buffer(np.full((c.V, ld), 777, t), gdtype)}
+    args = dict(dtype=dtype, grad_dtype=gdtype, N=c.N, D=c.D, V=c.V, ldx=ld, ldw=ld, lddx=ld, lddw=ld, grad_scale=256.0 if gdtype == L.AH_F16 else 1.0, **b)
+    ws = dev.buffer(np.full(dev.linear_ce_workspace(**args) // 4 + 4, np.nan, np.float32))
+    dev.linear_ce(ws=ws, **args)
+    dev.sync()
+    dX, dW = b["dX"].read().reshape(c.N, ld), b["dW"].read().reshape(c.V, ld)
+    got = {"loss": b["loss"].read(), "rowloss": b["rowloss"].read(), "dX": dX[:, :c.D].astype(np.float64), "dW": dW[:, :c.D].astype(np.float64)}
+    compare(got, c.exact(grad_scale=args["grad_scale"]))
+    assert np.all(dX[:, c.D:] == 777) and np.all(dW[:, c.D:] == 777)
+    loss = {"loss": dev.buffer(1)}   # and the loss alone
+    for k in ("dX", "dW", "rowloss", "loss"):
+        args.pop(k)
+    dev.linear_ce(ws=ws, **args, **loss)
+    dev.sync()
+    compare({"loss": loss["loss"].read()}, c.exact())
+    for v in list(b.values()) + list(loss.values()) + [ws]:
+        v.free()
+
+
 @pytest.mark.parametrize("types", TYPES, ids=["f32", "f16", "f16_f32grad"])
 def test_repeats_bit_for_bit_in_a_graph(dev, types):
     """Captured, then replayed between other work: the eager call's bits each time, also after new inputs."""

@@ -370,20 +370,35 @@ struct FewArgs {
     int D, Vp;
 };
 template <class C, int KEEP, bool F16>
-__global__ __launch_bounds__(C::NT, 2) void lce_few_logits_kernel(LogitArgs a, FewArgs f) {
-    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
-    if (M == 0) return;
+__device__ __forceinline__ void few_logits(const LogitArgs &a, const FewArgs &f, int M, char *smem) {
     int tile, slot, first, count, m0, n0;
     pg::pick(a.w, blockIdx.x, a.nk, tile, slot, first, count);
     logits_tile<C>(a, tile, m0, n0);
-    __shared__ __attribute__((aligned(16))) char smem[few::smem_bytes<C>()];
     floatx4 acc[C::FA][C::FB];
     few::contract_along<C, F16>(f.X, f.ldx, f.rowmap, M, f.W, f.ldw, a.V, f.D, n0, first, count, smem, acc);
-    if (slot >= 0) {
-        pg::store_partials<C>(a.w.part, slot, acc);
-        return;
-    }
-    logits_rows<C, KEEP, C::FA>(a, M, m0, n0, 0, acc);
+    if (slot >= 0) pg::store_partials<C>(a.w.part, slot, acc);
+    else logits_rows<C, KEEP, C::FA>(a, M, m0, n0, 0, acc);
+}
+// Room for 16 FA rows; the rows that count may be fewer, and then the tile is.
+template <int FA, int KEEP, bool F16>
+__global__ __launch_bounds__(256, 2) void lce_few_logits_kernel(LogitArgs a, FewArgs f) {
+    __shared__ __attribute__((aligned(16))) char smem[few::smem_bytes<few::Tile<FA, 2>>()];
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    if (M == 0) return;
+    few::with_rows<FA>(M, [&](auto fa) { few_logits<few::Tile<fa, 2>, KEEP, F16>(a, f, M, smem); });
+}
+template <int FA, int KEEP>
+__global__ __launch_bounds__(256) void lce_few_logits_join_kernel(LogitArgs a) {
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    if (16 * (int)blockIdx.y >= M) return;
+    few::with_rows<FA>(M, [&](auto fa) {
+        typedef few::Tile<fa, 2> C;
+        int m0, n0;
+        logits_tile<C>(a, a.w.whole + blockIdx.x, m0, n0);
+        floatx4 z[1][C::FB];
+        pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, z[0]);
+        logits_rows<C, KEEP, 1>(a, M, m0, n0, blockIdx.y, z);
+    });
 }
 
 template <class C, int KEEP>
@@ -653,27 +668,31 @@ __global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
 
 // dX from W as it lies, for few rows: one row of tiles.
 template <class C, int PP, bool F16>
-__global__ __launch_bounds__(C::NT, 2) void lce_few_dx_kernel(ProductArgs a, FewArgs f, const char *P) {
-    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
-    if (M == 0) return;
+__device__ __forceinline__ void few_dx(const ProductArgs &a, const FewArgs &f, const char *P, int M, char *smem) {
     int tile, slot, first, count;
     pg::pick(a.w, blockIdx.x, (a.k + few::across_v(PP) - 1) / few::across_v(PP), tile, slot, first, count);
-    __shared__ __attribute__((aligned(16))) char smem[few::smem_bytes<C>()];
     floatx4 acc[C::FA][C::FB];
     few::contract_across<C, PP, F16>(P, a.rows, f.Vp, f.W, f.ldw, a.k, a.N, tile * C::BN, first, count, smem, acc);
-    if (slot >= 0) {
-        pg::store_partials<C>(a.w.part, slot, acc);
-        return;
-    }
-    product_rows<C, C::FA>(a, M, 0, tile * C::BN, 0, acc);
+    if (slot >= 0) pg::store_partials<C>(a.w.part, slot, acc);
+    else product_rows<C, C::FA>(a, M, 0, tile * C::BN, 0, acc);
 }
-template <class C>
-__global__ __launch_bounds__(C::NT) void lce_few_dx_join_kernel(ProductArgs a) {
+template <int FA, int PP, bool F16>
+__global__ __launch_bounds__(256, 2) void lce_few_dx_kernel(ProductArgs a, FewArgs f, const char *P) {
+    __shared__ __attribute__((aligned(16))) char smem[few::smem_bytes<few::Tile<FA, 4>>()];
+    const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
+    if (M == 0) return;
+    few::with_rows<FA>(M, [&](auto fa) { few_dx<few::Tile<fa, 4>, PP, F16>(a, f, P, M, smem); });
+}
+template <int FA>
+__global__ __launch_bounds__(256) void lce_few_dx_join_kernel(ProductArgs a) {
     const int M = chunk_rows(&a.sc->count, a.row0, a.rows);
     if (16 * (int)blockIdx.y >= M) return;
-    floatx4 v[1][C::FB];
-    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, v[0]);
-    product_rows<C, 1>(a, M, 0, (a.w.whole + blockIdx.x) * C::BN, blockIdx.y, v);
+    few::with_rows<FA>(M, [&](auto fa) {
+        typedef few::Tile<fa, 4> C;
+        floatx4 v[1][C::FB];
+        pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, v[0]);
+        product_rows<C, 1>(a, M, 0, (a.w.whole + blockIdx.x) * C::BN, blockIdx.y, v);
+    });
 }
 
 template <class C>
@@ -807,13 +826,12 @@ void logits(const LogitArgs &a, int keep, hipStream_t s) {
 
 template <int FA, bool F16, int KEEP>
 void launch_few_logits(LogitArgs a, const FewArgs &f, hipStream_t s) {
-    typedef few::Tile<FA, 2> C;
     a.tiles_m = 1;
-    hipLaunchKernelGGL((lce_few_logits_kernel<C, KEEP, F16>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a, f);
-    if (a.w.splits > 1) hipLaunchKernelGGL((lce_logits_join_kernel<C, KEEP>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((lce_few_logits_kernel<FA, KEEP, F16>), dim3((unsigned)a.w.blocks()), dim3(256), 0, s, a, f);
+    if (a.w.splits > 1) hipLaunchKernelGGL((lce_few_logits_join_kernel<FA, KEEP>), dim3((unsigned)a.w.rest, FA), dim3(256), 0, s, a);
 }
 template <int FA>
-void few_logits(const LogitArgs &a, const FewArgs &f, const LinearCe &d, int keep, hipStream_t s) {
+void launch_few_logits(const LogitArgs &a, const FewArgs &f, const LinearCe &d, int keep, hipStream_t s) {
     if (!d.f16) keep == KEEP_NONE ? launch_few_logits<FA, false, KEEP_NONE>(a, f, s) : launch_few_logits<FA, false, KEEP_Z>(a, f, s);
     else if (keep == KEEP_NONE) launch_few_logits<FA, true, KEEP_NONE>(a, f, s);
     else if (keep == KEEP_EXP) launch_few_logits<FA, true, KEEP_EXP>(a, f, s);
@@ -822,9 +840,8 @@ void few_logits(const LogitArgs &a, const FewArgs &f, const LinearCe &d, int kee
 
 template <int PP, bool F16, int FA>
 void launch_few_dx(const ProductArgs &a, const FewArgs &f, const char *P, hipStream_t s) {
-    typedef few::Tile<FA, 4> C;
-    hipLaunchKernelGGL((lce_few_dx_kernel<C, PP, F16>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a, f, P);
-    if (a.w.splits > 1) hipLaunchKernelGGL((lce_few_dx_join_kernel<C>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
+    hipLaunchKernelGGL((lce_few_dx_kernel<FA, PP, F16>), dim3((unsigned)a.w.blocks()), dim3(256), 0, s, a, f, P);
+    if (a.w.splits > 1) hipLaunchKernelGGL((lce_few_dx_join_kernel<FA>), dim3((unsigned)a.w.rest, FA), dim3(256), 0, s, a);
 }
 
 template <class C>
@@ -954,9 +971,9 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         a.Vp = l.Vp;
         if (l.few) {
             const FewArgs f{d.X, d.W, d.ldx, d.ldw, rowmap, d.D, l.Vp};
-            if (l.few == 1) few_logits<1>(a, f, d, l.keep, s);
-            else if (l.few == 4) few_logits<4>(a, f, d, l.keep, s);
-            else few_logits<8>(a, f, d, l.keep, s);
+            if (l.few == 1) launch_few_logits<1>(a, f, d, l.keep, s);
+            else if (l.few == 4) launch_few_logits<4>(a, f, d, l.keep, s);
+            else launch_few_logits<8>(a, f, d, l.keep, s);
         } else if (l.P == 1) {
             if (plan.width == 256) logits<pg::Tile256<0, 0, 1, 1>>(a, l.keep, s);
             else if (plan.width == 128) logits<pg::Tile128<0, 0, 1, 1>>(a, l.keep, s);

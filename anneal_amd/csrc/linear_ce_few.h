@@ -20,6 +20,18 @@ struct Tile {
     static constexpr int FA = FA_, FB = FB_, WVM = 1, WVN = 4, NT = 256, WM = 16 * FA, WN = 16 * FB, BM = WM, BN = 4 * WN;
 };
 
+// Calls f with the constant for the smallest of 1, 2, 4, 6 and 8 tiles of 16 rows that hold M, of at most FA.
+template <int FA, class F>
+__device__ __forceinline__ void with_rows(int M, F f) {
+    if constexpr (FA == 1) f(std::integral_constant<int, 1>());
+    else if (M <= 16) f(std::integral_constant<int, 1>());
+    else if (M <= 32) f(std::integral_constant<int, 2>());
+    else if constexpr (FA == 4) f(std::integral_constant<int, 4>());
+    else if (M <= 64) f(std::integral_constant<int, 4>());
+    else if (M <= 96) f(std::integral_constant<int, 6>());
+    else f(std::integral_constant<int, 8>());
+}
+
 // The rows' side of a stage: 256 bytes of each row in LDS, shared by the waves (each wave fetching its own copy through the caches took
 // 984 us, not 432, at 64 rows of 4001 f16 features over 131072 classes). 16-byte pieces are swizzled by the row, so that a fragment's
 // 16 rows lie in different banks. Two buffers, one barrier a stage.
@@ -136,7 +148,7 @@ __device__ __forceinline__ void contract_across(const char *P, long prows, int V
     typedef typename std::conditional<F16, half_t, float>::type T;
     typedef T vec __attribute__((ext_vector_type(4)));
     typedef T vec_any __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    constexpr int NCH = across_v(PP) / 16, PF = C::FA == 8 && !F16 ? 2 : 4;
+    constexpr int NCH = across_v(PP) / 16, PF = C::FA == 8 || (C::FA == 6 && !F16) ? 2 : 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, row = lane & 15;
     const int nw = n0 + wave * C::WN, panels = Vp / (across_v(PP) / 2);
     const T *wp = (const T *)W + min(nw + 4 * (4 * (row & 3) + (row >> 2)), D - 4);

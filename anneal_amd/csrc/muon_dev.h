@@ -79,18 +79,20 @@ __device__ __forceinline__ void store_result(const Muon &d, long z, int r, int c
 
 // Steps of the longest group: |a + b x + c x^2| over what the squared singular values reach bounds a step's growth, and the planes
 // of three steps' Q hold its cube up to 43. A short side under 256 starts with larger singular values of X and has less to average
-// over: three steps at once cost it more than 32-bit products lose (16 x 64: 7 times the error of step by step).
+// over: three steps at once cost it more than 32-bit products lose (16 x 64: 7 times the error of step by step), and under 32 two at
+// once do (8 x 576: 1.6e-6 off, 32-bit products 0.7e-6).
 inline int longest_group(const Muon &d) {
     double grow = 0;
     for (int i = 0; i <= 60; i++) {
         const double x = i * 0.025;
         grow = std::max(grow, std::fabs(d.a + d.b * x + d.c * x * x));
     }
-    return grow <= 3.5 && std::min(d.rows, d.cols) >= 256 ? 3 : grow <= 5.0 ? 2 : 1;
+    const int side = std::min(d.rows, d.cols);
+    return grow <= 3.5 && side >= 256 ? 3 : grow <= 5.0 && side >= 32 ? 2 : 1;
 }
 // Steps of group `index` with `left` to go: 3, 2, 1, 1, .. or 2, 1, 1, .. Of the ways to cut five steps in 32-bit products these
 // stay nearest to step by step over short sides of 8 to 512 and flat and steep spectra (1.1 to 1.7 times its error at 3, 2 from 256
-// on, 1.0 to 1.3 at 2, 1, 1, 1 below; pairs throughout 1.2 to 2.8, other cuts 4 to 40). Step by step in planes has 0.6 (s = 4096) to
+// on, 1.0 to 1.3 at 2, 1, 1, 1 from 32 to there; pairs throughout 1.2 to 2.8, other cuts 4 to 40). Step by step in planes has 0.6 (s = 4096) to
 // 1.5 times (s = 8) the error of 32-bit products.
 inline int group_size(int longest, int index, int left) { return std::min(std::max(1, longest - index), left); }
 

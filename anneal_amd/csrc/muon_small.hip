@@ -77,12 +77,12 @@ __device__ __forceinline__ void multiply(uint32_t a, uint32_t b, int nst, floatx
             for (int j = 0; j < FB; j++) y[s][j] = B::read(bv, j, s);
         }
 #pragma unroll
-        for (int p = 0; p < 3; p++)   // hi hi, lo hi, hi lo
+        for (int p = 0; p < 3; p++)   // lo hi, hi lo, hi hi: the small ones first, so that a sum of 32 is rounded once at its full size
 #pragma unroll
             for (int i = 0; i < FA; i++)
 #pragma unroll
                 for (int j = 0; j < FB; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[p == 2][j], x[p == 1][i], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[p == 1][j], x[p == 0][i], acc[i][j], 0, 0, 0);
     }
 }
 

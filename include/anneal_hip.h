@@ -314,7 +314,8 @@ int ah_chain_step_noalloc(ah_device *dev, const float *X, const float *g, int32_
 /* ── The ends of a language model's training step ─────────────────────────────
  * No counterpart in the reference (no softmax, no cross-entropy and no update rule but SGD: tensor/nn/nn.go:69-106). All calls
  * are asynchronous on the device stream and allocate nothing, so they can be captured by ah_graph_begin; each takes a workspace
- * of the caller's, whose size the *_workspace call gives for the same descriptor (pointers set or not as in the call). The workspace needs 16-byte
+ * of the caller's, whose size the *_workspace call gives for the same descriptor (pointers set or not, and W at a multiple
+ * of 16 bytes or not, as in the call). The workspace needs 16-byte
  * alignment and no particular contents; calls of one device handle may share one. Graphs hold its address.
  *
  * Softmax cross-entropy of a linear head, without keeping the logits. X [N,D], W [V,D], bias [V] (may be null), labels [N]:

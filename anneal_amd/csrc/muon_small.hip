@@ -32,8 +32,8 @@ struct SmallArgs {
     float *out;
     const double *part;    // first kernel: sums of squares
     int parts;
-    int steps;             // of the group
-    float qi, qs;          // the group's polynomial is qi I + Q; 1 / the scale of Q's planes
+    int steps;             // of the group, 1 or 2
+    float qi;              // the group's polynomial is qi I + Q
 };
 
 // Byte offsets in an image of R rows: four values at row r, k c (T = 0), or at k r, row c (T = 1). The lo plane is at the offset xor 64.
@@ -214,8 +214,7 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
             for (int i = 0; i < FQ; i++)
 #pragma unroll
                 for (int j = 0; j < FQ; j++) Q[i][j] = B[i][j];
-            float qi = ca, sq = 1.0f;   // Q's planes hold 2^kSB sq Q
-            for (int g = 1; g < p.steps; g++) {
+            if (p.steps == 2) {
                 Square P;
                 put(square_img, B);   // nothing reads image 1 here
                 __syncthreads();
@@ -232,19 +231,12 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
                 put(slice_img, Q);
                 put(square_img, B);
                 __syncthreads();
-                const float to = g == 2 ? 0.25f : 1.0f;   // three steps' Q is up to 43: planes of 2^9
-                product(1, 0, to / (1 << kSB), Q, to * ca, B, to * sq * qi, Q);
-                qi *= ca;
-                sq *= to;
-                if (g + 1 < p.steps) {
-                    __syncthreads();
-                    put(slice_img, A);
-                }
+                product(1, 0, 1.0f / (1 << kSB), Q, ca, B, ca, Q);
             }
             __syncthreads();
             put(square_img, Q);
         }
-        const float qi = p.qi, qs = p.qs;
+        const float qi = p.qi, qs = 1.0f / (1 << kSB);
         for (int sl = blockIdx.x; sl < p.slices; sl += p.groups) {
             const int m0 = WIDE ? 0 : sl * kSlice, n0 = WIDE ? sl * kSlice : 0;
             __syncthreads();   // B is there; the slice image has been read
@@ -357,7 +349,6 @@ void run(const Muon &d, SmallArgs a, float *const (&parts)[2], hipStream_t s) {
         a.steps = group_size(longest_group(d), k, left);
         left -= a.steps;
         a.qi = (float)std::pow((double)d.a, a.steps);
-        a.qs = std::ldexp(1.0f, a.steps == 3 ? -(kSB - 2) : -kSB);
         a.in = parts[k & 1];
         a.out = parts[(k + 1) & 1];
         if (left) hipLaunchKernelGGL((muon_small_kernel<S, WIDE, STEP>), grid, dim3(S / 32 * (S / 32) * 64), 0, s, a, d);

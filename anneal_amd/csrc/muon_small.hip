@@ -60,8 +60,10 @@ __device__ __forceinline__ floatx4 image_load(const char *img, int off) {
     return v;
 }
 
-// acc += the products of nst stages of two images; a, b: LDS addresses of the wave's first fragments.
-template <int RA, int TA, int RB, int TB, int FA, int FB>
+// acc += the products of nst stages of two images; a, b: LDS addresses of the wave's first fragments. The small products come first, so
+// that a sum of 32 is rounded once at its full size. NP = 4: lo lo is one of them, which sums as short as a side under 64 show (0.85 of
+// the error of an 8 x 25 without; at 128 it would take 95 us, not 90, for 128 x 784 and show nothing).
+template <int NP, int RA, int TA, int RB, int TB, int FA, int FB>
 __device__ __forceinline__ void multiply(uint32_t a, uint32_t b, int nst, floatx4 (&acc)[FA][FB]) {
     using A = pg::PFrag<RA, TA, 2, 32>;
     using B = pg::PFrag<RB, TB, 2, 32>;
@@ -77,12 +79,12 @@ __device__ __forceinline__ void multiply(uint32_t a, uint32_t b, int nst, floatx
             for (int j = 0; j < FB; j++) y[s][j] = B::read(bv, j, s);
         }
 #pragma unroll
-        for (int p = 0; p < 3; p++)   // lo hi, hi lo, hi hi: the small ones first, so that a sum of 32 is rounded once at its full size
+        for (int p = 4 - NP; p < 4; p++)   // lo lo, lo hi, hi lo, hi hi
 #pragma unroll
             for (int i = 0; i < FA; i++)
 #pragma unroll
                 for (int j = 0; j < FB; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[p == 1][j], x[p == 0][i], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y[p == 0 || p == 2][j], x[p < 2][i], acc[i][j], 0, 0, 0);
     }
 }
 
@@ -101,7 +103,7 @@ enum { FIRST = 0, STEP = 1, LAST = 2 };
 // 64 x 64 a step of 128 x 784 took 20 us, not 16).
 template <int S, bool WIDE, int WHAT>
 __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(SmallArgs p, Muon d) {
-    constexpr int WV = S / 32, NT = WV * WV * 64;
+    constexpr int WV = S / 32, NT = WV * WV * 64, NP = S == 64 ? 4 : 3;   // (NP: products of planes)
     constexpr int FQ = 2;                                               // 16-row blocks a wave holds of a side of S
     constexpr int XM = WIDE ? S : kSlice, XN = WIDE ? kSlice : S;       // a slice of X
     constexpr int FM = XM / WV / 16, FN = XN / WV / 16;
@@ -127,13 +129,13 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
             f.init(slice_lds, wr * (S / WV), lane);
             const uint32_t a = f.first;
             f.init(slice_lds, wc * (S / WV), lane);
-            multiply<S, 0, S, 0>(a, f.first, kSlice / 32, gram);
+            multiply<NP, S, 0, S, 0>(a, f.first, kSlice / 32, gram);
         } else {
             pg::PFrag<S, 1, 2, 32> f;
             f.init(slice_lds, wr * (S / WV), lane);
             const uint32_t a = f.first;
             f.init(slice_lds, wc * (S / WV), lane);
-            multiply<S, 1, S, 1>(a, f.first, kSlice / 32, gram);
+            multiply<NP, S, 1, S, 1>(a, f.first, kSlice / 32, gram);
         }
     };
     const auto slice_at = [&](int m, int n) { return WIDE ? image0<S>(m, n) : image1<S>(m, n); };   // of the image that add_gram reads
@@ -168,7 +170,7 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
             const auto product = [&](int left, int right, float k, Square &p1, float k1, Square &p2, float k2, Square &v) {
                 Square t;
                 clear(t);
-                multiply<S, 0, S, 0>(row[left], col[right], S / 32, t);
+                multiply<NP, S, 0, S, 0>(row[left], col[right], S / 32, t);
 #pragma unroll
                 for (int i = 0; i < FQ; i++)
 #pragma unroll
@@ -260,13 +262,13 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
                 pg::PFrag<kSlice, 1, 2, 32> fx;
                 fb.init(square_lds, wr * (S / WV), lane);
                 fx.init(slice_lds, wc * (kSlice / WV), lane);
-                multiply<S, 0, kSlice, 1>(fb.first, fx.first, S / 32, x);
+                multiply<NP, S, 0, kSlice, 1>(fb.first, fx.first, S / 32, x);
             } else {
                 pg::PFrag<kSlice, 0, 2, 32> fx;
                 pg::PFrag<S, 0, 2, 32> fb;
                 fx.init(slice_lds, wr * (kSlice / WV), lane);
                 fb.init(square_lds, wc * (S / WV), lane);
-                multiply<kSlice, 0, S, 0>(fx.first, fb.first, S / 32, x);
+                multiply<NP, kSlice, 0, S, 0>(fx.first, fb.first, S / 32, x);
             }
 #pragma unroll
             for (int i = 0; i < FM; i++)

@@ -5,15 +5,14 @@
 //
 // The counted rows of X are gathered first (rows whose label is outside [0, V) cost nothing after that, and whatever they hold
 // stays out of the products), then worked on in pieces of rows. Per piece: the logits' product, whose epilogue keeps each row's
-// maximum and sum of exponentials per wave tile of the vocabulary and writes only exp(z - tile maximum) (f16 gradients) or z
-// (f32 gradients) of the piece; one pass that joins the statistics of a row; one pass that turns the piece into P in place; the
-// two gradient products. Keeping one piece costs 2 or 4 bytes of traffic five times per logit; computing it again would cost a
-// third product, 2 D operations per logit: at D = 1024 and 1 PFLOP/s that is 2 ps against 2 ps at 5 TB/s, and the gap widens
-// with D.
+// maximum and sum of exponentials per wave tile of the vocabulary and writes the piece's logits; one pass that joins the statistics of
+// a row; one pass that turns the piece into P in place; the two gradient products. Keeping a logit moves 14 (f16 gradients) or 20
+// bytes, computing it again would cost a third product, 2 D operations: at 5 TB/s and 1 PFLOP/s the two are even at D = 1400 and 2000, but
+// only 8 of the bytes stand outside a product that hides them (at 4096 x 4096 x 131072 P's pass is 4% of the time).
 //
 // Precision. f16 operands are exact in the products; f32 operands are carried as two f16 planes scaled by a power of two taken
-// from their largest magnitude (plane_gemm.h). P goes into the gradient products as 2^15 P in one f16 plane for f16 gradients
-// (relative 2^-12 for |P| above 2^-29, and a floor of 2^-40) and in two for f32 gradients (2^-23 above 2^-17, floor 2^-40).
+// from their largest magnitude (plane_gemm.h). P is formed in f32 and goes into the gradient products as 2^15 P in one f16 plane for f16
+// gradients (one rounding, 2^-11 of |P| above 2^-29 at most, 2^-40 below) and in two for f32 gradients (2^-22 above 2^-18, 2^-40 below).
 // Statistics, losses and sums are f32; sums over rows and pieces run in a fixed order, so results repeat bit for bit.
 #include "linear_ce.h"
 
@@ -239,7 +238,7 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, i
 
 // ── the logits' product ────────────────────────────────────────────────────────
 
-enum { KEEP_NONE = 0, KEEP_EXP = 1, KEEP_Z = 2 };
+enum { KEEP_NONE = 0, KEEP_Z = 1 };
 
 struct LogitArgs {
     pg::Operand X, W;
@@ -254,11 +253,12 @@ struct LogitArgs {
     float *zt;            // each row's logit of its label
     float2 *stats;        // [rows][T]: maximum and sum of exponentials of each wave tile's columns
     int T;
-    char *E;              // the piece in panels of 128 bytes: exp(z - tile maximum) 2^15 in f16, or z in f32
+    char *E;              // the piece's logits in panels of 128 bytes, 32 columns each
     int Vp;
 };
 
-// Bytes to an f32 logit of the piece: 32 columns fill a panel's row, as the planes that replace them do.
+// Bytes to a logit of the piece: 32 columns fill a panel's row, as the two planes that replace them do (one plane of 64 columns fills
+// every other panel).
 __device__ __forceinline__ long z_at(long rows, long r, long c) { return ((c >> 5) * rows + r) * 128 + (c & 31) * 4; }
 
 // Tiles are walked down the rows first: the tiles of one run share their columns of W, the larger operand.
@@ -288,10 +288,9 @@ __device__ __forceinline__ void logits_rows(const LogitArgs &a, int M, int m0, i
             const int n = at.n + 16 * j + r;
             bias[j][r] = n >= a.V ? ninf : !a.bias ? 0.0f : a.bias16 ? (float)((const half_t *)a.bias)[n] : ((const float *)a.bias)[n];
         }
-    // this lane's first column in E; 16 j columns on are (j & pm) further in the panel and j / (pm + 1) panels on
-    constexpr int LOG = KEEP == KEEP_EXP ? 6 : 5, PM = (1 << (LOG - 4)) - 1, SZ = KEEP == KEEP_EXP ? 2 : 4;
+    // this lane's first column in E; 16 j columns on are 64 (j & 1) bytes further in the panel and j / 2 panels on
     const int nw = n0 + (at.wave % C::WVN) * C::WN;
-    char *const tile = KEEP == KEEP_NONE ? nullptr : a.E + ((long)(nw >> LOG) * a.rows + m0) * 128 + (nw & ((1 << LOG) - 1)) * SZ;
+    char *const tile = KEEP == KEEP_NONE ? nullptr : a.E + z_at(a.rows, m0, nw);
     const uint32_t panel = (uint32_t)a.rows * 128;
 #pragma unroll
     for (int i = 0; i < NR; i++) {
@@ -318,26 +317,13 @@ __device__ __forceinline__ void logits_rows(const LogitArgs &a, int M, int m0, i
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         const float ref = mx == ninf ? 0.0f : mx;   // columns that are all -inf (a bias that rules them out) add nothing
         float sum = 0.0f;
-        const uint32_t off = (uint32_t)(m - m0) * 128 + 4 * (at.lane >> 4) * SZ;
+        const uint32_t off = (uint32_t)(m - m0) * 128 + (at.lane >> 4) * 16;
 #pragma unroll
         for (int j = 0; j < C::FB; j++) {
-            floatx4 ex;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                ex[r] = __builtin_amdgcn_exp2f((z[i][j][r] - ref) * kLog2e);
-                sum += ex[r];
-            }
-            if (KEEP != KEEP_NONE && m < M && (whole || at.n + 16 * j < a.Vp)) {
-                char *p = tile + (off + (uint32_t)(j / (PM + 1)) * panel) + (j & PM) * 16 * SZ;
-                if constexpr (KEEP == KEEP_EXP) {
-                    h4 h;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) h[r] = (half_t)(ex[r] * (float)(1 << kPScale));
-                    *(h4 *)p = h;
-                } else {
-                    *(floatx4 *)p = z[i][j];
-                }
-            }
+            for (int r = 0; r < 4; r++) sum += __builtin_amdgcn_exp2f((z[i][j][r] - ref) * kLog2e);
+            if (KEEP != KEEP_NONE && m < M && (whole || at.n + 16 * j < a.Vp))
+                *(floatx4 *)(tile + (off + (uint32_t)(j / 2) * panel) + (j & 1) * 64) = z[i][j];
         }
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
@@ -452,15 +438,14 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(const Scalars *sc, int ro
 
 struct GradArgs {
     const Scalars *sc;
-    int row0, rows, V, Vp, T, WN;   // WN: columns of a statistics tile
-    const float2 *stats;
+    int row0, rows, V, Vp;
     const float *lse, *zt;
     const int *lab;
-    char *E, *P;                    // what the product kept; P: E itself, or where one plane made of z goes
+    char *E;                        // the logits, then P
     float *dbpart;                  // [row block][V] column sums of P, or null
 };
 
-// e^x for f32 gradients: the product with log2 e carries what its rounding loses, which at x = -10 is 3e-7 of the result.
+// e^x: the product with log2 e carries what its rounding loses, which at x = -10 is 3e-7 of the result.
 __device__ __forceinline__ float exp_of(float x) {
     const float t = x * kLog2e, low = fmaf(x, kLog2e, -t) + x * 1.925963033500e-8f;   // log2 e less its f32 value
     const float r = __builtin_amdgcn_exp2f(t);
@@ -469,11 +454,12 @@ __device__ __forceinline__ float exp_of(float x) {
 
 constexpr int kGradRows = 64;       // rows of a block; also the k of a one-plane stage, up to which rows are cleared
 
-// A thread owns 8 (f16 kept) or 4 (f32 kept) columns, 8 threads a panel's 128 bytes of a row, and walks down kGradRows / 4 rows.
-// The in-place change of z to planes is sound because those 128 bytes belong to one wave, whose loads return before it stores.
-template <int KEEP, int PLANES>
+// A thread owns 4 columns, 8 threads a panel's 128 bytes of a row, and walks down kGradRows / 4 rows. The change in place is sound
+// because the 128 bytes of planes, or the 256 of 64 columns that one plane takes half of, belong to one wave, whose loads return before
+// it stores.
+template <int PLANES>
 __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
-    constexpr int NC = KEEP == KEEP_EXP ? 8 : 4;
+    constexpr int NC = 4;
     __shared__ float red[3][64][NC];
     const int M = chunk_rows(&a.sc->count, a.row0, a.rows), Mp = (M + 63) & ~63;
     const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * NC, w = threadIdx.x >> 6;
@@ -481,50 +467,32 @@ __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
     if (r0 >= Mp) return;
     float col[NC] = {};
     if (n < a.Vp) {
-        const int t = min(n / a.WN, a.T - 1);
         for (int k = w; k < kGradRows; k += 4) {
             const int m = r0 + k;
-            float p[NC];
-            char *at = a.E + (KEEP == KEEP_EXP ? pg::panel_at<1>(a.rows, m, n) * 2 : z_at(a.rows, m, n));
+            floatx4 p = {};
+            char *at = a.E + z_at(a.rows, m, n);
             if (m < M) {
                 const float lse = a.lse[m];
                 const int y = a.lab[m] - n;
-                if constexpr (KEEP == KEEP_EXP) {
-                    const float mt = a.stats[(long)m * a.T + t].x;
-                    const float f = mt == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((mt - lse) * kLog2e);
-                    const h8 v = *(const h8 *)at;
+                const floatx4 z = *(const floatx4 *)at;
 #pragma unroll
-                    for (int c = 0; c < NC; c++) p[c] = (float)v[c] * f;
-                } else {
-                    const floatx4 z = *(const floatx4 *)at;
-#pragma unroll
-                    for (int c = 0; c < NC; c++) p[c] = exp_of(z[c] - lse) * (float)(1 << kPScale);
-                }
+                for (int c = 0; c < NC; c++) p[c] = exp_of(z[c] - lse) * (float)(1 << kPScale);
                 if ((unsigned)y < (unsigned)NC) {
                     const float q = expm1f(a.zt[m] - lse) * (float)(1 << kPScale);
 #pragma unroll
                     for (int c = 0; c < NC; c++)
                         if (c == y) p[c] = q;
                 }
-            } else {
-#pragma unroll
-                for (int c = 0; c < NC; c++) p[c] = 0.0f;
             }
 #pragma unroll
             for (int c = 0; c < NC; c++) col[c] += p[c];
-            if constexpr (KEEP == KEEP_EXP) {
-                h8 h;
-#pragma unroll
-                for (int c = 0; c < NC; c++) h[c] = (half_t)p[c];
-                *(h8 *)at = h;
-            } else if constexpr (PLANES == 1) {
+            if constexpr (PLANES == 1) {
                 h4 h;
 #pragma unroll
                 for (int c = 0; c < NC; c++) h[c] = (half_t)p[c];
-                *(h4 *)((half_t *)a.P + pg::panel_at<1>(a.rows, m, n)) = h;
+                *(h4 *)((half_t *)a.E + pg::panel_at<1>(2l * a.rows, m, n)) = h;
             } else {
-                floatx4 v = {p[0], p[1], p[2], p[3]};
-                pg::plane_store((half_t *)a.P + pg::panel_at<2>(a.rows, m, n), v);
+                pg::plane_store((half_t *)a.E + pg::panel_at<2>(a.rows, m, n), p);
             }
         }
     }
@@ -672,7 +640,7 @@ __device__ __forceinline__ void few_dx(const ProductArgs &a, const FewArgs &f, c
     int tile, slot, first, count;
     pg::pick(a.w, blockIdx.x, (a.k + few::across_v(PP) - 1) / few::across_v(PP), tile, slot, first, count);
     floatx4 acc[C::FA][C::FB];
-    few::contract_across<C, PP, F16>(P, a.rows, f.Vp, f.W, f.ldw, a.k, a.N, tile * C::BN, first, count, smem, acc);
+    few::contract_across<C, PP, F16>(P, PP == 1 ? 2l * a.rows : a.rows, f.Vp, f.W, f.ldw, a.k, a.N, tile * C::BN, first, count, smem, acc);
     if (slot >= 0) pg::store_partials<C>(a.w.part, slot, acc);
     else product_rows<C, C::FA>(a, M, 0, tile * C::BN, 0, acc);
 }
@@ -709,7 +677,7 @@ __global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) 
 
 // ── host ───────────────────────────────────────────────────────────────────────
 
-constexpr int kPieceMb = 2048;   // MiB of kept exponentials or logits: one piece holds 8192 rows of 131072 f16 exponentials
+constexpr int kPieceMb = 2048;   // MiB of kept logits: one piece holds 4096 rows of 131072 classes
 constexpr int kMaxPieceRows = 1 << 20;          // a panel's offsets stay within 32 bits
 // Rows up to which a W that would have to be packed is read as it lies. 4096 features, 32000 classes in f32, with gradients, packed and as
 // it lies: 16 rows 731 and 438 us, 128 rows 823 and 850; the loss alone 433 and 139 us at 16 rows, 545 and 367 at 121 (2944 x 51416).
@@ -717,12 +685,12 @@ constexpr int kFewRows = 128;
 constexpr int kStatCols = 32;                  // the narrowest wave tile: bounds the statistics' columns
 
 struct Layout {
-    int Dp, Vp, P, KE;         // padded widths; planes of X and W; bytes of a kept logit (and of the P that takes its place)
-    int keep, PP;              // what the logits' product keeps; planes of P
+    int Dp, Vp, P;             // padded widths; planes of X and W
+    int PP;                    // planes of P, which takes the logits' place
     int rows, pieces;          // rows of a piece
     bool pack_w, grad;
     int few;                   // 16-row tiles of the form for few rows, or 0
-    int64_t maxes, rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, Pp, dbpart, dwacc, sums, total;
+    int64_t maxes, rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, dbpart, dwacc, sums, total;
 };
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -757,10 +725,7 @@ Layout layout(const LinearCe &d) {
     l.Vp = (d.V + 63) & ~63;
     l.P = d.f16 ? 1 : 2;
     l.grad = d.dX || d.dW || d.dbias;
-    // f16 gradients make do with exp(z - maximum) in f16; db, which is f32, takes the logits themselves
-    l.keep = !l.grad ? KEEP_NONE : d.g16 && !d.dbias ? KEEP_EXP : KEEP_Z;
     l.PP = d.g16 ? 1 : 2;
-    l.KE = l.keep == KEEP_NONE ? 0 : l.keep == KEEP_EXP ? 2 : d.g16 ? 6 : 4;
     l.pack_w = !d.f16 || d.D % 8 || d.ldw % 8 || ((uintptr_t)d.W & 15) || d.ldw > 1 << 22;
     if (l.pack_w && d.N <= kFewRows && d.D >= 8) {
         l.pack_w = false;
@@ -768,7 +733,7 @@ Layout layout(const LinearCe &d) {
     }
     const int64_t Np = ((int64_t)d.N + 63) & ~63ll;
     int64_t rows = Np;
-    if (l.KE) rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, ((int64_t)(d.piece_mb ? d.piece_mb : kPieceMb) << 20) / ((int64_t)l.Vp * l.KE) / 256 * 256)});
+    if (l.grad) rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, ((int64_t)(d.piece_mb ? d.piece_mb : kPieceMb) << 20) / ((int64_t)l.Vp * 4) / 256 * 256)});
     else rows = std::min<int64_t>(rows, 16384);
     l.pieces = (int)((Np + rows - 1) / rows);
     if (l.pieces > 1) rows = ((Np + l.pieces - 1) / l.pieces + 255) / 256 * 256;
@@ -791,8 +756,7 @@ Layout layout(const LinearCe &d) {
     l.stats = take(rows * ((l.Vp + 255) / 256 * 256 / kStatCols) * 8);
     l.Xp = take(Np * l.Dp * 2 * l.P);
     if (l.pack_w) l.Wp = take((int64_t)d.V * l.Dp * 2 * l.P);
-    if (l.KE) l.E = l.Pp = take(rows * l.Vp * std::min(l.KE, 4));
-    if (l.KE == 6) l.Pp = take(rows * l.Vp * 2);
+    if (l.grad) l.E = take(rows * l.Vp * 4);
     if (d.dbias) l.dbpart = take(Np / kGradRows * d.V * 4);
     if (d.dW && d.g16 && l.pieces > 1) l.dwacc = take((int64_t)d.V * d.D * 4);
     int64_t sums = 0;
@@ -818,10 +782,8 @@ void launch_logits(LogitArgs a, hipStream_t s) {
 }
 
 template <class C>
-void logits(const LogitArgs &a, int keep, hipStream_t s) {
-    if (keep == KEEP_NONE) launch_logits<C, KEEP_NONE>(a, s);
-    else if (keep == KEEP_Z) launch_logits<C, KEEP_Z>(a, s);
-    else if constexpr (C::PA == 1) launch_logits<C, KEEP_EXP>(a, s);
+void logits(const LogitArgs &a, bool keep, hipStream_t s) {
+    keep ? launch_logits<C, KEEP_Z>(a, s) : launch_logits<C, KEEP_NONE>(a, s);
 }
 
 template <int FA, bool F16, int KEEP>
@@ -831,11 +793,9 @@ void launch_few_logits(LogitArgs a, const FewArgs &f, hipStream_t s) {
     if (a.w.splits > 1) hipLaunchKernelGGL((lce_few_logits_join_kernel<FA, KEEP>), dim3((unsigned)a.w.rest, FA), dim3(256), 0, s, a);
 }
 template <int FA>
-void launch_few_logits(const LogitArgs &a, const FewArgs &f, const LinearCe &d, int keep, hipStream_t s) {
-    if (!d.f16) keep == KEEP_NONE ? launch_few_logits<FA, false, KEEP_NONE>(a, f, s) : launch_few_logits<FA, false, KEEP_Z>(a, f, s);
-    else if (keep == KEEP_NONE) launch_few_logits<FA, true, KEEP_NONE>(a, f, s);
-    else if (keep == KEEP_EXP) launch_few_logits<FA, true, KEEP_EXP>(a, f, s);
-    else launch_few_logits<FA, true, KEEP_Z>(a, f, s);
+void launch_few_logits(const LogitArgs &a, const FewArgs &f, const LinearCe &d, bool keep, hipStream_t s) {
+    if (d.f16) keep ? launch_few_logits<FA, true, KEEP_Z>(a, f, s) : launch_few_logits<FA, true, KEEP_NONE>(a, f, s);
+    else keep ? launch_few_logits<FA, false, KEEP_Z>(a, f, s) : launch_few_logits<FA, false, KEEP_NONE>(a, f, s);
 }
 
 template <int PP, bool F16, int FA>
@@ -863,7 +823,8 @@ void launch_product(const ProductArgs &a, int width, hipStream_t s) {
 template <int PP, int PO>
 void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Operand &W, const pg::Operand &X, int piece, char *ws, hipStream_t s) {
     const Scalars *sc = (const Scalars *)ws;
-    const char *P = ws + l.Pp;
+    const char *P = ws + l.E;
+    const int prows = PP == 1 ? 2 * a.rows : a.rows;   // rows that P's panels are apart
     if (d.dX) {
         ProductArgs b = a;
         b.N = d.D;
@@ -884,7 +845,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
             b.w = plan.w;
             b.w.part = (float *)(ws + l.sums);
             b.cap = dx_cap(plan);
-            b.A = pg::panels(P, a.rows, a.rows, a.rows);
+            b.A = pg::panels(P, prows, a.rows, a.rows);
             b.B = W;
             b.B.rows = l.pack_w ? l.Dp : d.D;
             b.B.k = d.V;
@@ -897,7 +858,7 @@ void gradients(const LinearCe &d, const Layout &l, ProductArgs a, const pg::Oper
         const pg::Plan plan = dw_plan(l, d, a.rows);
         b.w = plan.w;
         b.w.part = (float *)(ws + l.sums);
-        b.A = pg::panels(P, a.rows, l.Vp, a.rows);
+        b.A = pg::panels(P, prows, l.Vp, a.rows);
         b.B = X;
         b.B.rows = l.Dp;
         b.B.k = a.rows;
@@ -965,33 +926,30 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         a.lab = lab + row0;
         a.zt = zt + row0;
         a.stats = stats;
-        const int wave = l.few ? 32 : plan.width / 2;   // columns of a wave
         a.T = ceil_div(d.V, l.few ? 128 : plan.width) * (l.few ? 4 : 2);
         a.E = ws + l.E;
         a.Vp = l.Vp;
         if (l.few) {
             const FewArgs f{d.X, d.W, d.ldx, d.ldw, rowmap, d.D, l.Vp};
-            if (l.few == 1) launch_few_logits<1>(a, f, d, l.keep, s);
-            else if (l.few == 4) launch_few_logits<4>(a, f, d, l.keep, s);
-            else launch_few_logits<8>(a, f, d, l.keep, s);
+            if (l.few == 1) launch_few_logits<1>(a, f, d, l.grad, s);
+            else if (l.few == 4) launch_few_logits<4>(a, f, d, l.grad, s);
+            else launch_few_logits<8>(a, f, d, l.grad, s);
         } else if (l.P == 1) {
-            if (plan.width == 256) logits<pg::Tile256<0, 0, 1, 1>>(a, l.keep, s);
-            else if (plan.width == 128) logits<pg::Tile128<0, 0, 1, 1>>(a, l.keep, s);
-            else logits<pg::Tile64<0, 0, 1, 1>>(a, l.keep, s);
+            if (plan.width == 256) logits<pg::Tile256<0, 0, 1, 1>>(a, l.grad, s);
+            else if (plan.width == 128) logits<pg::Tile128<0, 0, 1, 1>>(a, l.grad, s);
+            else logits<pg::Tile64<0, 0, 1, 1>>(a, l.grad, s);
         } else {
-            if (plan.width == 256) logits<pg::Tile256<0, 0, 2, 2>>(a, l.keep, s);
-            else if (plan.width == 128) logits<pg::Tile128<0, 0, 2, 2>>(a, l.keep, s);
-            else logits<pg::Tile64<0, 0, 2, 2>>(a, l.keep, s);
+            if (plan.width == 256) logits<pg::Tile256<0, 0, 2, 2>>(a, l.grad, s);
+            else if (plan.width == 128) logits<pg::Tile128<0, 0, 2, 2>>(a, l.grad, s);
+            else logits<pg::Tile64<0, 0, 2, 2>>(a, l.grad, s);
         }
         hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, sc, row0, rows, stats, a.T, zt + row0, rowmap + row0,
                            lse + row0, loss + row0, d.rowloss, d.lse);
         if (!l.grad) continue;
-        const GradArgs g{sc, row0, rows, d.V, l.Vp, a.T, wave, stats, lse + row0, zt + row0, lab + row0, ws + l.E, ws + l.Pp,
-                         d.dbias ? (float *)(ws + l.dbpart) : nullptr};
-        const dim3 ggrid((unsigned)ceil_div(l.Vp, 64 * (l.keep == KEEP_EXP ? 8 : 4)), (unsigned)ceil_div(rows, kGradRows));
-        if (l.keep == KEEP_EXP) hipLaunchKernelGGL((lce_grad_kernel<KEEP_EXP, 1>), ggrid, dim3(256), 0, s, g);
-        else if (l.PP == 1) hipLaunchKernelGGL((lce_grad_kernel<KEEP_Z, 1>), ggrid, dim3(256), 0, s, g);
-        else hipLaunchKernelGGL((lce_grad_kernel<KEEP_Z, 2>), ggrid, dim3(256), 0, s, g);
+        const GradArgs g{sc, row0, rows, d.V, l.Vp, lse + row0, zt + row0, lab + row0, ws + l.E, d.dbias ? (float *)(ws + l.dbpart) : nullptr};
+        const dim3 ggrid((unsigned)ceil_div(l.Vp, 256), (unsigned)ceil_div(rows, kGradRows));
+        if (l.PP == 1) hipLaunchKernelGGL(lce_grad_kernel<1>, ggrid, dim3(256), 0, s, g);
+        else hipLaunchKernelGGL(lce_grad_kernel<2>, ggrid, dim3(256), 0, s, g);
         ProductArgs p{};
         p.sc = sc;
         p.row0 = row0;

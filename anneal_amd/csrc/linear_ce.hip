@@ -12,7 +12,8 @@
 //
 // Precision. f16 operands are exact in the products; f32 operands are carried as two f16 planes scaled by a power of two taken
 // from their largest magnitude (plane_gemm.h). P is formed in f32 and goes into the gradient products as 2^15 P in one f16 plane for f16
-// gradients (one rounding, 2^-11 of |P| above 2^-29 at most, 2^-40 below) and in two for f32 gradients (2^-22 above 2^-18, 2^-40 below).
+// gradients (one rounding, 2^-11 of |P| above 2^-29 at most, 2^-40 below; what it leaves at the label, mostly the largest entry, is added apart:
+// add_label_rows, add_labelled) and in two for f32 gradients (2^-22 above 2^-18, 2^-40 below).
 // Statistics, losses and sums are f32; sums over rows and pieces run in a fixed order, so results repeat bit for bit.
 #include "linear_ce.h"
 
@@ -442,6 +443,7 @@ struct GradArgs {
     const float *lse, *zt;
     const int *lab;
     char *E;                        // the logits, then P
+    float *res;                     // one plane: what its rounding leaves of each row's P at its label
     float *dbpart;                  // [row block][V] column sums of P, or null
 };
 
@@ -482,6 +484,7 @@ __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
 #pragma unroll
                     for (int c = 0; c < NC; c++)
                         if (c == y) p[c] = q;
+                    if constexpr (PLANES == 1) a.res[m] = q - (float)(half_t)q;
                 }
             }
 #pragma unroll
@@ -558,6 +561,11 @@ struct ProductArgs {
     const float *acc_in;   // dW: the earlier pieces' sum, or null
     float *acc_out;        // dW: the sum goes there in f32 and C is left, or null
     long ldacc;
+    // P in one plane: what its rounding left of each of the piece's rows at its label, the labels, and W as it lies
+    const float *res;
+    const int *lab;
+    const half_t *W;
+    long ldw;
 };
 
 __device__ __forceinline__ int product_size(const ProductArgs &a, int &nk, int BK) {
@@ -616,6 +624,101 @@ __device__ __forceinline__ void product_rows(const ProductArgs &a, int M, int m0
         if (row[i] >= 0) product_row<C>(a, m1 + 16 * i, row[i], n0, mult, e, acc[i]);
 }
 
+// P at the label is near -1 in most rows while the others are small, so in one plane its rounding (2^-11 of it at most) is most of what a
+// gradient is off by: 1.4e-4 beside the 2.1e-4 of an f16 output's own rounding. What is left of it there, res, is added to the products.
+// dX: row m gets res times the label's row of W, from the workgroup that has that class in its k range [k0, k1).
+template <class C>
+__device__ __forceinline__ void add_label_rows(const ProductArgs &a, int M, int m0, int n0, int k0, int k1, floatx4 (&acc)[C::FA][C::FB]) {
+    const pg::Place<C> at(m0, n0);
+    int y[C::FA];
+    float res[C::FA];
+#pragma unroll
+    for (int i = 0; i < C::FA; i++) {   // all together, for one wait
+        const int m = min(at.m + 16 * i, M - 1);
+        y[i] = a.lab[m];
+        res[i] = a.res[m];
+    }
+#pragma unroll
+    for (int i = 0; i < C::FA; i++) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (at.m + 16 * i >= M || y[i] < k0 || y[i] >= k1) continue;
+        const half_t *w = a.W + (long)y[i] * a.ldw;
+#pragma unroll
+        for (int j = 0; j < C::FB; j++) acc[i][j] += res[i] * pg::load4(w, at.n + 16 * j, a.N);
+    }
+}
+
+// dW: row v gets the sum of res times X over the rows n in [k0, k1) whose label it is. A wave lists those of its own rows, in order, and
+// adds them 32 at a time by one more product: A is res at (label, entry), B the listed rows of X. list: kListed entries of LDS, (row,
+// its label's place in the wave's rows).
+constexpr int kListed = 32 + 64;
+template <class C>
+__device__ __forceinline__ void add_labelled(const ProductArgs &a, int m0, int n0, int k0, int k1, int2 *list, floatx4 (&acc)[C::FA][C::FB]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15;
+    const int vw = m0 + wave / C::WVN * C::WM, nw = n0 + wave % C::WVN * C::WN;
+    int held = 0;
+    const auto add = [&](int n) {   // the first n entries, at most 32
+        if (lane >= n && lane < 32) list[lane] = make_int2(list[0].x, -1);
+        asm volatile("" ::: "memory");   // the wave's own LDS accesses complete in order
+        h8 x[C::FA];
+        int n8[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int2 e = list[8 * (lane >> 4) + k];
+            n8[k] = e.x;
+            const half_t r = (half_t)a.res[e.x];
+#pragma unroll
+            for (int i = 0; i < C::FA; i++) x[i][k] = e.y == 16 * i + col ? r : (half_t)0;
+        }
+#pragma unroll
+        for (int j = 0; j < C::FB; j++) {
+            const int c = nw + 16 * j + col;
+            const char *X = a.B.p + (long)(c >> 6) * a.B.ps + (c & 63) * 2;
+            h8 b = {};
+            if (c < a.N)
+#pragma unroll
+                for (int k = 0; k < 8; k++) b[k] = *(const half_t *)(X + (long)n8[k] * 128);
+#pragma unroll
+            for (int i = 0; i < C::FA; i++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, x[i], acc[i][j], 0, 0, 0);
+        }
+    };
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    for (int n0w = k0; n0w < k1; n0w += 1024) {
+        i4 y[4];
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int n = n0w + 256 * u + 4 * lane;
+            y[u] = n < k1 ? *(const i4 *)(a.lab + n) : (i4){-1, -1, -1, -1};
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                y[u][c] = n0w + 256 * u + 4 * lane + c < k1 ? y[u][c] - vw : -1;
+                any |= (unsigned)y[u][c] < (unsigned)C::WM;
+            }
+        if (!__ballot(any)) continue;
+#pragma unroll
+        for (int q = 0; q < 16; q++) {
+            const int n = n0w + 256 * (q >> 2) + 4 * lane + (q & 3), v = y[q >> 2][q & 3];
+            const bool hit = (unsigned)v < (unsigned)C::WM;
+            const uint64_t hits = __ballot(hit);
+            if (hit) list[held + __popcll(hits & ((1ull << lane) - 1))] = make_int2(n, v);
+            held += __popcll(hits);
+            while (held >= 32) {
+                add(32);
+                held -= 32;
+                asm volatile("" ::: "memory");
+                const int2 e = list[min(32 + lane, kListed - 1)];
+                asm volatile("" ::: "memory");
+                if (lane < held) list[lane] = e;
+            }
+        }
+    }
+    if (held) add(held);
+}
+
 template <class C>
 __global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
     __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
@@ -627,6 +730,15 @@ __global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
     product_tile<C>(a, tile, tiles_m, m0, n0);
     floatx4 acc[C::FA][C::FB];
     pg::contract<C>(a.A, a.B, m0, n0, first, count, smem, acc);
+    if constexpr (C::PA == 1) {
+        if constexpr (C::TA == 0) {
+            add_label_rows<C>(a, M, m0, n0, first * C::BK, (first + count) * C::BK, acc);
+        } else {
+            __syncthreads();   // the stages' buffers are free
+            const int rows = chunk_rows(&a.sc->count, a.row0, a.rows);
+            add_labelled<C>(a, m0, n0, first * C::BK, min(rows, (first + count) * C::BK), (int2 *)smem + (threadIdx.x >> 6) * kListed, acc);
+        }
+    }
     if (slot >= 0) {
         pg::store_partials<C>(w.part, slot, acc);
         return;
@@ -641,6 +753,7 @@ __device__ __forceinline__ void few_dx(const ProductArgs &a, const FewArgs &f, c
     pg::pick(a.w, blockIdx.x, (a.k + few::across_v(PP) - 1) / few::across_v(PP), tile, slot, first, count);
     floatx4 acc[C::FA][C::FB];
     few::contract_across<C, PP, F16>(P, PP == 1 ? 2l * a.rows : a.rows, f.Vp, f.W, f.ldw, a.k, a.N, tile * C::BN, first, count, smem, acc);
+    if constexpr (PP == 1) add_label_rows<C>(a, M, 0, tile * C::BN, first * few::across_v(PP), (first + count) * few::across_v(PP), acc);
     if (slot >= 0) pg::store_partials<C>(a.w.part, slot, acc);
     else product_rows<C, C::FA>(a, M, 0, tile * C::BN, 0, acc);
 }
@@ -690,7 +803,7 @@ struct Layout {
     int rows, pieces;          // rows of a piece
     bool pack_w, grad;
     int few;                   // 16-row tiles of the form for few rows, or 0
-    int64_t maxes, rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, dbpart, dwacc, sums, total;
+    int64_t maxes, rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, res, dbpart, dwacc, sums, total;
 };
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -757,6 +870,7 @@ Layout layout(const LinearCe &d) {
     l.Xp = take(Np * l.Dp * 2 * l.P);
     if (l.pack_w) l.Wp = take((int64_t)d.V * l.Dp * 2 * l.P);
     if (l.grad) l.E = take(rows * l.Vp * 4);
+    if (l.PP == 1) l.res = take(rows * 4);
     if (d.dbias) l.dbpart = take(Np / kGradRows * d.V * 4);
     if (d.dW && d.g16 && l.pieces > 1) l.dwacc = take((int64_t)d.V * d.D * 4);
     int64_t sums = 0;
@@ -946,7 +1060,7 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, sc, row0, rows, stats, a.T, zt + row0, rowmap + row0,
                            lse + row0, loss + row0, d.rowloss, d.lse);
         if (!l.grad) continue;
-        const GradArgs g{sc, row0, rows, d.V, l.Vp, lse + row0, zt + row0, lab + row0, ws + l.E, d.dbias ? (float *)(ws + l.dbpart) : nullptr};
+        const GradArgs g{sc, row0, rows, d.V, l.Vp, lse + row0, zt + row0, lab + row0, ws + l.E, (float *)(ws + l.res), d.dbias ? (float *)(ws + l.dbpart) : nullptr};
         const dim3 ggrid((unsigned)ceil_div(l.Vp, 256), (unsigned)ceil_div(rows, kGradRows));
         if (l.PP == 1) hipLaunchKernelGGL(lce_grad_kernel<1>, ggrid, dim3(256), 0, s, g);
         else hipLaunchKernelGGL(lce_grad_kernel<2>, ggrid, dim3(256), 0, s, g);
@@ -957,6 +1071,10 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         p.grad_scale = d.grad_scale;
         p.mean = d.mean;
         p.out16 = d.g16;
+        p.res = (const float *)(ws + l.res);
+        p.lab = lab + row0;
+        p.W = (const half_t *)d.W;
+        p.ldw = d.ldw;
         if (l.PP == 1) gradients<1, 1>(d, l, p, W, X, piece, ws, s);
         else if (d.f16) gradients<2, 1>(d, l, p, W, X, piece, ws, s);
         else gradients<2, 2>(d, l, p, W, X, piece, ws, s);

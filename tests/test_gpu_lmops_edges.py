@@ -29,3 +29,44 @@ def test_f16_gradients_round_p_once(dev, D, N, bias):
     tol = (U16 + (D / 32 + 40) * U32 * 16) * np.abs(want)
     worst = np.abs(got["dW"] - want) / tol
     assert worst.max() <= 1.0, worst.max()
+
+
+# rows, features, classes, and pieces of how many MiB: tiles of 64 features and more, either sum split, few rows of unaligned W, pieces
+LABELLED = [(130, 64, 1000, 0), (777, 96, 3003, 0), (2, 41, 300, 0), (100, 65, 2049, 0), (2500, 64, 200, 0), (150, 264, 20011, 0), (900, 130, 2100, 1),
+            (3000, 520, 5003, 0)]
+
+
+@pytest.mark.parametrize("labels", ["uniform", "few", "one"])
+@pytest.mark.parametrize("shape", LABELLED, ids=lambda s: "%dx%dx%d_%d" % s)
+def test_f16_gradients_keep_p_at_the_label(dev, shape, labels):
+    """P at the label is the largest entry of most rows. It takes part with 22 bits, as f16 and what that leaves, so a gradient is off
+    by its own rounding, by U16 of the other entries' share, and by f32 sums: with P at the label in f16 alone it is up to twice as far."""
+    N, D, V, mb = shape
+    r = np.random.default_rng([N, D])
+    y = {"uniform": r.integers(0, V, N), "few": np.exp(r.uniform(0, np.log(V), N)).astype(int) - 1, "one": np.full(N, V // 2)}[labels]
+    if N > 2:
+        y[r.random(N) < 0.2] = -1
+    c = TL.Case(N, D, V, dtype=L.AH_F16, grad_dtype=L.AH_F16, labels=y, bias=False)
+    s = 2.0 ** 10
+    got = TL.run(dev, c, want=("loss", "dX", "dW"), mean=False, grad_scale=s, piece_mb=mb)
+    X, W, on = c.X.astype(np.float64), c.W.astype(np.float64), np.flatnonzero(y >= 0)
+    X = X[on]
+    z = X @ W.T
+    p = np.exp(z - z.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    at = np.arange(len(on)), y[on]
+    dz = (np.abs(X) @ np.abs(W).T).max(1, keepdims=True) * (D / 32 + 32) * U32
+    dP = p * (3 * dz + (V / 64 + 40) * U32 + 2.0 ** -20) + U16 * p   # the logits, the statistics, exp; f16
+    P = p.copy()
+    P[at] -= 1.0
+    dP[at] = p[at] * (3 * dz[:, 0] + (V / 64 + 40) * U32 + 2.0 ** -20) + 2.0 ** -21 * np.abs(P[at])
+    dP += 2.0 ** -39
+    pieces = 4 if mb else 1
+    for name, a, da, b in (("dX", P, dP, W), ("dW", P.T, dP.T, X)):
+        want = a @ b * s
+        tol = s * (da @ np.abs(b) + (a.shape[1] / 32 + 32 * pieces) * U32 * (np.abs(a) @ np.abs(b))) + U16 * 1.01 * np.abs(want) + 2.0 ** -25
+        g = got[name][on] if name == "dX" else got[name]
+        over = np.abs(want) > 65504 - tol   # past f16's range (many rows of one label): infinite, or the largest value
+        assert np.all(np.sign(g[over]) == np.sign(want[over])) and np.all(np.abs(g[over]) >= np.minimum(np.abs(want), 65504)[over] - tol[over])
+        worst = np.where(over, 0.0, np.abs(np.where(over, 0.0, g) - want) / tol)
+        assert worst.max() <= 1.0, (name, worst.max(), np.argwhere(worst > 1)[:4].tolist())

@@ -195,9 +195,13 @@ __device__ __forceinline__ void pack_row(half_t *__restrict__ out, long rows, lo
 
 // A wave a row. Of the first N + 64, row r of X goes to its place among the counted rows, or its dX and outputs are cleared; the last
 // 64 clear the packed rows that fill up the last stage of the dW product. The others pack W.
+struct PackArgs {
+    half_t *X, *W;         // W: null where it is read as it lies
+    int Np, Dp, piece;     // padded rows and features; rows of a piece: each piece has panels of its own
+    int wshift, wstored;   // log2 of the rows of a block of W, and the rows that its panels are apart
+};
 template <int P>
-__global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, int Np, half_t *Wp, int Dp, const int *pos, Scalars *sc,
-                                                       const uint2 *maxes, int blocks) {
+__global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, PackArgs a, const int *pos, Scalars *sc, const uint2 *maxes, int blocks) {
     int ex = 0, ew = 0;
     if constexpr (P == 2) {
         const uint2 top = join_maxes(maxes, blocks);
@@ -209,13 +213,17 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, i
         ew = plane_exp(top.y);
     }
     constexpr int ESZ = P == 1 ? 2 : 4;
-    const int lane = threadIdx.x & 63, count = sc->count;
-    const long total = (long)d.N + 64 + (Wp ? d.V : 0);
+    const int lane = threadIdx.x & 63, count = sc->count, Dp = a.Dp;
+    const long total = (long)d.N + 64 + (a.W ? d.V : 0);
+    const auto xrow = [&](auto planes, int q, const void *in, int D, int width, int e) {   // row q of the counted ones
+        const int first = q / a.piece * a.piece;
+        pack_row<decltype(planes)::value>(a.X + (long)first * Dp * P, min(a.piece, a.Np - first), q - first, in, D, width, e);
+    };
     for (long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6); r < total; r += (long)gridDim.x * 4) {
         if (r < d.N) {
             const int q = pos[r];
             if (q >= 0) {
-                pack_row<P>(Xp, Np, q, (const char *)d.X + r * d.ldx * ESZ, d.D, Dp, ex);
+                xrow(std::integral_constant<int, P>(), q, (const char *)d.X + r * d.ldx * ESZ, d.D, Dp, ex);
                 continue;
             }
             if (d.dX)
@@ -228,11 +236,11 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(LinearCe d, half_t *Xp, i
                 if (d.lse) d.lse[r] = 0.0f;
             }
         } else if (r < d.N + 64) {
-            const long q = count + (r - d.N);
-            if (q < ((count + 63) & ~63)) pack_row<1>(Xp, Np, q, nullptr, 0, Dp * P, 0);
+            const int q = count + (int)(r - d.N);
+            if (q < ((count + 63) & ~63)) xrow(std::integral_constant<int, 1>(), q, nullptr, 0, Dp * P, 0);
         } else {
-            const long v = r - d.N - 64;
-            pack_row<P>(Wp, d.V, v, (const char *)d.W + v * d.ldw * ESZ, d.D, Dp, ew);
+            const int v = (int)(r - d.N - 64);
+            pack_row<P>(a.W + (long)(v >> a.wshift) * a.wstored * Dp * P, a.wstored, v & (int)((1u << a.wshift) - 1), (const char *)d.W + (long)v * d.ldw * ESZ, d.D, Dp, ew);
         }
     }
 }
@@ -341,7 +349,7 @@ __global__ __launch_bounds__(C::NT, 2) void lce_logits_kernel(LogitArgs a) {
     logits_tile<C>(a, tile, m0, n0);
     if (m0 >= M) return;
     floatx4 acc[C::FA][C::FB];
-    pg::contract<C>(a.X, a.W, m0, n0, first, count, smem, acc);
+    pg::contract<C, true>(a.X, a.W, m0, n0, first, count, smem, acc);
     if (slot >= 0) {
         pg::store_partials<C>(a.w.part, slot, acc);
         return;
@@ -729,7 +737,7 @@ __global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
     pg::pick(w, blockIdx.x, nk, tile, slot, first, count);
     product_tile<C>(a, tile, tiles_m, m0, n0);
     floatx4 acc[C::FA][C::FB];
-    pg::contract<C>(a.A, a.B, m0, n0, first, count, smem, acc);
+    pg::contract<C, C::TA == 0>(a.A, a.B, m0, n0, first, count, smem, acc);   // B is W for dX
     if constexpr (C::PA == 1) {
         if constexpr (C::TA == 0) {
             add_label_rows<C>(a, M, m0, n0, first * C::BK, (first + count) * C::BK, acc);
@@ -791,7 +799,8 @@ __global__ __launch_bounds__(C::NT) void lce_product_join_kernel(ProductArgs a) 
 // ── host ───────────────────────────────────────────────────────────────────────
 
 constexpr int kPieceMb = 2048;   // MiB of kept logits: one piece holds 4096 rows of 131072 classes
-constexpr int kMaxPieceRows = 1 << 20;          // a panel's offsets stay within 32 bits
+constexpr int kMaxPieceRows = 1 << 20;          // a tile's offsets over its panels stay within 32 bits (pg::kMaxPanelRows)
+constexpr int kBlockRowsLog = 17;               // rows of a block of packed W, where it has too many for one
 // Rows up to which a W that would have to be packed is read as it lies. 4096 features, 32000 classes in f32, with gradients, packed and as
 // it lies: 16 rows 731 and 438 us, 128 rows 823 and 850; the loss alone 433 and 139 us at 16 rows, 545 and 367 at 121 (2944 x 51416).
 constexpr int kFewRows = 128;
@@ -802,6 +811,7 @@ struct Layout {
     int PP;                    // planes of P, which takes the logits' place
     int rows, pieces;          // rows of a piece
     bool pack_w, grad;
+    int wshift, wstored;       // of packed W: PackArgs
     int few;                   // 16-row tiles of the form for few rows, or 0
     int64_t maxes, rowmap, pos, lab, zt, lse, loss, stats, Xp, Wp, E, res, dbpart, dwacc, sums, total;
 };
@@ -868,7 +878,9 @@ Layout layout(const LinearCe &d) {
     l.loss = take(Np * 4);
     l.stats = take(rows * ((l.Vp + 255) / 256 * 256 / kStatCols) * 8);
     l.Xp = take(Np * l.Dp * 2 * l.P);
-    if (l.pack_w) l.Wp = take((int64_t)d.V * l.Dp * 2 * l.P);
+    l.wshift = d.V <= pg::kMaxPanelRows ? 31 : kBlockRowsLog;
+    l.wstored = l.wshift == 31 ? d.V : 1 << kBlockRowsLog;
+    if (l.pack_w) l.Wp = take((((int64_t)d.V - 1 >> l.wshift) + 1) * l.wstored * l.Dp * 2 * l.P);
     if (l.grad) l.E = take(rows * l.Vp * 4);
     if (l.PP == 1) l.res = take(rows * 4);
     if (d.dbias) l.dbpart = take(Np / kGradRows * d.V * 4);
@@ -1016,13 +1028,15 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
     hipLaunchKernelGGL(lce_scan_kernel, dim3((unsigned)(1 + scans)), dim3(256), 0, s, scan);
     const dim3 pgrid((unsigned)std::min<int64_t>(((int64_t)d.N + 64 + (l.pack_w ? d.V : 0) + 3) / 4, 4096));
     const int Np = (d.N + 63) & ~63;
-    if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc, maxes, scans);
-    else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, Xp, Np, Wp, l.Dp, pos, sc, maxes, scans);
+    const PackArgs pack{Xp, Wp, Np, l.Dp, l.rows, l.wshift, l.wstored};
+    if (d.f16) hipLaunchKernelGGL(lce_pack_kernel<1>, pgrid, dim3(256), 0, s, d, pack, pos, sc, maxes, scans);
+    else hipLaunchKernelGGL(lce_pack_kernel<2>, pgrid, dim3(256), 0, s, d, pack, pos, sc, maxes, scans);
 
-    const pg::Operand W = l.pack_w ? pg::panels(Wp, d.V, d.V, l.Dp) : pg::row_major(d.W, d.ldw, d.V, d.D);
+    pg::Operand W = l.pack_w ? pg::panels(Wp, l.wstored, d.V, l.Dp) : pg::row_major(d.W, d.ldw, d.V, d.D);
+    if (l.pack_w && l.wshift < 31) W.shift = l.wshift, W.block = (long)l.wstored * l.Dp * 2 * l.P;
     for (int piece = 0; piece < l.pieces; piece++) {
         const int row0 = piece * l.rows, rows = std::min(l.rows, Np - row0);
-        const pg::Operand X = pg::panels(Xp + (long)row0 * 64, Np, rows, l.Dp);
+        const pg::Operand X = pg::panels(Xp + (long)row0 * l.Dp * l.P, rows, rows, l.Dp);
         const pg::Plan plan = logits_plan(l, d.V, rows);
         LogitArgs a{};
         a.X = X;

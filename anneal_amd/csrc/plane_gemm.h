@@ -190,7 +190,15 @@ struct Operand {
     long ps;         // bytes from 64 halves of a row to the next 64
     int rows;        // operand rows
     int k;           // k that there are (B's may end inside a stage: PFetch::issue)
+    // B of contract<C, true>: stored rows come in blocks of 2^shift, a multiple of a tile's and a stage's, each `block` bytes on with panels of its own
+    int shift = 31;
+    long block = 0;
 };
+
+// A lane's offset from its tile's corner is 32 bits wide and spans up to 8 panels (T = 1: 256 operand rows of two planes), so panels may
+// not be further apart than this many stored rows; more of them go in blocks.
+constexpr int kMaxPanelRows = 1 << 22;
+static_assert(7l * kMaxPanelRows * 128 + 64 * 128 < 1l << 32, "the last panel's rows are in reach");
 
 // `stored` rows in panels; rows of the operand, k as above.
 inline Operand panels(const void *p, long stored, int rows, int k) { return {(const char *)p, 64, stored * 128, rows, k}; }
@@ -203,7 +211,8 @@ inline Operand row_major(const void *p, long ld, int rows, int k) { return {(con
 //
 // The stage pipeline: NS buffers; the wait and barrier for stage t+1 stand before the last MFMA group of stage t, so that its
 // first fragments arrive during that group, and the refill of stage t's buffer goes out between that group's MFMAs.
-template <class C>
+// BLOCKS: B's stored rows may lie in blocks (always reckoned with, it costs the orthogonalisation of 4096 x 1024 2%).
+template <class C, bool BLOCKS = false>
 __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int m0, int n0, int kt0, int nk, char *smem,
                                          floatx4 (&acc)[C::FA][C::FB]) {
     constexpr int FA = C::FA, FB = C::FB, BK = C::BK, NS = C::NS, STAGE = C::STAGE, ABYTES = C::ABYTES;
@@ -225,11 +234,14 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
     fa.init(A.ld, A.ps, m0, A.rows, wave, lane);
     fb.init(B.ld, B.ps, n0, B.rows, wave, lane);
     const char *Ab = A.p + (C::TA == 0 ? (long)m0 * A.ld * 2 : (long)(m0 * C::PA / 64) * A.ps);
-    const char *Bb = B.p + (C::TB == 0 ? (long)n0 * B.ld * 2 : (long)(n0 * C::PB / 64) * B.ps);
+    const auto stored = [&](int r) {   // B's row r
+        return BLOCKS ? (long)(r >> B.shift) * B.block + (long)(r & (int)((1u << B.shift) - 1)) * B.ld * 2 : (long)r * B.ld * 2;
+    };
+    const char *Bb = B.p + (C::TB == 0 ? stored(n0) : (long)(n0 * C::PB / 64) * B.ps);
     const long da = C::TA == 0 ? A.ps : (long)BK * A.ld * 2, db = C::TB == 0 ? B.ps : (long)BK * B.ld * 2;   // bytes a stage
     auto issue_one = [&](int f, int t, int buf) {   // load f of stage t into buffer buf
         if (f < PERA) fa.issue(f, Ab + (kt0 + t) * da, A.ld, BK, lds + buf * STAGE, wave_u, lane);
-        else fb.issue(f - PERA, Bb + (kt0 + t) * db, B.ld, C::TB == 1 || C::PB == 1 ? B.k - (kt0 + t) * BK : BK, lds + buf * STAGE + ABYTES, wave_u, lane);
+        else fb.issue(f - PERA, Bb + (BLOCKS && C::TB == 1 ? stored((kt0 + t) * BK) : (kt0 + t) * db), B.ld, C::TB == 1 || C::PB == 1 ? B.k - (kt0 + t) * BK : BK, lds + buf * STAGE + ABYTES, wave_u, lane);
     };
     typename C::FragA ra;
     typename C::FragB rb;

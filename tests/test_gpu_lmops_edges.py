@@ -70,3 +70,85 @@ def test_f16_gradients_keep_p_at_the_label(dev, shape, labels):
         assert np.all(np.sign(g[over]) == np.sign(want[over])) and np.all(np.abs(g[over]) >= np.minimum(np.abs(want), 65504)[over] - tol[over])
         worst = np.where(over, 0.0, np.abs(np.where(over, 0.0, g) - want) / tol)
         assert worst.max() <= 1.0, (name, worst.max(), np.argwhere(worst > 1)[:4].tolist())
+
+
+# ── more rows or classes than one array of panels holds ────────────────────────
+
+def _repeated(dev, base, rows, dtype=L.AH_F32):
+    """Device memory of `rows` rows, row r that of base's r % len(base)."""
+    b = dev.buffer(rows * base.shape[1], dtype)
+    chunk = np.ascontiguousarray(np.tile(base.astype(TL.NP[dtype]), (256, 1)))
+    for r in range(0, rows, len(chunk)):
+        n = min(len(chunk), rows - r) * base.shape[1] * chunk.itemsize
+        L.check(dev.lib.ah_upload_bytes(dev.h, b.ptr + r * base.shape[1] * chunk.itemsize, chunk.ctypes.data, n))
+    return b
+
+
+def _run(dev, **args):
+    ws = dev.buffer(dev.linear_ce_workspace(**args) // 4 + 4)
+    dev.linear_ce(ws=ws, **args)
+    dev.sync()
+    ws.free()
+
+
+@pytest.mark.parametrize("dtype,N,D,V", [(L.AH_F32, 2048, 256, 5_000_000), (L.AH_F16, 300, 257, 4_300_003)], ids=["f32", "f16"])
+def test_millions_of_classes(dev, dtype, N, D, V):
+    """Packed W of more rows than a tile's 32-bit offsets span, with 256-wide tiles of dX in the f32 case: loss and dX against 64 bits. W
+    repeats 1021 rows, so that the sums over classes are short here. A row's P is off by a share e of it, from its logit and the
+    statistics, and dX by e |P| |W| and by f32 sums over V / splits, splits >= 8."""
+    r = np.random.default_rng(V)
+    base, X = (D ** -0.5 * r.standard_normal((1021, D))).astype(TL.NP[dtype]), r.standard_normal((N, D)).astype(TL.NP[dtype])
+    y = r.integers(0, V, N).astype(np.int32)
+    s, u16 = (1024.0, U16) if dtype == L.AH_F16 else (1.0, 0.0)
+    b = {"X": dev.buffer(X, dtype), "W": _repeated(dev, base, V, dtype), "labels": dev.buffer(y, L.AH_I32), "loss": dev.buffer(1), "rowloss": dev.buffer(N),
+         "dX": dev.buffer(N * D, dtype)}
+    _run(dev, dtype=dtype, grad_dtype=dtype, N=N, D=D, V=V, mean=False, grad_scale=s, piece_mb=48000, **b)
+    rowloss, dX = b["rowloss"].read(), b["dX"].read().reshape(N, D).astype(np.float64)
+    for v in b.values():
+        v.free()
+    X, base = X.astype(np.float64), base.astype(np.float64)
+    z = X @ base.T
+    times = np.bincount(np.arange(V) % 1021, minlength=1021)
+    m = z.max(1, keepdims=True)
+    lse = m + np.log((np.exp(z - m) * times).sum(1, keepdims=True))
+    want = lse[:, 0] - z[np.arange(N), y % 1021]
+    dz = (np.abs(X) @ np.abs(base).T).max(1) * ((3 * 2.0 ** -22 if dtype == L.AH_F32 else 0.0) + (D / 32 + 32) * U32)
+    # V / 128 = 39063 wave tiles, joined by a wave in chains of 610 f32 sums; lse is up to 18
+    dlse = dz + (640 + 64 + 40) * U32 + 18 * 2 * U32
+    assert np.all(np.abs(rowloss - want) <= dlse + dz + 20 * U32)
+    p = np.exp(z - lse) * times   # the repeated rows' P, summed
+    own = base[y % 1021]
+    e = 2 * dz + dlse + 2.0 ** -20 + (V / 8 / 32 + 64) * U32
+    want = p @ base - own
+    tol = (e + u16)[:, None] * (p @ np.abs(base)) + (e + 2.0 ** -20)[:, None] * np.abs(own) + 2.0 ** -39 * np.abs(base).sum(0) * V / 1021
+    off = np.abs(dX - s * want) / (s * (tol + (u16 + 2 * U32) * 1.01 * np.abs(want)) + 2.0 ** -25)
+    assert off.max() <= 1.0, off.max()
+
+
+def test_millions_of_rows(dev):
+    """dW over 5 million packed rows of X in pieces, with 256-wide tiles, against 64 bits; X repeats 1021 rows. e as above; f32 sums over a
+    piece's 262144 rows in at least 8 splits, and over 20 pieces."""
+    N, D, V = 5_000_000, 256, 2048
+    r = np.random.default_rng(N)
+    W, base = (D ** -0.5 * r.standard_normal((V, D))).astype(np.float32), r.standard_normal((1021, D)).astype(np.float32)
+    y = (np.arange(N, dtype=np.int64) * 7 % V).astype(np.int32)
+    b = {"X": _repeated(dev, base, N), "W": dev.buffer(W), "labels": dev.buffer(y, L.AH_I32), "loss": dev.buffer(1), "dW": dev.buffer(V * D)}
+    _run(dev, dtype=L.AH_F32, N=N, D=D, V=V, mean=False, **b)
+    loss, dW = float(b["loss"].read()[0]), b["dW"].read().reshape(V, D).astype(np.float64)
+    for v in b.values():
+        v.free()
+    base, W = base.astype(np.float64), W.astype(np.float64)
+    z = base @ W.T
+    m = z.max(1, keepdims=True)
+    lse = m + np.log(np.exp(z - m).sum(1, keepdims=True))
+    kind = np.arange(N) % 1021
+    times = np.bincount(kind, minlength=1021)
+    pairs = np.bincount(kind * V + y, minlength=1021 * V).reshape(1021, V).astype(np.float64)   # rows of each kind with each label
+    dz = float((np.abs(base) @ np.abs(W).T).max()) * (3 * 2.0 ** -22 + (D / 32 + 32) * U32)
+    total = (times * lse[:, 0]).sum() - (pairs * z).sum()
+    assert abs(loss - total) <= N * (2 * dz + 80 * U32 + 16 * 2 * U32) + 2 * U32 * total
+    p = np.exp(z - lse)
+    e = 3 * dz + 2.0 ** -19 + (262144 / 8 / 32 + 64 + 20) * U32
+    want = (p * times[:, None] - pairs).T @ base
+    off = np.abs(dW - want) / (e * ((p * times[:, None] + pairs).T @ np.abs(base)) + 2.0 ** -39 * N)
+    assert off.max() <= 1.0, off.max()

@@ -656,75 +656,97 @@ __device__ __forceinline__ void add_label_rows(const ProductArgs &a, int M, int 
     }
 }
 
-// dW: row v gets the sum of res times X over the rows n in [k0, k1) whose label it is. A wave lists those of its own rows, in order, and
-// adds them 32 at a time by one more product: A is res at (label, entry), B the listed rows of X. list: kListed entries of LDS, (row,
-// its label's place in the wave's rows).
-constexpr int kListed = 32 + 64;
+// dW: row v gets the sum of res times X over the rows n in [k0, k1) whose label it is. The workgroup looks through 512 labels a wave at a
+// time and lists those of each row of waves, in a fixed order; a wave adds its row's 32 at a time by one more product: A is res at
+// (label, entry), B the listed rows of X. (Every wave through all labels for itself took 11 us a tile of 4096 rows.)
 template <class C>
-__device__ __forceinline__ void add_labelled(const ProductArgs &a, int m0, int n0, int k0, int k1, int2 *list, floatx4 (&acc)[C::FA][C::FB]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15;
-    const int vw = m0 + wave / C::WVN * C::WM, nw = n0 + wave % C::WVN * C::WN;
-    int held = 0;
-    const auto add = [&](int n) {   // the first n entries, at most 32
-        if (lane >= n && lane < 32) list[lane] = make_int2(list[0].x, -1);
-        asm volatile("" ::: "memory");   // the wave's own LDS accesses complete in order
-        h8 x[C::FA];
-        int n8[8];
+__device__ __forceinline__ void add_labelled(const ProductArgs &a, int m0, int n0, int k0, int k1, char *smem, floatx4 (&acc)[C::FA][C::FB]) {
+    constexpr int G = C::WVM, R = C::NW * 512;
+    static_assert((G * R + C::NW * G) * 4 <= C::SMEM && R <= 1 << 16, "the lists fit the stages' buffers, an entry 16 + 16 bits");
+    uint32_t *const list = (uint32_t *)smem;   // [row of waves][R]: row of X from the chunk's first, the label's place in the waves' rows
+    int *const counts = (int *)smem + G * R;   // [wave][row of waves]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, nw = n0 + wave % C::WVN * C::WN;
+    for (int c0 = k0; c0 < k1; c0 += R) {
+        typedef int i4 __attribute__((ext_vector_type(4)));
+        const int n = c0 + wave * 512 + lane * 8;
+        int y[8], at[G];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int2 e = list[8 * (lane >> 4) + k];
-            n8[k] = e.x;
-            const half_t r = (half_t)a.res[e.x];
+        for (int q = 0; q < 8; q += 4) {
+            i4 l = {};
+            if (n + q < k1) l = *(const i4 *)(a.lab + n + q);
 #pragma unroll
-            for (int i = 0; i < C::FA; i++) x[i][k] = e.y == 16 * i + col ? r : (half_t)0;
+            for (int r = 0; r < 4; r++) y[q + r] = n + q + r < k1 ? l[r] - m0 : -1;
         }
+        const auto hit = [&](int q, int g) { return (unsigned)(y[q] - g * C::WM) < (unsigned)C::WM; };
 #pragma unroll
-        for (int j = 0; j < C::FB; j++) {
-            const int c = nw + 16 * j + col;
-            const char *X = a.B.p + (long)(c >> 6) * a.B.ps + (c & 63) * 2;
-            h8 b = {};
-            if (c < a.N)
+        for (int g = 0; g < G; g++) {
+            at[g] = 0;
 #pragma unroll
-                for (int k = 0; k < 8; k++) b[k] = *(const half_t *)(X + (long)n8[k] * 128);
-#pragma unroll
-            for (int i = 0; i < C::FA; i++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, x[i], acc[i][j], 0, 0, 0);
+            for (int q = 0; q < 8; q++) at[g] += __popcll(__ballot(hit(q, g)));
+            if (lane == 0) counts[wave * G + g] = at[g];
         }
-    };
-    typedef int i4 __attribute__((ext_vector_type(4)));
-    for (int n0w = k0; n0w < k1; n0w += 1024) {
-        i4 y[4];
-        bool any = false;
+        __syncthreads();
+        int mine = 0;   // entries of this wave's row
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int n = n0w + 256 * u + 4 * lane;
-            y[u] = n < k1 ? *(const i4 *)(a.lab + n) : (i4){-1, -1, -1, -1};
-        }
+        for (int g = 0; g < G; g++) {
+            at[g] = 0;
 #pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                y[u][c] = n0w + 256 * u + 4 * lane + c < k1 ? y[u][c] - vw : -1;
-                any |= (unsigned)y[u][c] < (unsigned)C::WM;
-            }
-        if (!__ballot(any)) continue;
-#pragma unroll
-        for (int q = 0; q < 16; q++) {
-            const int n = n0w + 256 * (q >> 2) + 4 * lane + (q & 3), v = y[q >> 2][q & 3];
-            const bool hit = (unsigned)v < (unsigned)C::WM;
-            const uint64_t hits = __ballot(hit);
-            if (hit) list[held + __popcll(hits & ((1ull << lane) - 1))] = make_int2(n, v);
-            held += __popcll(hits);
-            while (held >= 32) {
-                add(32);
-                held -= 32;
-                asm volatile("" ::: "memory");
-                const int2 e = list[min(32 + lane, kListed - 1)];
-                asm volatile("" ::: "memory");
-                if (lane < held) list[lane] = e;
+            for (int w = 0; w < C::NW; w++) {
+                const int c = counts[w * G + g];
+                if (w < wave) at[g] += c;
+                if (g == wave / C::WVN) mine += c;
             }
         }
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const uint64_t hits = __ballot(hit(q, g));
+                if (hit(q, g)) list[g * R + at[g] + __popcll(hits & ((1ull << lane) - 1))] = (uint32_t)(n + q - c0) | (uint32_t)(y[q] - g * C::WM) << 16;
+                at[g] += __popcll(hits);
+            }
+        __syncthreads();
+        const uint32_t *const own = list + wave / C::WVN * R;
+        for (int first = 0; first < mine; first += 32) {
+            uint32_t v[8];
+            const char *row[8];
+            float res[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = own[min(first + 8 * (lane >> 4) + k, mine - 1)];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                row[k] = a.B.p + (long)(c0 + (int)(v[k] & 0xffff)) * 128 + col * 2;
+                res[k] = a.res[c0 + (int)(v[k] & 0xffff)];
+            }
+            h8 x[C::FA];
+            constexpr int H = C::FB > 4 ? C::FB / 2 : C::FB;   // columns whose loads are in flight together
+#pragma unroll
+            for (int j0 = 0; j0 < C::FB; j0 += H) {
+                h8 b[H];
+#pragma unroll
+                for (int j = 0; j < H; j++) {
+                    const int c = min(nw + 16 * (j0 + j), a.B.rows - 16);   // past the last feature: those columns are not stored
+                    const long X = (long)(c >> 6) * a.B.ps + (c & 63) * 2;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) b[j][k] = *(const half_t *)(row[k] + X);
+                }
+                if (j0 == 0)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const half_t r = (half_t)res[k];
+#pragma unroll
+                        for (int i = 0; i < C::FA; i++)
+                            x[i][k] = first + 8 * (lane >> 4) + k < mine && (int)(v[k] >> 16) == 16 * i + col ? r : (half_t)0;
+                    }
+#pragma unroll
+                for (int j = 0; j < H; j++)
+#pragma unroll
+                    for (int i = 0; i < C::FA; i++) acc[i][j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[j], x[i], acc[i][j0 + j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        __syncthreads();   // the lists have been read
     }
-    if (held) add(held);
 }
 
 template <class C>
@@ -744,7 +766,7 @@ __global__ __launch_bounds__(C::NT, 2) void lce_product_kernel(ProductArgs a) {
         } else {
             __syncthreads();   // the stages' buffers are free
             const int rows = chunk_rows(&a.sc->count, a.row0, a.rows);
-            add_labelled<C>(a, m0, n0, first * C::BK, min(rows, (first + count) * C::BK), (int2 *)smem + (threadIdx.x >> 6) * kListed, acc);
+            add_labelled<C>(a, m0, n0, first * C::BK, min(rows, (first + count) * C::BK), smem, acc);
         }
     }
     if (slot >= 0) {

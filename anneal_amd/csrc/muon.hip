@@ -6,8 +6,8 @@
 // The iteration raises small singular values by a = 3.4 a step, 480-fold in five: what is lost of X to rounding grows as much. So
 // all matrices are carried as two f16 planes (22 bits, plane_gemm.h) and every product is three f16 products in an f32
 // accumulator; against 64 bits the result is about as far off as 32-bit products leave it, in 3/16 of the f32 MFMAs' time. Each
-// matrix is scaled by a power of two (kSX ..): with the singular values of X at most 1.2, as the iteration keeps them, entries stay
-// far below f16's largest value, and entries down to 2^-22 of the matrix's norm keep 22 bits less what they are below 2^-14.
+// matrix is scaled by a power of two (kSX, Scales), by how far the polynomial can take the singular values, up to 4: entries stay
+// below f16's largest value. Where they stay at 1.2, entries down to 2^-22 of the matrix's norm keep 22 bits less what they are below 2^-14.
 //
 // Several steps in one. A + (a I + B) A (a I + B) = the next step's A: all are polynomials of one symmetric matrix and commute. So a
 // group of g steps can be run on the s x s side (s the short side, l the long one) and applied to X once:
@@ -321,6 +321,7 @@ hipError_t muon(const Muon &d, void *wsp, hipStream_t s) {
                        dim3(256), 0, s, d, part, l.parts, X, l.Rp, l.Cp);
 
     const long sx = (long)l.Rp * l.Cp * 4, ss = (long)l.S * l.S * 4;
+    const Scales sc = scales(d);
     const auto buf = [&](int i) { return (half_t *)(ws + l.square_at[i]); };
     const auto square = [&](const half_t *p) { return pg::panels(p, l.S, l.S, l.S); };
     // out = k (left right) + k1 p1 + k2 p2, matrices without their planes' scales
@@ -345,7 +346,7 @@ hipError_t muon(const Muon &d, void *wsp, hipStream_t s) {
     for (int left = d.steps, index = 0; left > 0; index++) {
         const int g = group_size(l.group, index, left);
         left -= g;
-        Square A{buf(0), kSA}, B{buf(1), kSB};
+        Square A{buf(0), sc.A}, B{buf(1), sc.B};
         NsArgs q{};   // A = X X^T or X^T X
         q.M = q.N = l.S;
         q.nk = l.K / 32;
@@ -354,7 +355,7 @@ hipError_t muon(const Muon &d, void *wsp, hipStream_t s) {
         q.out = A.p;
         q.so = ss / 2;
         q.rows = l.S;
-        q.k0 = 1.0f / (1 << (2 * kSX - kSA));
+        q.k0 = (float)std::ldexp(1.0, sc.A - 2 * kSX);
         if (l.wide) product<0, 0, NS_SYM>(q, l.gram, d, sums, s);
         else product<1, 1, NS_SYM>(q, l.gram, d, sums, s);
 
@@ -362,7 +363,7 @@ hipError_t muon(const Muon &d, void *wsp, hipStream_t s) {
         Square Q = B;                               // the group's polynomial is qi I + Q
         double qi = d.a;
         for (int i = 1; i < g; i++) {
-            const Square BA{buf(2), kSBA}, Bn{buf(i == 1 ? 3 : 1), kSB}, Qn{buf(3 + i), i == 1 ? 11 : 9};
+            const Square BA{buf(2), sc.BA}, Bn{buf(i == 1 ? 3 : 1), sc.B}, Qn{buf(3 + i), i == 1 ? sc.Q2 : sc.Q3};
             symmetric(BA, B, A, 1, d.a, A, 0, none);       // (a I + B) A
             symmetric(A, BA, B, 1, d.a, BA, 0, none);      // (a I + B) A (a I + B)
             symmetric(Bn, A, A, d.c, d.b, A, 0, none);

@@ -13,7 +13,7 @@ using pg::h4;
 using pg::load4;
 using pg::store4;
 
-constexpr int kSX = 12, kSA = 13, kSB = 11, kSBA = 12;   // powers of two of the planes: X, A, B, (a I + B) A
+constexpr int kSX = 12;   // power of two of X's planes; of the short side's matrices: Scales
 
 __device__ __forceinline__ floatx4 load_g(const Muon &d, long z, int r, int c) {
     const long at = z * d.sg + r * d.ldg;
@@ -77,14 +77,56 @@ __device__ __forceinline__ void store_result(const Muon &d, long z, int r, int c
 
 }  // namespace ns
 
-// Steps of the longest group: |a + b x + c x^2| over what the squared singular values reach bounds a step's growth, and the planes
-// of three steps' Q hold its cube up to 43. A short side under 256 starts with larger singular values of X and has less to average
+// How large the polynomial's matrices become: over squared singular values x that the iterates before the last reach (1 at the start; the
+// caller keeps them to 16), the largest x, |a + b x + c x^2|, |b x + c x^2| and |a + b x + c x^2| x, from samples, with 2% for what lies
+// between them.
+struct Reach {
+    double x, step, b, ba;
+};
+inline Reach reach(const Muon &d) {
+    constexpr int n = 128;
+    const auto poly = [&](double x) { return d.a + d.b * x + d.c * x * x; };
+    double top = 1.0;
+    for (int k = 1; k < d.steps && top < 4.0; k++) {
+        double next = 0.0;
+        for (int i = 1; i <= n; i++) {
+            const double s = top * i / n;
+            next = std::max(next, 1.02 * std::fabs(s * poly(s * s)));
+        }
+        if (next <= top) break;
+        top = std::min(next, 4.0);
+    }
+    Reach r{top * top, 0, 0, 0};
+    for (int i = 0; i <= n; i++) {
+        const double x = r.x * i / n;
+        r.step = std::max(r.step, 1.02 * std::fabs(poly(x)));
+        r.b = std::max(r.b, 1.02 * std::fabs(d.b * x + d.c * x * x));
+        r.ba = std::max(r.ba, 1.02 * std::fabs(poly(x) * x));
+    }
+    return r;
+}
+
+// Powers of two of the planes of A, B, (a I + B) A and of the polynomials of groups of two and three steps (less their multiple of I). No
+// entry passes f16's largest value: an entry is at most the largest eigenvalue. The caps are what a polynomial that keeps the singular
+// values to 1.2 takes.
+struct Scales {
+    int A, B, BA, Q2, Q3;
+};
+inline Scales scales(const Muon &d) {
+    const Reach r = reach(d);
+    const auto most = [](double top, int cap) { return top * std::ldexp(1.0, cap) <= 65504.0 ? cap : (int)std::floor(std::log2(65504.0 / top)); };
+    const double a = std::fabs(d.a);
+    return {most(r.x, 13), most(r.b, 11), most(r.ba, 12), most(r.step * r.step + a * a, 11), most(r.step * r.step * r.step + a * a * a, 9)};
+}
+
+// Steps of the longest group: the largest |a + b x + c x^2| bounds a step's growth. A short side under 256 starts with larger singular values of X and has less to average
 // over: three steps at once cost it more than 32-bit products lose (16 x 64: 7 times the error of step by step), and under 32 two at
 // once do (8 x 8: 1.3e-6 off, step by step 0.7e-6, 32-bit products 0.6e-6).
 inline int longest_group(const Muon &d) {
     double grow = 0;
+    const double top = std::max(1.5, reach(d).x);
     for (int i = 0; i <= 60; i++) {
-        const double x = i * 0.025;
+        const double x = i * top / 60;
         grow = std::max(grow, std::fabs(d.a + d.b * x + d.c * x * x));
     }
     const int side = std::min(d.rows, d.cols);

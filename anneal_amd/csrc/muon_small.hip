@@ -34,6 +34,11 @@ struct SmallArgs {
     int parts;
     int steps;             // of the group, 1 or 2
     float qi;              // the group's polynomial is qi I + Q
+    float ga;              // A's planes from the Gram matrix of X's
+    float b2, b1;          // c A A and b A in B's planes
+    float p2, p1;          // B A and a A in those of (a I + B) A
+    float a2, a1;          // times B, and times a, in A's
+    float q2, q1, qs;      // B Q and a Q + a B in those of a group of two; what its planes are scaled by
 };
 
 // Byte offsets in an image of R rows: four values at row r, k c (T = 0), or at k r, row c (T = 1). The lo plane is at the offset xor 64.
@@ -155,7 +160,6 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
             add_gram();
         }
     } else {
-        const float ca = d.a, cb = d.b, cc = d.c;
         {   // A, then the group's Q, by the products that muon.hip describes
             typedef floatx4 Square[FQ][FQ];
             // v = k (image 0 or 1 times image 0 or 1) + k1 p + k2 q
@@ -184,7 +188,6 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
 #pragma unroll
                     for (int j = 0; j < FQ; j++) image_store(img, image0<S>(qm + 16 * i, qn + 16 * j), v[i][j]);
             };
-            constexpr float kB2 = 1.0f / (1 << (2 * kSA - kSB)), kB1 = 1.0f / (1 << (kSA - kSB));   // of c A A and of b A
             Square A, B, Q;
             clear(A);
             const floatx4 *in = (const floatx4 *)p.in + z * p.groups * (S * S / 4) + tid;
@@ -208,10 +211,10 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
 #pragma unroll
             for (int i = 0; i < FQ; i++)
 #pragma unroll
-                for (int j = 0; j < FQ; j++) A[i][j] *= 1.0f / (1 << (2 * kSX - kSA));
+                for (int j = 0; j < FQ; j++) A[i][j] *= p.ga;
             put(slice_img, A);
             __syncthreads();
-            product(0, 0, cc * kB2, A, cb * kB1, A, 0.0f, B);
+            product(0, 0, p.b2, A, p.b1, A, 0.0f, B);
 #pragma unroll
             for (int i = 0; i < FQ; i++)
 #pragma unroll
@@ -220,25 +223,25 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
                 Square P;
                 put(square_img, B);   // nothing reads image 1 here
                 __syncthreads();
-                product(1, 0, 1.0f / (1 << (kSA + kSB - kSBA)), A, ca / (1 << (kSA - kSBA)), A, 0.0f, P);   // (a I + B) A
+                product(1, 0, p.p2, A, p.p1, A, 0.0f, P);   // (a I + B) A
                 __syncthreads();
                 put(slice_img, P);
                 __syncthreads();
-                product(0, 1, 1.0f / (1 << (kSB + kSBA - kSA)), P, ca * (1 << (kSA - kSBA)), P, 0.0f, A);   // (a I + B) A (a I + B)
+                product(0, 1, p.a2, P, p.a1, P, 0.0f, A);   // (a I + B) A (a I + B)
                 __syncthreads();
                 put(slice_img, A);
                 __syncthreads();
-                product(0, 0, cc * kB2, A, cb * kB1, A, 0.0f, B);
+                product(0, 0, p.b2, A, p.b1, A, 0.0f, B);
                 __syncthreads();
                 put(slice_img, Q);
                 put(square_img, B);
                 __syncthreads();
-                product(1, 0, 1.0f / (1 << kSB), Q, ca, B, ca, Q);
+                product(1, 0, p.q2, Q, p.q1, B, p.q1, Q);
             }
             __syncthreads();
             put(square_img, Q);
         }
-        const float qi = p.qi, qs = 1.0f / (1 << kSB);
+        const float qi = p.qi, qs = p.qs;
         for (int sl = blockIdx.x; sl < p.slices; sl += p.groups) {
             const int m0 = WIDE ? 0 : sl * kSlice, n0 = WIDE ? sl * kSlice : 0;
             __syncthreads();   // B is there; the slice image has been read
@@ -345,12 +348,24 @@ SmallLayout small_layout(const Muon &d) {
 template <int S, bool WIDE>
 void run(const Muon &d, SmallArgs a, float *const (&parts)[2], hipStream_t s) {
     const dim3 grid((unsigned)a.groups, (unsigned)d.batch);
+    const Scales c = scales(d);
+    const auto p2 = [](double v, int e) { return (float)std::ldexp(v, e); };
+    a.ga = p2(1, c.A - 2 * kSX);
+    a.b2 = p2(d.c, c.B - 2 * c.A);
+    a.b1 = p2(d.b, c.B - c.A);
+    a.p2 = p2(1, c.BA - c.A - c.B);
+    a.p1 = p2(d.a, c.BA - c.A);
+    a.a2 = p2(1, c.A - c.B - c.BA);
+    a.a1 = p2(d.a, c.A - c.BA);
+    a.q2 = p2(1, c.Q2 - 2 * c.B);
+    a.q1 = p2(d.a, c.Q2 - c.B);
     a.out = parts[0];
     hipLaunchKernelGGL((muon_small_kernel<S, WIDE, FIRST>), grid, dim3(S / 32 * (S / 32) * 64), 0, s, a, d);
     for (int left = d.steps, k = 0; left > 0; k++) {
         a.steps = group_size(longest_group(d), k, left);
         left -= a.steps;
         a.qi = (float)std::pow((double)d.a, a.steps);
+        a.qs = p2(1, a.steps == 2 ? -c.Q2 : -c.B);
         a.in = parts[k & 1];
         a.out = parts[(k + 1) & 1];
         if (left) hipLaunchKernelGGL((muon_small_kernel<S, WIDE, STEP>), grid, dim3(S / 32 * (S / 32) * 64), 0, s, a, d);

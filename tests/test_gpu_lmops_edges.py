@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import test_gpu_linear_ce as TL
+import test_gpu_muon as TM
 from anneal_amd import _lib as L
 
 pytestmark = pytest.mark.gpu
@@ -152,3 +153,35 @@ def test_millions_of_rows(dev):
     want = (p * times[:, None] - pairs).T @ base
     off = np.abs(dW - want) / (e * ((p * times[:, None] + pairs).T @ np.abs(base)) + 2.0 ** -39 * N)
     assert off.max() <= 1.0, off.max()
+
+
+# ── polynomials whose iterates come near the largest singular value that is allowed, 4 ──
+
+FAR = [(2, (4.15, -1.25, 0.1)), (2, (3.375, -0.375, 0.0)), (3, (3.375, -0.375, 0.0)), (2, (4.0, 0.0, 0.0)), (2, (-4.0, 0.0, 0.0)), (2, (2.0, 1.0, 1.0)),
+       (2, (14.0, -0.5, 0.5))]
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (20, 30), (50, 90), (130, 100), (280, 260), (300, 700), (640, 300)], ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("steps,coef", FAR, ids=str)
+@pytest.mark.parametrize("axis", [False, True], ids=["", "axis"])
+def test_singular_values_up_to_4(dev, shape, steps, coef, axis):
+    """A single value, which starts at 1, and matrices with one strong direction, spread out or along an axis (where one entry of the Gram
+    matrix has all of its eigenvalue). The bound is iterate()'s, with (14, -0.5, 0.5) after one
+    step at 14, which only the last iterate may be."""
+    if coef[0] == 14.0:
+        steps = 1
+    r = np.random.default_rng(shape)
+    G = np.outer(r.standard_normal(shape[0]), r.standard_normal(shape[1])) + 0.02 * r.standard_normal(shape)
+    if axis:
+        G = 1e-4 * r.standard_normal(shape)
+        G[shape[0] // 2, shape[1] // 3] = 1.0
+    G = G.astype(np.float32)
+    want, err = TM.iterate(G.astype(np.float64), steps, coef)
+    a, b, c = coef
+    s = np.linalg.svd(G.astype(np.float64), compute_uv=False)
+    s = s / np.linalg.norm(s)
+    for _ in range(steps - 1):
+        s = a * s + b * s ** 3 + c * s ** 5
+        assert np.abs(s).max() <= 4.0
+    got = TM.ortho(dev, G, L.AH_F32, steps=steps, coef=coef)[0]
+    assert np.linalg.norm(got - want) <= err + U32 * np.linalg.norm(want), (np.linalg.norm(got - want), err, np.linalg.norm(want))

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(Muon d, const double *pa
     __shared__ double red[4];
     const long z = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (Cp + kSegment - 1) / kSegment;
-    const float inv = inverse_norm<256>(d, part, parts, z, red);
+    const double inv = inverse_norm<256>(d, part, parts, z, red);
     half_t *out = X + z * (long)Rp * Cp * 2;
     for (long q = (long)blockIdx.x * 4 + wave; q < (long)Rp * segs; q += (long)gridDim.x * 4) {
         const int r = (int)(q / segs), c0 = (int)(q - (long)r * segs) * kSegment + lane * 4;

@@ -32,21 +32,21 @@ __device__ __forceinline__ floatx4 update_of(const Muon &d, floatx4 g, floatx4 m
 // The elementwise passes give a wave one segment of a row at a time.
 constexpr int kSegment = 1024;
 
-// Four values of the update, at column c of row r of matrix z, times inv; zeros past the matrix.
-__device__ __forceinline__ floatx4 scaled_update(const Muon &d, long z, int r, int c, float inv) {
+// Four values of the update, at column c of row r of matrix z, times inv, which may pass f32's range; zeros past the matrix.
+__device__ __forceinline__ floatx4 scaled_update(const Muon &d, long z, int r, int c, double inv) {
     floatx4 v = {};
     if (r < d.rows && c < d.cols) {
         v = load_g(d, z, r, c);
         if (d.W) v = update_of(d, v, load4(d.M_out + z * d.sw + r * d.ldw, c, d.cols));
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] *= inv;
+        for (int k = 0; k < 4; k++) v[k] = (float)((double)v[k] * inv);
     }
     return v;
 }
 
-// 2^kSX / (|U| + eps) from the blocks' sums of squares; red: NT / 64 doubles of LDS. All NT threads of a workgroup.
+// 2^kSX / (|U| + eps), or 0 for a zero matrix, from the blocks' sums of squares; red: NT / 64 doubles of LDS. All NT threads of a workgroup.
 template <int NT>
-__device__ __forceinline__ float inverse_norm(const Muon &d, const double *part, int parts, long z, double *red) {
+__device__ __forceinline__ double inverse_norm(const Muon &d, const double *part, int parts, long z, double *red) {
     double s = 0.0;
     for (int i = threadIdx.x; i < parts; i += NT) s += part[z * parts + i];
     for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -54,7 +54,7 @@ __device__ __forceinline__ float inverse_norm(const Muon &d, const double *part,
     __syncthreads();
     s = red[0];
     for (int w = 1; w < NT / 64; w++) s += red[w];
-    return (float)((double)(1 << kSX) / (sqrt(s) + (double)d.eps));
+    return s == 0.0 ? 0.0 : (double)(1 << kSX) / (sqrt(s) + (double)d.eps);
 }
 
 // Four values of the last iterate (without the planes' scale) at column c of row r: into O, or into the weights.

@@ -146,7 +146,7 @@ __global__ __launch_bounds__(S / 32 * (S / 32) * 64, 1) void muon_small_kernel(S
     const auto slice_at = [&](int m, int n) { return WIDE ? image0<S>(m, n) : image1<S>(m, n); };   // of the image that add_gram reads
 
     if constexpr (WHAT == FIRST) {
-        const float inv = inverse_norm<NT>(d, p.part, p.parts, z, red);
+        const double inv = inverse_norm<NT>(d, p.part, p.parts, z, red);
         for (int sl = blockIdx.x; sl < p.slices; sl += p.groups) {
             const int m0 = WIDE ? 0 : sl * kSlice, n0 = WIDE ? sl * kSlice : 0;
             __syncthreads();

@@ -359,9 +359,9 @@ int ah_linear_ce(ah_device *dev, const ah_linear_ce_desc *d);
 
 /* Newton-Schulz orthogonalisation of a matrix G [rows, cols], or of `batch` of them:
  *   X = G / (|G|_F + eps); steps times: A = X X^T (X^T X if rows > cols), X <- (a I + b A + c A A) X (X (..)); O = X
- * dtype (of G) and out_dtype AH_F32 or AH_F16. The norm is summed in f64; products keep 22 bits of their operands and sum in
- * f32. The iterates before the last have to keep their singular values at 4 or less (a = 3.4445, b = -4.7750, c = 2.0315 keeps them
- * below 1.3; larger ones may end as infinities or NaN); |a| + |b| + |c| may be at most 15 and steps 1 to 64. A zero matrix gives zeros, a non-finite one NaN. O may be G. ldg, ldo: row
+ * dtype (of G) and out_dtype AH_F32 or AH_F16. The norm is summed in f64; products keep 22 bits of their operands (X down to
+ * 2^-37) and sum in f32. The iterates before the last have to keep their singular values at 4 or less (a = 3.4445, b = -4.7750, c = 2.0315 keeps them
+ * below 1.3; larger ones may end as infinities or NaN); |a| + |b| + |c| may be at most 15 and steps 1 to 64. A zero matrix gives zeros, whatever eps, a non-finite one NaN. O may be G. ldg, ldo: row
  * strides; stride_g, stride_o: from matrix to matrix, in elements (read only for batch > 1). */
 typedef struct {
     int32_t dtype, out_dtype;

@@ -185,3 +185,40 @@ def test_singular_values_up_to_4(dev, shape, steps, coef, axis):
         assert np.abs(s).max() <= 4.0
     got = TM.ortho(dev, G, L.AH_F32, steps=steps, coef=coef)[0]
     assert np.linalg.norm(got - want) <= err + U32 * np.linalg.norm(want), (np.linalg.norm(got - want), err, np.linalg.norm(want))
+
+
+# ── zero and tiny matrices ─────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("eps", [0.0, 1e-45, 1e-36, 1e-7])
+@pytest.mark.parametrize("shape", [(1, 1), (40, 70), (128, 300), (300, 280), (700, 300)], ids=lambda s: "%dx%d" % s)
+def test_zero_matrices_and_tiny_ones_in_a_batch(dev, shape, eps):
+    """Zero stays zero without a norm to divide by, beside others, and values of 2^-130 and less, whose norm's inverse passes f32's range, are
+    orthogonalised as they are. Planes end at 2^-24 of values scaled by 2^12: X is off by 2^-37 an entry where eps leaves it that small, and
+    five steps raise that by at most 3.4445^5 = 485."""
+    r = np.random.default_rng(shape)
+    big = TM.gradient(r, *shape, L.AH_F32)
+    tiny = (big * np.float32(2.0 ** -60)) * np.float32(2.0 ** -60)
+    G = np.stack([big, 0 * big, tiny, 0 * big])
+    assert 0 < np.abs(tiny).max() < 2.0 ** -120
+    got = TM.ortho(dev, G, L.AH_F32, eps=eps)
+    assert not got[1].any() and not got[3].any()
+    for z in (0, 2):
+        want, err = TM.iterate(G[z].astype(np.float64), eps=eps)
+        assert np.linalg.norm(got[z] - want) <= err + U32 * np.linalg.norm(want) + 485 * 2.0 ** -37 * want.size ** 0.5, z
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-45])
+@pytest.mark.parametrize("shape", [(64, 100), (300, 280)], ids=lambda s: "%dx%d" % s)
+def test_a_step_without_a_gradient_decays_the_weights(dev, shape, eps):
+    W = np.random.default_rng(3).standard_normal(shape).astype(np.float32)
+    bG, bM, bW, b16 = dev.buffer(np.zeros(shape, np.float32)), dev.buffer(np.zeros(shape, np.float32)), dev.buffer(W), dev.buffer(W.size, L.AH_F16)
+    args = dict(dtype=L.AH_F32, rows=shape[0], cols=shape[1], G=bG, M=bM, W=bW, W16_out=b16, lr=0.125, decay=0.5, eps=eps)
+    ws = dev.buffer(dev.muon_step_workspace(**args) // 4 + 4)
+    dev.muon_step(ws=ws, **args)
+    dev.sync()
+    want = np.float32(1 - 0.125 * 0.5) * W
+    np.testing.assert_array_equal(bW.read().reshape(shape), want)
+    np.testing.assert_array_equal(b16.read().reshape(shape), want.astype(np.float16))
+    assert not bM.read().any()
+    for b in (bG, bM, bW, b16, ws):
+        b.free()

@@ -40,6 +40,10 @@ struct TemplateKernel {
     std::function<std::vector<int64_t>(int64_t symval)> bytes;
     void *ws = nullptr;
     int64_t ws_bytes = 0;
+    // A graph that the caller captured from a launch may replay at any time: workspaces it holds are kept when a larger one replaces
+    // them (a plan captures again instead).
+    bool held = false;
+    std::vector<void *> kept;
     std::function<int(ah_device *, TemplateKernel *self, void *const *ptrs, int32_t n_ptrs, const int32_t *scalars,
                       int32_t n_scalars)>
         run;
@@ -73,6 +77,8 @@ struct ah_device {
     // f16 GEMM variant chosen by ah_gemm_tune per (ta, tb, M, N, K); used when a launch asks for
     // variant 0 (the role of BEAM's cache, codegen/beam.go:118-169).
     std::unordered_map<std::string, int> gemm_variant;
+    // A plan is capturing its items: the graph is its own, and it drops it when a workspace moves.
+    bool plan_capture = false;
     // This device's address of the chain's file-scope workspace (ah_chain_step_noalloc), set by ah_open.
     float *chain_scratch = nullptr;
     // This handle's counters of the chain's strip kernel (chain_sync_max_ints, zero between launches), for ah_chain_step_noalloc.
@@ -94,7 +100,7 @@ int template_create(const std::string &source, TemplateKernel **out);
 // "tmpl:<name>;k=v;..." -> name and the k=v map.
 std::unordered_map<std::string, std::string> template_key_params(const std::string &key, std::string *name);
 // Grows the template's workspace for the binding symval (before a graph capture).
-int template_prepare(TemplateKernel *t, int64_t symval);
+int template_prepare(ah_device *d, TemplateKernel *t, int64_t symval);
 std::string wgsl_to_hip(const std::string &src, std::string *err, bool *wave = nullptr);
 // A "tmpl:gemm" key for a WGSL kernel that is a plain contraction (wgsl_match.cpp), else false.
 bool wgsl_match_contraction(const std::string &src, std::string *key);

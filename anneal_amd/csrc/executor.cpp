@@ -56,6 +56,7 @@ struct ah_plan {
         int n_sym = 0;
         int32_t ls[3], wg[3];
         ah_kernel *k = nullptr;
+        void *ws = nullptr;        // the template's workspace at the last run
         std::vector<int> writes;   // PARAM positions written: 0 plus the template's side outputs
         std::vector<bool> clear;   // per entry of writes: zero before the launch
     };
@@ -239,7 +240,8 @@ int plan_run(ah_plan *p, const ah_input *inputs, int32_t n_inputs, int64_t n, bo
     *n_outputs = 0;
     if (p->items.empty()) return AH_OK;
     if (int rc = plan_alloc(p, n)) return rc;
-    // Template workspaces for this binding; a workspace that moves invalidates captured graphs. First,
+    // Template workspaces for this binding; one that is not where it was at the last run, whoever moved it (launches of one key share
+    // a workspace, other plans' among them), invalidates captured graphs. First,
     // every buffer a template reads or writes must hold what its key's shape needs: the hand-written
     // kernels index by the key's M, N, K (and the like), not by the buffer sizes.
     for (size_t i = 0; i < p->items.size(); i++) {
@@ -261,9 +263,9 @@ int plan_run(ah_plan *p, const ah_input *inputs, int32_t n_inputs, int64_t n, bo
     for (size_t i = 0; i < p->items.size(); i++) {
         TemplateKernel *t = p->items[i].k->tmpl;
         if (!t) continue;
-        void *before = t->ws;
-        if (int rc = template_prepare(t, symbolic ? n : 0)) return set_error(rc, "ah_run: kernel %zu: %s", i, ah_last_error());
-        if (t->ws != before) p->drop_graphs();
+        if (int rc = template_prepare(d, t, symbolic ? n : 0)) return set_error(rc, "ah_run: kernel %zu: %s", i, ah_last_error());
+        if (t->ws != p->items[i].ws) p->drop_graphs();
+        p->items[i].ws = t->ws;
     }
     // Leaves: the input's elements, zeros after them (fresh-buffer semantics); no input: all zeros.
     std::map<uint32_t, const ah_input *> in;
@@ -285,7 +287,9 @@ int plan_run(ah_plan *p, const ah_input *inputs, int32_t n_inputs, int64_t n, bo
         auto g = p->graphs.find(key);
         if (g == p->graphs.end()) {
             if (int rc = ah_graph_begin(d)) return rc;
+            d->plan_capture = true;
             int rc = plan_enqueue(p, n, symbolic);
+            d->plan_capture = false;
             ah_graph *cg = nullptr;
             int rc2 = ah_graph_end(d, &cg);
             if (rc) { ah_graph_destroy(cg); return rc; }
@@ -411,7 +415,7 @@ int ah_benchmark(ah_device *d, const ah_exec_item *item, int32_t warmup, int32_t
     ah_kernel *k = nullptr;
     int rc = ah_module_get(d, item->source, "kernel", &k);
     if (rc) return rc;
-    if (k->tmpl && (rc = template_prepare(k->tmpl, 0))) return rc;
+    if (k->tmpl && (rc = template_prepare(d, k->tmpl, 0))) return rc;
     if (k->tmpl && k->tmpl->bytes) {   // buffers sized below what the key's shape needs: refuse before launching
         const std::vector<int64_t> want = k->tmpl->bytes(0);
         if ((int32_t)want.size() > item->n_bufs)

@@ -132,10 +132,14 @@ int need(const char *key, int32_t n_ptrs, int want) {
 }
 
 // Grows the template's own device workspace (kept for the device's lifetime; never under capture when
-// the caller prepares items first, as ah_plan does). A new workspace starts zeroed.
-int ensure_ws(TemplateKernel *t, int64_t bytes) {
+// the caller prepares items first, as ah_plan does). A new workspace starts zeroed. Launches of one key share it.
+int ensure_ws(ah_device *d, TemplateKernel *t, int64_t bytes) {
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (!t->held && !d->plan_capture && hipStreamIsCapturing(d->stream, &capture) == hipSuccess && capture == hipStreamCaptureStatusActive)
+        t->held = true;
     if (bytes <= t->ws_bytes) return AH_OK;
-    if (t->ws) AH_HIP(hipFree(t->ws));
+    if (t->ws && t->held) t->kept.push_back(t->ws);
+    else if (t->ws) AH_HIP(hipFree(t->ws));
     t->ws = nullptr;
     t->ws_bytes = 0;
     AH_HIP(hipMalloc(&t->ws, (size_t)bytes));
@@ -280,7 +284,7 @@ int template_gemm(const Params &P, TemplateKernel *t) {
             const int64_t sv = (M.sym || N.sym || K.sym) && ns > 0 ? sc[0] : 0;
             int64_t offB = 0;
             const int64_t bytes = ws_layout(sv, &offB);
-            if (int rc = ensure_ws(self, bytes)) return rc;
+            if (int rc = ensure_ws(d, self, bytes)) return rc;
             const bool f16 = base.dtype == GEMM_F16;
             if (proA) {
                 void *dst = self->ws;
@@ -378,7 +382,7 @@ int template_reduce(const Params &P, TemplateKernel *t) {
         if (axis == 1) {
             AH_HIP(reduce_rows(ptrs[1], f16, (int)m, (int)n, op, scale, (float *)ptrs[0], d->stream));
         } else {
-            if (int rc = ensure_ws(self, reduce_cols_workspace((int)m, (int)n) * 4)) return rc;
+            if (int rc = ensure_ws(d, self, reduce_cols_workspace((int)m, (int)n) * 4)) return rc;
             AH_HIP(reduce_cols(ptrs[pA], f16, (int)m, (int)n, op, scale, (float *)self->ws, (float *)ptrs[0], d->stream,
                                mask ? ptrs[pZ] : nullptr, wz));
         }
@@ -512,7 +516,7 @@ int template_conv(const Params &P, TemplateKernel *t, ConvKind kind) {
             break;
         case CONV_BWD_W: {
             const int64_t bytes = (int64_t)conv_bwd_w_splits((int)n, (int)Ci.v, (int)H.v, (int)Co.v) * Co.v * Ci.v * 10 * 4;
-            if (int rc = ensure_ws(self, bytes)) return rc;
+            if (int rc = ensure_ws(d, self, bytes)) return rc;
             AH_HIP(conv_bwd_w_partial(in1, in2, (int)n, (int)Ci.v, (int)H.v, (int)Co.v, (float *)self->ws, d->stream));
             AH_HIP(conv_bwd_w_finalize((const float *)self->ws, (int)n, (int)Ci.v, (int)H.v, (int)Co.v, nullptr, nullptr, 0.0f,
                                        (float *)ptrs[0], nullptr, d->stream));
@@ -573,7 +577,7 @@ int template_chain(const Params &P, TemplateKernel *t) {
     const std::string key = t->key;
     t->run = [=](ah_device *d, TemplateKernel *self, void *const *ptrs, int32_t n_ptrs, const int32_t *, int32_t) -> int {
         if (int rc = need(key.c_str(), n_ptrs, 5)) return rc;
-        if (int rc = ensure_ws(self, chain_workspace_floats((int)R.v, (int)Cc.v) * 4)) return rc;
+        if (int rc = ensure_ws(d, self, chain_workspace_floats((int)R.v, (int)Cc.v) * 4)) return rc;
         AH_HIP(chain_step((const float *)ptrs[1], (const float *)ptrs[2], (int)R.v, (int)Cc.v, (float *)self->ws,
                           (float *)ptrs[0], (float *)ptrs[3], (float *)ptrs[4], d->stream, -1, nullptr, spin));
         return AH_OK;
@@ -641,7 +645,7 @@ int template_linear_ce(const Params &P, TemplateKernel *t) {
         AT(N, n);
         if (n < 1 || n > 1 << 27 || n * D.v > 1l << 40) return set_error(AH_ERR_INVALID, "%s: N=%ld", key.c_str(), n);
         const LinearCe a = with(n, ptrs);
-        if (int rc = ensure_ws(self, linear_ce_workspace(a))) return rc;
+        if (int rc = ensure_ws(d, self, linear_ce_workspace(a))) return rc;
         AH_HIP(linear_ce(a, self->ws, d->stream));
         return AH_OK;
     };
@@ -686,7 +690,7 @@ int template_orthogonalize(const Params &P, TemplateKernel *t) {
     t->workspace = [=](int64_t) { return muon_workspace(m); };
     t->run = [=](ah_device *d, TemplateKernel *self, void *const *ptrs, int32_t n_ptrs, const int32_t *, int32_t) -> int {
         if (int rc = need(key.c_str(), n_ptrs, 2)) return rc;
-        if (int rc = ensure_ws(self, muon_workspace(m))) return rc;
+        if (int rc = ensure_ws(d, self, muon_workspace(m))) return rc;
         Muon a = m;
         a.O = ptrs[0];
         a.G = ptrs[1];
@@ -713,7 +717,7 @@ int template_muon(const Params &P, TemplateKernel *t) {
     t->workspace = [=](int64_t) { return muon_workspace(m); };
     t->run = [=](ah_device *d, TemplateKernel *self, void *const *ptrs, int32_t n_ptrs, const int32_t *, int32_t) -> int {
         if (int rc = need(key.c_str(), n_ptrs, 5)) return rc;
-        if (int rc = ensure_ws(self, muon_workspace(m))) return rc;
+        if (int rc = ensure_ws(d, self, muon_workspace(m))) return rc;
         Muon a = m;
         a.W_out = (float *)ptrs[0];
         a.W = (const float *)ptrs[1];
@@ -730,11 +734,12 @@ int template_muon(const Params &P, TemplateKernel *t) {
 
 TemplateKernel::~TemplateKernel() {
     if (ws) (void)hipFree(ws);
+    for (void *p : kept) (void)hipFree(p);
 }
 
-int template_prepare(TemplateKernel *t, int64_t symval) {
+int template_prepare(ah_device *d, TemplateKernel *t, int64_t symval) {
     if (!t->workspace) return AH_OK;
-    return ensure_ws(t, t->workspace(symval));
+    return ensure_ws(d, t, t->workspace(symval));
 }
 
 int template_create(const std::string &source, TemplateKernel **out) {

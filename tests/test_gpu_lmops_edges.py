@@ -1,9 +1,12 @@
 """Single roundings, limits and rare states of ah_linear_ce, ah_orthogonalize and ah_muon_step (GPU). Tolerances as in
 test_gpu_linear_ce.py and test_gpu_muon.py where none is derived here."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import test_gpu_linear_ce as TL
+import test_gpu_lmops_run as TR
 import test_gpu_muon as TM
 from anneal_amd import _lib as L
 
@@ -222,3 +225,73 @@ def test_a_step_without_a_gradient_decays_the_weights(dev, shape, eps):
     assert not bM.read().any()
     for b in (bG, bM, bW, b16, ws):
         b.free()
+
+
+# ── a key's workspace, which all of its launches share ─────────────────────────
+
+def _traps(dev, mib):
+    """Memory of the sizes that a workspace may have left behind, filled with NaN."""
+    return [dev.buffer(np.full(m << 18, np.nan, np.float32)) for m in mib]
+
+
+def _untouched(traps):
+    for t in traps:
+        assert np.isnan(t.read()).all()
+        t.free()
+
+
+def test_plans_of_one_key_with_other_batches(dev):
+    """A second plan's larger batch moves the workspace that the first one's graph holds."""
+    key = dict(dtype=L.AH_F32, bias=True)
+    small, large = TL.Case(70, 47, 530, **key), TL.Case(900, 47, 530, **key)
+    item = TR._head_item(small, sym=True)[0]
+    plans = [TR.Plan(dev, [item], graph=True) for _ in range(2)]
+    TL.compare(TR._head_values(small, plans[0].run(TR._head_item(small)[1], {"n": 70})), small.exact())
+    TL.compare(TR._head_values(large, plans[1].run(TR._head_item(large)[1], {"n": 900})), large.exact())
+    traps = _traps(dev, (1, 1, 2, 2, 4))
+    for seed in (1, 2):
+        c = TL.Case(70, 47, 530, seed=seed, **key)
+        TL.compare(TR._head_values(c, plans[0].run(TR._head_item(c)[1], {"n": 70})), c.exact())
+    TL.compare(TR._head_values(large, plans[1].run(TR._head_item(large)[1], {"n": 900})), large.exact())
+    _untouched(traps)
+    captures, replays = plans[0].stats()
+    assert captures <= 2 and replays >= 1   # captured again at most once
+    for p in plans:
+        p.close()
+
+
+def test_a_callers_graph_keeps_the_workspace(dev):
+    """A launch of a key that the caller captured replays soundly after a larger launch of the key."""
+    c, large = TL.Case(66, 43, 270, dtype=L.AH_F32, bias=True), TL.Case(1000, 43, 270, dtype=L.AH_F32, bias=True)
+    key = ("tmpl:linear_ce;dtype=f32;grad=f32;N=sym;D=43;V=270;bias=1").encode()
+    k = C.c_void_p()
+    L.check(dev.lib.ah_module_get(dev.h, key, b"kernel", C.byref(k)))
+
+    def launch(c, b):
+        order = [b[n].ptr for n in ("dX", "X", "W", "labels", "bias", "dW", "loss", "dbias")]
+        one = (C.c_uint32 * 3)(1, 1, 1)
+        L.check(dev.lib.ah_launch(dev.h, k, one, one, (C.c_void_p * 8)(*order), 8, (C.c_int32 * 4)(*[c.N] * 4), 4))
+
+    want = ("dX", "dW", "loss", "dbias")
+    bufs = [TL.buffers(dev, x, want) for x in (c, large)]
+    launch(c, bufs[0])
+    dev.sync()
+    g = C.c_void_p()
+    L.check(dev.lib.ah_graph_begin(dev.h))
+    launch(c, bufs[0])
+    L.check(dev.lib.ah_graph_end(dev.h, C.byref(g)))
+    launch(large, bufs[1])
+    dev.sync()
+    traps = _traps(dev, (1, 1, 2))
+    for _ in range(3):
+        for n in want:
+            bufs[0][n].write(np.zeros(bufs[0][n].n, np.float32))
+        L.check(dev.lib.ah_graph_replay(dev.h, g))
+        dev.sync()
+        shapes = {"dX": (c.N, c.D), "dW": (c.V, c.D)}
+        TL.compare({n: bufs[0][n].read().astype(np.float64).reshape(shapes.get(n, -1)) for n in want}, c.exact())
+    _untouched(traps)
+    dev.lib.ah_graph_destroy(g)
+    for b in bufs:
+        for v in b.values():
+            v.free()

@@ -39,10 +39,10 @@ struct Scalars {
     int pad;
 };
 
-// Power of two that brings the largest magnitude into [2^14, 2^15); 0 for all-zero or non-finite operands.
+// Power of two that brings the largest finite magnitude into [2^14, 2^15); 0 where there is none but 0.
 __device__ __forceinline__ int plane_exp(unsigned maxbits) {
     const float m = __uint_as_float(maxbits);
-    if (!(m > 0.0f) || maxbits >= 0x7f800000u) return 0;
+    if (!(m > 0.0f)) return 0;
     return min(14 - ilogbf(m), 120);
 }
 
@@ -113,7 +113,12 @@ __device__ __forceinline__ void index_rows(const ScanArgs &a) {
 }
 
 // Workgroup 0 indexes the rows; the others (f32 operands) find the largest magnitudes of W and of the counted rows of X, a wave per
-// stretch of 2048 values of a row. The bits of non-negative floats order as integers.
+// stretch of 2048 values of a row. The bits of non-negative floats order as integers. Infinities and NaN are passed over: they make their
+// own row's logits NaN under any scale, and the other rows' scale is not theirs.
+__device__ __forceinline__ unsigned magnitude(uint32_t bits) {
+    bits &= 0x7fffffffu;
+    return bits < 0x7f800000u ? bits : 0;
+}
 __global__ __launch_bounds__(256) void lce_scan_kernel(ScanArgs a) {
     if (blockIdx.x == 0) {
         index_rows(a);
@@ -134,10 +139,10 @@ __global__ __launch_bounds__(256) void lce_scan_kernel(ScanArgs a) {
         for (int k = 0; k < 2048; k += 256) {
             const int c = c0 + k;
             if (c + 3 < end) {
-                const u4 v = *(const u4 *)(p + c) & 0x7fffffffu;
-                m = max(m, max(max(v[0], v[1]), max(v[2], v[3])));
+                const u4 v = *(const u4 *)(p + c);
+                m = max(m, max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3]))));
             } else {
-                for (int u = c; u < end; u++) m = max(m, p[u] & 0x7fffffffu);
+                for (int u = c; u < end; u++) m = max(m, magnitude(p[u]));
             }
         }
         if (x) mx = max(mx, m);

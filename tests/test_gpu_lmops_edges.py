@@ -295,3 +295,28 @@ def test_a_callers_graph_keeps_the_workspace(dev):
     for b in bufs:
         for v in b.values():
             v.free()
+
+
+# ── rows that are not finite ───────────────────────────────────────────────────
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf], ids=str)
+@pytest.mark.parametrize("scale", [1e6, 1e-6, 1.0])
+@pytest.mark.parametrize("N", [60, 200])
+@pytest.mark.parametrize("types", TL.TYPES, ids=["f32", "f16", "f16_f32grad"])
+def test_rows_that_are_not_finite_leave_the_others(dev, types, N, scale, bad):
+    """A counted row with an infinity or NaN has a NaN loss and dX, and the weights' gradients are NaN; the other rows are as they are without
+    it, whatever the size of their values (f32 operands share one power of two)."""
+    if types[0] == L.AH_F16 and scale != 1.0:
+        scale = 2.0 ** 8 if scale > 1 else 2.0 ** -6
+    c = TL.Case(N, 64, 300, dtype=types[0], grad_dtype=types[1], std=scale, wstd=0.125 / scale)
+    c.X[9, 3] = bad
+    s = 64.0 * (scale if types[1] == L.AH_F16 else 1.0)
+    got = TL.run(dev, c, want=("loss", "rowloss", "lse", "dX", "dW"), mean=False, grad_scale=s)
+    c.labels[9] = -1   # the oracle without the row
+    exact = c.exact(mean=False, grad_scale=s)
+    keep = np.arange(N) != 9
+    for k in ("rowloss", "lse", "dX"):
+        assert np.isnan(got[k][9]).all()
+        v, tol = exact[k]
+        assert np.all(np.abs(got[k][keep] - v[keep]) <= tol[keep]), k
+    assert np.isnan(got["loss"][0]) and np.isnan(got["dW"]).all()

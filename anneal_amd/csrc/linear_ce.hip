@@ -831,7 +831,6 @@ constexpr int kBlockRowsLog = 17;               // rows of a block of packed W, 
 // Rows up to which a W that would have to be packed is read as it lies. 4096 features, 32000 classes in f32, with gradients, packed and as
 // it lies: 16 rows 731 and 438 us, 128 rows 823 and 850; the loss alone 433 and 139 us at 16 rows, 545 and 367 at 121 (2944 x 51416).
 constexpr int kFewRows = 128;
-constexpr int kStatCols = 32;                  // the narrowest wave tile: bounds the statistics' columns
 
 struct Layout {
     int Dp, Vp, P;             // padded widths; planes of X and W
@@ -849,6 +848,8 @@ pg::Plan plan_of(int64_t M, int64_t N, int64_t k, int pa, int pb, bool narrow) {
     return pg::plan([&](int w) { return (long)ceil_div(M, w) * ceil_div(N, w); }, k, pa, pb, narrow);
 }
 pg::Plan logits_plan(const Layout &l, int V, int rows) { return plan_of(rows, V, l.Dp, l.P, l.P, true); }
+// Statistics of a row: one for each wave tile of the logits' product.
+int stat_tiles(const Layout &l, int V, int rows) { return l.few ? ceil_div(V, 128) * 4 : ceil_div(V, logits_plan(l, V, rows).width) * 2; }
 // (64-wide tiles of one plane have no layout for operands along k)
 pg::Plan dx_plan(const Layout &l, const LinearCe &d, int rows) { return plan_of(rows, d.D, d.V, l.PP, l.P, l.P == 2); }
 // Room for partial tiles: four rounds of them where half a round to two rounds of tiles may turn out to be fewer (below that, what
@@ -882,9 +883,14 @@ Layout layout(const LinearCe &d) {
         l.few = d.N <= 16 ? 1 : d.N <= 64 ? 4 : 8;
     }
     const int64_t Np = ((int64_t)d.N + 63) & ~63ll;
+    const int64_t piece = (int64_t)(d.piece_mb ? d.piece_mb : kPieceMb) << 20;
     int64_t rows = Np;
-    if (l.grad) rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, ((int64_t)(d.piece_mb ? d.piece_mb : kPieceMb) << 20) / ((int64_t)l.Vp * 4) / 256 * 256)});
-    else rows = std::min<int64_t>(rows, 16384);
+    if (l.grad) {
+        rows = std::min({rows, (int64_t)kMaxPieceRows, std::max<int64_t>(256, piece / ((int64_t)l.Vp * 4) / 256 * 256)});
+    } else {   // without gradients the statistics are what a piece keeps
+        rows = std::min<int64_t>(rows, 16384);
+        while (rows > 256 && rows * stat_tiles(l, d.V, (int)rows) * 8 > piece) rows = (rows / 2 + 255) / 256 * 256;
+    }
     l.pieces = (int)((Np + rows - 1) / rows);
     if (l.pieces > 1) rows = ((Np + l.pieces - 1) / l.pieces + 255) / 256 * 256;
     l.rows = (int)rows;
@@ -903,7 +909,8 @@ Layout layout(const LinearCe &d) {
     l.zt = take(Np * 4);
     l.lse = take(Np * 4);
     l.loss = take(Np * 4);
-    l.stats = take(rows * ((l.Vp + 255) / 256 * 256 / kStatCols) * 8);
+    const int64_t last = Np - (l.pieces - 1) * rows;   // the last piece has fewer rows, and its own plan
+    l.stats = take(std::max(rows * stat_tiles(l, d.V, (int)rows), last * stat_tiles(l, d.V, (int)last)) * 8);
     l.Xp = take(Np * l.Dp * 2 * l.P);
     l.wshift = d.V <= pg::kMaxPanelRows ? 31 : kBlockRowsLog;
     l.wstored = l.wshift == 31 ? d.V : 1 << kBlockRowsLog;
@@ -913,7 +920,7 @@ Layout layout(const LinearCe &d) {
     if (d.dbias) l.dbpart = take(Np / kGradRows * d.V * 4);
     if (d.dW && d.g16 && l.pieces > 1) l.dwacc = take((int64_t)d.V * d.D * 4);
     int64_t sums = 0;
-    for (const int64_t r : {rows, Np - (l.pieces - 1) * rows}) {   // the last piece has fewer rows, and its own plan
+    for (const int64_t r : {rows, last}) {
         sums = std::max(sums, l.few ? few_part_bytes(l, few_logits_work(l, d), 128) : (int64_t)logits_plan(l, d.V, (int)r).part_bytes());
         if (d.dX && l.few) sums = std::max(sums, few_part_bytes(l, few_dx_work(l, d), 256));
         else if (d.dX) {
@@ -1081,7 +1088,7 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         a.lab = lab + row0;
         a.zt = zt + row0;
         a.stats = stats;
-        a.T = ceil_div(d.V, l.few ? 128 : plan.width) * (l.few ? 4 : 2);
+        a.T = stat_tiles(l, d.V, rows);
         a.E = ws + l.E;
         a.Vp = l.Vp;
         if (l.few) {

@@ -350,7 +350,7 @@ typedef struct {
     int64_t lddw;
     float *dbias;
     float grad_scale;
-    int32_t piece_mb;      /* MiB of logits that are kept at a time with gradients; 0: 2048. At least 256 rows are */
+    int32_t piece_mb;      /* MiB of logits that are kept at a time with gradients, or of statistics without; 0: 2048. At least 256 rows are */
     void *ws;
     int64_t ws_bytes;
 } ah_linear_ce_desc;

@@ -297,6 +297,20 @@ def test_a_callers_graph_keeps_the_workspace(dev):
             v.free()
 
 
+# ── pieces ─────────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("dtype", [L.AH_F32, L.AH_F16], ids=["f32", "f16"])
+def test_the_loss_alone_in_pieces(dev, dtype):
+    """Statistics of 1 MiB: 256 rows at a time, the same losses bit for bit."""
+    y = np.random.default_rng(4).integers(-5000, 30001, 900)
+    c = TL.Case(900, 64, 30001, dtype=dtype, grad_dtype=dtype, labels=y)
+    want = ("loss", "rowloss", "lse")
+    one, many = TL.run(dev, c, want=want), TL.run(dev, c, want=want, piece_mb=1)
+    TL.compare(one, c.exact())
+    for k in want:
+        np.testing.assert_array_equal(one[k], many[k], err_msg=k)
+
+
 # ── rows that are not finite ───────────────────────────────────────────────────
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf], ids=str)

@@ -457,7 +457,7 @@ struct GradArgs {
     const int *lab;
     char *E;                        // the logits, then P
     float *res;                     // one plane: what its rounding leaves of each row's P at its label
-    float *dbpart;                  // [row block][V] column sums of P, or null
+    float *dbpart;                  // [row block of the piece][V] column sums of P, or null
 };
 
 // e^x: the product with log2 e carries what its rounding loses, which at x = -10 is 3e-7 of the result.
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256) void lce_grad_kernel(GradArgs a) {
 #pragma unroll
         for (int c = 0; c < NC; c++)
             if (n + c < a.V)
-                a.dbpart[((long)(a.row0 + r0) / kGradRows) * a.V + n + c] =
+                a.dbpart[(long)blockIdx.y * a.V + n + c] =
                     col[c] + red[0][threadIdx.x][c] + red[1][threadIdx.x][c] + red[2][threadIdx.x][c];
 }
 
@@ -529,16 +529,27 @@ __device__ __forceinline__ float grad_mult(const Scalars *sc, float grad_scale, 
     return mean ? grad_scale / (float)max(1, sc->count) : grad_scale;
 }
 
-// Workgroup 0: the loss, in f64. The others: db, the row blocks' sums in order.
-__global__ __launch_bounds__(256) void lce_finish_kernel(const Scalars *sc, const float *loss_c, int mean, float *loss, const float *part, int V,
-                                                         float grad_scale, float *dbias) {
+// db's sum of P over the rows to the end of the piece [row0, row0 + rows): what the pieces before left in dbias, then the piece's row
+// blocks in order.
+__device__ __forceinline__ float db_sum(const Scalars *sc, int row0, int rows, const float *part, int V, const float *dbias, int n) {
+    const int blocks = (chunk_rows(&sc->count, row0, rows) + kGradRows - 1) / kGradRows;
+    float s = row0 ? dbias[n] : 0.0f;
+    for (int b = 0; b < blocks; b++) s += part[(long)b * V + n];
+    return s;
+}
+// After a piece that others follow.
+__global__ __launch_bounds__(256) void lce_db_kernel(const Scalars *sc, int row0, int rows, const float *part, int V, float *dbias) {
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n < V) dbias[n] = db_sum(sc, row0, rows, part, V, dbias, n);
+}
+
+// Workgroup 0: the loss, in f64. The others: db, after the last piece.
+__global__ __launch_bounds__(256) void lce_finish_kernel(const Scalars *sc, const float *loss_c, int mean, float *loss, int row0, int rows,
+                                                         const float *part, int V, float grad_scale, float *dbias) {
     const int c = sc->count, t = threadIdx.x;
     if (blockIdx.x > 0) {
-        const int n = (blockIdx.x - 1) * 256 + t, blocks = (c + kGradRows - 1) / kGradRows;
-        if (n >= V) return;
-        float s = 0.0f;
-        for (int b = 0; b < blocks; b++) s += part[(long)b * V + n];
-        dbias[n] = ldexpf(s, -kPScale) * grad_mult(sc, grad_scale, mean);
+        const int n = (blockIdx.x - 1) * 256 + t;
+        if (n < V) dbias[n] = ldexpf(db_sum(sc, row0, rows, part, V, dbias, n), -kPScale) * grad_mult(sc, grad_scale, mean);
         return;
     }
     __shared__ double red[4];
@@ -917,7 +928,7 @@ Layout layout(const LinearCe &d) {
     if (l.pack_w) l.Wp = take((((int64_t)d.V - 1 >> l.wshift) + 1) * l.wstored * l.Dp * 2 * l.P);
     if (l.grad) l.E = take(rows * l.Vp * 4);
     if (l.PP == 1) l.res = take(rows * 4);
-    if (d.dbias) l.dbpart = take(Np / kGradRows * d.V * 4);
+    if (d.dbias) l.dbpart = take(rows / kGradRows * d.V * 4);
     if (d.dW && d.g16 && l.pieces > 1) l.dwacc = take((int64_t)d.V * d.D * 4);
     int64_t sums = 0;
     for (const int64_t r : {rows, last}) {
@@ -1112,6 +1123,8 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         const dim3 ggrid((unsigned)ceil_div(l.Vp, 256), (unsigned)ceil_div(rows, kGradRows));
         if (l.PP == 1) hipLaunchKernelGGL(lce_grad_kernel<1>, ggrid, dim3(256), 0, s, g);
         else hipLaunchKernelGGL(lce_grad_kernel<2>, ggrid, dim3(256), 0, s, g);
+        if (d.dbias && piece + 1 < l.pieces)
+            hipLaunchKernelGGL(lce_db_kernel, dim3((unsigned)ceil_div(d.V, 256)), dim3(256), 0, s, sc, row0, rows, g.dbpart, d.V, d.dbias);
         ProductArgs p{};
         p.sc = sc;
         p.row0 = row0;
@@ -1127,8 +1140,9 @@ hipError_t linear_ce(const LinearCe &d, void *wsp, hipStream_t s) {
         else if (d.f16) gradients<2, 1>(d, l, p, W, X, piece, ws, s);
         else gradients<2, 2>(d, l, p, W, X, piece, ws, s);
     }
-    hipLaunchKernelGGL(lce_finish_kernel, dim3((unsigned)(1 + (d.dbias ? ceil_div(d.V, 256) : 0))), dim3(256), 0, s, sc, loss, d.mean, d.loss,
-                       (const float *)(ws + l.dbpart), d.V, d.grad_scale, d.dbias);
+    const int last = (l.pieces - 1) * l.rows;
+    hipLaunchKernelGGL(lce_finish_kernel, dim3((unsigned)(1 + (d.dbias ? ceil_div(d.V, 256) : 0))), dim3(256), 0, s, sc, loss, d.mean, d.loss, last,
+                       Np - last, (const float *)(ws + l.dbpart), d.V, d.grad_scale, d.dbias);
     return hipGetLastError();
 }
 

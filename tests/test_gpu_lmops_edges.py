@@ -311,6 +311,19 @@ def test_the_loss_alone_in_pieces(dev, dtype):
         np.testing.assert_array_equal(one[k], many[k], err_msg=k)
 
 
+@pytest.mark.parametrize("types", TL.TYPES, ids=["f32", "f16", "f16_f32grad"])
+def test_db_adds_up_over_pieces_in_order(dev, types):
+    """db is summed in place over pieces, some of which have no row that counts. (Pieces of other sizes may have other tiles, whose statistics
+    round otherwise: each result has the bound of the whole, and repeats bit for bit by itself.)"""
+    y = np.random.default_rng(6).integers(0, 2100, 1100)
+    y[300:900] = -1
+    c = TL.Case(1100, 72, 2100, dtype=types[0], grad_dtype=types[1], labels=y)
+    one, many, again = (TL.run(dev, c, want=("loss", "dX", "dbias"), piece_mb=mb) for mb in (0, 1, 1))
+    for got in (one, many):
+        TL.compare(got, c.exact())
+    np.testing.assert_array_equal(many["dbias"], again["dbias"])
+
+
 # ── rows that are not finite ───────────────────────────────────────────────────
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf], ids=str)

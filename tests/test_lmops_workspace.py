@@ -39,3 +39,11 @@ def test_piece_mb_bounds_the_statistics(mb, dtype):
     packed = 2 * e * D * (N + (V + (1 << 17) if e == 2 else 0))
     bound = max((mb or 2048) * MB, 256 * V // 32 * 8) + packed + 64 * N + 256 * MB
     assert workspace((), N=N, D=D, V=V, dtype=dtype, grad_dtype=dtype, piece_mb=mb) <= bound
+
+
+@pytest.mark.parametrize("dtype", [L.AH_F16, L.AH_F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("mb", [0, 512])
+def test_a_bias_adds_a_64th_of_a_piece(mb, dtype):
+    """db's partial sums are a float a class for 64 rows of the piece that is worked on, not of all rows."""
+    kw = dict(N=1 << 20, D=64, V=131072, dtype=dtype, grad_dtype=dtype, piece_mb=mb)
+    assert workspace(("dX", "dbias"), **kw) - workspace(("dX",), **kw) <= (mb or 2048) * MB // 64 + 4096

@@ -23,6 +23,7 @@ struct OnDevice {
 };
 
 constexpr int64_t kMaxSide = 1 << 20, kMaxRows = 1 << 27, kMaxStride = 1ll << 40, kMaxElems = 1ll << 40;
+constexpr int64_t kMaxSpan = 1ll << 48;   // elements from a strided array's first to its last: their bytes stay within 64 bits
 
 // A block of device memory: rows of `width` bytes, `ld` bytes apart.
 struct Span {
@@ -71,6 +72,9 @@ int linear_ce_args(ah_device *dev, const ah_linear_ce_desc *d, LinearCe *o) {
     if (d->ldx < d->D || d->ldw < d->D || (d->dX && d->lddx < d->D) || (d->dW && d->lddw < d->D) || d->ldx > kMaxStride || d->ldw > kMaxStride ||
         (d->dX && d->lddx > kMaxStride) || (d->dW && d->lddw > kMaxStride))
         return set_error(AH_ERR_INVALID, "%s: a row stride is less than D=%d or past 2^40", fn, d->D);
+    const auto spans = [](int64_t rows, int64_t ld) { return rows > 1 && ld > kMaxSpan / (rows - 1); };
+    if (spans(d->N, d->ldx) || spans(d->V, d->ldw) || (d->dX && spans(d->N, d->lddx)) || (d->dW && spans(d->V, d->lddw)))
+        return set_error(AH_ERR_INVALID, "%s: rows that span more than 2^48 elements", fn);
     if (!std::isfinite(d->grad_scale)) return set_error(AH_ERR_INVALID, "%s: grad_scale is not finite", fn);
     if (d->piece_mb < 0) return set_error(AH_ERR_INVALID, "%s: piece_mb=%d", fn, d->piece_mb);
     const int e = esize(d->dtype), g = esize(d->grad_dtype);

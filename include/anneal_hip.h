@@ -329,7 +329,8 @@ int ah_chain_step_noalloc(ah_device *dev, const float *X, const float *g, int32_
  * (dX, dW) AH_F32, or AH_F16 where dtype is AH_F16. loss, rowloss, lse and dbias are f32; losses and statistics are computed in
  * f32 or wider. f32 operands take part in the products with 22 bits of each value (less below 2^-14 of the operand's largest
  * magnitude), and P with 22 bits for f32 gradients and 11 for f16 ones, down to an absolute 2^-40. Gradients of f16 that would
- * underflow take a loss scale as grad_scale. Results repeat bit for bit (for one piece_mb: more pieces round dW more often). Row strides ldx, ldw, lddx, lddw are in elements.
+ * underflow take a loss scale as grad_scale. Results repeat bit for bit (for one piece_mb: more pieces round dW more often). Row strides ldx, ldw, lddx, lddw are in elements
+ * (an array's rows may span 2^48 of them).
  * Outputs may not overlap inputs or one another. */
 typedef struct {
     int32_t dtype, grad_dtype;

@@ -132,7 +132,7 @@ class Device:
                                    ws_bytes=ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
 
     def linear_ce(self, **kw) -> None:
-        """Softmax cross-entropy of the linear head X W^T + bias, without keeping the logits; with dX, dW or dbias given also
+        """Softmax cross-entropy of the linear head X W^T + bias, its logits in pieces of piece_mb MiB; with dX, dW or dbias given also
         those gradients (keyword arguments mirror ah_linear_ce_desc; strides default to contiguous rows, ws_bytes to ws.nbytes)."""
         L.check(self.lib.ah_linear_ce(self.h, C.byref(self._linear_ce_desc(**kw))))
 

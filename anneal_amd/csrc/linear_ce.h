@@ -1,4 +1,4 @@
-// linear_ce.h — softmax cross-entropy of a linear head, without keeping the logits (kernels in linear_ce.hip).
+// linear_ce.h — softmax cross-entropy of a linear head, its logits in pieces of rows (kernels in linear_ce.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -18,7 +18,7 @@ struct LinearCe {
     long lddx, lddw;
     float *dbias;               // [V] or null
     float grad_scale;
-    int piece_mb;               // MiB of kept logits, at most (0: 2048)
+    int piece_mb;               // MiB of kept logits (of statistics, for the loss alone), at most (0: 2048)
     int mean;                   // divide loss and gradients by the number of counted rows
 };
 

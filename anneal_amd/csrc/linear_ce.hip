@@ -1,4 +1,4 @@
-// linear_ce.hip — loss and gradients of softmax cross-entropy over a linear head's logits, which are never whole in memory.
+// linear_ce.hip — loss and gradients of softmax cross-entropy over a linear head's logits, of which a piece of rows is in memory at a time.
 //
 //   z = X W^T + b,  lse_n = log sum_v exp z_nv,  l_n = lse_n - z_n,y(n),  P = exp(z - lse) - onehot(y)
 //   dX = s P W,  dW = s P^T X,  db = s sum_n P        (s: the gradient's scale, divided by the number of counted rows for a mean)

@@ -5,7 +5,8 @@
 //
 // An f32 matrix x is carried as hi = f16(2^s x), lo = f16(2^s x - hi): 22 bits of each value whose magnitude is within 2^14 of
 // 2^15, with an absolute floor of 2^-24 (an f16 subnormal) below that. A product of two such matrices is three f16 products,
-// hi*hi + lo*hi + hi*lo (lo*lo is below the rounding of the sum), accumulated in one f32 accumulator; every f16 product is exact
+// hi*hi + lo*hi + hi*lo (lo*lo, at most 2^-22 of the product, is left out: as much as the operands' own planes lose, and shows in sums as
+// short as muon_small.hip has them alone), accumulated in one f32 accumulator; every f16 product is exact
 // in f32. Three f16 MFMAs do the work of one f32 MFMA of the same shape in 3/16 of its time.
 //
 // Layout of a two-plane matrix: each stored row holds groups of 32 hi values and then their 32 lo values (128 bytes, one cache
@@ -524,7 +525,7 @@ template <class Tiles>
 Plan plan(Tiles tiles, long k, int pa, int pb, bool narrow, long piece = 1l << 40) {
     const int row = pa == 1 ? 0 : pb == 1 ? 1 : 2;
     constexpr double kFew[3] = {1.22, 1.18, 1.53}, kMore[3] = {0.55, 0.40, 0.77};
-    constexpr double k128[3][2] = {{0.72, 1.15}, {0.61, 0.97}, {0.68, 1.33}}, k64[3][2] = {{0.22, 0.36}, {0.30, 0.50}, {0.26, 0.41}};
+    constexpr double k128[3][2] = {{0.72, 1.15}, {0.61, 0.97}, {0.68, 1.33}}, k64[2][2] = {{0.22, 0.36}, {0.26, 0.41}};
     const long nk = (k + (row == 0 ? 63 : 31)) / (row == 0 ? 64 : 32);
     Plan best{};
     double best_us = 1e30;
@@ -532,7 +533,7 @@ Plan plan(Tiles tiles, long k, int pa, int pb, bool narrow, long piece = 1l << 4
         if (width == 64 && !narrow) break;
         const long n = tiles(width), slots = width == 256 ? 256 : 512;
         const auto stage = [&](long wg) {
-            return width == 256 ? kFew[row] + kMore[row] * (double)wg / 256 : width == 128 ? k128[row][wg > 256] : k64[row][wg > 256];
+            return width == 256 ? kFew[row] + kMore[row] * (double)wg / 256 : width == 128 ? k128[row][wg > 256] : k64[row / 2][wg > 256];   // (not with planes 2 x 1)
         };
         const double fixed = width == 256 ? 7.0 : 5.0;   // launch, first loads, the epilogue
         const long least = (nk * (row == 0 ? 64 : 32) + piece - 1) / piece;

@@ -318,20 +318,26 @@ int ah_chain_step_noalloc(ah_device *dev, const float *X, const float *g, int32_
  * of 16 bytes or not, as in the call). The workspace needs 16-byte
  * alignment and no particular contents; calls of one device handle may share one. Graphs hold its address.
  *
- * Softmax cross-entropy of a linear head, without keeping the logits. X [N,D], W [V,D], bias [V] (may be null), labels [N]:
+ * Softmax cross-entropy of a linear head, whose logits are worked on in pieces of rows. X [N,D], W [V,D], bias [V] (may be null),
+ * labels [N]:
  *   z = X W^T + bias, lse_n = log sum_v exp z_nv, rowloss_n = lse_n - z_n,label(n)
  *   P = exp(z - lse) - onehot(label), s = grad_scale (over the number of counted rows, if mean)
  *   dX = s P W, dW = s P^T X, dbias = s sum_n P
  * A row whose label is outside [0, V) does not count: its rowloss, lse and dX are 0, and what X holds there is not used (it
  * may be NaN). loss is the counted rows' sum, divided by their number if mean (0 when there are none; all gradients are 0 then).
- * Null dX, dW or dbias are not computed; with all three null the call does the loss alone. A bias of -inf rules a class out.
- * A non-finite logit makes its row's loss and gradients NaN. dtype (X, W, bias) AH_F32 or AH_F16; grad_dtype
- * (dX, dW) AH_F32, or AH_F16 where dtype is AH_F16. loss, rowloss, lse and dbias are f32; losses and statistics are computed in
- * f32 or wider. f32 operands take part in the products with 22 bits of each value (less below 2^-14 of the operand's largest
- * magnitude), and P with 22 bits for f32 gradients and 11 for f16 ones, down to an absolute 2^-40. Gradients of f16 that would
- * underflow take a loss scale as grad_scale. Results repeat bit for bit (for one piece_mb: more pieces round dW more often). Row strides ldx, ldw, lddx, lddw are in elements
- * (an array's rows may span 2^48 of them).
- * Outputs may not overlap inputs or one another. */
+ * Null dX, dW or dbias are not computed; with all three null the call does the loss alone. A bias of -inf rules a class out (as a
+ * label it gives an infinite loss and the gradient above). A logit of +inf or NaN makes its row's loss, lse and dX NaN, and dW and
+ * dbias, which sum over rows; the other rows are as without it.
+ * dtype (X, W, bias) AH_F32 or AH_F16; grad_dtype (dX, dW) AH_F32, or AH_F16 where dtype is AH_F16. loss, rowloss, lse and dbias are
+ * f32; losses and statistics are computed in f32 or wider. f32 operands take part in the products with 22 bits of each value (less
+ * below 2^-14 of the operand's largest magnitude). P takes part with 22 bits for f32 gradients, for f16 ones with 11, and 22 at the
+ * label; all down to an absolute 2^-40. Gradients of f16 that would underflow take a loss scale as grad_scale. Results repeat bit for
+ * bit (for one piece_mb: more pieces round dW more often). Row strides ldx, ldw, lddx, lddw are in elements (an array's rows may
+ * span 2^48 of them). Outputs may not overlap inputs or one another, from their first element to their last.
+ * With gradients, up to piece_mb MiB of f32 logits are in the workspace at a time (whole, if they take no more). Beside them there are
+ * X's counted rows and, if W is f32 or its rows are not 16-byte aligned (and there are more than 128 rows of X), W, each once more;
+ * at most an eighth of a piece for statistics and db; V D floats for dW in f16 over several pieces; and partial sums of products, some
+ * hundred MiB at most. */
 typedef struct {
     int32_t dtype, grad_dtype;
     int32_t N, D, V;
@@ -361,9 +367,10 @@ int ah_linear_ce(ah_device *dev, const ah_linear_ce_desc *d);
 /* Newton-Schulz orthogonalisation of a matrix G [rows, cols], or of `batch` of them:
  *   X = G / (|G|_F + eps); steps times: A = X X^T (X^T X if rows > cols), X <- (a I + b A + c A A) X (X (..)); O = X
  * dtype (of G) and out_dtype AH_F32 or AH_F16. The norm is summed in f64; products keep 22 bits of their operands (X down to
- * 2^-37) and sum in f32. The iterates before the last have to keep their singular values at 4 or less (a = 3.4445, b = -4.7750, c = 2.0315 keeps them
- * below 1.3; larger ones may end as infinities or NaN); |a| + |b| + |c| may be at most 15 and steps 1 to 64. A zero matrix gives zeros, whatever eps, a non-finite one NaN. O may be G. ldg, ldo: row
- * strides; stride_g, stride_o: from matrix to matrix, in elements (read only for batch > 1). */
+ * 2^-37) and sum in f32. The iterates before the last have to keep their singular values at 4 or less (a = 3.4445, b = -4.7750,
+ * c = 2.0315 keeps them below 1.3; larger ones may end as infinities or NaN); |a| + |b| + |c| may be at most 15 and steps 1 to 64.
+ * A zero matrix gives zeros, whatever eps, a non-finite one NaN. O may be G. ldg, ldo: row strides; stride_g, stride_o: from matrix
+ * to matrix, in elements (read only for batch > 1). */
 typedef struct {
     int32_t dtype, out_dtype;
     int32_t rows, cols, batch;

@@ -347,3 +347,19 @@ def test_rows_that_are_not_finite_leave_the_others(dev, types, N, scale, bad):
         v, tol = exact[k]
         assert np.all(np.abs(got[k][keep] - v[keep]) <= tol[keep]), k
     assert np.isnan(got["loss"][0]) and np.isnan(got["dW"]).all()
+
+
+@pytest.mark.parametrize("N", [40, 150])
+@pytest.mark.parametrize("types", TL.TYPES, ids=["f32", "f16", "f16_f32grad"])
+def test_a_label_that_is_ruled_out(dev, types, N):
+    """A bias of -inf at some rows' labels: their loss is infinite, and P there -1, as the formulas have it."""
+    c = TL.Case(N, 64, 300, dtype=types[0], grad_dtype=types[1], labels=np.arange(N) * 5 % 300)
+    c.b[::10] = -np.inf
+    out = c.labels % 10 == 0
+    got, exact = TL.run(dev, c, want=("rowloss", "lse", "loss", "dX", "dW", "dbias")), c.exact()
+    assert np.isposinf(got["rowloss"][out]).all() and np.isposinf(got["loss"][0])
+    for k in ("lse", "dX", "dW", "dbias"):
+        v, tol = exact[k]
+        assert np.all(np.abs(got[k] - v) <= tol), k
+    v, tol = exact["rowloss"]
+    assert np.all(np.abs(got["rowloss"][~out] - v[~out]) <= tol[~out])

@@ -349,6 +349,7 @@ template <int S, bool WIDE>
 void run(const Muon &d, SmallArgs a, float *const (&parts)[2], hipStream_t s) {
     const dim3 grid((unsigned)a.groups, (unsigned)d.batch);
     const Scales c = scales(d);
+    const int longest = longest_group(d);
     const auto p2 = [](double v, int e) { return (float)std::ldexp(v, e); };
     a.ga = p2(1, c.A - 2 * kSX);
     a.b2 = p2(d.c, c.B - 2 * c.A);
@@ -362,7 +363,7 @@ void run(const Muon &d, SmallArgs a, float *const (&parts)[2], hipStream_t s) {
     a.out = parts[0];
     hipLaunchKernelGGL((muon_small_kernel<S, WIDE, FIRST>), grid, dim3(S / 32 * (S / 32) * 64), 0, s, a, d);
     for (int left = d.steps, k = 0; left > 0; k++) {
-        a.steps = group_size(longest_group(d), k, left);
+        a.steps = group_size(longest, k, left);
         left -= a.steps;
         a.qi = (float)std::pow((double)d.a, a.steps);
         a.qs = p2(1, a.steps == 2 ? -c.Q2 : -c.B);

@@ -210,6 +210,18 @@ def test_zero_matrices_and_tiny_ones_in_a_batch(dev, shape, eps):
         assert np.linalg.norm(got[z] - want) <= err + U32 * np.linalg.norm(want) + 485 * 2.0 ** -37 * want.size ** 0.5, z
 
 
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf], ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (40, 70), (300, 128), (300, 280)], ids=lambda s: "%dx%d" % s)
+def test_a_matrix_that_is_not_finite_is_nan_alone(dev, shape, bad):
+    G = np.stack([TM.gradient(np.random.default_rng([z, *shape]), *shape, L.AH_F32) for z in range(3)])
+    alone = [TM.ortho(dev, g, L.AH_F32)[0] for g in G]
+    G[1, shape[0] // 2, shape[1] // 3] = bad
+    got = TM.ortho(dev, G, L.AH_F32)
+    assert np.isnan(got[1]).all()
+    for z in (0, 2):
+        np.testing.assert_allclose(got[z], alone[z], rtol=0, atol=2e-5 * np.linalg.norm(alone[z]))
+
+
 @pytest.mark.parametrize("eps", [0.0, 1e-45])
 @pytest.mark.parametrize("shape", [(64, 100), (300, 280)], ids=lambda s: "%dx%d" % s)
 def test_a_step_without_a_gradient_decays_the_weights(dev, shape, eps):

@@ -409,9 +409,9 @@ def _call(s):
         return "linear_grad", dict(kw, grad_dtype=_AH[c["out"]], F=c["F"], act=_ACTS[c["act"]], X=p["X"], W=p["W"], Z=p["Z"], U=p.get("U"), dY=p["dY"],
                                    dX=o["dX"], dW=o["dW"], dbias=o.get("db"), dU=o.get("dU"))
     kw.update(res_dtype=_AH[c["res"]], Y=p["Y"], gate=p.get("gate"), rows_per_gate=c["per"], post=_NORMS[c["post"]], pre=_NORMS[c["pre"]], eps=_EPS, skip=_SKIP)
-    kw.update({k: p.get(k) for k in ("post_w", "post_b", "pre_w", "pre_b")})
+    kw.update({k: p.get(k) for k in ("post_w", "post_b", "pre_w")})
     if kind == "norm":
-        return "residual_norm", dict(kw, H=p["H"], H_out=o["H"], O=o["O"])
+        return "residual_norm", dict(kw, pre_b=p.get("pre_b"), H=p["H"], H_out=o["H"], O=o["O"])
     kw.update({k: o.get(k) for k in ("dH", "dY", "dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b")})
     return "residual_norm_grad", dict(kw, H_out=p["H"], dH_out=p["dH"], dO=p["dO"])
 

@@ -14,6 +14,8 @@ LIB_PATH = os.path.join(HERE, "libanneal_hip.so")
 AH_OK = 0
 AH_F32, AH_F16, AH_BF16, AH_I32, AH_BOOL, AH_U32 = 0, 1, 2, 3, 4, 5
 EPI_STORE, EPI_BIAS, EPI_BIAS_RELU, EPI_MSE, EPI_MASK, EPI_SGD = range(6)
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
 TRAIN_MLP_CE, TRAIN_CONVNET, TRAIN_MLP3_F16, TRAIN_CHAIN = 1, 2, 3, 4
 STEP_STORE_GRADS, STEP_GRAPH = 1, 2
 PLAN_GRAPH = 1
@@ -81,6 +83,48 @@ class ah_muon_desc(C.Structure):
                 ("W", C.c_void_p), ("W_out", C.c_void_p), ("W16_out", C.c_void_p), ("ldw", C.c_int64), ("stride_w", C.c_int64),
                 ("lr", C.c_float), ("momentum", C.c_float), ("decay", C.c_float), ("scale", C.c_float),
                 ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class ah_linear_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("act", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("F", C.c_int32), ("scale", C.c_float),
+                ("X", C.c_void_p), ("ldx", C.c_int64), ("W", C.c_void_p), ("ldw", C.c_int64), ("bias", C.c_void_p), ("U", C.c_void_p),
+                ("ldu", C.c_int64), ("R", C.c_void_p), ("ldr", C.c_int64), ("Y", C.c_void_p), ("ldy", C.c_int64), ("Z", C.c_void_p),
+                ("ldz", C.c_int64), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class ah_linear_grad_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("grad_dtype", C.c_int32), ("act", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("F", C.c_int32),
+                ("scale", C.c_float), ("X", C.c_void_p), ("ldx", C.c_int64), ("W", C.c_void_p), ("ldw", C.c_int64), ("Z", C.c_void_p),
+                ("ldz", C.c_int64), ("U", C.c_void_p), ("ldu", C.c_int64), ("dY", C.c_void_p), ("lddy", C.c_int64), ("dX", C.c_void_p),
+                ("lddx", C.c_int64), ("dW", C.c_void_p), ("lddw", C.c_int64), ("dbias", C.c_void_p), ("dU", C.c_void_p),
+                ("lddu", C.c_int64), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class ah_residual_norm_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("res_dtype", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("post", C.c_int32),
+                ("pre", C.c_int32), ("rows_per_gate", C.c_int32), ("eps", C.c_float), ("skip", C.c_float), ("scale", C.c_float),
+                ("H", C.c_void_p), ("ldh", C.c_int64), ("Y", C.c_void_p), ("ldy", C.c_int64), ("gate", C.c_void_p), ("ldgate", C.c_int64),
+                ("post_w", C.c_void_p), ("post_b", C.c_void_p), ("pre_w", C.c_void_p), ("pre_b", C.c_void_p), ("H_out", C.c_void_p),
+                ("ldh_out", C.c_int64), ("O", C.c_void_p), ("ldo", C.c_int64)]
+
+
+class ah_residual_norm_grad_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("res_dtype", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("post", C.c_int32),
+                ("pre", C.c_int32), ("rows_per_gate", C.c_int32), ("eps", C.c_float), ("skip", C.c_float), ("scale", C.c_float),
+                ("Y", C.c_void_p), ("ldy", C.c_int64), ("gate", C.c_void_p), ("ldgate", C.c_int64), ("post_w", C.c_void_p),
+                ("post_b", C.c_void_p), ("pre_w", C.c_void_p), ("H_out", C.c_void_p), ("ldh_out", C.c_int64), ("dH_out", C.c_void_p),
+                ("lddh_out", C.c_int64), ("dO", C.c_void_p), ("lddo", C.c_int64), ("dH", C.c_void_p), ("lddh", C.c_int64),
+                ("dY", C.c_void_p), ("lddy", C.c_int64), ("dgate", C.c_void_p), ("lddgate", C.c_int64), ("dpost_w", C.c_void_p),
+                ("dpost_b", C.c_void_p), ("dpre_w", C.c_void_p), ("dpre_b", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+class ah_tensor(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("count", C.c_int64), ("dtype", C.c_int32), ("out_dtype", C.c_int32)]
+
+
+class ah_clip_desc(C.Structure):
+    _fields_ = [("n", C.c_int32), ("max_norm", C.c_float), ("eps", C.c_float), ("unscale", C.c_float), ("tensors", C.c_void_p),
+                ("norm", C.c_void_p), ("coef", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
 
 
 class ah_opt(C.Structure):
@@ -161,6 +205,15 @@ SIGNATURES = {
     "ah_orthogonalize": (C.c_int, [_P, C.POINTER(ah_orthogonalize_desc)]),
     "ah_muon_workspace": (C.c_int, [_P, C.POINTER(ah_muon_desc), C.POINTER(C.c_int64)]),
     "ah_muon_step": (C.c_int, [_P, C.POINTER(ah_muon_desc)]),
+    "ah_linear_workspace": (C.c_int, [_P, C.POINTER(ah_linear_desc), C.POINTER(C.c_int64)]),
+    "ah_linear": (C.c_int, [_P, C.POINTER(ah_linear_desc)]),
+    "ah_linear_grad_workspace": (C.c_int, [_P, C.POINTER(ah_linear_grad_desc), C.POINTER(C.c_int64)]),
+    "ah_linear_grad": (C.c_int, [_P, C.POINTER(ah_linear_grad_desc)]),
+    "ah_residual_norm": (C.c_int, [_P, C.POINTER(ah_residual_norm_desc)]),
+    "ah_residual_norm_grad_workspace": (C.c_int, [_P, C.POINTER(ah_residual_norm_grad_desc), C.POINTER(C.c_int64)]),
+    "ah_residual_norm_grad": (C.c_int, [_P, C.POINTER(ah_residual_norm_grad_desc)]),
+    "ah_clip_norm_workspace": (C.c_int, [_P, C.POINTER(ah_clip_desc), C.POINTER(C.c_int64)]),
+    "ah_clip_norm": (C.c_int, [_P, C.POINTER(ah_clip_desc)]),
     "ah_trainer_create": (C.c_int, [_P, C.c_int32, C.POINTER(C.c_int64), C.c_int32, C.c_float, C.POINTER(_P)]),
     "ah_trainer_destroy": (None, [_P]),
     "ah_trainer_set": (C.c_int, [_P, C.c_int32, _P, C.c_int64]),

@@ -183,6 +183,93 @@ class Device:
         """Bytes of workspace that muon_step needs for the same arguments (ws left out)."""
         return self._sized(self.lib.ah_muon_workspace, self._muon_desc(**kw))
 
+    def _fill(self, cls, rows, **kw):
+        """A descriptor from keyword arguments: buffers become pointers, strides that are not given those of contiguous rows."""
+        d = {}
+        for name, t in cls._fields_:
+            v = kw.pop(name, None)
+            if name.startswith("ld"):
+                v = rows[name] if v is None else v
+            elif t is C.c_void_p:
+                v = v if v is None or isinstance(v, int) else v.ptr
+            elif name == "ws_bytes":
+                ws = kw.get("_ws")
+                v = v if v is not None else 0 if ws is None else ws.nbytes
+            d[name] = v
+        kw.pop("_ws", None)
+        if kw:
+            raise TypeError(f"unknown arguments: {', '.join(sorted(kw))}")
+        return cls(**d)
+
+    def _linear_desc(self, dtype, N, D, F, X, W, Y, act=L.ACT_NONE, scale=1.0, ws=None, **kw):
+        return self._fill(L.ah_linear_desc, dict(ldx=D, ldw=D, ldu=F, ldr=F, ldy=F, ldz=F), dtype=dtype, N=N, D=D, F=F, X=X, W=W, Y=Y, act=act,
+                          scale=scale, ws=ws, _ws=ws, **kw)
+
+    def linear(self, **kw) -> None:
+        """Y = R + scale act(Z) U, Z = X W^T + bias (keyword arguments mirror ah_linear_desc; bias, U, R and Z may be left out, strides
+        default to contiguous rows, ws_bytes to ws.nbytes)."""
+        L.check(self.lib.ah_linear(self.h, C.byref(self._linear_desc(**kw))))
+
+    def linear_workspace(self, **kw) -> int:
+        """Bytes of workspace that linear needs for the same arguments (ws left out)."""
+        return self._sized(self.lib.ah_linear_workspace, self._linear_desc(**kw))
+
+    def _linear_grad_desc(self, dtype, N, D, F, dY, grad_dtype=L.AH_F32, act=L.ACT_NONE, scale=1.0, ws=None, **kw):
+        return self._fill(L.ah_linear_grad_desc, dict(ldx=D, ldw=D, ldz=F, ldu=F, lddy=F, lddx=D, lddw=D, lddu=F), dtype=dtype, grad_dtype=grad_dtype,
+                          N=N, D=D, F=F, dY=dY, act=act, scale=scale, ws=ws, _ws=ws, **kw)
+
+    def linear_grad(self, **kw) -> None:
+        """The gradients of linear that are given buffers: dX, dW, dbias, dU (keyword arguments mirror ah_linear_grad_desc)."""
+        L.check(self.lib.ah_linear_grad(self.h, C.byref(self._linear_grad_desc(**kw))))
+
+    def linear_grad_workspace(self, **kw) -> int:
+        """Bytes of workspace that linear_grad needs for the same arguments (ws left out)."""
+        return self._sized(self.lib.ah_linear_grad_workspace, self._linear_grad_desc(**kw))
+
+    def _residual_norm_args(self, cls, strides, dtype, N, D, res_dtype=None, post=L.NORM_NONE, pre=L.NORM_NONE, rows_per_gate=0, eps=1e-6, skip=1.0,
+                            scale=1.0, **kw):
+        return self._fill(cls, dict.fromkeys(strides, D), dtype=dtype, res_dtype=dtype if res_dtype is None else res_dtype, N=N, D=D, post=post, pre=pre,
+                          rows_per_gate=rows_per_gate, eps=eps, skip=skip, scale=scale, **kw)
+
+    def residual_norm(self, **kw) -> None:
+        """H_out = skip H + scale gate post(Y), O = pre(H_out) (keyword arguments mirror ah_residual_norm_desc; res_dtype defaults to dtype,
+        arrays may be left out as ah_residual_norm says, strides default to contiguous rows)."""
+        d = self._residual_norm_args(L.ah_residual_norm_desc, ("ldh", "ldy", "ldgate", "ldh_out", "ldo"), **kw)
+        L.check(self.lib.ah_residual_norm(self.h, C.byref(d)))
+
+    def _residual_norm_grad_desc(self, ws=None, **kw):
+        return self._residual_norm_args(L.ah_residual_norm_grad_desc, ("ldy", "ldgate", "ldh_out", "lddh_out", "lddo", "lddh", "lddy", "lddgate"), ws=ws,
+                                        _ws=ws, **kw)
+
+    def residual_norm_grad(self, **kw) -> None:
+        """The gradients of residual_norm that are given buffers: dH, dY, dgate and the weights' (keyword arguments mirror
+        ah_residual_norm_grad_desc)."""
+        L.check(self.lib.ah_residual_norm_grad(self.h, C.byref(self._residual_norm_grad_desc(**kw))))
+
+    def residual_norm_grad_workspace(self, **kw) -> int:
+        """Bytes of workspace that residual_norm_grad needs for the same arguments (ws left out)."""
+        return self._sized(self.lib.ah_residual_norm_grad_workspace, self._residual_norm_grad_desc(**kw))
+
+    @staticmethod
+    def tensor_list(tensors):
+        """The tensors of clip_norm, to be kept by a program whose gradients stay where they are: (src, dst or None, count, dtype,
+        out_dtype) each."""
+        return (L.ah_tensor * len(tensors))(*[(s.ptr, None if o is None else o.ptr, n, t, to) for s, o, n, t, to in tensors])
+
+    def _clip_desc(self, tensors, max_norm, norm=None, coef=None, eps=1e-6, unscale=1.0, ws=None, ws_bytes=None):
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        return L.ah_clip_desc(n=len(tensors), max_norm=max_norm, eps=eps, unscale=unscale, tensors=C.addressof(tensors), norm=p(norm), coef=p(coef),
+                              ws=p(ws), ws_bytes=ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
+
+    def clip_norm(self, **kw) -> None:
+        """norm = unscale times the norm of all tensors together, coef = min(1, max_norm / (norm + eps)), dst = unscale coef src for each
+        (tensors: a tensor_list; the other keyword arguments mirror ah_clip_desc)."""
+        L.check(self.lib.ah_clip_norm(self.h, C.byref(self._clip_desc(**kw))))
+
+    def clip_norm_workspace(self, **kw) -> int:
+        """Bytes of workspace that clip_norm needs for the same arguments (ws left out)."""
+        return self._sized(self.lib.ah_clip_norm_workspace, self._clip_desc(**kw))
+
     def close(self) -> None:
         if self.h:
             self.lib.ah_close(self.h)

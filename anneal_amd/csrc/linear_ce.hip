@@ -19,6 +19,7 @@
 
 #include <algorithm>
 
+#include "act.h"
 #include "linear_ce_few.h"
 #include "plane_gemm.h"
 
@@ -27,9 +28,11 @@ namespace {
 
 using pg::h4;
 using pg::h8;
+using pg::magnitude;
+using pg::pack_row;
+using pg::plane_exp;
 typedef half_t h2 __attribute__((ext_vector_type(2)));
 
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kPScale = 15;   // P is carried as 2^15 P: |P| <= 1, so the largest value is 2^15
 
 // Device scalars at the workspace's start.
@@ -38,13 +41,6 @@ struct Scalars {
     unsigned xmax, wmax;      // bits of the largest magnitudes (f32 operands)
     int pad;
 };
-
-// Power of two that brings the largest finite magnitude into [2^14, 2^15); 0 where there is none but 0.
-__device__ __forceinline__ int plane_exp(unsigned maxbits) {
-    const float m = __uint_as_float(maxbits);
-    if (!(m > 0.0f)) return 0;
-    return min(14 - ilogbf(m), 120);
-}
 
 __device__ __forceinline__ int chunk_rows(const int *count, int row0, int rows) { return max(0, min(rows, *count - row0)); }
 
@@ -115,10 +111,6 @@ __device__ __forceinline__ void index_rows(const ScanArgs &a) {
 // Workgroup 0 indexes the rows; the others (f32 operands) find the largest magnitudes of W and of the counted rows of X, a wave per
 // stretch of 2048 values of a row. The bits of non-negative floats order as integers. Infinities and NaN are passed over: they make their
 // own row's logits NaN under any scale, and the other rows' scale is not theirs.
-__device__ __forceinline__ unsigned magnitude(uint32_t bits) {
-    bits &= 0x7fffffffu;
-    return bits < 0x7f800000u ? bits : 0;
-}
 __global__ __launch_bounds__(256) void lce_scan_kernel(ScanArgs a) {
     if (blockIdx.x == 0) {
         index_rows(a);
@@ -171,31 +163,6 @@ __device__ __forceinline__ uint2 join_maxes(const uint2 *maxes, int n) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     return make_uint2(max(max(red[0].x, red[1].x), max(red[2].x, red[3].x)), max(max(red[0].y, red[1].y), max(red[2].y, red[3].y)));
-}
-
-// One wave: row r of the packed operand (panels of `rows` rows): Dp columns, zeros past D. f32 values go to two planes, f16 ones stay.
-template <int P>
-__device__ __forceinline__ void pack_row(half_t *__restrict__ out, long rows, long r, const void *__restrict__ in, int D, int Dp, int e) {
-    const int t = threadIdx.x & 63;
-    if constexpr (P == 1) {
-        const half_t *p = (const half_t *)in;
-#pragma unroll 2
-        for (int i = t * 8; i < Dp; i += 64 * 8) {
-            h8 v = {};
-            if (i + 7 < D) v = *(const pg::h8_any *)(p + i);
-            else
-                for (int k = 0; i + k < D; k++) v[k] = p[i + k];
-            *(h8 *)(out + pg::panel_at<1>(rows, r, i)) = v;
-        }
-    } else {
-#pragma unroll 4
-        for (int i = t * 4; i < Dp; i += 64 * 4) {
-            floatx4 v = pg::load4((const float *)in, i, D);
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = ldexpf(v[k], e);
-            pg::plane_store(out + pg::panel_at<2>(rows, r, i), v);
-        }
-    }
 }
 
 // A wave a row. Of the first N + 64, row r of X goes to its place among the counted rows, or its dX and outputs are cleared; the last
@@ -459,13 +426,6 @@ struct GradArgs {
     float *res;                     // one plane: what its rounding leaves of each row's P at its label
     float *dbpart;                  // [row block of the piece][V] column sums of P, or null
 };
-
-// e^x: the product with log2 e carries what its rounding loses, which at x = -10 is 3e-7 of the result.
-__device__ __forceinline__ float exp_of(float x) {
-    const float t = x * kLog2e, low = fmaf(x, kLog2e, -t) + x * 1.925963033500e-8f;   // log2 e less its f32 value
-    const float r = __builtin_amdgcn_exp2f(t);
-    return t > -126.0f ? fmaf(r, low * 0.69314718f, r) : r;   // -inf stays away from the correction
-}
 
 constexpr int kGradRows = 64;       // rows of a block; also the k of a one-plane stage, up to which rows are cleared
 

@@ -85,8 +85,8 @@ __device__ __forceinline__ void stages(int first, int count, char *smem, Fetch f
 // k of a stage of the logits' product: 256 bytes of a row.
 constexpr int along_k(bool f16) { return f16 ? 128 : 64; }
 
-// acc[i][j] += X(m, k) W(n, k) over stages [first, first + count) of k, four chunks of 64 bytes each. Rows m of X are rowmap[m], the
-// last of M for those past it; past the last class the last row of W is read (the epilogue leaves those columns out). Where a lane's
+// acc[i][j] += X(m, k) W(n, k) over stages [first, first + count) of k, four chunks of 64 bytes each. Rows m of X are rowmap[m]
+// (m without one), the last of M for those past it; past the last class the last row of W is read (the epilogue leaves those columns out). Where a lane's
 // 16 bytes end past D (D >= 8), both operands read the row's last 16, and the rows' side has zeros for the k that were there before.
 template <class C, bool F16>
 __device__ __forceinline__ void contract_along(const void *X, long ldx, const int *rowmap, int M, const void *W, long ldw, int V, int D, int n0,
@@ -98,7 +98,10 @@ __device__ __forceinline__ void contract_along(const void *X, long ldx, const in
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
     const T *xp[C::FA], *wp[C::FB];
 #pragma unroll
-    for (int i = 0; i < C::FA; i++) xp[i] = (const T *)X + (long)rowmap[min(16 * i + (int)(threadIdx.x >> 4), M - 1)] * ldx;
+    for (int i = 0; i < C::FA; i++) {
+        const int m = min(16 * i + (int)(threadIdx.x >> 4), M - 1);
+        xp[i] = (const T *)X + (long)(rowmap ? rowmap[m] : m) * ldx;
+    }
 #pragma unroll
     for (int j = 0; j < C::FB; j++) wp[j] = (const T *)W + (long)min(n0 + wave * C::WN + 16 * j + row, V - 1) * ldw;
 #pragma unroll

@@ -95,6 +95,43 @@ __device__ __forceinline__ void plane_store(half_t *p, floatx4 v) {
     *(h4 *)(p + 32) = lo;
 }
 
+// Power of two that brings the largest finite magnitude into [2^14, 2^15); 0 where there is none but 0.
+__device__ __forceinline__ int plane_exp(unsigned maxbits) {
+    const float m = __uint_as_float(maxbits);
+    if (!(m > 0.0f)) return 0;
+    return min(14 - ilogbf(m), 120);
+}
+// The bits of non-negative floats order as integers; 0 for infinities and NaN, which leave the others' scale alone.
+__device__ __forceinline__ unsigned magnitude(uint32_t bits) {
+    bits &= 0x7fffffffu;
+    return bits < 0x7f800000u ? bits : 0;
+}
+
+// One wave: row r of the packed operand (panels of `rows` rows): Dp columns, zeros past D. f32 values go to two planes, f16 ones stay.
+template <int P>
+__device__ __forceinline__ void pack_row(half_t *__restrict__ out, long rows, long r, const void *__restrict__ in, int D, int Dp, int e) {
+    const int t = threadIdx.x & 63;
+    if constexpr (P == 1) {
+        const half_t *p = (const half_t *)in;
+#pragma unroll 2
+        for (int i = t * 8; i < Dp; i += 64 * 8) {
+            h8 v = {};
+            if (i + 7 < D) v = *(const h8_any *)(p + i);
+            else
+                for (int k = 0; i + k < D; k++) v[k] = p[i + k];
+            *(h8 *)(out + panel_at<1>(rows, r, i)) = v;
+        }
+    } else {
+#pragma unroll 4
+        for (int i = t * 4; i < Dp; i += 64 * 4) {
+            floatx4 v = load4((const float *)in, i, D);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = ldexpf(v[k], e);
+            plane_store(out + panel_at<2>(rows, r, i), v);
+        }
+    }
+}
+
 // One stage's 1 KiB blocks that a wave fetches: R operand rows x BK k in P planes. Offsets are relative to the tile's corner.
 template <int R, int T, int P, int BK, int NW>
 struct PFetch {
@@ -121,7 +158,7 @@ struct PFetch {
             }
         }
     }
-    // krem: k of the operand from the stage's first on. Past them T = 1 reads the last k-row and T = 0 the stage's first chunk of the
+    // krem: k of the operand from the stage's first on, at least 1 (a stage wholly past them would be off by 2^32 bytes). Past them T = 1 reads the last k-row and T = 0 the stage's first chunk of the
     // row (krem is then a multiple of a chunk's 8): the other operand is 0 there, and nothing behind the array is read.
     __device__ __forceinline__ void issue(int j, const char *base, long ld, int krem, uint32_t lds, int wave_u, int lane) const {
         uint32_t o = off[j];

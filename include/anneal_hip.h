@@ -411,6 +411,162 @@ typedef struct {
 int ah_muon_workspace(ah_device *dev, const ah_muon_desc *d, int64_t *bytes);
 int ah_muon_step(ah_device *dev, const ah_muon_desc *d);
 
+/* ── A residual block of a training step, and clipping before its update ──────
+ * No counterpart in the reference (no activation but ReLU, no norm layer, no clipping). As above: asynchronous on the device stream,
+ * nothing allocated, a workspace of the caller's (where there is one) that calls of one handle may share and graphs hold.
+ *
+ * Linear layer with its epilogue. X [N,D], W [F,D], bias [F]; U, R, Y, Z [N,F]:
+ *   Z = X W^T + bias,  Y = R + scale act(Z) U        (elementwise; bias, U, R may be null: 0, 1, 0)
+ * act: ReLU, GELU by erf or by tanh(sqrt(2/pi) (z + 0.044715 z^3)), SiLU z / (1 + exp(-z)). Z may be null; a backward pass needs it.
+ * dtype (all arrays) AH_F32 or AH_F16; everything is computed in f32 from an f32 Z and each output rounded once. f32 operands take part in
+ * the product with 22 bits of each value (less below 2^-14 of its row's largest magnitude), or with all 24 where there are at most 64
+ * rows. Y may be R. What is not finite in a row of X or W makes that row or column of the outputs infinite or NaN, and no other.
+ * N to 2^21, D and F to 2^20. Row strides ld* are in elements. */
+enum { AH_ACT_NONE = 0, AH_ACT_RELU = 1, AH_ACT_GELU = 2, AH_ACT_GELU_TANH = 3, AH_ACT_SILU = 4 };
+typedef struct {
+    int32_t dtype, act;
+    int32_t N, D, F;
+    float scale;
+    const void *X;
+    int64_t ldx;
+    const void *W;
+    int64_t ldw;
+    const void *bias;
+    const void *U;
+    int64_t ldu;
+    const void *R;
+    int64_t ldr;
+    void *Y;
+    int64_t ldy;
+    void *Z;
+    int64_t ldz;
+    void *ws;
+    int64_t ws_bytes;
+} ah_linear_desc;
+int ah_linear_workspace(ah_device *dev, const ah_linear_desc *d, int64_t *bytes);
+int ah_linear(ah_device *dev, const ah_linear_desc *d);
+
+/* Its gradients, given dY:
+ *   dZ = scale dY U act'(Z),  dX = dZ W,  dW = dZ^T X,  dbias = sum_n dZ,  dU = scale dY act(Z);  dR is dY itself
+ * act'(0) of ReLU is 0. Null dX, dW, dbias, dU are not computed; X is read for dW alone, W for dX alone (null otherwise), Z for an
+ * act other than none and for dU. dtype (X, W, Z, U, dY, dU) AH_F32 or AH_F16, grad_dtype (dX, dW) AH_F32, or AH_F16 where dtype is; dbias
+ * is f32. dZ takes part in the products with 22 bits for f32 gradients, 11 for f16 ones, f32 operands with 22 (all less below 2^-14 of
+ * the array's largest magnitude). Results repeat bit for bit. */
+typedef struct {
+    int32_t dtype, grad_dtype, act;
+    int32_t N, D, F;
+    float scale;
+    const void *X;
+    int64_t ldx;
+    const void *W;
+    int64_t ldw;
+    const void *Z;
+    int64_t ldz;
+    const void *U;
+    int64_t ldu;
+    const void *dY;
+    int64_t lddy;
+    void *dX;
+    int64_t lddx;
+    void *dW;
+    int64_t lddw;
+    float *dbias;
+    void *dU;
+    int64_t lddu;
+    void *ws;
+    int64_t ws_bytes;
+} ah_linear_grad_desc;
+int ah_linear_grad_workspace(ah_device *dev, const ah_linear_grad_desc *d, int64_t *bytes);
+int ah_linear_grad(ah_device *dev, const ah_linear_grad_desc *d);
+
+/* Norms after and before a block, fused with its gate and the residual sum. H, H_out (the residual stream), Y (the block's output), O (the
+ * next block's input) [N,D]; row n of gate is row n / rows_per_gate (0: one row for all):
+ *   H_out = skip H + scale gate post(Y),  O = pre(H_out)
+ * post, pre: none, RMS x / sqrt(mean x^2 + eps) w, or layer (x - mean) / sqrt(var + eps) w + b; weights [D], may be null (1 and 0).
+ * H null: no first term. Y null: no second one (gate and post then none). H_out or O may be null (O where pre is none); O is the norm of
+ * H_out before its rounding. dtype (Y, O, gate, weights) AH_F32 or AH_F16; res_dtype (H, H_out) AH_F32, or AH_F16 where dtype is.
+ * Computed in f32; H_out may be H. A row that is not finite leaves the others alone. N to 2^27, D to 2^20. No workspace. */
+enum { AH_NORM_NONE = 0, AH_NORM_RMS = 1, AH_NORM_LAYER = 2 };
+typedef struct {
+    int32_t dtype, res_dtype;
+    int32_t N, D;
+    int32_t post, pre;
+    int32_t rows_per_gate;
+    float eps, skip, scale;
+    const void *H;
+    int64_t ldh;
+    const void *Y;
+    int64_t ldy;
+    const void *gate;
+    int64_t ldgate;
+    const void *post_w, *post_b, *pre_w, *pre_b;
+    void *H_out;
+    int64_t ldh_out;
+    void *O;
+    int64_t ldo;
+} ah_residual_norm_desc;
+int ah_residual_norm(ah_device *dev, const ah_residual_norm_desc *d);
+
+/* Its gradients, given those of H_out and O (dH_out null: 0; dO is needed unless pre is none), from Y and the stored H_out:
+ *   t = dH_out + pre'(dO),  dH = skip t,  dY = post'(scale gate t),  dgate = sum over its rows of scale t post(Y)
+ * and the weights' gradients, sums over all rows. Null outputs are not computed. dgate is of dtype, the weights' gradients are
+ * f32. Y is needed for dgate and where post is not none, H_out where pre is not none. Sums over rows run in a fixed order: results repeat
+ * bit for bit. dH may be dH_out. */
+typedef struct {
+    int32_t dtype, res_dtype;
+    int32_t N, D;
+    int32_t post, pre;
+    int32_t rows_per_gate;
+    float eps, skip, scale;
+    const void *Y;
+    int64_t ldy;
+    const void *gate;
+    int64_t ldgate;
+    const void *post_w, *post_b, *pre_w;
+    const void *H_out;
+    int64_t ldh_out;
+    const void *dH_out;
+    int64_t lddh_out;
+    const void *dO;
+    int64_t lddo;
+    void *dH;
+    int64_t lddh;
+    void *dY;
+    int64_t lddy;
+    void *dgate;
+    int64_t lddgate;
+    float *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+    void *ws;
+    int64_t ws_bytes;
+} ah_residual_norm_grad_desc;
+int ah_residual_norm_grad_workspace(ah_device *dev, const ah_residual_norm_grad_desc *d, int64_t *bytes);
+int ah_residual_norm_grad(ah_device *dev, const ah_residual_norm_grad_desc *d);
+
+/* The global norm of many tensors, and clipping by it:
+ *   norm = unscale sqrt(sum over all entries of src^2),  coef = min(1, max_norm / (norm + eps)),  dst = unscale coef src
+ * unscale: the inverse of a loss scale, or 1. A tensor is `count` consecutive elements (0 is allowed) of dtype AH_F32 or AH_F16, out_dtype
+ * AH_F32, or AH_F16 where dtype is. dst null: the tensor is only counted; dst may be src where the types are the same, and is then
+ * left alone where unscale coef is 1. norm and coef [1] are on the device and may be null. Squares are summed in f64 in a fixed order. If an entry
+ * is infinite or NaN, so is norm; coef is then 0 and every dst is 0, so that the update that follows takes no step from them. max_norm may
+ * be infinite. The array `tensors` is host memory and read during the call alone. 1 to 2^16 tensors of up to 2^40 elements in all. */
+typedef struct {
+    const void *src;
+    void *dst;
+    int64_t count;
+    int32_t dtype, out_dtype;
+} ah_tensor;
+typedef struct {
+    int32_t n;
+    float max_norm, eps, unscale;
+    const ah_tensor *tensors;
+    float *norm;
+    float *coef;
+    void *ws;
+    int64_t ws_bytes;
+} ah_clip_desc;
+int ah_clip_norm_workspace(ah_device *dev, const ah_clip_desc *d, int64_t *bytes);
+int ah_clip_norm(ah_device *dev, const ah_clip_desc *d);
+
 /* ── Device-resident training steps (one BASELINE config each) ───────────────
  * Replaces the reference step pattern: graph build -> tensor.Backward -> one tensor.Realize per gradient
  * -> host SGD (examples/mlp.go:112-142, tensor/nn/nn.go:69-106). Parameters stay resident as f32 masters

@@ -183,27 +183,13 @@ class Device:
         """Bytes of workspace that muon_step needs for the same arguments (ws left out)."""
         return self._sized(self.lib.ah_muon_workspace, self._muon_desc(**kw))
 
-    def _fill(self, cls, rows, **kw):
-        """A descriptor from keyword arguments: buffers become pointers, strides that are not given those of contiguous rows."""
-        d = {}
-        for name, t in cls._fields_:
-            v = kw.pop(name, None)
-            if name.startswith("ld"):
-                v = rows[name] if v is None else v
-            elif t is C.c_void_p:
-                v = v if v is None or isinstance(v, int) else v.ptr
-            elif name == "ws_bytes":
-                ws = kw.get("_ws")
-                v = v if v is not None else 0 if ws is None else ws.nbytes
-            d[name] = v
-        kw.pop("_ws", None)
-        if kw:
-            raise TypeError(f"unknown arguments: {', '.join(sorted(kw))}")
-        return cls(**d)
-
-    def _linear_desc(self, dtype, N, D, F, X, W, Y, act=L.ACT_NONE, scale=1.0, ws=None, **kw):
-        return self._fill(L.ah_linear_desc, dict(ldx=D, ldw=D, ldu=F, ldr=F, ldy=F, ldz=F), dtype=dtype, N=N, D=D, F=F, X=X, W=W, Y=Y, act=act,
-                          scale=scale, ws=ws, _ws=ws, **kw)
+    @staticmethod
+    def _linear_desc(dtype, N, D, F, X, W, Y, act=L.ACT_NONE, scale=1.0, bias=None, U=None, R=None, Z=None, ldx=None, ldw=None, ldu=None, ldr=None,
+                     ldy=None, ldz=None, ws=None, ws_bytes=None):
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        ld = lambda v, n: n if v is None else v     # noqa: E731
+        return L.ah_linear_desc(dtype, act, N, D, F, scale, X.ptr, ld(ldx, D), W.ptr, ld(ldw, D), p(bias), p(U), ld(ldu, F), p(R), ld(ldr, F), Y.ptr,
+                                ld(ldy, F), p(Z), ld(ldz, F), p(ws), ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
 
     def linear(self, **kw) -> None:
         """Y = R + scale act(Z) U, Z = X W^T + bias (keyword arguments mirror ah_linear_desc; bias, U, R and Z may be left out, strides
@@ -214,9 +200,14 @@ class Device:
         """Bytes of workspace that linear needs for the same arguments (ws left out)."""
         return self._sized(self.lib.ah_linear_workspace, self._linear_desc(**kw))
 
-    def _linear_grad_desc(self, dtype, N, D, F, dY, grad_dtype=L.AH_F32, act=L.ACT_NONE, scale=1.0, ws=None, **kw):
-        return self._fill(L.ah_linear_grad_desc, dict(ldx=D, ldw=D, ldz=F, ldu=F, lddy=F, lddx=D, lddw=D, lddu=F), dtype=dtype, grad_dtype=grad_dtype,
-                          N=N, D=D, F=F, dY=dY, act=act, scale=scale, ws=ws, _ws=ws, **kw)
+    @staticmethod
+    def _linear_grad_desc(dtype, N, D, F, dY, grad_dtype=L.AH_F32, act=L.ACT_NONE, scale=1.0, X=None, W=None, Z=None, U=None, dX=None, dW=None, dbias=None,
+                          dU=None, ldx=None, ldw=None, ldz=None, ldu=None, lddy=None, lddx=None, lddw=None, lddu=None, ws=None, ws_bytes=None):
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        ld = lambda v, n: n if v is None else v     # noqa: E731
+        return L.ah_linear_grad_desc(dtype, grad_dtype, act, N, D, F, scale, p(X), ld(ldx, D), p(W), ld(ldw, D), p(Z), ld(ldz, F), p(U), ld(ldu, F), dY.ptr,
+                                     ld(lddy, F), p(dX), ld(lddx, D), p(dW), ld(lddw, D), p(dbias), p(dU), ld(lddu, F), p(ws),
+                                     ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
 
     def linear_grad(self, **kw) -> None:
         """The gradients of linear that are given buffers: dX, dW, dbias, dU (keyword arguments mirror ah_linear_grad_desc)."""
@@ -226,20 +217,28 @@ class Device:
         """Bytes of workspace that linear_grad needs for the same arguments (ws left out)."""
         return self._sized(self.lib.ah_linear_grad_workspace, self._linear_grad_desc(**kw))
 
-    def _residual_norm_args(self, cls, strides, dtype, N, D, res_dtype=None, post=L.NORM_NONE, pre=L.NORM_NONE, rows_per_gate=0, eps=1e-6, skip=1.0,
-                            scale=1.0, **kw):
-        return self._fill(cls, dict.fromkeys(strides, D), dtype=dtype, res_dtype=dtype if res_dtype is None else res_dtype, N=N, D=D, post=post, pre=pre,
-                          rows_per_gate=rows_per_gate, eps=eps, skip=skip, scale=scale, **kw)
-
-    def residual_norm(self, **kw) -> None:
-        """H_out = skip H + scale gate post(Y), O = pre(H_out) (keyword arguments mirror ah_residual_norm_desc; res_dtype defaults to dtype,
-        arrays may be left out as ah_residual_norm says, strides default to contiguous rows)."""
-        d = self._residual_norm_args(L.ah_residual_norm_desc, ("ldh", "ldy", "ldgate", "ldh_out", "ldo"), **kw)
+    def residual_norm(self, dtype, N, D, res_dtype=None, post=L.NORM_NONE, pre=L.NORM_NONE, rows_per_gate=0, eps=1e-6, skip=1.0, scale=1.0, H=None, Y=None,
+                      gate=None, post_w=None, post_b=None, pre_w=None, pre_b=None, H_out=None, O=None, ldh=None, ldy=None, ldgate=None, ldh_out=None,
+                      ldo=None) -> None:
+        """H_out = skip H + scale gate post(Y), O = pre(H_out) (arguments mirror ah_residual_norm_desc; res_dtype defaults to dtype, arrays may
+        be left out as ah_residual_norm says, strides default to contiguous rows)."""
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        ld = lambda v: D if v is None else v        # noqa: E731
+        d = L.ah_residual_norm_desc(dtype, dtype if res_dtype is None else res_dtype, N, D, post, pre, rows_per_gate, eps, skip, scale, p(H), ld(ldh), p(Y),
+                                    ld(ldy), p(gate), ld(ldgate), p(post_w), p(post_b), p(pre_w), p(pre_b), p(H_out), ld(ldh_out), p(O), ld(ldo))
         L.check(self.lib.ah_residual_norm(self.h, C.byref(d)))
 
-    def _residual_norm_grad_desc(self, ws=None, **kw):
-        return self._residual_norm_args(L.ah_residual_norm_grad_desc, ("ldy", "ldgate", "ldh_out", "lddh_out", "lddo", "lddh", "lddy", "lddgate"), ws=ws,
-                                        _ws=ws, **kw)
+    @staticmethod
+    def _residual_norm_grad_desc(dtype, N, D, res_dtype=None, post=L.NORM_NONE, pre=L.NORM_NONE, rows_per_gate=0, eps=1e-6, skip=1.0, scale=1.0, Y=None,
+                                 gate=None, post_w=None, post_b=None, pre_w=None, H_out=None, dH_out=None, dO=None, dH=None, dY=None, dgate=None,
+                                 dpost_w=None, dpost_b=None, dpre_w=None, dpre_b=None, ldy=None, ldgate=None, ldh_out=None, lddh_out=None, lddo=None,
+                                 lddh=None, lddy=None, lddgate=None, ws=None, ws_bytes=None):
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        ld = lambda v: D if v is None else v        # noqa: E731
+        return L.ah_residual_norm_grad_desc(dtype, dtype if res_dtype is None else res_dtype, N, D, post, pre, rows_per_gate, eps, skip, scale, p(Y), ld(ldy),
+                                            p(gate), ld(ldgate), p(post_w), p(post_b), p(pre_w), p(H_out), ld(ldh_out), p(dH_out), ld(lddh_out), p(dO),
+                                            ld(lddo), p(dH), ld(lddh), p(dY), ld(lddy), p(dgate), ld(lddgate), p(dpost_w), p(dpost_b), p(dpre_w), p(dpre_b),
+                                            p(ws), ws_bytes if ws_bytes is not None else 0 if ws is None else ws.nbytes)
 
     def residual_norm_grad(self, **kw) -> None:
         """The gradients of residual_norm that are given buffers: dH, dY, dgate and the weights' (keyword arguments mirror

@@ -29,7 +29,7 @@ __device__ __forceinline__ float sigmoid(float t, float &slope) {
 // rounded to f16.
 template <bool FAST>
 __device__ __forceinline__ float normal(float z, float &g) {
-    const float e = exp_of(-0.5f * z * z);
+    const float e = FAST ? __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z) : exp_of(-0.5f * z * z);
     g = 0.3989422804014327f * e;
     if constexpr (FAST) {
         const float t = __builtin_amdgcn_rcpf(fmaf(0.305f, fabsf(z), 1.0f));
@@ -47,14 +47,28 @@ __device__ __forceinline__ float normal(float z, float &g) {
     }
 }
 
-// act(z). NaN stays NaN under each of them.
+// FAST forms, for results that are rounded to f16: s(t) = 1 / (1 + 2^(-t log2 e)) without the exponent's correction and folding of signs
+// (within 2^-20 up to |t| = 16, past which s is 0 or 1 to 2^-22), and 1 - s by subtraction (off by 2^-24 of 1).
+template <bool FAST>
+__device__ __forceinline__ float gate_of(int act, float z, float &q) {   // s(z (a + q)), q = b z^2
+    const float a = act == AH_ACT_SILU ? 1.0f : kTanhA, b = act == AH_ACT_SILU ? 0.0f : kTanhB;
+    if constexpr (FAST) {
+        q = b * (z * z);
+        return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * (fmaf(z * z, -kLog2e * b, -kLog2e * a))));
+    } else {
+        float unused;
+        q = b * fminf(z * z, 1e30f);   // (0 times an infinite square would be NaN)
+        return sigmoid(z * (a + q), unused);
+    }
+}
+
+// act(z). NaN stays NaN under each of them. FAST takes z of at most 2^63.
 template <bool FAST>
 __device__ __forceinline__ float act_of(int act, float z) {
     float unused;
     if (act <= AH_ACT_RELU) return act == AH_ACT_RELU && z < 0.0f ? 0.0f : z;
     if (act == AH_ACT_GELU) return z * normal<FAST>(z, unused);
-    const float a = act == AH_ACT_SILU ? 1.0f : kTanhA, b = act == AH_ACT_SILU ? 0.0f : kTanhB;
-    return z * sigmoid(z * fmaf(b, fminf(z * z, 1e30f), a), unused);   // (0 times an infinite square would be NaN)
+    return z * gate_of<FAST>(act, z, unused);
 }
 
 // act(z) and act'(z). Past |z| = 1e4 the slopes of both GELUs are 0 and 1 exactly, and their formulas would meet infinities.
@@ -71,11 +85,22 @@ __device__ __forceinline__ float act_slope(int act, float z, float &slope) {
         slope = g > 0.0f ? fmaf(z, g, p) : p;
         return z * p;
     }
-    const float a = act == AH_ACT_SILU ? 1.0f : kTanhA, b = act == AH_ACT_SILU ? 0.0f : kTanhB, q = b * fminf(z * z, 1e8f);
-    float s1;
-    const float s = sigmoid(z * (a + q), s1);
-    slope = s1 > 0.0f ? fmaf(z * s1, fmaf(3.0f, q, a), s) : s;
-    return z * s;
+    const float a = act == AH_ACT_SILU ? 1.0f : kTanhA;
+    if constexpr (FAST) {
+        float q;
+        const float s = gate_of<true>(act, z, q);
+        slope = fmaf(z * (s - s * s), fmaf(3.0f, q, a), s);
+        return z * s;
+    } else {
+        const float b = act == AH_ACT_SILU ? 0.0f : kTanhB, q = b * fminf(z * z, 1e8f);
+        float s1;
+        const float s = sigmoid(z * (a + q), s1);
+        slope = s1 > 0.0f ? fmaf(z * s1, fmaf(3.0f, q, a), s) : s;
+        return z * s;
+    }
 }
+
+// No act's slope is larger than this: the GELUs' largest is 1.129, SiLU's 1.0999.
+__device__ __forceinline__ float slope_bound(int act) { return act <= AH_ACT_RELU ? 1.0f : 1.13f; }
 
 }  // namespace ah

@@ -64,10 +64,9 @@ __device__ __forceinline__ void layer_rows(const Layer &l, int m0, int n0, int i
     }
     raw b = {};
     if (l.bias && in) b = load_raw8((const T *)l.bias, out.n, l.F);
-    int ew[8] = {};
-    if (l.ew && in)
-#pragma unroll
-        for (int k = 0; k < 8; k++) ew[k] = l.ew[min(out.n + k, l.F - 1)];
+    typedef int i8 __attribute__((ext_vector_type(8), aligned(4)));
+    i8 ew = {};
+    if (l.ew && in) ew = *(const i8 *)(l.ew + out.n);   // (there is room behind the last)
     out.put(acc);
     if (!in) return;
 #pragma unroll
@@ -241,7 +240,7 @@ Layout layout(const ah_linear_desc &d) {
     if (l.pack_w) l.Wp = take((int64_t)d.F * l.Dp * 2 * l.P);
     if (!f16 && !l.few) {
         l.ex = take((int64_t)d.N * 4);
-        l.ew = take((int64_t)d.F * 4);
+        l.ew = take(((int64_t)d.F + 7) * 4);
     }
     if (l.few) {
         const pg::Work w = few_work(d, l);

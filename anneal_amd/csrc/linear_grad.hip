@@ -2,12 +2,14 @@
 //
 //   dZ = s dY U act'(Z),  dX = dZ W,  dW = dZ^T X,  db = sum_n dZ,  dU = s dY act(Z)
 //
-// dZ is formed twice: once for its largest magnitude, which sets the power of two that its planes are scaled by, and once to be stored as
-// one f16 plane (f16 gradients) or two (f32 ones), which both products then read (plane_gemm.h); the second pass also writes dU and
-// leaves db's sums of 64 rows. f32 X and W are scanned with it and packed as two planes; f16 ones are read as they lie where their
+// A first pass bounds dZ's largest magnitude, which sets the power of two that its planes are scaled by; a second one stores it as
+// one f16 plane (f16 gradients) or two (f32 ones), which both products then read (plane_gemm.h), also writes dU and
+// leaves db's sums of 32 rows. f32 X and W are scanned with it and packed as two planes; f16 ones are read as they lie where their
 // rows are aligned. Up to 128 rows (64 in f16) dX reads W once, as it lies (linear_ce_few.h). Sums run in a fixed order. Bound by the
 // matrix cores: two products of 2 N D F operations; dZ's passes move 10 (f16) to 28 (f32) bytes an element.
 #include "linear.h"
+
+#include <string.h>
 
 #include <algorithm>
 
@@ -19,7 +21,7 @@ namespace ah {
 namespace {
 
 constexpr int kScans = 1024;   // workgroups that look for an array's largest magnitude, at most
-constexpr int kRows = 64;      // rows of a block of dZ; also the k of a one-plane stage, up to which rows are cleared
+constexpr int kRows = 32;      // rows of a block of dZ
 
 struct GradIn {
     int N, D, F, act;
@@ -30,19 +32,29 @@ struct GradIn {
     long ldx, ldw;
 };
 
-// dZ and dU at row n, columns c .. c+3.
+// What a row's eight columns of dZ are made of, as it lies.
 template <class T>
-__device__ __forceinline__ floatx4 dz_at(const GradIn &g, long n, int c, floatx4 &du) {
-    const floatx4 dy = pg::load4((const T *)g.dY + n * g.lddy, c, g.F);
-    floatx4 z = {}, u = {1.0f, 1.0f, 1.0f, 1.0f}, v;
-    if (g.Z) z = pg::load4((const T *)g.Z + n * g.ldz, c, g.F);
-    if (g.U) u = pg::load4((const T *)g.U + n * g.ldu, c, g.F);
+struct Line {
+    typename Raw8<T>::type dy, z, u;
+};
+template <class T>
+__device__ __forceinline__ Line<T> load_line(const GradIn &g, long n, int c) {
+    Line<T> l = {};
+    l.dy = load_raw8((const T *)g.dY + n * g.lddy, c, g.F);
+    if (g.Z) l.z = load_raw8((const T *)g.Z + n * g.ldz, c, g.F);
+    if (g.U) l.u = load_raw8((const T *)g.U + n * g.ldu, c, g.F);
+    return l;
+}
+// dZ and dU.
+template <class T>
+__device__ __forceinline__ f8 dz_of(const GradIn &g, const Line<T> &l, f8 &du) {
+    f8 v;
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
+    for (int k = 0; k < 8; k++) {
         float slope;
-        const float y = act_slope<sizeof(T) == 2>(g.act, z[k], slope), t = g.scale * dy[k];
-        v[k] = t * slope * u[k];
-        du[k] = t * y;
+        const float y = act_slope<sizeof(T) == 2>(g.act, (float)l.z[k], slope), t = g.scale * (float)l.dy[k];
+        v.v[k] = g.U ? t * slope * (float)l.u[k] : t * slope;
+        du.v[k] = t * y;
     }
     return v;
 }
@@ -53,29 +65,49 @@ struct ScanArgs {
     int zblocks, xblocks, wblocks;   // workgroups of each array, in this order
     unsigned *maxes;                 // [3][kScans]
 };
-__device__ __forceinline__ unsigned max4(unsigned m, floatx4 v) {
+template <class T>
+__device__ __forceinline__ unsigned max8(unsigned m, const T &v) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) m = max(m, pg::magnitude(__float_as_uint(v[k])));
+    for (int k = 0; k < 8; k++) m = max(m, pg::magnitude(__float_as_uint((float)v[k])));
     return m;
 }
-// A wave a stretch of 1024 values of a row.
+// A wave a stretch of 2048 values of a row. dZ's magnitude is bounded by that of s dY U times the largest slope: neither Z is read for it nor
+// an activation evaluated, and where the bound is loose by 2^n the planes lose n of the 29 (one plane) or 18 binades that they have to spare.
 template <class T>
 __global__ __launch_bounds__(256) void linear_grad_scan_kernel(GradIn g, ScanArgs a) {
     __shared__ unsigned red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, which = (int)blockIdx.x < a.zblocks ? 0 : (int)blockIdx.x < a.zblocks + a.xblocks ? 1 : 2;
     const int b = blockIdx.x - (which == 0 ? 0 : which == 1 ? a.zblocks : a.zblocks + a.xblocks), blocks = which == 0 ? a.zblocks : which == 1 ? a.xblocks : a.wblocks;
-    const int width = which == 0 ? g.F : g.D, segs = (width + 1023) / 1024;
+    const int width = which == 0 ? g.F : g.D, segs = (width + 2047) / 2048;
     const long rows = which == 2 ? g.F : g.N;
     unsigned m = 0;
     for (long q = (long)b * 4 + wave; q < rows * segs; q += (long)blocks * 4) {
         const long r = q / segs;
-        const int c0 = (int)(q - r * segs) * 1024 + lane * 4;
+        const int c0 = (int)(q - r * segs) * 2048 + lane * 8;
+        if (which == 0) {
+            typename Raw8<T>::type dy[4] = {}, u[4] = {};
 #pragma unroll
-        for (int k = 0; k < 1024; k += 256) {
-            if (c0 + k >= width) continue;
-            floatx4 unused;
-            if (which == 0) m = max4(m, dz_at<T>(g, r, c0 + k, unused));
-            else m = max4(m, pg::load4(which == 1 ? (const float *)g.X + r * g.ldx : (const float *)g.W + r * g.ldw, c0 + k, width));
+            for (int k = 0; k < 4; k++) {
+                if (c0 + k * 512 >= width) continue;
+                dy[k] = load_raw8((const T *)g.dY + r * g.lddy, c0 + k * 512, width);
+                if (g.U) u[k] = load_raw8((const T *)g.U + r * g.ldu, c0 + k * 512, width);
+            }
+            const float s = g.scale * slope_bound(g.act);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = s * (float)dy[k][e] * (g.U ? (float)u[k][e] : 1.0f);
+                m = max8(m, v);
+            }
+        } else {
+            const float *p = which == 1 ? (const float *)g.X + r * g.ldx : (const float *)g.W + r * g.ldw;
+            raw8_f32 v[4] = {};
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (c0 + k * 512 < width) v[k] = load_raw8(p, c0 + k * 512, width);
+#pragma unroll
+            for (int k = 0; k < 4; k++) m = max8(m, v[k]);
         }
     }
     for (int o = 32; o >= 1; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
@@ -110,47 +142,50 @@ struct PackArgs {
 // P: planes of dZ; PO: of X and W.
 template <class T, int P, int PO>
 __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArgs a, ScanArgs s) {
-    __shared__ float red[3][64][4];
+    __shared__ float red[3][64][8];
     int e[3] = {};
     if (s.zblocks) e[0] = pg::plane_exp(join_maxes(s.maxes, s.zblocks));
     if (s.xblocks) e[1] = pg::plane_exp(join_maxes(s.maxes + kScans, s.xblocks));
     if (s.wblocks) e[2] = pg::plane_exp(join_maxes(s.maxes + 2 * kScans, s.wblocks));
     if (blockIdx.x == 0 && threadIdx.x < 3) a.exps[threadIdx.x] = threadIdx.x == 0 ? e[0] : threadIdx.x == 1 ? e[1] : e[2];
-    if ((int)blockIdx.x < a.zblocks) {   // 64 rows by 256 columns: a thread has four columns of every fourth row
-        const int rb = blockIdx.x / a.zcols, n = ((int)blockIdx.x - rb * a.zcols) * 256 + (threadIdx.x & 63) * 4, w = threadIdx.x >> 6;
-        floatx4 col = {};
+    if ((int)blockIdx.x < a.zblocks) {   // kRows rows by 512 columns: a thread has eight columns of every fourth row
+        const int rb = blockIdx.x / a.zcols, n = ((int)blockIdx.x - rb * a.zcols) * 512 + (threadIdx.x & 63) * 8, w = threadIdx.x >> 6;
+        constexpr int B = sizeof(T) == 2 ? 4 : 2;   // rows whose loads are in flight together
+        f8 col = {};
         if (n < a.Fp) {
-#pragma unroll 4
-            for (int k = w; k < kRows; k += 4) {
-                const int m = rb * kRows + k;
-                floatx4 v = {}, du;
-                if (m < g.N && n < g.F) {
-                    v = dz_at<T>(g, m, n, du);
-                    if (a.dU) pg::store4((T *)a.dU + (long)m * a.lddu, n, g.F, du);
-                    col += v;
+            for (int k0 = w; k0 < kRows; k0 += 4 * B) {
+                Line<T> line[B] = {};
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    const int m = rb * kRows + k0 + 4 * b;
+                    if (m < g.N && n < g.F) line[b] = load_line<T>(g, m, n);
                 }
-                if (!a.dZ) continue;
 #pragma unroll
-                for (int c = 0; c < 4; c++) v[c] = n + c < g.F ? ldexpf(v[c], e[0]) : 0.0f;
-                if constexpr (P == 1) {
-                    pg::h4 h;
+                for (int b = 0; b < B; b++) {
+                    const int m = rb * kRows + k0 + 4 * b;
+                    f8 v = {}, du;
+                    if (m < g.N && n < g.F) {
+                        v = dz_of<T>(g, line[b], du);
+                        if (a.dU) store_f8((T *)a.dU + (long)m * a.lddu, n, g.F, du);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) h[c] = (half_t)v[c];
-                    *(pg::h4 *)(a.dZ + pg::panel_at<1>(a.Np, m, n)) = h;
-                } else {
-                    pg::plane_store(a.dZ + pg::panel_at<2>(a.Np, m, n), v);
+                        for (int c = 0; c < 8; c++) col.v[c] += v.v[c];
+                    }
+                    if (!a.dZ) continue;
+#pragma unroll
+                    for (int c = 0; c < 8; c++) v.v[c] = n + c < g.F ? ldexpf(v.v[c], e[0]) : 0.0f;
+                    plane_store8<P>(a.dZ + pg::panel_at<P>(a.Np, m, n), v);
                 }
             }
         }
         if (!a.dbpart) return;
         if (w > 0)
 #pragma unroll
-            for (int c = 0; c < 4; c++) red[w - 1][threadIdx.x & 63][c] = col[c];
+            for (int c = 0; c < 8; c++) red[w - 1][threadIdx.x & 63][c] = col.v[c];
         __syncthreads();
         if (w == 0)
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (n + c < g.F) a.dbpart[(long)rb * g.F + n + c] = col[c] + red[0][threadIdx.x][c] + red[1][threadIdx.x][c] + red[2][threadIdx.x][c];
+            for (int c = 0; c < 8; c++)
+                if (n + c < g.F) a.dbpart[(long)rb * g.F + n + c] = col.v[c] + red[0][threadIdx.x][c] + red[1][threadIdx.x][c] + red[2][threadIdx.x][c];
         return;
     }
     constexpr int ESZ = PO == 1 ? 2 : 4;
@@ -161,22 +196,9 @@ __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArg
     }
 }
 
-// db: the row blocks' sums in order, 64 columns a workgroup and 16 runs of blocks.
-__global__ __launch_bounds__(1024) void linear_grad_db_kernel(const float *part, int blocks, int F, float *db) {
-    __shared__ float red[16][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6, each = (blocks + 15) / 16;
-    float s = 0.0f;
-    if (c < F)
-#pragma unroll 8
-        for (int b = k * each; b < min(blocks, (k + 1) * each); b++) s += part[(long)b * F + c];
-    red[k][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (k || c >= F) return;
-    for (int r = 1; r < 16; r++) s += red[r][threadIdx.x];
-    db[c] = s;
-}
-
 // ── the products ───────────────────────────────────────────────────────────────
+// dX and dW go in one launch (and what was split of them is joined in one), dX's workgroups first: what one leaves idle in its last round the
+// other fills (1999 x 776 x 3104 in f32: 49 and 50 us one after the other, 73 together). db's workgroups follow.
 
 struct ProductArgs {
     pg::Operand A, B;
@@ -187,6 +209,29 @@ struct ProductArgs {
     long ldc;
     int out16;
 };
+struct PairArgs {
+    ProductArgs x, w;      // dX, dW
+    int xblocks, wblocks;  // workgroups; dX's a multiple of 8, some of which may have nothing to do
+    const float *dbpart;
+    int dbrows, F;
+    float *db;
+};
+
+// db: the row blocks' sums in order, 64 columns a workgroup and NT / 64 runs of blocks.
+template <int NT>
+__device__ __forceinline__ void sum_db(const PairArgs &a, int block, char *smem) {
+    float(*red)[64] = (float(*)[64])smem;
+    const int c = block * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6, each = (a.dbrows + NT / 64 - 1) / (NT / 64);
+    float s = 0.0f;
+    if (c < a.F)
+#pragma unroll 8
+        for (int b = k * each; b < min(a.dbrows, (k + 1) * each); b++) s += a.dbpart[(long)b * a.F + c];
+    red[k][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (k || c >= a.F) return;
+    for (int r = 1; r < NT / 64; r++) s += red[r][threadIdx.x];
+    a.db[c] = s;
+}
 
 template <class C>
 __device__ __forceinline__ void tile_at(const ProductArgs &a, int tile, int &m0, int &n0) {
@@ -216,11 +261,10 @@ __device__ __forceinline__ void product_rows(const ProductArgs &a, int m0, int n
 }
 
 template <class C>
-__global__ __launch_bounds__(C::NT, 2) void linear_grad_kernel(ProductArgs a) {
-    __shared__ __attribute__((aligned(1024))) char smem[C::SMEM];
+__device__ __forceinline__ void product(const ProductArgs &a, int block, char *smem) {
     static_assert(tile_out_bytes<C>() <= C::SMEM, "the tile leaves through the stages' buffers");
     int tile, slot, first, count, m0, n0;
-    pg::pick(a.w, blockIdx.x, a.nk, tile, slot, first, count);
+    pg::pick(a.w, block, a.nk, tile, slot, first, count);
     tile_at<C>(a, tile, m0, n0);
     floatx4 acc[C::FA][C::FB];
     pg::contract<C>(a.A, a.B, m0, n0, first, count, smem, acc);
@@ -236,13 +280,34 @@ __global__ __launch_bounds__(C::NT, 2) void linear_grad_kernel(ProductArgs a) {
     }
 }
 template <class C>
-__global__ __launch_bounds__(C::NT) void linear_grad_join_kernel(ProductArgs a) {
-    __shared__ __attribute__((aligned(16))) char smem[tile_out_bytes<C>()];
+__device__ __forceinline__ void join(const ProductArgs &a, int tile, int row, char *smem) {
     int m0, n0;
-    tile_at<C>(a, a.w.whole + blockIdx.x, m0, n0);
+    tile_at<C>(a, a.w.whole + tile, m0, n0);
     floatx4 v[C::FB];
-    pg::sum_partials<C>(a.w, blockIdx.x, blockIdx.y, v);
-    product_rows<C>(a, m0, n0, blockIdx.y, v, smem);
+    pg::sum_partials<C>(a.w, tile, row, v);
+    product_rows<C>(a, m0, n0, row, v, smem);
+}
+
+template <class X, class W>
+__global__ __launch_bounds__(X::NT, 2) void linear_grad_kernel(PairArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[std::max(X::SMEM, W::SMEM)];
+    static_assert(X::NT == W::NT, "one launch");
+    const int b = blockIdx.x;
+    if (b < a.xblocks) {
+        if (b < a.x.w.blocks()) product<X>(a.x, b, smem);
+    } else if (b < a.xblocks + a.wblocks) {
+        product<W>(a.w, b - a.xblocks, smem);
+    } else {
+        sum_db<X::NT>(a, b - a.xblocks - a.wblocks, smem);
+    }
+}
+// A workgroup for each 16 rows of a tile's waves; xblocks, wblocks count those.
+template <class X, class W>
+__global__ __launch_bounds__(X::NT) void linear_grad_join_kernel(PairArgs a) {
+    __shared__ __attribute__((aligned(16))) char smem[std::max(tile_out_bytes<X>(), tile_out_bytes<W>())];
+    const int b = blockIdx.x;
+    if (b < a.xblocks) join<X>(a.x, b / X::FA, b % X::FA, smem);
+    else join<W>(a.w, (b - a.xblocks) / W::FA, (b - a.xblocks) % W::FA, smem);
 }
 
 // dX from W as it lies, for few rows: one row of tiles.
@@ -291,19 +356,85 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 bool rows_aligned(const void *p, int64_t ld, int D) { return D % 8 == 0 && ld % 8 == 0 && ((uintptr_t)p & 15) == 0 && ld <= 1 << 22; }
 
+// How the two products are cut: widths of the tiles and splits of K, by a model of the time they take together. Stage times are those of
+// pg::plan; tiles of 256 go with each other, and narrower ones, which have half the threads. (64-wide tiles of one plane have no
+// layout along k.)
+struct Cut {
+    int width;
+    pg::Work w;
+    long part_bytes() const { return w.splits > 1 ? (long)w.rest * w.splits * width * width * 4 : 0; }
+};
+struct Cuts {
+    Cut x, w;
+};
+constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
+
+// n jobs of p us and then m of q on `slots` machines: when the last is done.
+double makespan(long n, double p, long m, double q, long slots) {
+    const long a = n / slots, r = n % slots;   // r machines have a + 1 of the first, the others a
+    if (m == 0) return (a + (r > 0)) * p;
+    double t = (n * p + m * q) / slots;
+    for (int i = 0; i < 64; i++) {
+        const auto fit = [&](double from) { return t <= from ? 0l : (long)((t - from) / q + 1e-6); };
+        const long can = r * fit((a + 1) * p) + (slots - r) * fit(a * p);
+        if (can >= m) break;
+        t += std::max(q * (m - can) / slots, q / 64);
+    }
+    return std::max(t, (a + (r > 0)) * p);
+}
+
+Cuts cuts_of(int N, int D, int F, int P, int PO, bool with_x) {
+    struct Key {
+        int v[6];
+    };
+    const Key key{{N, D, F, P, PO, with_x}};
+    static thread_local Key last_key{};
+    static thread_local Cuts last{};
+    if (!memcmp(&key, &last_key, sizeof key)) return last;   // of the call's own workspace query, or the step before
+    const int row = P == 1 ? 0 : PO == 1 ? 1 : 2;
+    // us a stage of 256, 128 and 64, with one workgroup on each CU (of 256: one alone on the chip) and with as many as there is room for
+    constexpr double kFirst[3][3] = {{1.22, 0.72, 0}, {1.18, 0.61, 0}, {1.53, 0.68, 0.26}}, kFull[3][3] = {{1.77, 1.15, 0}, {1.73, 0.97, 0}, {2.30, 1.33, 0.41}};
+    const int bk = row == 0 ? 64 : 32;
+    const long nx = ceil_div(F, bk), nw = ceil_div(N, bk);
+    double best = 1e30;
+    Cuts c{};
+    for (int kind = 0; kind < 2; kind++) {
+        const long slots = kind == 0 ? 256 : 512;
+        for (int ix = kind; ix <= (kind && PO == 2 ? 2 : kind); ix++)
+            for (int iw = kind; iw <= (kind && PO == 2 ? 2 : kind); iw++) {
+                const int wx = 256 >> ix, ww = 256 >> iw;
+                const long tx = with_x ? (long)ceil_div(N, wx) * ceil_div(D, wx) : 0, tw = (long)ceil_div(F, ww) * ceil_div(D, ww);
+                for (const int sx : kSplits) {
+                    if (sx > 1 && (!with_x || nx < 2 * sx || tx * sx > 4 * slots)) break;
+                    for (const int sw : kSplits) {
+                        if (sw > 1 && (nw < 2 * sw || tw * sw > 4 * slots)) break;
+                        const double busy = (double)std::min(slots, tx * sx + tw * sw) / 256, fixed = kind == 0 ? 7.0 : 5.0;
+                        const double load = kind == 0 ? busy : std::max(0.0, busy - 1.0);
+                        const auto stage = [&](int i) { return kFirst[row][i] + (kFull[row][i] - kFirst[row][i]) * load; };
+                        const double px = (nx + sx - 1) / sx * stage(ix) + fixed, pw = (nw + sw - 1) / sw * stage(iw) + fixed;
+                        double us = makespan(tx * sx, px, tw * sw, pw, slots);
+                        if (sx > 1 || sw > 1) us += 4.0 + ((sx > 1 ? (double)tx * sx * wx * wx : 0.0) + (sw > 1 ? (double)tw * sw * ww * ww : 0.0)) * 8 / 4e6;
+                        if (us < best) {
+                            best = us;
+                            c.x = {wx, sx > 1 ? pg::Work{0, (int)tx, sx, nullptr} : pg::Work{(int)tx, 0, 1, nullptr}};
+                            c.w = {ww, sw > 1 ? pg::Work{0, (int)tw, sw, nullptr} : pg::Work{(int)tw, 0, 1, nullptr}};
+                        }
+                    }
+                }
+            }
+    }
+    last_key = key;
+    last = c;
+    return c;
+}
 struct Layout {
     int P, PO;                 // planes of dZ; of X and W
     int Np, Fp, Dp, few;
     bool products, pack_x, pack_w;
-    int64_t exps, maxes, dbpart, dZ, Xp, Wp, sums, total;
+    Cuts cuts;
+    int64_t exps, maxes, dbpart, dZ, Xp, Wp, sums, wsums, total;
 };
 
-pg::Plan dx_plan(const ah_linear_grad_desc &d, const Layout &l) {
-    return pg::plan([&](int w) { return (long)ceil_div(d.N, w) * ceil_div(d.D, w); }, d.F, l.P, l.PO, l.PO == 2);   // (64-wide tiles of one plane
-}
-pg::Plan dw_plan(const ah_linear_grad_desc &d, const Layout &l) {
-    return pg::plan([&](int w) { return (long)ceil_div(d.F, w) * ceil_div(d.D, w); }, d.N, l.P, l.PO, l.PO == 2);   // have no layout along k)
-}
 pg::Work few_work(const ah_linear_grad_desc &d, const Layout &l) {
     return few::work(ceil_div(d.D, 256), ceil_div(d.F, few::across_v(l.P)), 2 * std::max(1.75, d.dtype == AH_F16 ? 0.0 : 0.43 * l.few), l.few * 16l * 256 * 4);
 }
@@ -332,31 +463,48 @@ Layout layout(const ah_linear_grad_desc &d) {
     if (l.products) l.dZ = take((int64_t)l.Np * l.Fp * 2 * l.P);
     if (l.pack_x) l.Xp = take((int64_t)d.N * l.Dp * 2 * l.PO);
     if (l.pack_w) l.Wp = take((int64_t)d.F * l.Dp * 2 * l.PO);
-    int64_t sums = 0;
+    const bool few = d.N <= (f16 ? kFewF16 : kFewF32) && d.D >= 8;
+    if (l.products) l.cuts = cuts_of(d.N, d.D, d.F, l.P, l.PO, !few);   // of both products, whichever are asked for: the same bits
     if (l.few) {
         const pg::Work w = few_work(d, l);
-        sums = w.splits > 1 ? (int64_t)w.rest * w.splits * l.few * 16 * 256 * 4 : 0;
+        l.sums = take(w.splits > 1 ? (int64_t)w.rest * w.splits * l.few * 16 * 256 * 4 : 0);
     } else if (d.dX) {
-        sums = dx_plan(d, l).part_bytes();
+        l.sums = take(l.cuts.x.part_bytes());
     }
-    if (d.dW) sums = std::max<int64_t>(sums, dw_plan(d, l).part_bytes());
-    l.sums = take(sums);
+    if (d.dW) l.wsums = take(l.cuts.w.part_bytes());
     l.total = at;
     return l;
 }
 
-template <class C>
-void launch(ProductArgs a, hipStream_t s) {
-    a.tiles_m = ceil_div(a.M, C::BM);
-    a.tiles_n = ceil_div(a.N, C::BN);
-    hipLaunchKernelGGL((linear_grad_kernel<C>), dim3((unsigned)a.w.blocks()), dim3(C::NT), 0, s, a);
-    if (a.w.splits > 1) hipLaunchKernelGGL((linear_grad_join_kernel<C>), dim3((unsigned)a.w.rest, C::FA), dim3(C::NT), 0, s, a);
+template <class X, class W>
+void launch(PairArgs a, bool x, bool w, hipStream_t s) {
+    a.x.tiles_m = ceil_div(a.x.M, X::BM);
+    a.x.tiles_n = ceil_div(a.x.N, X::BN);
+    a.w.tiles_m = ceil_div(a.w.M, W::BM);
+    a.w.tiles_n = ceil_div(a.w.N, W::BN);
+    a.xblocks = x ? (a.x.w.blocks() + 7) & ~7 : 0;
+    a.wblocks = w ? a.w.w.blocks() : 0;
+    hipLaunchKernelGGL((linear_grad_kernel<X, W>), dim3((unsigned)(a.xblocks + a.wblocks + (a.db ? ceil_div(a.F, 64) : 0))), dim3(X::NT), 0, s, a);
+    a.xblocks = x && a.x.w.splits > 1 ? a.x.w.rest * X::FA : 0;
+    a.wblocks = w && a.w.w.splits > 1 ? a.w.w.rest * W::FA : 0;
+    if (a.xblocks + a.wblocks) hipLaunchKernelGGL((linear_grad_join_kernel<X, W>), dim3((unsigned)(a.xblocks + a.wblocks)), dim3(X::NT), 0, s, a);
 }
-template <int TA, int TB, int PA, int PB>
-void launch(const ProductArgs &a, int width, hipStream_t s) {
-    if (width == 256) launch<pg::Tile256<TA, TB, PA, PB>>(a, s);
-    else if (width == 128) launch<pg::Tile128<TA, TB, PA, PB>>(a, s);
-    else if constexpr (PB == 2) launch<pg::Tile64<TA, TB, PA, PB>>(a, s);
+template <int PA, int PB>
+void launch(const PairArgs &a, const Cuts &c, bool x, bool w, hipStream_t s) {
+    typedef pg::Tile128<0, 1, PA, PB> X128;
+    typedef pg::Tile128<1, 1, PA, PB> W128;
+    if (c.w.width == 256) {
+        launch<pg::Tile256<0, 1, PA, PB>, pg::Tile256<1, 1, PA, PB>>(a, x, w, s);
+        return;
+    }
+    if constexpr (PB == 2) {
+        typedef pg::Tile64<0, 1, PA, PB> X64;
+        typedef pg::Tile64<1, 1, PA, PB> W64;
+        if (c.x.width == 64 && c.w.width == 64) return launch<X64, W64>(a, x, w, s);
+        if (c.x.width == 64) return launch<X64, W128>(a, x, w, s);
+        if (c.w.width == 64) return launch<X128, W64>(a, x, w, s);
+    }
+    launch<X128, W128>(a, x, w, s);
 }
 
 template <int P, bool F16, int FA>
@@ -369,7 +517,7 @@ template <class T, int P, int PO>
 void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     char *ws = (char *)d.ws;
     const GradIn g{d.N, d.D, d.F, d.act, d.scale, d.dY, d.Z, d.U, d.lddy, d.ldz, d.ldu, d.X, d.W, d.ldx, d.ldw};
-    const auto scans = [](int64_t rows, int64_t width) { return (int)std::min<int64_t>((rows * ((width + 1023) / 1024) + 3) / 4, kScans); };
+    const auto scans = [](int64_t rows, int64_t width) { return (int)std::min<int64_t>((rows * ((width + 2047) / 2048) + 3) / 4, kScans); };
     ScanArgs sc{};
     sc.zblocks = l.products ? scans(d.N, d.F) : 0;
     sc.xblocks = l.pack_x && PO == 2 ? scans(d.N, d.D) : 0;
@@ -387,55 +535,55 @@ void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     p.Np = l.Np;
     p.Fp = l.Fp;
     p.Dp = l.Dp;
-    p.zcols = ceil_div(l.Fp, 256);
+    p.zcols = ceil_div(l.Fp, 512);
     p.zblocks = l.Np / kRows * p.zcols;
     p.rest = (int)std::min<int64_t>(((l.pack_x ? d.N : 0) + (int64_t)(l.pack_w ? d.F : 0) + 3) / 4, 4096);
     p.exps = (int *)(ws + l.exps);
     hipLaunchKernelGGL((linear_grad_pack_kernel<T, P, PO>), dim3((unsigned)(p.zblocks + p.rest)), dim3(256), 0, s, g, p, sc);
-    if (d.dbias) hipLaunchKernelGGL(linear_grad_db_kernel, dim3((unsigned)ceil_div(d.F, 64)), dim3(1024), 0, s, p.dbpart, l.Np / kRows, d.F, d.dbias);
-
-    ProductArgs a{};
-    a.ea = p.exps;
-    a.out16 = d.grad_dtype == AH_F16;
-    a.N = d.D;
-    if (d.dX) {
-        ProductArgs b = a;
-        b.M = d.N;
-        b.C = d.dX;
-        b.ldc = d.lddx;
-        if (l.few) {
-            const FewArgs f{ws + l.dZ, l.Np, l.Fp, d.F, d.W, d.ldw};
-            b.nk = ceil_div(d.F, few::across_v(P));
-            b.w = few_work(d, l);
-            b.w.part = (float *)(ws + l.sums);
-            if (l.few == 1) launch_few<P, PO == 1, 1>(b, f, s);
-            else if (l.few == 4) launch_few<P, PO == 1, 4>(b, f, s);
-            else if constexpr (PO == 2) launch_few<P, PO == 1, 8>(b, f, s);
-        } else {
-            const pg::Plan plan = dx_plan(d, l);
-            b.w = plan.w;
-            b.w.part = (float *)(ws + l.sums);
-            b.A = pg::panels(p.dZ, l.Np, l.Np, l.Fp);
-            b.B = l.pack_w ? pg::panels(p.Wp, d.F, l.Dp, d.F) : pg::row_major(d.W, d.ldw, d.D, d.F);
-            b.nk = ceil_div(d.F, P == 1 ? 64 : 32);   // every stage begins at a row of W that there is
-            b.eb = PO == 2 ? p.exps + 2 : nullptr;
-            launch<0, 1, P, PO>(b, plan.width, s);
-        }
+    PairArgs a{};
+    a.x.ea = a.w.ea = p.exps;
+    a.x.out16 = a.w.out16 = d.grad_dtype == AH_F16;
+    a.x.N = a.w.N = d.D;
+    a.x.M = d.N;
+    a.x.C = d.dX;
+    a.x.ldc = d.lddx;
+    a.w.M = d.F;
+    a.w.C = d.dW;
+    a.w.ldc = d.lddw;
+    a.db = d.dbias;
+    a.dbpart = p.dbpart;
+    a.dbrows = l.Np / kRows;
+    a.F = d.F;
+    if (l.few) {
+        ProductArgs b = a.x;
+        const FewArgs f{ws + l.dZ, l.Np, l.Fp, d.F, d.W, d.ldw};
+        b.nk = ceil_div(d.F, few::across_v(P));
+        b.w = few_work(d, l);
+        b.w.part = (float *)(ws + l.sums);
+        if (l.few == 1) launch_few<P, PO == 1, 1>(b, f, s);
+        else if (l.few == 4) launch_few<P, PO == 1, 4>(b, f, s);
+        else if constexpr (PO == 2) launch_few<P, PO == 1, 8>(b, f, s);
+    }
+    const bool x = d.dX && !l.few;
+    if (!x && !d.dW && !d.dbias) return;
+    constexpr int BK = P == 1 ? 64 : 32;   // every stage begins at a row of W or X that there is
+    if (x) {
+        a.x.w = l.cuts.x.w;
+        a.x.w.part = (float *)(ws + l.sums);
+        a.x.A = pg::panels(p.dZ, l.Np, l.Np, l.Fp);
+        a.x.B = l.pack_w ? pg::panels(p.Wp, d.F, l.Dp, d.F) : pg::row_major(d.W, d.ldw, d.D, d.F);
+        a.x.nk = ceil_div(d.F, BK);
+        a.x.eb = PO == 2 ? p.exps + 2 : nullptr;
     }
     if (d.dW) {
-        ProductArgs b = a;
-        const pg::Plan plan = dw_plan(d, l);
-        b.M = d.F;
-        b.C = d.dW;
-        b.ldc = d.lddw;
-        b.w = plan.w;
-        b.w.part = (float *)(ws + l.sums);
-        b.A = pg::panels(p.dZ, l.Np, l.Fp, l.Np);
-        b.B = l.pack_x ? pg::panels(p.Xp, d.N, l.Dp, d.N) : pg::row_major(d.X, d.ldx, d.D, d.N);
-        b.nk = ceil_div(d.N, P == 1 ? 64 : 32);
-        b.eb = PO == 2 ? p.exps + 1 : nullptr;
-        launch<1, 1, P, PO>(b, plan.width, s);
+        a.w.w = l.cuts.w.w;
+        a.w.w.part = (float *)(ws + l.wsums);
+        a.w.A = pg::panels(p.dZ, l.Np, l.Fp, l.Np);
+        a.w.B = l.pack_x ? pg::panels(p.Xp, d.N, l.Dp, d.N) : pg::row_major(d.X, d.ldx, d.D, d.N);
+        a.w.nk = ceil_div(d.N, BK);
+        a.w.eb = PO == 2 ? p.exps + 1 : nullptr;
     }
+    launch<P, PO>(a, l.cuts, x, d.dW != nullptr, s);
 }
 
 }  // namespace

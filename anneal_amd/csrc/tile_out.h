@@ -55,6 +55,19 @@ __device__ __forceinline__ void store_f8(T *row, int c, int D, const f8 &v) {
     store_raw8(row, c, D, x);
 }
 
+// The two planes of eight values at p (hi) and p + 32 (lo), or one.
+template <int P>
+__device__ __forceinline__ void plane_store8(half_t *p, const f8 &v) {
+    pg::h8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        hi[k] = (half_t)v.v[k];
+        lo[k] = (half_t)(v.v[k] - (float)hi[k]);
+    }
+    *(pg::h8 *)p = hi;
+    if constexpr (P == 2) *(pg::h8 *)(p + 32) = lo;
+}
+
 template <class C>
 constexpr int tile_out_bytes() {
     return C::NT / 64 * 16 * (C::WN + 4) * 4;

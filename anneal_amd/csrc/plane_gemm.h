@@ -315,9 +315,10 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
     constexpr std::integral_constant<int, FB *(C::TB ? 2 : 1)> NRB{};                                // of B's,
     constexpr std::integral_constant<int, decltype(NRA)::value + decltype(NRB)::value> NRAB{};       // of both
     // the last group of stage t, with the refill of its buffer spread between the MFMAs (the tail re-fetches the last stage into
-    // idle buffers, so that the number of loads in flight stays the same)
+    // idle buffers, so that the number of loads in flight stays the same). One plane by one, whose stage is the shortest: a load every second
+    // MFMA gives them half a group more to arrive in (8192 x 4096 -> 16384 988 -> 967 us; every MFMA 974)
     auto mma_refill = [&](h8 (&a)[FA], h8 (&b)[FB], int t, int buf) {
-        constexpr int NM = FA * FB, STEP = NM >= PERS ? NM / PERS : 1, EACH = NM >= PERS ? 1 : (PERS + NM - 1) / NM;
+        constexpr int NM = FA * FB, EVEN = NM >= PERS ? NM / PERS : 1, STEP = C::PA == 1 && C::PB == 1 && EVEN > 2 ? 2 : EVEN, EACH = NM >= PERS ? 1 : (PERS + NM - 1) / NM;
         const int tr = min(t + NS, nk - 1);
         __builtin_amdgcn_sched_barrier(0);
         int f = 0;

@@ -15,129 +15,70 @@
 #include "resnorm.h"
 
 #include <algorithm>
+#include <type_traits>
 
-#include "ah_common.h"
+#include "vec8.h"
 
 namespace ah {
 namespace {
 
 constexpr int kVec = 8;            // columns of a thread
 constexpr int kWide = 8192;        // columns that a workgroup's registers hold
+constexpr int kTermsT = 512;       // threads of a row whose terms are a launch of their own
 
-struct f8 {
-    float v[kVec];
-};
 template <class T>
-struct Raw {   // eight values as they lie; rows may start anywhere
-    typedef T type __attribute__((ext_vector_type(kVec), aligned(sizeof(T))));
-};
-template <class T>
-__device__ __forceinline__ typename Raw<T>::type load_raw(const T *row, int c, int D) {
-    typename Raw<T>::type x = {};
-    if (c + kVec <= D) {
-        x = *(const typename Raw<T>::type *)(row + c);
-    } else {
-#pragma unroll
-        for (int k = 0; k < kVec; k++)
-            if (c + k < D) x[k] = row[c + k];
+__device__ __forceinline__ f8 load8_or(const T *row, int c, int D, float other) {
+    return row ? load8(row, c, D) : all_of<kVec>(other);
+}
+
+// x from another lane of the row of 16: CTRL is a lane permutation of the cross-lane adder.
+template <int CTRL>
+__device__ __forceinline__ float lane_of(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+// Sum over groups of G lanes, in each of them: neighbours, pairs, then mirrored within 8 and 16 lanes, and the halves of 32 and 64 exchanged.
+template <int G>
+__device__ __forceinline__ float lanes_sum(float x) {
+    if constexpr (G >= 2) x += lane_of<0xB1>(x);    // 1 0 3 2
+    if constexpr (G >= 4) x += lane_of<0x4E>(x);    // 2 3 0 1
+    if constexpr (G >= 8) x += lane_of<0x141>(x);   // 7 .. 0
+    if constexpr (G >= 16) x += lane_of<0x140>(x);  // 15 .. 0
+    if constexpr (G >= 32) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    }
+    if constexpr (G >= 64) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
     }
     return x;
 }
-template <class V>
-__device__ __forceinline__ f8 widen(V x) {
-    f8 r;
-#pragma unroll
-    for (int k = 0; k < kVec; k++) r.v[k] = (float)x[k];
-    return r;
-}
-template <class T>
-__device__ __forceinline__ f8 load8(const T *row, int c, int D) {
-    return widen(load_raw(row, c, D));
-}
-__device__ __forceinline__ f8 all8(float x) {
-    f8 r;
-#pragma unroll
-    for (int k = 0; k < kVec; k++) r.v[k] = x;
-    return r;
-}
-template <class T>
-__device__ __forceinline__ f8 load8_or(const T *row, int c, int D, float other) {
-    return row ? load8(row, c, D) : all8(other);
-}
-template <class T>
-__device__ __forceinline__ void store8(T *row, int c, int D, const f8 &x) {
-    typename Raw<T>::type o;
-#pragma unroll
-    for (int k = 0; k < kVec; k++) o[k] = (T)x.v[k];
-    if (c + kVec <= D) {
-        *(typename Raw<T>::type *)(row + c) = o;
-    } else {
-#pragma unroll
-        for (int k = 0; k < kVec; k++)
-            if (c + k < D) row[c + k] = o[k];
-    }
-}
-
-// K sums over the TPR threads of a row, in every one of them. Over several waves through LDS: `turn` alternates between two
-// buffers, so that one barrier a sum is enough.
+// K sums over the TPR threads of a row, in every one of them. Over several waves through LDS, where each lane then reads one wave's sums
+// and groups of lanes add those: `turn` alternates between two buffers, so that one barrier is enough.
 template <int TPR, int K>
 __device__ __forceinline__ void row_sums(float (&s)[K], int &turn) {
 #pragma unroll
-    for (int o = (TPR < 64 ? TPR : 64) / 2; o >= 1; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < K; k++) s[k] += __shfl_xor(s[k], o, 64);
+    for (int k = 0; k < K; k++) s[k] = lanes_sum<TPR < 64 ? TPR : 64>(s[k]);
     if constexpr (TPR > 64) {
-        constexpr int W = TPR / 64;
-        __shared__ float red[2][2][W];
-        static_assert(K <= 2, "two sums at a time");
+        constexpr int W = TPR / 64, KP = K + (K & 1);   // (8-byte accesses)
+        __shared__ __attribute__((aligned(16))) float red[2][W][KP];
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
-            for (int k = 0; k < K; k++) red[turn][k][threadIdx.x >> 6] = s[k];
+            for (int k = 0; k < K; k++) red[turn][threadIdx.x >> 6][k] = s[k];
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            s[k] = red[turn][k][0];
+        for (int k = 0; k < K; k++) s[k] = red[turn][threadIdx.x & (W - 1)][k];
 #pragma unroll
-            for (int w = 1; w < W; w++) s[k] += red[turn][k][w];
-        }
+        for (int k = 0; k < K; k++) s[k] = lanes_sum<W>(s[k]);
         turn ^= 1;
     }
 }
 
-// Mean and inverse deviation of two rows at once (a, b: their eight columns from c on here, for every c).
 struct Stats {
     float m, r;
 };
-// each(f): f(c, a, b) for each of this thread's column groups. One pass for the sums, and one for layer norms' squares about the mean.
-template <int TPR, class Each>
-__device__ __forceinline__ void stats2(int D, int ka, int kb, float eps, Each each, Stats &A, Stats &B, int &turn) {
-    const float n = 1.0f / (float)D;
-    float s[2] = {};
-    if (ka == AH_NORM_LAYER || kb == AH_NORM_LAYER) {
-        each([&](int, const f8 &a, const f8 &b) {
-#pragma unroll
-            for (int k = 0; k < kVec; k++) {
-                s[0] += a.v[k];
-                s[1] += b.v[k];
-            }
-        });
-        row_sums<TPR>(s, turn);
-    }
-    A.m = ka == AH_NORM_LAYER ? s[0] * n : 0.0f;
-    B.m = kb == AH_NORM_LAYER ? s[1] * n : 0.0f;
-    s[0] = s[1] = 0.0f;
-    each([&](int c, const f8 &a, const f8 &b) {
-#pragma unroll
-        for (int k = 0; k < kVec; k++) {
-            const float x = c + k < D ? a.v[k] - A.m : 0.0f, y = c + k < D ? b.v[k] - B.m : 0.0f;
-            s[0] = fmaf(x, x, s[0]);
-            s[1] = fmaf(y, y, s[1]);
-        }
-    });
-    row_sums<TPR>(s, turn);
-    A.r = 1.0f / sqrtf(s[0] * n + eps);
-    B.r = 1.0f / sqrtf(s[1] * n + eps);
-}
+// Mean and inverse deviation of a row. each(f): f(c, a) for each of this thread's column groups. One pass for the sum, and one for layer
+// norms' squares about the mean.
 template <int TPR, class Each>
 __device__ __forceinline__ Stats stats1(int D, int kind, float eps, Each each, int &turn) {
     const float n = 1.0f / (float)D;
@@ -164,96 +105,147 @@ __device__ __forceinline__ Stats stats1(int D, int kind, float eps, Each each, i
     return S;
 }
 
+// x less its mean, zeros past the row's end.
+template <int V, bool LAYER>
+__device__ __forceinline__ fN<V> less(fN<V> x, float m, int c, int D) {
+    if constexpr (LAYER)
+#pragma unroll
+        for (int k = 0; k < V; k++) x.v[k] = c + k < D ? x.v[k] - m : 0.0f;
+    return x;
+}
+template <int V>
+__device__ __forceinline__ fN<V> times(float s, fN<V> a, const fN<V> &b) {   // s a b
+#pragma unroll
+    for (int k = 0; k < V; k++) a.v[k] = s * a.v[k] * b.v[k];
+    return a;
+}
+
 // ── forward ────────────────────────────────────────────────────────────────────
 
-// T: Y, O, gate and weights; R: the residual stream. VPT: column groups that a thread holds; 0: rows are read again for each pass.
-template <class T, class R, int TPR, int VPT>
-__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void resnorm_kernel(ah_residual_norm_desc d) {
-    constexpr int PER = TPR <= 64 ? 256 / TPR : 1, V = VPT ? VPT : 1;
+// T: Y, O, gate and weights; R: the residual stream. Rows of up to 8 TPR columns. Weights are loaded where they are needed, from L2: held from the
+// start they cost half the waves (16384 x 4096: 232 us against 160).
+// G: groups of eight columns that a thread has.
+template <class T, class R, int TPR, int G>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, G == 1 ? 8 : 4) void resnorm_kernel(ah_residual_norm_desc d) {
+    constexpr int PER = TPR <= 64 ? 256 / TPR : 1, V = kVec;
+    constexpr bool NARROW = TPR == 8;   // there may be fewer than eight columns
     const int t = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x, D = d.D;
-    int turn = 0;
-    const T *pw = (const T *)d.post_w, *pb = (const T *)d.post_b, *nw = (const T *)d.pre_w, *nb = (const T *)d.pre_b;
+    int c0 = t * V, turn = 0;
+    const auto col = [&](int g) { return c0 + g * TPR * V; };
+    const auto weights = [&](const void *w, int g, float other) {
+        return w && col(g) < D ? widen<V>(settle<T, V, NARROW>(load_raw<T, V, NARROW>((const T *)w, col(g), D), col(g), D)) : all_of<V>(other);
+    };
+    const auto normed = [&](int kind, f8 (&x)[G], const void *w, const void *b) {
+        const float n = 1.0f / (float)D;
+        float s[1] = {};
+        if (kind == AH_NORM_LAYER) {
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int k = 0; k < V; k++) s[0] += x[g].v[k];
+            row_sums<TPR>(s, turn);
+            const float m = s[0] * n;
+#pragma unroll
+            for (int g = 0; g < G; g++) x[g] = less<V, true>(x[g], m, col(g), D);
+        }
+        s[0] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int k = 0; k < V; k++) s[0] = fmaf(x[g].v[k], x[g].v[k], s[0]);
+        row_sums<TPR>(s, turn);
+        const float r = 1.0f / sqrtf(s[0] * n + d.eps);
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const f8 ww = weights(w, g, 1.0f), bb = weights(b, g, 0.0f);
+#pragma unroll
+            for (int k = 0; k < V; k++) x[g].v[k] = fmaf(x[g].v[k] * r, ww.v[k], bb.v[k]);
+        }
+    };
     for (long r = (long)blockIdx.x * PER + (TPR <= 64 ? threadIdx.x / TPR : 0); r < ((d.N + PER - 1) / PER) * (long)PER; r += (long)gridDim.x * PER) {
+        asm volatile("" : "+v"(c0));   // addresses are formed anew for each row: kept, they cost waves
         const bool on = PER == 1 || r < d.N;   // lanes past the last row keep their wave company
         const long row = on ? r : d.N - 1;
-        const R *H = d.H ? (const R *)d.H + row * d.ldh : nullptr;
-        const T *Y = d.Y ? (const T *)d.Y + row * d.ldy : nullptr;
-        const T *G = d.gate ? (const T *)d.gate + (long)(d.rows_per_gate ? (int)row / d.rows_per_gate : 0) * d.ldgate : nullptr;
-        f8 y[V], h[V];
-        const auto groups = [&](auto f) {   // f(v, c): this thread's column groups
-            if constexpr (VPT == 0) {
-                for (int c = t * kVec; c < D; c += TPR * kVec) f(0, c);
-            } else {
+        typename RawN<T, V>::type ry[G] = {};
+        typename RawN<R, V>::type rh[G] = {};
 #pragma unroll
-                for (int v = 0; v < VPT; v++)
-                    if ((v * TPR + t) * kVec < D) f(v, (v * TPR + t) * kVec);
+        for (int g = 0; g < G; g++) {
+            if (col(g) >= D) continue;
+            if (d.Y) ry[g] = load_raw<T, V, NARROW>((const T *)d.Y + row * d.ldy, col(g), D);
+            if (d.H) rh[g] = load_raw<R, V, NARROW>((const R *)d.H + row * d.ldh, col(g), D);
+        }
+        f8 s[G] = {};
+        if (d.Y) {
+#pragma unroll
+            for (int g = 0; g < G; g++) s[g] = widen<V>(settle<T, V, NARROW>(ry[g], col(g), D));
+            if (d.post != AH_NORM_NONE) normed(d.post, s, d.post_w, d.post_b);
+            const T *gate = d.gate ? (const T *)d.gate + (long)(d.rows_per_gate ? (int)row / d.rows_per_gate : 0) * d.ldgate : nullptr;
+#pragma unroll
+            for (int g = 0; g < G; g++) s[g] = times<V>(d.scale, weights(gate, g, 1.0f), s[g]);
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            if (d.H) {
+                const f8 h = widen<V>(settle<R, V, NARROW>(rh[g], col(g), D));
+#pragma unroll
+                for (int k = 0; k < V; k++) s[g].v[k] = fmaf(d.skip, h.v[k], s[g].v[k]);
             }
-        };
-        if constexpr (VPT > 0)
-            groups([&](int v, int c) {
-                if (Y) y[v] = load8(Y, c, D);
-                if (H) h[v] = load8(H, c, D);
-            });
-        const auto y_at = [&](int v, int c) {
-            if constexpr (VPT == 0) return load8(Y, c, D);
-            else return y[v];
-        };
-        Stats P{0.0f, 1.0f};
-        if (Y && d.post != AH_NORM_NONE)
-            P = stats1<TPR>(D, d.post, d.eps, [&](auto f) { groups([&](int v, int c) { f(c, y_at(v, c)); }); }, turn);
-        const auto sum_at = [&](int v, int c) {
+            if (d.H_out && on && col(g) < D) store8((R *)d.H_out + row * d.ldh_out, col(g), D, s[g]);
+        }
+        if (!d.O) continue;
+        normed(d.pre, s, d.pre_w, d.pre_b);
+#pragma unroll
+        for (int g = 0; g < G; g++)
+            if (on && col(g) < D) store8((T *)d.O + row * d.ldo, col(g), D, s[g]);
+    }
+}
+
+// Rows of any width, a workgroup a row: read again for each pass.
+constexpr int kWideT = 1024;
+template <class T, class R>
+__global__ __launch_bounds__(kWideT) void resnorm_wide_kernel(ah_residual_norm_desc d) {
+    const int D = d.D;
+    int turn = 0;
+    const T *pw = (const T *)d.post_w, *pb = (const T *)d.post_b, *nw = (const T *)d.pre_w, *nb = (const T *)d.pre_b;
+    const auto groups = [&](auto f) {
+        for (int c = threadIdx.x * kVec; c < D; c += kWideT * kVec) f(c);
+    };
+    for (long r = blockIdx.x; r < d.N; r += gridDim.x) {
+        const R *H = d.H ? (const R *)d.H + r * d.ldh : nullptr;
+        const T *Y = d.Y ? (const T *)d.Y + r * d.ldy : nullptr;
+        const T *G = d.gate ? (const T *)d.gate + (long)(d.rows_per_gate ? (int)r / d.rows_per_gate : 0) * d.ldgate : nullptr;
+        Stats P{0.0f, 1.0f}, Q{0.0f, 1.0f};
+        if (d.post != AH_NORM_NONE) P = stats1<kWideT>(D, d.post, d.eps, [&](auto f) { groups([&](int c) { f(c, load8(Y, c, D)); }); }, turn);
+        const auto sum_at = [&](int c) {
             f8 s = {};
             if (Y) {
-                s = y_at(v, c);
+                s = load8(Y, c, D);
                 if (d.post != AH_NORM_NONE) {
-                    const f8 w = load8_or(pw, c, D, 1.0f);
+                    const f8 w = load8_or(pw, c, D, 1.0f), b = load8_or(pb, c, D, 0.0f);
 #pragma unroll
-                    for (int k = 0; k < kVec; k++) s.v[k] = (s.v[k] - P.m) * P.r * w.v[k];
-                    if (d.post == AH_NORM_LAYER && pb) {
-                        const f8 b = load8(pb, c, D);
-#pragma unroll
-                        for (int k = 0; k < kVec; k++) s.v[k] += b.v[k];
-                    }
+                    for (int k = 0; k < kVec; k++) s.v[k] = fmaf((s.v[k] - P.m) * P.r, w.v[k], b.v[k]);
                 }
                 const f8 g = load8_or(G, c, D, 1.0f);
 #pragma unroll
                 for (int k = 0; k < kVec; k++) s.v[k] *= d.scale * g.v[k];
             }
             if (H) {
-                f8 x;
-                if constexpr (VPT == 0) x = load8(H, c, D);
-                else x = h[v];
+                const f8 h = load8(H, c, D);
 #pragma unroll
-                for (int k = 0; k < kVec; k++) s.v[k] = fmaf(d.skip, x.v[k], s.v[k]);
+                for (int k = 0; k < kVec; k++) s.v[k] = fmaf(d.skip, h.v[k], s.v[k]);
             }
             return s;
         };
-        if constexpr (VPT > 0)
-            groups([&](int v, int c) {
-                h[v] = sum_at(v, c);
-                if (d.H_out && on) store8((R *)d.H_out + row * d.ldh_out, c, D, h[v]);
-            });
-        const auto h_at = [&](int v, int c) {
-            if constexpr (VPT == 0) return sum_at(v, c);
-            else return h[v];
-        };
-        Stats Q{0.0f, 1.0f};
-        if (d.O) Q = stats1<TPR>(D, d.pre, d.eps, [&](auto f) { groups([&](int v, int c) { f(c, h_at(v, c)); }); }, turn);
-        if (d.O || VPT == 0)
-            groups([&](int v, int c) {
-                f8 s = h_at(v, c);
-                if (VPT == 0 && d.H_out) store8((R *)d.H_out + row * d.ldh_out, c, D, s);   // after the row's last reading: H_out may be H
-                if (!d.O) return;
-                const f8 w = load8_or(nw, c, D, 1.0f);
+        if (d.O) Q = stats1<kWideT>(D, d.pre, d.eps, [&](auto f) { groups([&](int c) { f(c, sum_at(c)); }); }, turn);
+        groups([&](int c) {
+            f8 s = sum_at(c);
+            if (d.H_out) store8((R *)d.H_out + r * d.ldh_out, c, D, s);   // after the row's last reading: H_out may be H
+            if (!d.O) return;
+            const f8 w = load8_or(nw, c, D, 1.0f), b = load8_or(nb, c, D, 0.0f);
 #pragma unroll
-                for (int k = 0; k < kVec; k++) s.v[k] = (s.v[k] - Q.m) * Q.r * w.v[k];
-                if (d.pre == AH_NORM_LAYER && nb) {
-                    const f8 b = load8(nb, c, D);
-#pragma unroll
-                    for (int k = 0; k < kVec; k++) s.v[k] += b.v[k];
-                }
-                if (on) store8((T *)d.O + row * d.ldo, c, D, s);
-            });
+            for (int k = 0; k < kVec; k++) s.v[k] = fmaf((s.v[k] - Q.m) * Q.r, w.v[k], b.v[k]);
+            store8((T *)d.O + r * d.ldo, c, D, s);
+        });
     }
 }
 
@@ -270,283 +262,245 @@ struct Runs {
     __host__ __device__ int row(int w) const { return (int)((long)w * n / workers); }
 };
 
-// What a row's gradient needs of its statistics.
-struct RowStats {
-    Stats y, h;
-    float q1, qx, p1, px;  // means of q, q xh, p, p yh
+// What a row's gradients need of its sums:
+//   t = dh + c1 q - c2 h - c0,  c1 = r_h,  c2 = r_h^3 mean(q h),  c0 = r_h mean(q)
+//   dY = r_y p - px y - p1,     px = r_y^3 mean(p y),  p1 = r_y mean(p),  p = a t,  a = scale g w_post
+// (y, h less their means my, mh; c0, p1 of layer norms alone). The sums of p come from those of t's terms, so that all are taken at once:
+//   sum p y = sum a y dh + c1 sum a y q - c2 sum a y h - c0 sum a y,  and sum p likewise
+struct RowTerms {
+    float my, mh, ry, c1, c2, c0, px, p1;
 };
-
-struct Slots {   // a thread's sums over rows
-    f8 wpre, bpre, wpost, bpost, gate;
-};
-
-struct RowCols {   // a row's values in a thread's columns
-    f8 y, h, dh, dO, g;
-};
-
-// t from the row's values: the gradient of h.
-__device__ __forceinline__ f8 grad_h(const RowCols &x, const f8 &wn, const RowStats &s, int pre) {
-    f8 t = x.dh;
-    if (pre != AH_NORM_NONE) {
-#pragma unroll
-        for (int k = 0; k < kVec; k++) {
-            const float xh = (x.h.v[k] - s.h.m) * s.h.r, q = x.dO.v[k] * wn.v[k];
-            t.v[k] += s.h.r * (q - s.qx * xh - s.q1);
-        }
-    }
-    return t;
-}
-
-// The columns' sums gain a row. layer: some norm has a bias.
 template <bool LAYER>
-__device__ __forceinline__ void add_row(Slots &a, const RowCols &x, const f8 &t, const f8 &wp, const f8 &bp, const RowStats &s, float scale) {
+constexpr int kSums = LAYER ? 12 : 6;
+template <int V, bool LAYER>
+__device__ __forceinline__ void add_terms(float (&s)[kSums<LAYER>], const fN<V> &y, const fN<V> &h, const fN<V> &q, const fN<V> &dh, const fN<V> &a, int c, int D) {
 #pragma unroll
-    for (int k = 0; k < kVec; k++) {
-        const float xh = (x.h.v[k] - s.h.m) * s.h.r, yh = (x.y.v[k] - s.y.m) * s.y.r, v = scale * t.v[k];
-        a.wpre.v[k] = fmaf(x.dO.v[k], xh, a.wpre.v[k]);
-        a.wpost.v[k] = fmaf(v * x.g.v[k], yh, a.wpost.v[k]);
-        float u = yh * wp.v[k];
+    for (int k = 0; k < V; k++) {
+        const float ay = a.v[k] * y.v[k];
+        s[0] = fmaf(y.v[k], y.v[k], s[0]);
+        s[1] = fmaf(h.v[k], h.v[k], s[1]);
+        s[2] = fmaf(q.v[k], h.v[k], s[2]);
+        s[3] = fmaf(ay, dh.v[k], s[3]);
+        s[4] = fmaf(ay, q.v[k], s[4]);
+        s[5] = fmaf(ay, h.v[k], s[5]);
         if constexpr (LAYER) {
-            a.bpre.v[k] += x.dO.v[k];
-            a.bpost.v[k] = fmaf(v, x.g.v[k], a.bpost.v[k]);
-            u += bp.v[k];
+            s[6] += q.v[k];
+            s[7] = fmaf(a.v[k], dh.v[k], s[7]);
+            s[8] = fmaf(a.v[k], q.v[k], s[8]);
+            s[9] = fmaf(a.v[k], h.v[k], s[9]);
+            s[10] += c + k < D ? a.v[k] : 0.0f;
+            s[11] += ay;
         }
-        a.gate.v[k] = fmaf(v, u, a.gate.v[k]);
     }
 }
+template <bool LAYER>
+__device__ __forceinline__ RowTerms terms_of(const ah_residual_norm_grad_desc &d, const float (&m)[2], const float (&s)[kSums<LAYER>], float n) {
+    const bool pre = d.pre != AH_NORM_NONE, post = d.post != AH_NORM_NONE;
+    RowTerms x{m[0], m[1], 1.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (post) x.ry = 1.0f / sqrtf(s[0] * n + d.eps);
+    if (pre) {
+        x.c1 = 1.0f / sqrtf(s[1] * n + d.eps);
+        x.c2 = x.c1 * x.c1 * (x.c1 * (s[2] * n));
+    }
+    float py = s[3] + x.c1 * s[4] - x.c2 * s[5];
+    if constexpr (LAYER) {
+        if (d.pre == AH_NORM_LAYER) x.c0 = x.c1 * (s[6] * n);
+        py -= x.c0 * s[11];
+        if (d.post == AH_NORM_LAYER) x.p1 = x.ry * n * (s[7] + x.c1 * s[8] - x.c2 * s[9] - x.c0 * s[10]);
+    }
+    if (post) x.px = x.ry * x.ry * x.ry * (n * py);
+    return x;
+}
+template <int V>
+struct Slots {   // a thread's sums over rows
+    fN<V> wpre, bpre, wpost, bpost;
+};
 
 // Gate `index`, whose rows the run [a, b) of worker w has come to the end of: into dgate if they are all in the run, else into one
 // of the worker's two places.
-template <class T>
-__device__ __forceinline__ void put_gate(const ah_residual_norm_grad_desc &d, const Runs &u, int w, int a, int b, long index, int c, const f8 &v) {
+template <class T, int V>
+__device__ __forceinline__ void put_gate(const ah_residual_norm_grad_desc &d, const Runs &u, int w, int a, int b, long index, int c, const fN<V> &v) {
     const long first = index * u.per, end = min(first + (long)u.per, (long)u.n);
-    if (first >= a && end <= b) store8((T *)d.dgate + index * d.lddgate, c, d.D, v);
-    else store8(u.gates + ((long)w * 2 + (first < a ? 0 : 1)) * d.D, c, d.D, v);
+    if (first >= a && end <= b) store_cols<T, V>((T *)d.dgate + index * d.lddgate, c, d.D, v);
+    else store_cols<float, V>(u.gates + ((long)w * 2 + (first < a ? 0 : 1)) * d.D, c, d.D, v);
 }
 
-__device__ __forceinline__ void put_sums(const Runs &u, int w, int c, int D, const Slots &s) {
+template <int V>
+__device__ __forceinline__ void put_sums(const Runs &u, int w, int c, int D, const Slots<V> &s) {
     float *p = u.sums + (long)w * u.arrays * D;
-    if (u.wpre >= 0) store8(p + (long)u.wpre * D, c, D, s.wpre);
-    if (u.bpre >= 0) store8(p + (long)u.bpre * D, c, D, s.bpre);
-    if (u.wpost >= 0) store8(p + (long)u.wpost * D, c, D, s.wpost);
-    if (u.bpost >= 0) store8(p + (long)u.bpost * D, c, D, s.bpost);
+    if (u.wpre >= 0) store_cols<float, V>(p + (long)u.wpre * D, c, D, s.wpre);
+    if (u.bpre >= 0) store_cols<float, V>(p + (long)u.bpre * D, c, D, s.bpre);
+    if (u.wpost >= 0) store_cols<float, V>(p + (long)u.wpost * D, c, D, s.wpost);
+    if (u.bpost >= 0) store_cols<float, V>(p + (long)u.bpost * D, c, D, s.bpost);
 }
 
-// Rows of up to 8 TPR columns, TPR threads a worker. AHEAD: the next row's loads go out before this row's work (its values as they lie, 20
-// or 40 registers).
-template <class T, class R, int TPR, bool LAYER, bool AHEAD>
-__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void resnorm_grad_kernel(ah_residual_norm_grad_desc d, Runs u) {
+// Rows of up to V TPR columns, TPR threads a worker. The next row's loads go out before this row's work; a row costs its threads one barrier (two
+// with layer norms, which need the means first). GIVEN: rows of any width whose terms are known, V TPR columns a workgroup. The gradients of the
+// gate and the second norm's weights share sums over a gate's rows: sum t yh and sum t. LAYER: some norm has a mean and a bias.
+template <class T, class R, int TPR, int V, bool LAYER, bool GIVEN>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR <= 64 ? 3 : 4) void resnorm_grad_kernel(ah_residual_norm_grad_desc d, Runs u, const RowTerms *rows) {
     constexpr int PER = TPR <= 64 ? 256 / TPR : 1;
-    const int t = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x, D = d.D, c = t * kVec;
+    const int t = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x, D = d.D;
+    int c = (GIVEN ? (int)blockIdx.y * TPR + t : t) * V;
     const int w = blockIdx.x * PER + (TPR <= 64 ? threadIdx.x / TPR : 0);
-    if (PER > 1 && w >= u.workers) return;   // whole groups of lanes; shuffles stay within a group
+    if (PER > 1 && w >= u.workers) return;   // whole groups of lanes; sums stay within a group
     const int a = u.row(w), b = u.row(w + 1);
-    const bool in = c < D, ln_pre = d.pre == AH_NORM_LAYER, ln_post = d.post == AH_NORM_LAYER;
-    const bool rd_y = in && d.Y, rd_h = in && d.H_out, rd_dh = in && d.dH_out, rd_dO = in && d.dO, rd_g = in && d.gate;
+    const bool in = c < D, pre = d.pre != AH_NORM_NONE, post = d.post != AH_NORM_NONE;
+    const bool rd_y = in && d.Y, rd_h = in && pre, rd_dh = in && d.dH_out, rd_g = in && d.gate;
+    constexpr bool NARROW = TPR == 8;   // there may be fewer than V columns
     int turn = 0;
-    typedef typename Raw<T>::type rawT;
-    typedef typename Raw<R>::type rawR;
+    typedef typename RawN<T, V>::type rawT;
+    typedef typename RawN<R, V>::type rawR;
     struct Line {
-        rawT y, dO, g;
+        rawT y, dO;
         rawR h, dh;
     };
-    const auto fetch = [&](int r, long gate) {
+    const auto fetch = [&](int r) {
         Line l = {};
-        if (rd_y) l.y = load_raw((const T *)d.Y + (long)r * d.ldy, c, D);
-        if (rd_dO) l.dO = load_raw((const T *)d.dO + (long)r * d.lddo, c, D);
-        if (rd_h) l.h = load_raw((const R *)d.H_out + (long)r * d.ldh_out, c, D);
-        if (rd_dh) l.dh = load_raw((const R *)d.dH_out + (long)r * d.lddh_out, c, D);
-        if (rd_g) l.g = load_raw((const T *)d.gate + gate * d.ldgate, c, D);
+        if (rd_y) l.y = load_raw<T, V, NARROW>((const T *)d.Y + (long)r * d.ldy, c, D);
+        if (rd_dh) l.dh = load_raw<R, V, NARROW>((const R *)d.dH_out + (long)r * d.lddh_out, c, D);
+        if (rd_h) {
+            l.h = load_raw<R, V, NARROW>((const R *)d.H_out + (long)r * d.ldh_out, c, D);
+            l.dO = load_raw<T, V, NARROW>((const T *)d.dO + (long)r * d.lddo, c, D);
+        }
         return l;
     };
-    f8 wn = all8(1.0f), wp = all8(1.0f), bp = all8(0.0f);
-    if (in) {
-        if (d.pre_w) wn = load8((const T *)d.pre_w, c, D);
-        if (d.post_w) wp = load8((const T *)d.post_w, c, D);
-        if (LAYER && ln_post && d.post_b) bp = load8((const T *)d.post_b, c, D);
-    }
-    Slots sums = {};
+    rawT rg = {}, rwn = {}, rwp = {}, rbp = {};   // gate and weights as they lie: half the registers in f16
+    const auto fetch_gate = [&](long gate) {
+        if (rd_g) rg = settle<T, V, NARROW>(load_raw<T, V, NARROW>((const T *)d.gate + gate * d.ldgate, c, D), c, D);
+    };
+    if (in && d.pre_w) rwn = settle<T, V, NARROW>(load_raw<T, V, NARROW>((const T *)d.pre_w, c, D), c, D);
+    if (in && d.post_w) rwp = settle<T, V, NARROW>(load_raw<T, V, NARROW>((const T *)d.post_w, c, D), c, D);
+    if (in && LAYER && d.post_b) rbp = settle<T, V, NARROW>(load_raw<T, V, NARROW>((const T *)d.post_b, c, D), c, D);
+    const auto or_one = [&](bool there, rawT x) { return there ? widen<V>(x) : all_of<V>(1.0f); };
+    Slots<V> sums = {};
+    fN<V> ty = {}, ts = {};   // of a gate's rows: sum t yh, sum t
     long gate = a / u.per;
     int left = (int)min((long)u.per - a % u.per, (long)0x7fffffff);   // rows to the gate's end
     Line next = {};
-    if (AHEAD && a < b) next = fetch(a, gate);
+    if (a < b) {
+        next = fetch(a);
+        fetch_gate(gate);
+    }
     const float n = 1.0f / (float)D;
     for (int r = a; r < b; r++) {
-        Line l;
-        const long gate_next = left == 1 ? gate + 1 : gate;
-        if constexpr (AHEAD) {
-            l = next;
-            if (r + 1 < b) next = fetch(r + 1, gate_next);
+        asm volatile("" : "+v"(c));   // addresses are formed anew for each row: kept, they spill
+        Line l = next;
+        if (r + 1 < b) next = fetch(r + 1);
+        l.y = settle<T, V, NARROW>(l.y, c, D);
+        l.h = settle<R, V, NARROW>(l.h, c, D);
+        l.dO = settle<T, V, NARROW>(l.dO, c, D);
+        l.dh = settle<R, V, NARROW>(l.dh, c, D);
+        const auto gain = [&] { return times<V>(d.scale, or_one(d.gate, rg), or_one(d.post_w, rwp)); };
+        const auto grad = [&] { return times<V>(1.0f, widen<V>(l.dO), or_one(d.pre_w, rwn)); };
+        if constexpr (LAYER) {
+            const fN<V> q = widen<V>(l.dO);
+#pragma unroll
+            for (int k = 0; k < V; k++) sums.bpre.v[k] += q.v[k];
+        }
+        RowTerms x;
+        if constexpr (GIVEN) {
+            x = rows[r];
         } else {
-            l = fetch(r, gate);
-        }
-        RowCols x{widen(l.y), widen(l.h), widen(l.dh), widen(l.dO), rd_g ? widen(l.g) : all8(1.0f)};
-        RowStats s{{0.0f, 1.0f}, {0.0f, 1.0f}, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (d.pre != AH_NORM_NONE || d.post != AH_NORM_NONE) {
-            stats2<TPR>(D, d.post, d.pre, d.eps, [&](auto f) { f(c, x.y, x.h); }, s.y, s.h, turn);
-            if (d.post == AH_NORM_NONE) s.y = {0.0f, 1.0f};
-            if (d.pre == AH_NORM_NONE) s.h = {0.0f, 1.0f};
-        }
-        if (d.pre != AH_NORM_NONE) {
-            float m[2] = {};
+            float m[2] = {}, s[kSums<LAYER>] = {};
+            if constexpr (LAYER) {
+                const fN<V> y = widen<V>(l.y), h = widen<V>(l.h);
 #pragma unroll
-            for (int k = 0; k < kVec; k++) {   // dO is 0 past the last column
-                const float q = x.dO.v[k] * wn.v[k];
-                m[0] = fmaf(q, (x.h.v[k] - s.h.m) * s.h.r, m[0]);
-                m[1] += q;
-            }
-            row_sums<TPR>(m, turn);
-            s.qx = m[0] * n;
-            s.q1 = ln_pre ? m[1] * n : 0.0f;
-        }
-        const f8 tt = grad_h(x, wn, s, d.pre);
-        if (d.dH && in) {
-            f8 o;
-#pragma unroll
-            for (int k = 0; k < kVec; k++) o.v[k] = d.skip * tt.v[k];
-            store8((R *)d.dH + (long)r * d.lddh, c, D, o);
-        }
-        if (d.dY) {
-            f8 p;
-#pragma unroll
-            for (int k = 0; k < kVec; k++) p.v[k] = d.scale * x.g.v[k] * tt.v[k];
-            if (d.post != AH_NORM_NONE) {
-                float m[2] = {};
-#pragma unroll
-                for (int k = 0; k < kVec; k++) {
-                    p.v[k] = c + k < D ? p.v[k] * wp.v[k] : 0.0f;
-                    m[0] = fmaf(p.v[k], (x.y.v[k] - s.y.m) * s.y.r, m[0]);
-                    m[1] += p.v[k];
+                for (int k = 0; k < V; k++) {
+                    m[0] += y.v[k];
+                    m[1] += h.v[k];
                 }
                 row_sums<TPR>(m, turn);
-                s.px = m[0] * n;
-                s.p1 = ln_post ? m[1] * n : 0.0f;
-#pragma unroll
-                for (int k = 0; k < kVec; k++) p.v[k] = s.y.r * (p.v[k] - s.px * ((x.y.v[k] - s.y.m) * s.y.r) - s.p1);
+                m[0] = d.post == AH_NORM_LAYER ? m[0] * n : 0.0f;
+                m[1] = d.pre == AH_NORM_LAYER ? m[1] * n : 0.0f;
             }
-            if (in) store8((T *)d.dY + (long)r * d.lddy, c, D, p);
+            if (pre || post) {
+                add_terms<V, LAYER>(s, less<V, LAYER>(widen<V>(l.y), m[0], c, D), less<V, LAYER>(widen<V>(l.h), m[1], c, D), grad(), widen<V>(l.dh), gain(), c, D);
+                row_sums<TPR>(s, turn);
+            }
+            x = terms_of<LAYER>(d, m, s, n);
         }
-        add_row<LAYER>(sums, x, tt, wp, bp, s, d.scale);
+        // the row as it lies is widened again, rather than kept
+        asm volatile("" : "+v"(l.y), "+v"(l.h), "+v"(l.dO), "+v"(l.dh));
+        const fN<V> y = less<V, LAYER>(widen<V>(l.y), x.my, c, D);
+        fN<V> tt, o;
+        {
+            const fN<V> h = less<V, LAYER>(widen<V>(l.h), x.mh, c, D), dO = widen<V>(l.dO), q = grad(), dh = widen<V>(l.dh);
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                tt.v[k] = dh.v[k];
+                if (pre) tt.v[k] += fmaf(-x.c2, h.v[k], x.c1 * q.v[k]) - x.c0;
+                sums.wpre.v[k] = fmaf(dO.v[k], x.c1 * h.v[k], sums.wpre.v[k]);
+                ty.v[k] = fmaf(tt.v[k], x.ry * y.v[k], ty.v[k]);
+                if constexpr (LAYER) ts.v[k] += tt.v[k];
+            }
+        }
+        if (d.dH && in) {
+#pragma unroll
+            for (int k = 0; k < V; k++) o.v[k] = d.skip * tt.v[k];
+            store_cols<R, V>((R *)d.dH + (long)r * d.lddh, c, D, o);
+        }
+        if (d.dY && in) {
+            const fN<V> gw = gain();
+#pragma unroll
+            for (int k = 0; k < V; k++) o.v[k] = fmaf(-x.px, y.v[k], x.ry * (gw.v[k] * tt.v[k])) - x.p1;
+            store_cols<T, V>((T *)d.dY + (long)r * d.lddy, c, D, o);
+        }
         if (--left == 0 || r + 1 == b) {
-            if (d.dgate && in) put_gate<T>(d, u, w, a, b, gate, c, sums.gate);
-            sums.gate = all8(0.0f);
-            gate = gate_next;
+            const fN<V> g = or_one(d.gate, rg), wp = or_one(d.post_w, rwp), bp = widen<V>(rbp);
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                sums.wpost.v[k] = fmaf(d.scale * g.v[k], ty.v[k], sums.wpost.v[k]);
+                if constexpr (LAYER) sums.bpost.v[k] = fmaf(d.scale * g.v[k], ts.v[k], sums.bpost.v[k]);
+                o.v[k] = d.scale * fmaf(wp.v[k], ty.v[k], LAYER ? bp.v[k] * ts.v[k] : 0.0f);
+            }
+            if (d.dgate && in) put_gate<T, V>(d, u, w, a, b, gate, c, o);
+            ty = ts = all_of<V>(0.0f);
+            gate++;
             left = u.per;
+            if (r + 1 < b) fetch_gate(gate);
         }
     }
     if (u.arrays && in) put_sums(u, w, c, D, sums);
 }
 
-// Rows of any width, a workgroup a row: dH and dY by several readings of the row, and its statistics for the columns' sums.
-constexpr int kWideT = 1024;
-template <class T, class R>
-__global__ __launch_bounds__(kWideT) void resnorm_grad_wide_kernel(ah_residual_norm_grad_desc d, RowStats *rows) {
+// The terms of rows of any width, a workgroup a row; layer norms read it again, from caches.
+template <class T, class R, bool LAYER>
+__global__ __launch_bounds__(kTermsT) void resnorm_grad_terms_kernel(ah_residual_norm_grad_desc d, RowTerms *rows) {
     const int D = d.D;
     const float n = 1.0f / (float)D;
-    const T *wn = (const T *)d.pre_w, *wp = (const T *)d.post_w;
+    const bool pre = d.pre != AH_NORM_NONE, post = d.post != AH_NORM_NONE;
     int turn = 0;
-    const auto groups = [&](auto f) {
-        for (int c = threadIdx.x * kVec; c < D; c += kWideT * kVec) f(c);
-    };
     for (long r = blockIdx.x; r < d.N; r += gridDim.x) {
-        const T *Y = d.Y ? (const T *)d.Y + r * d.ldy : nullptr, *dO = d.dO ? (const T *)d.dO + r * d.lddo : nullptr;
-        const T *G = d.gate ? (const T *)d.gate + (long)(d.rows_per_gate ? (int)r / d.rows_per_gate : 0) * d.ldgate : nullptr;
-        const R *H = d.H_out ? (const R *)d.H_out + r * d.ldh_out : nullptr, *dh = d.dH_out ? (const R *)d.dH_out + r * d.lddh_out : nullptr;
-        RowStats s{{0.0f, 1.0f}, {0.0f, 1.0f}, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (d.post != AH_NORM_NONE) s.y = stats1<kWideT>(D, d.post, d.eps, [&](auto f) { groups([&](int c) { f(c, load8(Y, c, D)); }); }, turn);
-        if (d.pre != AH_NORM_NONE) {
-            s.h = stats1<kWideT>(D, d.pre, d.eps, [&](auto f) { groups([&](int c) { f(c, load8(H, c, D)); }); }, turn);
-            float m[2] = {};
-            groups([&](int c) {
-                const f8 h = load8(H, c, D), g = load8(dO, c, D), w = load8_or(wn, c, D, 1.0f);
+        const T *Y = d.Y ? (const T *)d.Y + r * d.ldy : nullptr, *G = d.gate ? (const T *)d.gate + (long)(d.rows_per_gate ? (int)r / d.rows_per_gate : 0) * d.ldgate : nullptr;
+        const T *dO = pre ? (const T *)d.dO + r * d.lddo : nullptr;
+        const R *H = pre ? (const R *)d.H_out + r * d.ldh_out : nullptr, *dh = d.dH_out ? (const R *)d.dH_out + r * d.lddh_out : nullptr;
+        float m[2] = {}, s[kSums<LAYER>] = {};
+        if constexpr (LAYER) {
+            for (int c = threadIdx.x * kVec; c < D; c += kTermsT * kVec) {
+                const f8 y = load8_or(Y, c, D, 0.0f), h = load8_or(H, c, D, 0.0f);
 #pragma unroll
                 for (int k = 0; k < kVec; k++) {
-                    const float q = g.v[k] * w.v[k];
-                    m[0] = fmaf(q, (h.v[k] - s.h.m) * s.h.r, m[0]);
-                    m[1] += q;
+                    m[0] += y.v[k];
+                    m[1] += h.v[k];
                 }
-            });
-            row_sums<kWideT>(m, turn);
-            s.qx = m[0] * n;
-            s.q1 = d.pre == AH_NORM_LAYER ? m[1] * n : 0.0f;
-        }
-        const auto t_at = [&](int c) {
-            RowCols x{};
-            if (H) x.h = load8(H, c, D);
-            if (dO) x.dO = load8(dO, c, D);
-            if (dh) x.dh = load8(dh, c, D);
-            return grad_h(x, load8_or(wn, c, D, 1.0f), s, d.pre);
-        };
-        const auto p_at = [&](int c) {
-            f8 t = t_at(c);
-            const f8 g = load8_or(G, c, D, 1.0f), w = d.post != AH_NORM_NONE ? load8_or(wp, c, D, 1.0f) : all8(1.0f);
-#pragma unroll
-            for (int k = 0; k < kVec; k++) t.v[k] = c + k < D ? d.scale * g.v[k] * t.v[k] * w.v[k] : 0.0f;
-            return t;
-        };
-        if (d.dY && d.post != AH_NORM_NONE) {
-            float m[2] = {};
-            groups([&](int c) {
-                const f8 p = p_at(c), y = load8(Y, c, D);
-#pragma unroll
-                for (int k = 0; k < kVec; k++) {
-                    m[0] = fmaf(p.v[k], (y.v[k] - s.y.m) * s.y.r, m[0]);
-                    m[1] += p.v[k];
-                }
-            });
-            row_sums<kWideT>(m, turn);
-            s.px = m[0] * n;
-            s.p1 = d.post == AH_NORM_LAYER ? m[1] * n : 0.0f;
-        }
-        groups([&](int c) {
-            if (d.dY) {
-                f8 p = p_at(c);
-                if (d.post != AH_NORM_NONE) {
-                    const f8 y = load8(Y, c, D);
-#pragma unroll
-                    for (int k = 0; k < kVec; k++) p.v[k] = s.y.r * (p.v[k] - s.px * ((y.v[k] - s.y.m) * s.y.r) - s.p1);
-                }
-                store8((T *)d.dY + r * d.lddy, c, D, p);
             }
-        });
-        if (rows && threadIdx.x == 0) rows[r] = s;
-    }
-}
-// The columns' sums, and dH last of all: it may be dH_out, which the rows' gradients are read from. A workgroup has 2048 columns.
-template <class T, class R>
-__global__ __launch_bounds__(256) void resnorm_grad_columns_kernel(ah_residual_norm_grad_desc d, Runs u, const RowStats *rows) {
-    const int D = d.D, c = (blockIdx.x * 256 + threadIdx.x) * kVec, w = blockIdx.y;
-    if (c >= D) return;
-    const int a = u.row(w), b = u.row(w + 1);
-    const f8 wn = load8_or((const T *)d.pre_w, c, D, 1.0f), wp = load8_or((const T *)d.post_w, c, D, 1.0f);
-    const f8 bp = load8_or(d.post == AH_NORM_LAYER ? (const T *)d.post_b : nullptr, c, D, 0.0f);
-    Slots sums = {};
-    long gate = a / u.per;
-    int left = u.per - a % u.per;
-    for (int r = a; r < b; r++) {
-        RowCols x{};
-        if (d.Y) x.y = load8((const T *)d.Y + (long)r * d.ldy, c, D);
-        if (d.H_out) x.h = load8((const R *)d.H_out + (long)r * d.ldh_out, c, D);
-        if (d.dH_out) x.dh = load8((const R *)d.dH_out + (long)r * d.lddh_out, c, D);
-        if (d.dO) x.dO = load8((const T *)d.dO + (long)r * d.lddo, c, D);
-        x.g = load8_or(d.gate ? (const T *)d.gate + gate * d.ldgate : nullptr, c, D, 1.0f);
-        const RowStats s = rows[r];
-        const f8 t = grad_h(x, wn, s, d.pre);
-        if (d.dH) {
-            f8 o;
-#pragma unroll
-            for (int k = 0; k < kVec; k++) o.v[k] = d.skip * t.v[k];
-            store8((R *)d.dH + (long)r * d.lddh, c, D, o);
+            row_sums<kTermsT>(m, turn);
+            m[0] = d.post == AH_NORM_LAYER ? m[0] * n : 0.0f;
+            m[1] = d.pre == AH_NORM_LAYER ? m[1] * n : 0.0f;
         }
-        add_row<true>(sums, x, t, wp, bp, s, d.scale);
-        if (--left == 0 || r + 1 == b) {
-            if (d.dgate) put_gate<T>(d, u, w, a, b, gate, c, sums.gate);
-            sums.gate = all8(0.0f);
-            gate++;
-            left = u.per;
+        if (pre || post) {
+            for (int c = threadIdx.x * kVec; c < D; c += kTermsT * kVec) {
+                const f8 y = load8_or(Y, c, D, 0.0f), h = load8_or(H, c, D, 0.0f), q = load8_or(dO, c, D, 0.0f), g = load8_or(dh, c, D, 0.0f);
+                const f8 a = times<kVec>(d.scale, load8_or(G, c, D, 1.0f), load8_or((const T *)d.post_w, c, D, 1.0f));
+                add_terms<kVec, LAYER>(s, less<kVec, LAYER>(y, m[0], c, D), less<kVec, LAYER>(h, m[1], c, D), times<kVec>(1.0f, q, load8_or((const T *)d.pre_w, c, D, 1.0f)),
+                                       g, a, c, D);
+            }
+            row_sums<kTermsT>(s, turn);
         }
+        const RowTerms x = terms_of<LAYER>(d, m, s, n);
+        if (threadIdx.x == 0) rows[r] = x;
     }
-    if (u.arrays) put_sums(u, w, c, D, sums);
 }
 
 // The workers' sums added in order: 64 columns a workgroup, 16 threads a column with neighbouring workers each. blockIdx.y: an array, or past
@@ -601,18 +555,19 @@ __global__ __launch_bounds__(1024) void resnorm_join_kernel(ah_residual_norm_gra
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Threads a row: the power of two that holds it in groups of eight columns.
-int threads_of(int D) {
+// Threads a row: the power of two that holds it in groups of `cols` columns.
+int threads_of(int D, int cols) {
     int t = 8;
-    while (t < 1024 && t * kVec < D) t *= 2;
+    while (t < 1024 && t * cols < D) t *= 2;
     return t;
 }
+bool has_layer(const ah_residual_norm_grad_desc &d) { return d.pre == AH_NORM_LAYER || d.post == AH_NORM_LAYER; }
 
 template <class T, class R>
 void launch_forward(const ah_residual_norm_desc &d, hipStream_t s) {
-    const int tpr = threads_of(d.D), per = tpr <= 64 ? 256 / tpr : 1;
+    const int tpr = threads_of(d.D, kVec), per = tpr <= 64 ? 256 / tpr : 1;
     const dim3 grid((unsigned)std::min<int64_t>(ceil_div(d.N, per), 16384)), block(tpr <= 64 ? 256 : tpr);
-    switch (d.D > kWide ? 0 : tpr) {
+    switch (d.D > 2 * kWide ? 0 : d.D > kWide ? 2048 : tpr) {
         case 8: hipLaunchKernelGGL((resnorm_kernel<T, R, 8, 1>), grid, block, 0, s, d); break;
         case 16: hipLaunchKernelGGL((resnorm_kernel<T, R, 16, 1>), grid, block, 0, s, d); break;
         case 32: hipLaunchKernelGGL((resnorm_kernel<T, R, 32, 1>), grid, block, 0, s, d); break;
@@ -621,20 +576,24 @@ void launch_forward(const ah_residual_norm_desc &d, hipStream_t s) {
         case 256: hipLaunchKernelGGL((resnorm_kernel<T, R, 256, 1>), grid, block, 0, s, d); break;
         case 512: hipLaunchKernelGGL((resnorm_kernel<T, R, 512, 1>), grid, block, 0, s, d); break;
         case 1024: hipLaunchKernelGGL((resnorm_kernel<T, R, 1024, 1>), grid, block, 0, s, d); break;
-        default: hipLaunchKernelGGL((resnorm_kernel<T, R, 1024, 0>), grid, block, 0, s, d);
+        case 2048: hipLaunchKernelGGL((resnorm_kernel<T, R, 1024, 2>), grid, block, 0, s, d); break;
+        default: hipLaunchKernelGGL((resnorm_wide_kernel<T, R>), grid, block, 0, s, d);
     }
 }
 
 struct Plan {
-    int tpr;             // 0: wide rows
+    int tpr;             // threads of a row (0: wide rows)
     Runs u;
     int gates, by_bound; // gates that workers may share, and how the join finds them
-    int64_t rows, total; // of the workspace: the wide rows' statistics
+    int64_t rows, total; // of the workspace: the wide rows' terms
 };
 
 Plan plan_of(const ah_residual_norm_grad_desc &d) {
     Plan p{};
-    p.tpr = d.D > kWide ? 0 : threads_of(d.D);
+    // Eight columns a thread where its registers hold them and the next row's; four for f32 streams and for layer norms' sums. Rows past
+    // 1024 threads' columns take two launches (4000 x 12000 f16: 410 us by readings of whole rows, see below for both).
+    const int cols = d.res_dtype == AH_F32 || has_layer(d) ? 4 : kVec;
+    p.tpr = d.D > 1024 * cols ? 0 : threads_of(d.D, cols);
     Runs &u = p.u;
     u.n = d.N;
     u.per = d.rows_per_gate && d.rows_per_gate < d.N ? d.rows_per_gate : d.N;
@@ -644,7 +603,7 @@ Plan plan_of(const ah_residual_norm_grad_desc &d) {
     if (d.dpost_w) u.wpost = u.arrays++;
     if (d.dpost_b) u.bpost = u.arrays++;
     // Workers: enough to fill the chip, with at least four rows each where there are many (a worker's sums cross memory twice).
-    const int cap = p.tpr == 0 ? 256 : p.tpr <= 64 ? 512 * (256 / p.tpr) : p.tpr == 128 ? 1024 : p.tpr == 256 ? 512 : 256;
+    const int cap = p.tpr == 0 ? 256 : p.tpr <= 64 ? 512 * (256 / p.tpr) : p.tpr == 1024 ? 256 : (1 << 18) / p.tpr;
     u.workers = std::max(1, std::min(cap, std::max(std::min(d.N, 256), d.N / 4)));
     u.workers = std::min(u.workers, d.N);
     int64_t at = 0;
@@ -661,17 +620,30 @@ Plan plan_of(const ah_residual_norm_grad_desc &d) {
         p.by_bound = gates > u.workers - 1;
         p.gates = std::min(gates, u.workers - 1);
     }
-    p.rows = take(p.tpr == 0 ? (int64_t)d.N * sizeof(RowStats) : 0);
+    p.rows = take(p.tpr == 0 ? (int64_t)d.N * sizeof(RowTerms) : 0);
     p.total = std::max<int64_t>(at, 16);
     return p;
 }
 
-template <class T, class R, int TPR>
-void launch_grad_rows(const ah_residual_norm_grad_desc &d, const Plan &p, hipStream_t s) {
-    const dim3 grid((unsigned)ceil_div(p.u.workers, TPR <= 64 ? 256 / TPR : 1)), block(TPR <= 64 ? 256 : TPR);
-    constexpr bool AHEAD = TPR <= 512;
-    if (d.pre == AH_NORM_LAYER || d.post == AH_NORM_LAYER) hipLaunchKernelGGL((resnorm_grad_kernel<T, R, TPR, true, AHEAD>), grid, block, 0, s, d, p.u);
-    else hipLaunchKernelGGL((resnorm_grad_kernel<T, R, TPR, false, AHEAD>), grid, block, 0, s, d, p.u);
+template <class T, class R, int V, bool LAYER>
+void launch_grad_rows(const ah_residual_norm_grad_desc &d, const Plan &p, RowTerms *rows, hipStream_t s) {
+    const auto go = [&](auto tpr) {
+        constexpr int TPR = tpr;
+        const dim3 grid((unsigned)ceil_div(p.u.workers, TPR <= 64 ? 256 / TPR : 1)), block(TPR <= 64 ? 256 : TPR);
+        hipLaunchKernelGGL((resnorm_grad_kernel<T, R, TPR, V, LAYER, false>), grid, block, 0, s, d, p.u, rows);
+    };
+    switch (p.tpr) {
+        case 8: return go(std::integral_constant<int, 8>());
+        case 16: return go(std::integral_constant<int, 16>());
+        case 32: return go(std::integral_constant<int, 32>());
+        case 64: return go(std::integral_constant<int, 64>());
+        case 128: return go(std::integral_constant<int, 128>());
+        case 256: return go(std::integral_constant<int, 256>());
+        case 512: return go(std::integral_constant<int, 512>());
+        case 1024: return go(std::integral_constant<int, 1024>());
+    }
+    hipLaunchKernelGGL((resnorm_grad_terms_kernel<T, R, LAYER>), dim3((unsigned)std::min(d.N, 16384)), dim3(kTermsT), 0, s, d, rows);
+    hipLaunchKernelGGL((resnorm_grad_kernel<T, R, 256, V, LAYER, true>), dim3((unsigned)p.u.workers, (unsigned)ceil_div(d.D, 256 * V)), dim3(256), 0, s, d, p.u, rows);
 }
 
 template <class T, class R>
@@ -679,21 +651,9 @@ void launch_grad(const ah_residual_norm_grad_desc &d, Plan p, hipStream_t s) {
     char *ws = (char *)d.ws;
     p.u.sums = (float *)(ws + (uintptr_t)p.u.sums);
     p.u.gates = (float *)(ws + (uintptr_t)p.u.gates);
-    switch (p.tpr) {
-        case 8: launch_grad_rows<T, R, 8>(d, p, s); break;
-        case 16: launch_grad_rows<T, R, 16>(d, p, s); break;
-        case 32: launch_grad_rows<T, R, 32>(d, p, s); break;
-        case 64: launch_grad_rows<T, R, 64>(d, p, s); break;
-        case 128: launch_grad_rows<T, R, 128>(d, p, s); break;
-        case 256: launch_grad_rows<T, R, 256>(d, p, s); break;
-        case 512: launch_grad_rows<T, R, 512>(d, p, s); break;
-        case 1024: launch_grad_rows<T, R, 1024>(d, p, s); break;
-        default: {
-            RowStats *rows = (RowStats *)(ws + p.rows);
-            hipLaunchKernelGGL((resnorm_grad_wide_kernel<T, R>), dim3((unsigned)std::min(d.N, 16384)), dim3(kWideT), 0, s, d, rows);
-            hipLaunchKernelGGL((resnorm_grad_columns_kernel<T, R>), dim3((unsigned)ceil_div(d.D, 256 * kVec), (unsigned)p.u.workers), dim3(256), 0, s, d, p.u, rows);
-        }
-    }
+    RowTerms *rows = (RowTerms *)(ws + p.rows);
+    if (has_layer(d)) launch_grad_rows<T, R, 4, true>(d, p, rows, s);
+    else launch_grad_rows<T, R, sizeof(R) == 2 ? 8 : 4, false>(d, p, rows, s);
     if (p.u.arrays + p.gates)
         hipLaunchKernelGGL(resnorm_join_kernel<T>, dim3((unsigned)ceil_div(d.D, 64), (unsigned)(p.u.arrays + p.gates)), dim3(1024), 0, s, d, p.u, p.gates, p.by_bound);
 }

@@ -6,7 +6,7 @@
 // of a stage's 64), others packed into panels. f32 operands are packed as two f16 planes, each row scaled by a power of two of its own
 // that brings its largest magnitude to 2^15: the row's exponent leaves the product in the epilogue, so nothing but the row itself has
 // to be read before it is packed, and a row keeps 22 bits whatever the others hold. Few rows: linear_ce_few.h, which reads W once, as it
-// lies (f32 on the f32 matrix instruction, all 24 bits).
+// lies (f32 on the f32 matrix instruction, all 24 bits), or K over the waves of small workgroups where one launch is worth more.
 //
 // The epilogue takes Z from the accumulators in f32 through LDS (tile_out.h), eight columns of a row to a lane, so that U, R, Z and Y are
 // read and written in 16 bytes; the loads of 16 rows are in flight together. Bound by the matrix cores for many rows, by W's bytes for few.
@@ -163,6 +163,84 @@ __global__ __launch_bounds__(256) void linear_few_join_kernel(ProductArgs a) {
     });
 }
 
+// ── few rows, K split over a workgroup's waves ─────────────────────────────────
+
+// 16 columns a workgroup: its waves read their rows of W in turns of 128 bytes (two chunks of 64), each with the rows of X that go with
+// them, and add their sums in LDS, in order. W goes from memory to registers once, all of its workgroups are at work from the start, and nothing
+// has to be joined by another launch. Where a lane's 16 bytes end past D (D >= 8), it reads the row's last 16 and those that were there before
+// are zeros.
+struct RowArgs {
+    FewArgs f;
+    Layer l;
+};
+template <int FA, class T>
+__global__ __launch_bounds__(1024) void linear_rows_kernel(RowArgs a) {
+    constexpr bool F16 = sizeof(T) == 2;
+    constexpr int E = 16 / sizeof(T), K = 4 * E, U = F16 && FA == 1 ? 8 : 4;   // k of a lane's load, of a chunk; chunks in flight
+    typedef T vec __attribute__((ext_vector_type(E)));
+    typedef T vec_any __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+    __shared__ floatx4 red[16][FA][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, row = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, D = a.f.D, nc = (D + K - 1) / K;
+    const T *w = (const T *)a.f.W + (long)min(n0 + row, a.l.F - 1) * a.f.ldw, *x[FA];
+#pragma unroll
+    for (int i = 0; i < FA; i++) x[i] = (const T *)a.f.X + (long)min(16 * i + row, a.l.N - 1) * a.f.ldx;
+    floatx4 acc[FA];
+#pragma unroll
+    for (int i = 0; i < FA; i++) acc[i] = (floatx4){};
+    const auto chunk = [&](int c) { return (c >> 1) * 2 * waves + 2 * wave + (c & 1); };   // this wave's c-th
+    for (int c0 = 0; chunk(c0) < nc; c0 += U) {
+        vec wv[U], xv[U][FA];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = min(chunk(c0 + u) * K + g * E, D - E);
+            wv[u] = *(const vec_any *)(w + at);
+#pragma unroll
+            for (int i = 0; i < FA; i++) xv[u][i] = *(const vec_any *)(x[i] + at);
+        }
+        if (chunk(c0 + U - 1) * K + K > D)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k = chunk(c0 + u) * K + g * E, at = min(k, D - E);
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const bool again = at + e < k;
+                    wv[u][e] = again ? (T)0 : wv[u][e];
+#pragma unroll
+                    for (int i = 0; i < FA; i++) xv[u][i][e] = again ? (T)0 : xv[u][i][e];
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < FA; i++) {
+                if constexpr (F16) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv[u], xv[u][i], acc[i], 0, 0, 0);
+                else
+#pragma unroll
+                    for (int e = 0; e < E; e++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[u][e], xv[u][i][e], acc[i], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < FA; i++) red[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int i = wave; i < FA; i += waves) {   // a wave 16 rows: a lane one of them and four columns
+        floatx4 z = red[0][i][lane];
+        for (int v = 1; v < waves; v++) z += red[v][i][lane];
+        const Layer &l = a.l;
+        const long m = 16 * i + row;
+        const int n = n0 + 4 * g;
+        if (m >= l.N || n >= l.F) continue;
+        if (l.bias) z += pg::load4((const T *)l.bias, n, l.F);
+        if (l.Z) pg::store4((T *)l.Z + m * l.ldz, n, l.F, z);
+        floatx4 u = {1.0f, 1.0f, 1.0f, 1.0f}, r = {};
+        if (l.U) u = pg::load4((const T *)l.U + m * l.ldu, n, l.F);
+        if (l.R) r = pg::load4((const T *)l.R + m * l.ldr, n, l.F);
+#pragma unroll
+        for (int k = 0; k < 4; k++) z[k] = r[k] + l.scale * act_of<F16>(l.act, z[k]) * u[k];
+        pg::store4((T *)l.Y + m * l.ldy, n, l.F, z);
+    }
+}
+
 // ── packing ────────────────────────────────────────────────────────────────────
 
 struct PackArgs {
@@ -206,8 +284,8 @@ constexpr int kFewF32 = 128, kFewF16 = 64;   // rows up to which W is read as it
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 struct Layout {
-    int P, Dp, few;          // planes; padded D; 16-row tiles of the form for few rows, or 0
-    bool pack_x, pack_w;
+    int P, Dp, few;          // planes; padded D; 16-row tiles of the forms for few rows, or 0
+    bool rows, pack_x, pack_w;   // rows: K over a workgroup's waves
     int64_t Xp, Wp, ex, ew, sums, total;
 };
 
@@ -222,12 +300,25 @@ pg::Work few_work(const ah_linear_desc &d, const Layout &l) {
     return few::work(ceil_div(d.F, 128), ceil_div(d.D, few::along_k(f16)), std::max(1.75, f16 ? 0.0 : 0.43 * l.few), l.few * 16l * 128 * 4);
 }
 
+// Which form for few rows. K over the waves reads all of X beside every 16 rows of W, at 33 GB/s a CU of both; tiles of 128 columns read W at 6.6
+// (f16) or 5 TB/s, and then 3.5 us go into a second launch. Measured, K over the waves | tiles: f16 1 x 4096 -> 16384 25.7 | 28.5 us,
+// 8 x 2048 -> 8192 9.6 | 13.5, 16 x 8192 -> 2048 17.3 | 15.8, 64 x 1024 -> 1024 7.6 | 8.9, 64 x 4096 -> 16384 82 | 38; f32 1 x 4096 -> 16384 58 | 70,
+// 16 x 4096 -> 1024 17.1 | 12.6.
+bool over_waves(const ah_linear_desc &d) {
+    if (d.N > 64) return false;
+    const bool f16 = d.dtype == AH_F16;
+    const double tiles = ceil_div(d.F, 16), row = (double)d.D * (f16 ? 2 : 4), bytes = row * d.F;
+    const double both = tiles * row * (16 + d.N) / (33e3 * std::min(256.0, tiles));
+    return std::max(both, bytes / 5.3e6) <= 6.0 + bytes / (f16 ? 6.6e6 : 5e6);
+}
+
 Layout layout(const ah_linear_desc &d) {
     Layout l{};
     const bool f16 = d.dtype == AH_F16;
     l.P = f16 ? 1 : 2;
     l.Dp = (d.D + 63) & ~63;
     if (d.N <= (f16 ? kFewF16 : kFewF32) && d.D >= 8) l.few = d.N <= 16 ? 1 : d.N <= 64 ? 4 : 8;
+    l.rows = l.few && over_waves(d);
     l.pack_x = !l.few && (!f16 || d.D % 64 || !rows_aligned(d.X, d.ldx, d.D));
     l.pack_w = !l.few && (!f16 || !rows_aligned(d.W, d.ldw, d.D));
     int64_t at = 0;
@@ -242,10 +333,10 @@ Layout layout(const ah_linear_desc &d) {
         l.ex = take((int64_t)d.N * 4);
         l.ew = take(((int64_t)d.F + 7) * 4);
     }
-    if (l.few) {
+    if (l.few && !l.rows) {
         const pg::Work w = few_work(d, l);
         l.sums = take(w.splits > 1 ? (int64_t)w.rest * w.splits * l.few * 16 * 128 * 4 : 0);
-    } else {
+    } else if (!l.few) {
         l.sums = take(plan_of(d, l).part_bytes());
     }
     l.total = std::max<int64_t>(at, 16);
@@ -264,6 +355,19 @@ void launch(const ProductArgs &a, int width, hipStream_t s) {
     if (width == 256) launch<pg::Tile256<0, 0, P, P>, T>(a, s);
     else if (width == 128) launch<pg::Tile128<0, 0, P, P>, T>(a, s);
     else launch<pg::Tile64<0, 0, P, P>, T>(a, s);
+}
+void launch_rows(const ah_linear_desc &d, const RowArgs &r, hipStream_t s) {
+    const bool f16 = d.dtype == AH_F16;
+    const int tiles = ceil_div(d.F, 16), chunks = ceil_div(d.D, f16 ? 32 : 16);
+    int waves = 4;   // up to 16 on each CU, of four pairs of chunks or more
+    while (waves < 16 && tiles * waves < 4096 && chunks >= waves * 8) waves *= 2;
+    const auto go = [&](auto fa) {
+        if (f16) hipLaunchKernelGGL((linear_rows_kernel<fa, half_t>), dim3((unsigned)tiles), dim3(64 * waves), 0, s, r);
+        else hipLaunchKernelGGL((linear_rows_kernel<fa, float>), dim3((unsigned)tiles), dim3(64 * waves), 0, s, r);
+    };
+    if (d.N <= 16) go(std::integral_constant<int, 1>());
+    else if (d.N <= 32) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 4>());
 }
 template <int FA, class T>
 void launch_few(const ProductArgs &a, const FewArgs &f, hipStream_t s) {
@@ -289,6 +393,10 @@ hipError_t linear(const ah_linear_desc &d, hipStream_t s) {
     a.l = {d.N, d.F, d.act, d.scale, d.bias, d.U, d.R, d.Y, d.Z, d.ldu, d.ldr, d.ldy, d.ldz, nullptr, nullptr};
     if (l.few) {
         const FewArgs f{d.X, d.W, d.ldx, d.ldw, d.D};
+        if (l.rows) {
+            launch_rows(d, RowArgs{f, a.l}, s);
+            return hipGetLastError();
+        }
         a.nk = ceil_div(d.D, few::along_k(f16));
         a.w = few_work(d, l);
         a.w.part = (float *)(ws + l.sums);

@@ -267,3 +267,24 @@ def test_gradients_against_differences(dev):
         want = float(((y[0] - y[1]) * c.dY).sum()) / (2 * h)
         noise = 2.0 ** -20 * np.linalg.norm(c.dY) * np.abs(y[0]).max() / h
         assert abs(float((g[grad].reshape(base.shape) * d).sum()) - want) <= noise + h * h * np.linalg.norm(c.dY), name
+
+
+@pytest.mark.parametrize("gap", [0, 3])
+@pytest.mark.parametrize("dtype", [L.AH_F32, L.AH_F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("shape", [(1, 8, 1), (2, 9, 33), (5, 31, 16), (17, 100, 70), (33, 776, 333), (64, 1001, 131), (16, 8192, 2000), (64, 4096, 1000), (48, 4100, 2050),
+                                   (16, 1000, 16400)], ids=lambda s: "%dx%dx%d" % s)
+def test_few_rows(dev, shape, dtype, gap):
+    """W read as it lies: K over 4, 8 and 16 waves with ends inside a lane's load, a chunk and a wave's turn, and tiles of 128 columns."""
+    c = Case(*shape, dtype=dtype, kind=L.ACT_SILU)
+    O.compare(c.forward(dev, gap=gap), c.expected())
+
+
+@pytest.mark.parametrize("dtype", [L.AH_F32, L.AH_F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("D", [9, 33, 130])
+def test_few_rows_read_twice_at_the_end(dev, D, dtype):
+    """An infinity among the columns that two lanes read: it counts once, and where X is positive Z is infinite, not NaN."""
+    c = Case(5, D, 40, dtype=dtype, kind=L.ACT_NONE, bias=False, factor=False, res=False)
+    c.X = np.abs(c.X)
+    c.W[3, D - 2] = np.inf
+    z = c.forward(dev)["Z"]
+    assert np.all(z[:, 3] == np.inf) and np.isfinite(np.delete(z, 3, axis=1)).all()

@@ -211,7 +211,7 @@ struct Tile {
     static constexpr int BM = BM_, BN = BN_, WVM = WVM_, WVN = WVN_, TA = TA_, TB = TB_, PA = PA_, PB = PB_, NS = NS_;
     static constexpr int NW = WVM * WVN, NT = 64 * NW, WM = BM / WVM, WN = BN / WVN, FA = WM / 16, FB = WN / 16;
     static constexpr int BK = PA == 1 && PB == 1 ? 64 : 32;
-    static constexpr int ABYTES = BM * BK * PA * 2, STAGE = ABYTES + BN * BK * PB * 2, SMEM = NS * STAGE;
+    static constexpr int ABYTES = BM * BK * PA * 2, STAGE = ABYTES + BN * BK * PB * 2, SMEM = PA == 1 && PB == 1 && NW == 8 ? 5 * ABYTES : NS * STAGE;   // contract_ring's five
     using FetchA = PFetch<BM, TA, PA, BK, NW>;
     using FetchB = PFetch<BN, TB, PB, BK, NW>;
     using FragA = PFrag<BM, TA, PA, BK>;
@@ -284,7 +284,7 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
     typename C::FragA ra;
     typename C::FragB rb;
     ra.init(lds, wm0, lane);
-    rb.init(lds + ABYTES, wn0, lane);
+    rb.init(C::PA == 1 && C::PB == 1 && C::NW == 8 ? lds : lds + ABYTES, wn0, lane);
     auto fragA = [&](h8 (&v)[FA], int buf, int s) {
         uint32_t at = ra.first + buf * STAGE;
         asm volatile("" : "+v"(at));
@@ -343,70 +343,125 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    g16::lds_barrier();   // the LDS may still be read by a caller's earlier tile
+    if constexpr (C::PA == 1 && C::PB == 1 && C::NW == 8) {
+        // One plane by one: A's and B's stages go round five buffers of 32 KiB, A of stage t in buffer 2 t mod 5 and B in the next, so that half a
+        // stage's loads go out in each half of a stage, one every eight MFMAs: sixteen in a row queue up, and the waves with them.
+        // Buffers are free from the barrier in their stage's middle: B of t+2 follows into that of A of t in the second half, A of t+3 into that
+        // of B of t in the next stage's first.
+        static_assert(FA == 4 && FB == 8 && PERA == 4 && PERS == 8 && NS == 2, "four parts of eight MFMAs and a load");
+        h8 a0[FA], a1[FA], b0[FB], b1[FB];
+        const auto next = [](int b, int by) { return b + by >= 5 ? b + by - 5 : b + by; };
+        const auto load_a = [&](int f, int t, int buf) { fa.issue(f, Ab + (kt0 + min(t, nk - 1)) * da, A.ld, BK, lds + buf * ABYTES, wave_u, lane); };
+        const auto load_b = [&](int f, int t, int buf) { fb.issue(f, Bb + (BLOCKS && C::TB == 1 ? stored((kt0 + min(t, nk - 1)) * BK) : (kt0 + min(t, nk - 1)) * db), B.ld, B.k - (kt0 + min(t, nk - 1)) * BK, lds + buf * ABYTES, wave_u, lane); };
+        // the MFMAs of one k-step, the reads of the next one (k-step s of the buffers at A and B) and four loads
+        const auto half = [&](h8 (&a)[FA], h8 (&b)[FB], h8 (&an)[FA], h8 (&bn)[FB], int bufa, int bufb, int s, auto load) {
+            uint32_t at = ra.first + bufa * ABYTES, bt = rb.first + bufb * ABYTES;
+            asm volatile("" : "+v"(at), "+v"(bt));
 #pragma unroll
-    for (int p = 0; p < NS; p++)
+            for (int i = 0; i < FA; i++) {
+                an[i] = C::FragA::read(at, i, s);
+                bn[2 * i] = C::FragB::read(bt, 2 * i, s);
+                bn[2 * i + 1] = C::FragB::read(bt, 2 * i + 1, s);
 #pragma unroll
-        for (int f = 0; f < PERS; f++) issue_one(f, min(p, nk - 1), p);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"i"((NS - 1) * PERS) : "memory");
-    g16::lds_barrier();
-
-    h8 a0[FA], a1[FA], b0[FB], b1[FB];
-    fragA(a0, 0, 0);
-    fragB(b0, 0, 0);
-    // One stage. On entry a and b hold its first fragments; on exit `an` and `bn` those of the next stage.
-    if constexpr (C::PB == 2) {
-        auto stage = [&](int t, int buf, h8 (&a)[FA], h8 (&an)[FA]) {
-            const int nbuf = buf + 1 == NS ? 0 : buf + 1;
-            fragA(an, buf, 1);   // lo
-            mma(a, b0, NRA);
-            fragB(b1, buf, 1);   // lo
-            mma(an, b0, NRB);
-            open_next();
-            fragA(an, nbuf, 0);
-            fragB(b0, nbuf, 0);
-            mma_refill(a, b1, t, buf);
-        };
-        int buf = 0;
-        for (int t = 0; t < nk; t += 2) {
-            stage(t, buf, a0, a1);
-            buf = buf + 1 == NS ? 0 : buf + 1;
-            if (t + 1 < nk) {
-                stage(t + 1, buf, a1, a0);
-                buf = buf + 1 == NS ? 0 : buf + 1;
+                for (int j = 0; j < FB; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[j], a[i], acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                load(i);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        g16::lds_barrier();   // the LDS may still be read by a caller's earlier tile
+#pragma unroll
+        for (int p = 0; p < 5; p++)
+#pragma unroll
+            for (int f = 0; f < PERA; f++) p & 1 ? load_b(f, p / 2, p) : load_a(f, p / 2, p);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(3 * PERA) : "memory");
+        g16::lds_barrier();
+        fragA(a0, 0, 0);
+        {
+            uint32_t bt = rb.first + ABYTES;
+            asm volatile("" : "+v"(bt));
+#pragma unroll
+            for (int j = 0; j < FB; j++) b0[j] = C::FragB::read(bt, j, 0);
         }
-    } else if constexpr (C::PA == 2) {
-        auto stage = [&](int t, int buf, h8 (&b)[FB], h8 (&bn)[FB]) {
-            const int nbuf = buf + 1 == NS ? 0 : buf + 1;
-            fragA(a1, buf, 1);   // lo
-            mma(a0, b, NRA);
-            open_next();
-            fragA(a0, nbuf, 0);
-            fragB(bn, nbuf, 0);
-            mma_refill(a1, b, t, buf);
-        };
-        int buf = 0;
-        for (int t = 0; t < nk; t += 2) {
-            stage(t, buf, b0, b1);
-            buf = buf + 1 == NS ? 0 : buf + 1;
-            if (t + 1 < nk) {
-                stage(t + 1, buf, b1, b0);
-                buf = buf + 1 == NS ? 0 : buf + 1;
-            }
+        int buf = 0;   // A's of stage t
+        for (int t = 0; t < nk; t++) {
+            half(a0, b0, a1, b1, buf, next(buf, 1), 1, [&](int f) {
+                if (t) load_a(f, t + 2, next(buf, 4));
+            });
+            // stage t+1 has landed (the next A may be on its way), and every wave has read stage t
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"i"(PERA) : "memory");
+            g16::lds_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            half(a1, b1, a0, b0, next(buf, 2), next(buf, 3), 0, [&](int f) { load_b(f, t + 2, buf); });
+            buf = next(buf, 2);
         }
     } else {
-        int buf = 0;
-        for (int t = 0; t < nk; t++) {
-            const int nbuf = buf + 1 == NS ? 0 : buf + 1;
-            fragA(a1, buf, 1);   // second k-step
-            fragB(b1, buf, 1);
-            mma(a0, b0, NRAB);
-            open_next();
-            fragA(a0, nbuf, 0);
-            fragB(b0, nbuf, 0);
-            mma_refill(a1, b1, t, buf);
-            buf = nbuf;
+        g16::lds_barrier();   // the LDS may still be read by a caller's earlier tile
+#pragma unroll
+        for (int p = 0; p < NS; p++)
+#pragma unroll
+            for (int f = 0; f < PERS; f++) issue_one(f, min(p, nk - 1), p);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"((NS - 1) * PERS) : "memory");
+        g16::lds_barrier();
+
+        h8 a0[FA], a1[FA], b0[FB], b1[FB];
+        fragA(a0, 0, 0);
+        fragB(b0, 0, 0);
+        // One stage. On entry a and b hold its first fragments; on exit `an` and `bn` those of the next stage.
+        if constexpr (C::PB == 2) {
+            auto stage = [&](int t, int buf, h8 (&a)[FA], h8 (&an)[FA]) {
+                const int nbuf = buf + 1 == NS ? 0 : buf + 1;
+                fragA(an, buf, 1);   // lo
+                mma(a, b0, NRA);
+                fragB(b1, buf, 1);   // lo
+                mma(an, b0, NRB);
+                open_next();
+                fragA(an, nbuf, 0);
+                fragB(b0, nbuf, 0);
+                mma_refill(a, b1, t, buf);
+            };
+            int buf = 0;
+            for (int t = 0; t < nk; t += 2) {
+                stage(t, buf, a0, a1);
+                buf = buf + 1 == NS ? 0 : buf + 1;
+                if (t + 1 < nk) {
+                    stage(t + 1, buf, a1, a0);
+                    buf = buf + 1 == NS ? 0 : buf + 1;
+                }
+            }
+        } else if constexpr (C::PA == 2) {
+            auto stage = [&](int t, int buf, h8 (&b)[FB], h8 (&bn)[FB]) {
+                const int nbuf = buf + 1 == NS ? 0 : buf + 1;
+                fragA(a1, buf, 1);   // lo
+                mma(a0, b, NRA);
+                open_next();
+                fragA(a0, nbuf, 0);
+                fragB(bn, nbuf, 0);
+                mma_refill(a1, b, t, buf);
+            };
+            int buf = 0;
+            for (int t = 0; t < nk; t += 2) {
+                stage(t, buf, b0, b1);
+                buf = buf + 1 == NS ? 0 : buf + 1;
+                if (t + 1 < nk) {
+                    stage(t + 1, buf, b1, b0);
+                    buf = buf + 1 == NS ? 0 : buf + 1;
+                }
+            }
+        } else {
+            int buf = 0;
+            for (int t = 0; t < nk; t++) {
+                const int nbuf = buf + 1 == NS ? 0 : buf + 1;
+                fragA(a1, buf, 1);   // second k-step
+                fragB(b1, buf, 1);
+                mma(a0, b0, NRAB);
+                open_next();
+                fragA(a0, nbuf, 0);
+                fragB(b0, nbuf, 0);
+                mma_refill(a1, b1, t, buf);
+                buf = nbuf;
+            }
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the tail's re-fetches land before the LDS is given up

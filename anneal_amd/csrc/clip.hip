@@ -6,7 +6,7 @@
 // order: 16 KB from the L2) and scales. Tensors are cut into chunks of 2048 elements that are numbered through; a workgroup takes a run of
 // neighbouring chunks, so it looks for its first tensor once (a binary search) and then walks on. The table of tensors travels with the
 // launch where it fits there, else small launches lay it down in the workspace first: no host memory has to outlive the call, and
-// a graph holds the table itself.
+// a graph holds the table itself. The second launch goes through a workgroup's run from its end, which the first has left in the caches.
 //
 // Bound by memory: every entry is read twice and written once. Squares go to f64 at once (f32 squares of entries under 2^-63 would vanish
 // and of those over 2^64 be infinite); squares of f16 are exact in f32 and are summed there eight at a time.
@@ -45,22 +45,33 @@ static_assert(sizeof(Args) + sizeof(Inline) <= 4096, "the arguments of a launch"
 
 int64_t chunks_of(int64_t count) { return (count + kChunk - 1) / kChunk; }
 
-// f(entry, from, to) for each stretch of a tensor among this workgroup's chunks; at(i): entry i.
-template <class At, class F>
+// f(entry, from, to) for each stretch of a tensor among this workgroup's chunks, from the first to the last or (BACK) the other way; at(i):
+// entry i.
+template <bool BACK, class At, class F>
 __device__ __forceinline__ void walk(const Args &a, At at, F f) {
-    long c = a.chunks * blockIdx.x / a.blocks;
-    const long end = a.chunks * (blockIdx.x + 1) / a.blocks;
+    const long begin = a.chunks * blockIdx.x / a.blocks, end = a.chunks * (blockIdx.x + 1) / a.blocks;
+    if (begin >= end) return;
+    long c = BACK ? end - 1 : begin;
     int t = 0;
     for (int hi = a.n - 1; t < hi;) {   // the last tensor that starts at or before c (empty ones start where the next does)
         const int mid = (t + hi + 1) / 2;
         if (at(mid).first <= c) t = mid;
         else hi = mid - 1;
     }
-    for (; c < end; t++) {
-        const Entry e = at(t);
-        const long stop = min(end, e.first + (e.count + kChunk - 1) / kChunk);
-        f(e, (c - e.first) * kChunk, min(e.count, (stop - e.first) * kChunk));
-        c = stop;
+    if constexpr (BACK) {
+        for (c = end; c > begin; t--) {
+            const Entry e = at(t);
+            const long start = max(begin, e.first);
+            f(e, (start - e.first) * kChunk, min(e.count, (c - e.first) * kChunk));
+            c = start;
+        }
+    } else {
+        for (; c < end; t++) {
+            const Entry e = at(t);
+            const long stop = min(end, e.first + (e.count + kChunk - 1) / kChunk);
+            f(e, (c - e.first) * kChunk, min(e.count, (stop - e.first) * kChunk));
+            c = stop;
+        }
     }
 }
 
@@ -121,7 +132,7 @@ __device__ __forceinline__ double block_sum(double s) {
 template <class At>
 __device__ __forceinline__ void norm_part(const Args &a, At at) {
     double s = 0.0;
-    walk(a, at, [&](const Entry &e, long from, long to) {
+    walk<false>(a, at, [&](const Entry &e, long from, long to) {
         s += e.half ? sum_squares((const half_t *)e.src, from, to) : sum_squares((const float *)e.src, from, to);
     });
     s = block_sum(s);
@@ -146,20 +157,22 @@ __device__ __forceinline__ void scale_range(const T *p, O *q, long from, long to
         for (int k = 0; k < V::N; k++) o[k] = (O)f.of((float)v[k]);
         *(out *)(q + i) = o;
     };
-    long i = from + threadIdx.x * V::N;
-    for (; i - threadIdx.x * V::N + 256 * V::N * kAhead <= to; i += 256 * V::N * kAhead) {
-        typename V::type v[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) v[u] = *(const typename V::type *)(p + i + u * 256 * V::N);
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) put(i + u * 256 * V::N, v[u]);
-    }
-    for (; i < to; i += 256 * V::N) {
+    constexpr long step = 256 * V::N * kAhead;
+    const long whole = (to - from) / step;
+    for (long i = from + whole * step + threadIdx.x * V::N; i < to; i += 256 * V::N) {
         if (i + V::N <= to) {
             put(i, *(const typename V::type *)(p + i));
         } else {
             for (long k = i; k < to; k++) q[k] = (O)f.of((float)p[k]);
         }
+    }
+    for (long s = whole - 1; s >= 0; s--) {
+        const long i = from + s * step + threadIdx.x * V::N;
+        typename V::type v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) v[u] = *(const typename V::type *)(p + i + u * 256 * V::N);
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) put(i + u * 256 * V::N, v[u]);
     }
 }
 
@@ -177,7 +190,7 @@ __device__ __forceinline__ void scale_part(const Args &a, At at) {
         if (a.norm) *a.norm = (float)norm;
         if (a.coef) *a.coef = (float)c;
     }
-    walk(a, at, [&](const Entry &e, long from, long to) {
+    walk<true>(a, at, [&](const Entry &e, long from, long to) {
         if (!e.dst || (e.dst == e.src && f.pre * f.m == 1.0f)) return;
         if (!e.half) scale_range((const float *)e.src, (float *)e.dst, from, to, f);
         else if (e.half_out) scale_range((const half_t *)e.src, (half_t *)e.dst, from, to, f);

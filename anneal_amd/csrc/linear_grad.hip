@@ -149,7 +149,8 @@ __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArg
     if (s.wblocks) e[2] = pg::plane_exp(join_maxes(s.maxes + 2 * kScans, s.wblocks));
     if (blockIdx.x == 0 && threadIdx.x < 3) a.exps[threadIdx.x] = threadIdx.x == 0 ? e[0] : threadIdx.x == 1 ? e[1] : e[2];
     if ((int)blockIdx.x < a.zblocks) {   // kRows rows by 512 columns: a thread has eight columns of every fourth row
-        const int rb = blockIdx.x / a.zcols, n = ((int)blockIdx.x - rb * a.zcols) * 512 + (threadIdx.x & 63) * 8, w = threadIdx.x >> 6;
+        // the last rows first, which the scan has left in the caches (16384 x 1024 -> 4096, both passes and the products: 420 -> 414 us)
+        const int zb = a.zblocks - 1 - (int)blockIdx.x, rb = zb / a.zcols, n = (zb - rb * a.zcols) * 512 + (threadIdx.x & 63) * 8, w = threadIdx.x >> 6;
         constexpr int B = sizeof(T) == 2 ? 4 : 2;   // rows whose loads are in flight together
         f8 col = {};
         if (n < a.Fp) {

@@ -250,7 +250,7 @@ struct PackArgs {
     half_t *Xp, *Wp;
     int *ex, *ew;
 };
-// A wave a row, of X and then of W. f32: the row's largest magnitude first, then its planes; the second reading comes from the caches.
+// A wave a row, of X and then of W. f32: the row's largest magnitude first, then its planes; a longer row's second reading comes from the caches.
 template <int P>
 __global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
     constexpr int E = P == 1 ? 2 : 4;
@@ -262,16 +262,37 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
         const char *in = x ? (const char *)a.X + r * a.ldx * E : (const char *)a.W + r * a.ldw * E;
         int e = 0;
         if constexpr (P == 2) {
+            constexpr int HELD = 8;   // 256 columns each: rows that a wave's registers hold are read once (777 + 2003 rows of 1001: HELD_US)
+            floatx4 v[HELD];
+            const bool held = a.D <= 256 * HELD;
             unsigned m = 0;
-#pragma unroll 4
-            for (int c = lane * 4; c < a.D; c += 256) {
-                const floatx4 v = pg::load4((const float *)in, c, a.D);
+            const auto most = [&](floatx4 y) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) m = max(m, pg::magnitude(__float_as_uint(v[k])));
+                for (int k = 0; k < 4; k++) m = max(m, pg::magnitude(__float_as_uint(y[k])));
+            };
+            if (held) {
+#pragma unroll
+                for (int j = 0; j < HELD; j++) v[j] = j * 256 < a.D ? pg::load4((const float *)in, lane * 4 + 256 * j, a.D) : (floatx4){};
+#pragma unroll
+                for (int j = 0; j < HELD; j++) most(v[j]);
+            } else {
+#pragma unroll 4
+                for (int c = lane * 4; c < a.D; c += 256) most(pg::load4((const float *)in, c, a.D));
             }
             for (int o = 32; o >= 1; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
             e = pg::plane_exp(m);
             if (lane == 0) (x ? a.ex : a.ew)[r] = e;
+            if (held) {
+#pragma unroll
+                for (int j = 0; j < HELD; j++) {
+                    const int c = lane * 4 + 256 * j;
+                    if (c >= a.Dp) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) v[j][k] = ldexpf(v[j][k], e);
+                    pg::plane_store((x ? a.Xp : a.Wp) + pg::panel_at<2>(x ? a.N : a.F, r, c), v[j]);
+                }
+                continue;
+            }
         }
         pg::pack_row<P>(x ? a.Xp : a.Wp, x ? a.N : a.F, r, in, a.D, a.Dp, e);
     }

@@ -21,7 +21,7 @@ namespace ah {
 namespace {
 
 constexpr int kScans = 1024;   // workgroups that look for an array's largest magnitude, at most
-constexpr int kRows = 32;      // rows of a block of dZ
+constexpr int kRows = 32, kFewRows = 8;   // rows of a block of dZ: fewer where those blocks would not fill the chip (300 x 1024 -> 1024 29 -> 23 us)
 
 struct GradIn {
     int N, D, F, act;
@@ -136,7 +136,7 @@ struct PackArgs {
     long lddu;
     float *dbpart;             // [row block][F] or null
     int Np, Fp, Dp;
-    int zblocks, zcols, rest;  // workgroups for dZ (zcols a row block), and for X's and W's rows
+    int zblocks, zcols, zrows, rest;  // workgroups for dZ (zcols a block of zrows rows), and for X's and W's rows
     int *exps;                 // [3]: exponents of dZ, X and W
 };
 // P: planes of dZ; PO: of X and W.
@@ -148,22 +148,23 @@ __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArg
     if (s.xblocks) e[1] = pg::plane_exp(join_maxes(s.maxes + kScans, s.xblocks));
     if (s.wblocks) e[2] = pg::plane_exp(join_maxes(s.maxes + 2 * kScans, s.wblocks));
     if (blockIdx.x == 0 && threadIdx.x < 3) a.exps[threadIdx.x] = threadIdx.x == 0 ? e[0] : threadIdx.x == 1 ? e[1] : e[2];
-    if ((int)blockIdx.x < a.zblocks) {   // kRows rows by 512 columns: a thread has eight columns of every fourth row
+    if ((int)blockIdx.x < a.zblocks) {   // zrows rows by 512 columns: a thread has eight columns of every fourth row
         // the last rows first, which the scan has left in the caches (16384 x 1024 -> 4096, both passes and the products: 420 -> 414 us)
         const int zb = a.zblocks - 1 - (int)blockIdx.x, rb = zb / a.zcols, n = (zb - rb * a.zcols) * 512 + (threadIdx.x & 63) * 8, w = threadIdx.x >> 6;
         constexpr int B = sizeof(T) == 2 ? 4 : 2;   // rows whose loads are in flight together
         f8 col = {};
         if (n < a.Fp) {
-            for (int k0 = w; k0 < kRows; k0 += 4 * B) {
+            for (int k0 = w; k0 < a.zrows; k0 += 4 * B) {
                 Line<T> line[B] = {};
 #pragma unroll
                 for (int b = 0; b < B; b++) {
-                    const int m = rb * kRows + k0 + 4 * b;
-                    if (m < g.N && n < g.F) line[b] = load_line<T>(g, m, n);
+                    const int m = rb * a.zrows + k0 + 4 * b;
+                    if (k0 + 4 * b < a.zrows && m < g.N && n < g.F) line[b] = load_line<T>(g, m, n);
                 }
 #pragma unroll
                 for (int b = 0; b < B; b++) {
-                    const int m = rb * kRows + k0 + 4 * b;
+                    if (k0 + 4 * b >= a.zrows) break;
+                    const int m = rb * a.zrows + k0 + 4 * b;
                     f8 v = {}, du;
                     if (m < g.N && n < g.F) {
                         v = dz_of<T>(g, line[b], du);
@@ -319,23 +320,31 @@ struct FewArgs {
     const void *W;
     long ldw;
 };
-template <int FA, int PP, bool F16>
-__global__ __launch_bounds__(256, 2) void linear_grad_few_kernel(ProductArgs a, FewArgs f) {
-    __shared__ __attribute__((aligned(16))) char smem[std::max(few::smem_bytes<few::Tile<FA, 4>>(), tile_out_bytes<few::Tile<FA, 4>>())];
-    few::with_rows<FA>(a.M, [&](auto fa) {
-        typedef few::Tile<fa, 4> C;
-        int tile, slot, first, count;
-        pg::pick(a.w, blockIdx.x, a.nk, tile, slot, first, count);
-        floatx4 acc[C::FA][C::FB];
-        few::contract_across<C, PP, F16>(f.P, f.prows, f.Fp, f.W, f.ldw, f.F, a.N, tile * C::BN, first, count, smem, acc);
-        if (slot >= 0) {
-            pg::store_partials<C>(a.w.part, slot, acc);
-            return;
-        }
-        few::sync();
+template <int FA, int PP, bool F16, class W>
+__global__ __launch_bounds__(256, 2) void linear_grad_few_kernel(PairArgs a, FewArgs f) {
+    __shared__ __attribute__((aligned(1024))) char smem[std::max({few::smem_bytes<few::Tile<FA, 4>>(), tile_out_bytes<few::Tile<FA, 4>>(), W::SMEM})];
+    static_assert(W::NT == 256, "one launch");
+    const int b = blockIdx.x;
+    if (b >= a.xblocks + a.wblocks) {
+        sum_db<256>(a, b - a.xblocks - a.wblocks, smem);
+    } else if (b >= a.xblocks) {
+        product<W>(a.w, b - a.xblocks, smem);
+    } else if (b < a.x.w.blocks()) {
+        few::with_rows<FA>(a.x.M, [&](auto fa) {
+            typedef few::Tile<fa, 4> C;
+            int tile, slot, first, count;
+            pg::pick(a.x.w, b, a.x.nk, tile, slot, first, count);
+            floatx4 acc[C::FA][C::FB];
+            few::contract_across<C, PP, F16>(f.P, f.prows, f.Fp, f.W, f.ldw, f.F, a.x.N, tile * C::BN, first, count, smem, acc);
+            if (slot >= 0) {
+                pg::store_partials<C>(a.x.w.part, slot, acc);
+                return;
+            }
+            few::sync();
 #pragma unroll
-        for (int i = 0; i < C::FA; i++) product_rows<C>(a, 0, tile * C::BN, i, acc[i], smem);
-    });
+            for (int i = 0; i < C::FA; i++) product_rows<C>(a.x, 0, tile * C::BN, i, acc[i], smem);
+        });
+    }
 }
 template <int FA>
 __global__ __launch_bounds__(256) void linear_grad_few_join_kernel(ProductArgs a) {
@@ -430,7 +439,7 @@ Cuts cuts_of(int N, int D, int F, int P, int PO, bool with_x) {
 }
 struct Layout {
     int P, PO;                 // planes of dZ; of X and W
-    int Np, Fp, Dp, few;
+    int Np, Fp, Dp, few, zrows;
     bool products, pack_x, pack_w;
     Cuts cuts;
     int64_t exps, maxes, dbpart, dZ, Xp, Wp, sums, wsums, total;
@@ -449,6 +458,7 @@ Layout layout(const ah_linear_grad_desc &d) {
     l.Fp = (d.F + 63) & ~63;
     l.Dp = (d.D + 63) & ~63;
     l.products = d.dX || d.dW;
+    l.zrows = (int64_t)(l.Np / kRows) * ceil_div(l.Fp, 512) < 256 ? kFewRows : kRows;
     if (d.dX && d.N <= (f16 ? kFewF16 : kFewF32) && d.D >= 8) l.few = d.N <= 16 ? 1 : d.N <= 64 ? 4 : 8;
     l.pack_x = d.dW && (!f16 || !rows_aligned(d.X, d.ldx, d.D));
     l.pack_w = d.dX && !l.few && (!f16 || !rows_aligned(d.W, d.ldw, d.D));
@@ -460,7 +470,7 @@ Layout layout(const ah_linear_grad_desc &d) {
     };
     l.exps = take(16);
     l.maxes = take(3 * kScans * 4);
-    if (d.dbias) l.dbpart = take((int64_t)(l.Np / kRows) * d.F * 4);
+    if (d.dbias) l.dbpart = take((int64_t)(l.Np / l.zrows) * d.F * 4);
     if (l.products) l.dZ = take((int64_t)l.Np * l.Fp * 2 * l.P);
     if (l.pack_x) l.Xp = take((int64_t)d.N * l.Dp * 2 * l.PO);
     if (l.pack_w) l.Wp = take((int64_t)d.F * l.Dp * 2 * l.PO);
@@ -508,10 +518,28 @@ void launch(const PairArgs &a, const Cuts &c, bool x, bool w, hipStream_t s) {
     launch<X128, W128>(a, x, w, s);
 }
 
-template <int P, bool F16, int FA>
-void launch_few(const ProductArgs &a, const FewArgs &f, hipStream_t s) {
-    hipLaunchKernelGGL((linear_grad_few_kernel<FA, P, F16>), dim3((unsigned)a.w.blocks()), dim3(256), 0, s, a, f);
-    if (a.w.splits > 1) hipLaunchKernelGGL((linear_grad_few_join_kernel<FA>), dim3((unsigned)a.w.rest, FA), dim3(256), 0, s, a);
+template <int P, bool F16, int FA, class W>
+void launch_few(PairArgs a, const FewArgs &f, bool w, hipStream_t s) {
+    a.w.tiles_m = ceil_div(a.w.M, W::BM);
+    a.w.tiles_n = ceil_div(a.w.N, W::BN);
+    a.xblocks = (a.x.w.blocks() + 7) & ~7;
+    a.wblocks = w ? a.w.w.blocks() : 0;
+    hipLaunchKernelGGL((linear_grad_few_kernel<FA, P, F16, W>), dim3((unsigned)(a.xblocks + a.wblocks + (a.db ? ceil_div(a.F, 64) : 0))), dim3(256), 0, s, a, f);
+    if (a.x.w.splits > 1) hipLaunchKernelGGL((linear_grad_few_join_kernel<FA>), dim3((unsigned)a.x.w.rest, FA), dim3(256), 0, s, a.x);
+    if (w && a.w.w.splits > 1) {
+        a.xblocks = 0;
+        a.wblocks = a.w.w.rest * W::FA;
+        hipLaunchKernelGGL((linear_grad_join_kernel<W, W>), dim3((unsigned)a.wblocks), dim3(256), 0, s, a);
+    }
+}
+// dX of few rows, and in its launch dW and db where their tiles have as many threads (7 x 1024 -> 4096 f16: 27.6 -> 22 us for all four).
+template <int P, int PO, int FA>
+void launch_few(const PairArgs &a, const FewArgs &f, int width, bool w, hipStream_t s) {
+    constexpr bool F16 = PO == 1;
+    if constexpr (PO == 2) {
+        if (width == 64) return launch_few<P, F16, FA, pg::Tile64<1, 1, P, PO>>(a, f, w, s);
+    }
+    launch_few<P, F16, FA, pg::Tile128<1, 1, P, PO>>(a, f, w, s);
 }
 
 template <class T, int P, int PO>
@@ -537,7 +565,8 @@ void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     p.Fp = l.Fp;
     p.Dp = l.Dp;
     p.zcols = ceil_div(l.Fp, 512);
-    p.zblocks = l.Np / kRows * p.zcols;
+    p.zrows = l.zrows;
+    p.zblocks = l.Np / l.zrows * p.zcols;
     p.rest = (int)std::min<int64_t>(((l.pack_x ? d.N : 0) + (int64_t)(l.pack_w ? d.F : 0) + 3) / 4, 4096);
     p.exps = (int *)(ws + l.exps);
     hipLaunchKernelGGL((linear_grad_pack_kernel<T, P, PO>), dim3((unsigned)(p.zblocks + p.rest)), dim3(256), 0, s, g, p, sc);
@@ -553,20 +582,10 @@ void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     a.w.ldc = d.lddw;
     a.db = d.dbias;
     a.dbpart = p.dbpart;
-    a.dbrows = l.Np / kRows;
+    a.dbrows = l.Np / l.zrows;
     a.F = d.F;
-    if (l.few) {
-        ProductArgs b = a.x;
-        const FewArgs f{ws + l.dZ, l.Np, l.Fp, d.F, d.W, d.ldw};
-        b.nk = ceil_div(d.F, few::across_v(P));
-        b.w = few_work(d, l);
-        b.w.part = (float *)(ws + l.sums);
-        if (l.few == 1) launch_few<P, PO == 1, 1>(b, f, s);
-        else if (l.few == 4) launch_few<P, PO == 1, 4>(b, f, s);
-        else if constexpr (PO == 2) launch_few<P, PO == 1, 8>(b, f, s);
-    }
     const bool x = d.dX && !l.few;
-    if (!x && !d.dW && !d.dbias) return;
+    if (!d.dX && !d.dW && !d.dbias) return;
     constexpr int BK = P == 1 ? 64 : 32;   // every stage begins at a row of W or X that there is
     if (x) {
         a.x.w = l.cuts.x.w;
@@ -583,6 +602,19 @@ void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
         a.w.B = l.pack_x ? pg::panels(p.Xp, d.N, l.Dp, d.N) : pg::row_major(d.X, d.ldx, d.D, d.N);
         a.w.nk = ceil_div(d.N, BK);
         a.w.eb = PO == 2 ? p.exps + 1 : nullptr;
+    }
+    if (l.few) {
+        const FewArgs f{ws + l.dZ, l.Np, l.Fp, d.F, d.W, d.ldw};
+        const bool with_w = d.dW && l.cuts.w.width < 256;
+        PairArgs b = a;
+        b.x.nk = ceil_div(d.F, few::across_v(P));
+        b.x.w = few_work(d, l);
+        b.x.w.part = (float *)(ws + l.sums);
+        if (!with_w && d.dW) b.db = nullptr;   // db goes with dW
+        if (l.few == 1) launch_few<P, PO, 1>(b, f, l.cuts.w.width, with_w, s);
+        else if (l.few == 4) launch_few<P, PO, 4>(b, f, l.cuts.w.width, with_w, s);
+        else if constexpr (PO == 2) launch_few<P, PO, 8>(b, f, l.cuts.w.width, with_w, s);
+        if (with_w || !d.dW) return;
     }
     launch<P, PO>(a, l.cuts, x, d.dW != nullptr, s);
 }

@@ -262,9 +262,10 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
         const char *in = x ? (const char *)a.X + r * a.ldx * E : (const char *)a.W + r * a.ldw * E;
         int e = 0;
         if constexpr (P == 2) {
-            constexpr int HELD = 8;   // 256 columns each: rows that a wave's registers hold are read once (777 + 2003 rows of 1001: HELD_US)
+            constexpr int HELD = 8;   // 256 columns each: longer rows that a wave's registers hold are read once
             floatx4 v[HELD];
-            const bool held = a.D <= 256 * HELD;
+            // 200 x 2048 -> 8192 71 -> 64 us, 777 x 1001 -> 2003 31.6 -> 30.2; shorter rows, in the loop below as in registers, 118 | 121 us at 4000 x 768 -> 3000
+            const bool held = a.D > 768 && a.D <= 256 * HELD;
             unsigned m = 0;
             const auto most = [&](floatx4 y) {
 #pragma unroll

@@ -10,6 +10,8 @@
 //
 // The epilogue takes Z from the accumulators in f32 through LDS (tile_out.h), eight columns of a row to a lane, so that U, R, Z and Y are
 // read and written in 16 bytes; the loads of 16 rows are in flight together. Bound by the matrix cores for many rows, by W's bytes for few.
+// f16 8192 x 4096 -> 16384 with bias, GELU and Z: 960-980 us (1135 TFLOP/s), 60 of them the epilogue; 1 x 4096 -> 16384 with a factor 26 (5.2 TB/s);
+// 48 x 8192 -> 2048 14; f32 777 x 1001 -> 2003 29.
 #include "linear.h"
 
 #include <algorithm>
@@ -80,7 +82,7 @@ __device__ __forceinline__ void layer_rows(const Layer &l, int m0, int n0, int i
         }
 #pragma unroll
         for (int k = 0; k < 8; k++) z.v[k] += (float)b[k];
-        if (l.Z) store_f8((T *)l.Z + row(p) * l.ldz, out.n, l.F, z);
+        if (l.Z) store8((T *)l.Z + row(p) * l.ldz, out.n, l.F, z);
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             float y = l.scale * act_of<sizeof(T) == 2>(l.act, z.v[k]);
@@ -88,7 +90,7 @@ __device__ __forceinline__ void layer_rows(const Layer &l, int m0, int n0, int i
             if (l.R) y += (float)r[p][k];
             z.v[k] = y;
         }
-        store_f8((T *)l.Y + row(p) * l.ldy, out.n, l.F, z);
+        store8((T *)l.Y + row(p) * l.ldy, out.n, l.F, z);
     }
 }
 
@@ -264,7 +266,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
         if constexpr (P == 2) {
             constexpr int HELD = 8;   // 256 columns each: longer rows that a wave's registers hold are read once
             floatx4 v[HELD];
-            // 200 x 2048 -> 8192 71 -> 64 us, 777 x 1001 -> 2003 31.6 -> 30.2; shorter rows, in the loop below as in registers, 118 | 121 us at 4000 x 768 -> 3000
+            // 200 x 2048 -> 8192 71 -> 64 us, 777 x 1001 -> 2003 31.6 -> 30.2; shorter rows are no faster from registers (4000 x 768 -> 3000 118 | 121)
             const bool held = a.D > 768 && a.D <= 256 * HELD;
             unsigned m = 0;
             const auto most = [&](floatx4 y) {

@@ -4,9 +4,12 @@
 //
 // A first pass bounds dZ's largest magnitude, which sets the power of two that its planes are scaled by; a second one stores it as
 // one f16 plane (f16 gradients) or two (f32 ones), which both products then read (plane_gemm.h), also writes dU and
-// leaves db's sums of 32 rows. f32 X and W are scanned with it and packed as two planes; f16 ones are read as they lie where their
+// leaves db's sums of up to 64 rows. f32 X and W are scanned with it and packed as two planes; f16 ones are read as they lie where their
 // rows are aligned. Up to 128 rows (64 in f16) dX reads W once, as it lies (linear_ce_few.h). Sums run in a fixed order. Bound by the
 // matrix cores: two products of 2 N D F operations; dZ's passes move 10 (f16) to 28 (f32) bytes an element.
+//
+// f16 gradients of 8192 x 2048 -> 8192 with a factor: bound 61 us, dZ and dU 131, products 473 (1160 TFLOP/s), 588 together. dZ in one plane has the 11
+// bits that a program's own f16 dZ has (off by 2.9e-4 of the norm, 2.1e-4 of it the output's rounding); two planes, as for f32 gradients, 990 us.
 #include "linear.h"
 
 #include <string.h>
@@ -21,7 +24,11 @@ namespace ah {
 namespace {
 
 constexpr int kScans = 1024;   // workgroups that look for an array's largest magnitude, at most
-constexpr int kRows = 32, kFewRows = 8;   // rows of a block of dZ: fewer where those blocks would not fill the chip (300 x 1024 -> 1024 29 -> 23 us)
+// Rows of a block of dZ: 64, or fewer where those blocks would not fill the chip (300 x 1024 -> 1024 in 8 rather than 32: 29 -> 23 us).
+int block_rows(int Np, int Fp) {
+    const int64_t blocks = (int64_t)(Np / 64) * ((Fp + 511) / 512);
+    return blocks >= 512 ? 64 : blocks >= 128 ? 32 : 8;
+}
 
 struct GradIn {
     int N, D, F, act;
@@ -168,7 +175,7 @@ __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArg
                     f8 v = {}, du;
                     if (m < g.N && n < g.F) {
                         v = dz_of<T>(g, line[b], du);
-                        if (a.dU) store_f8((T *)a.dU + (long)m * a.lddu, n, g.F, du);
+                        if (a.dU) store8((T *)a.dU + (long)m * a.lddu, n, g.F, du);
 #pragma unroll
                         for (int c = 0; c < 8; c++) col.v[c] += v.v[c];
                     }
@@ -257,8 +264,8 @@ __device__ __forceinline__ void product_rows(const ProductArgs &a, int m0, int n
         f8 v = out.get(p);
 #pragma unroll
         for (int k = 0; k < 8; k++) v.v[k] = ldexpf(v.v[k], e);
-        if (a.out16) store_f8((half_t *)a.C + m * a.ldc, out.n, a.N, v);
-        else store_f8((float *)a.C + m * a.ldc, out.n, a.N, v);
+        if (a.out16) store8((half_t *)a.C + m * a.ldc, out.n, a.N, v);
+        else store8((float *)a.C + m * a.ldc, out.n, a.N, v);
     }
 }
 
@@ -458,7 +465,7 @@ Layout layout(const ah_linear_grad_desc &d) {
     l.Fp = (d.F + 63) & ~63;
     l.Dp = (d.D + 63) & ~63;
     l.products = d.dX || d.dW;
-    l.zrows = (int64_t)(l.Np / kRows) * ceil_div(l.Fp, 512) < 256 ? kFewRows : kRows;
+    l.zrows = block_rows(l.Np, l.Fp);
     if (d.dX && d.N <= (f16 ? kFewF16 : kFewF32) && d.D >= 8) l.few = d.N <= 16 ? 1 : d.N <= 64 ? 4 : 8;
     l.pack_x = d.dW && (!f16 || !rows_aligned(d.X, d.ldx, d.D));
     l.pack_w = d.dX && !l.few && (!f16 || !rows_aligned(d.W, d.ldw, d.D));

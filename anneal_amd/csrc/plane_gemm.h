@@ -211,7 +211,7 @@ struct Tile {
     static constexpr int BM = BM_, BN = BN_, WVM = WVM_, WVN = WVN_, TA = TA_, TB = TB_, PA = PA_, PB = PB_, NS = NS_;
     static constexpr int NW = WVM * WVN, NT = 64 * NW, WM = BM / WVM, WN = BN / WVN, FA = WM / 16, FB = WN / 16;
     static constexpr int BK = PA == 1 && PB == 1 ? 64 : 32;
-    static constexpr int ABYTES = BM * BK * PA * 2, STAGE = ABYTES + BN * BK * PB * 2, SMEM = PA == 1 && PB == 1 && NW == 8 ? 5 * ABYTES : NS * STAGE;   // contract_ring's five
+    static constexpr int ABYTES = BM * BK * PA * 2, STAGE = ABYTES + BN * BK * PB * 2, SMEM = PA == 1 && PB == 1 && NW == 8 ? 5 * ABYTES : NS * STAGE;   // (contract's five buffers)
     using FetchA = PFetch<BM, TA, PA, BK, NW>;
     using FetchB = PFetch<BN, TB, PB, BK, NW>;
     using FragA = PFrag<BM, TA, PA, BK>;
@@ -315,10 +315,9 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
     constexpr std::integral_constant<int, FB *(C::TB ? 2 : 1)> NRB{};                                // of B's,
     constexpr std::integral_constant<int, decltype(NRA)::value + decltype(NRB)::value> NRAB{};       // of both
     // the last group of stage t, with the refill of its buffer spread between the MFMAs (the tail re-fetches the last stage into
-    // idle buffers, so that the number of loads in flight stays the same). One plane by one, whose stage is the shortest: a load every second
-    // MFMA gives them half a group more to arrive in (8192 x 4096 -> 16384 988 -> 967 us; every MFMA 974)
+    // idle buffers, so that the number of loads in flight stays the same).
     auto mma_refill = [&](h8 (&a)[FA], h8 (&b)[FB], int t, int buf) {
-        constexpr int NM = FA * FB, EVEN = NM >= PERS ? NM / PERS : 1, STEP = C::PA == 1 && C::PB == 1 && EVEN > 2 ? 2 : EVEN, EACH = NM >= PERS ? 1 : (PERS + NM - 1) / NM;
+        constexpr int NM = FA * FB, STEP = NM >= PERS ? NM / PERS : 1, EACH = NM >= PERS ? 1 : (PERS + NM - 1) / NM;
         const int tr = min(t + NS, nk - 1);
         __builtin_amdgcn_sched_barrier(0);
         int f = 0;
@@ -352,7 +351,10 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
         h8 a0[FA], a1[FA], b0[FB], b1[FB];
         const auto next = [](int b, int by) { return b + by >= 5 ? b + by - 5 : b + by; };
         const auto load_a = [&](int f, int t, int buf) { fa.issue(f, Ab + (kt0 + min(t, nk - 1)) * da, A.ld, BK, lds + buf * ABYTES, wave_u, lane); };
-        const auto load_b = [&](int f, int t, int buf) { fb.issue(f, Bb + (BLOCKS && C::TB == 1 ? stored((kt0 + min(t, nk - 1)) * BK) : (kt0 + min(t, nk - 1)) * db), B.ld, B.k - (kt0 + min(t, nk - 1)) * BK, lds + buf * ABYTES, wave_u, lane); };
+        const auto load_b = [&](int f, int t, int buf) {
+            const int kt = kt0 + min(t, nk - 1);
+            fb.issue(f, Bb + (BLOCKS && C::TB == 1 ? stored(kt * BK) : kt * db), B.ld, B.k - kt * BK, lds + buf * ABYTES, wave_u, lane);
+        };
         // the MFMAs of one k-step, the reads of the next one (k-step s of the buffers at A and B) and four loads
         const auto half = [&](h8 (&a)[FA], h8 (&b)[FB], h8 (&an)[FA], h8 (&bn)[FB], int bufa, int bufb, int s, auto load) {
             uint32_t at = ra.first + bufa * ABYTES, bt = rb.first + bufb * ABYTES;

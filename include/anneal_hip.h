@@ -419,8 +419,9 @@ int ah_muon_step(ah_device *dev, const ah_muon_desc *d);
  *   Z = X W^T + bias,  Y = R + scale act(Z) U        (elementwise; bias, U, R may be null: 0, 1, 0)
  * act: ReLU, GELU by erf or by tanh(sqrt(2/pi) (z + 0.044715 z^3)), SiLU z / (1 + exp(-z)). Z may be null; a backward pass needs it.
  * dtype (all arrays) AH_F32 or AH_F16; everything is computed in f32 from an f32 Z and each output rounded once. f32 operands take part in
- * the product with 22 bits of each value (less below 2^-14 of its row's largest magnitude), or with all 24 where there are at most 64
- * rows. Y may be R. What is not finite in a row of X or W makes that row or column of the outputs infinite or NaN, and no other.
+ * the product with 22 bits of each value (less below 2^-14 of its row's largest magnitude), or with all 24 where there are at most 128
+ * rows of 8 features or more. Y may be R. What is not finite in a row of X or W makes that row or column of the outputs infinite or NaN, and no
+ * other.
  * N to 2^21, D and F to 2^20. Row strides ld* are in elements. */
 enum { AH_ACT_NONE = 0, AH_ACT_RELU = 1, AH_ACT_GELU = 2, AH_ACT_GELU_TANH = 3, AH_ACT_SILU = 4 };
 typedef struct {
@@ -511,7 +512,8 @@ int ah_residual_norm(ah_device *dev, const ah_residual_norm_desc *d);
  *   t = dH_out + pre'(dO),  dH = skip t,  dY = post'(scale gate t),  dgate = sum over its rows of scale t post(Y)
  * and the weights' gradients, sums over all rows. Null outputs are not computed. dgate is of dtype, the weights' gradients are
  * f32. Y is needed for dgate and where post is not none, H_out where pre is not none. Sums over rows run in a fixed order: results repeat
- * bit for bit. dH may be dH_out. */
+ * bit for bit. dH may be dH_out. A row's sums hold products of a gradient's entry with Y's and H_out's (less their means), gate and weights, in
+ * f32: where those are past its range, so is the row. */
 typedef struct {
     int32_t dtype, res_dtype;
     int32_t N, D;

@@ -224,3 +224,26 @@ def test_gradients_against_differences(dev):
         want = (values[0] - values[1]) / (2 * h)
         noise = 2.0 ** -21 * 8 * (np.linalg.norm(c.dH_out) + np.linalg.norm(c.dO)) / h
         assert abs(float((g[grad].reshape(base.shape) * d).sum()) - want) <= noise + h * h * 16, name
+
+
+@pytest.mark.parametrize("kinds", [(RMS, RMS), (LAYER, LAYER), (NONE, RMS), (LAYER, NONE)], ids=lambda k: "%d_%d" % k)
+@pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** 40])
+@pytest.mark.parametrize("shape", [(9, 100), (9, 1001), (3, 5000)], ids=lambda s: "%dx%d" % s)
+def test_sizes_of_gradients(dev, shape, size, kinds):
+    """Gradients far from 1 beside a stream and a branch of 2^10 (f32): a row's sums of products keep to the bounds of one norm after the other."""
+    c = Case(*shape, post=kinds[0], pre=kinds[1], per=2)
+    c.H, c.Y = c.H * np.float32(2.0 ** 10), c.Y * np.float32(2.0 ** 10)
+    c.dH_out = c.dH_out * np.float32(size)
+    if c.dO is not None:
+        c.dO = c.dO * np.float32(size)
+    O.compare(c.backward(dev), c.gradients())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("D", [8193, 12000, 16384, 16385])
+def test_two_groups_of_columns(dev, D, types):
+    """Rows past 8192 columns, held in registers up to 16384, and the first that is not."""
+    c = Case(3, D, types=types, post=RMS, pre=LAYER, per=2)
+    O.compare(c.forward(dev, gap=1), c.expected())
+    O.compare(c.forward(dev, gap=1, in_place=True), c.expected())
+    O.compare(c.backward(dev, gap=1, in_place=True), c.gradients())

@@ -2,9 +2,12 @@
 //
 //   dZ = s dY U act'(Z),  dX = dZ W,  dW = dZ^T X,  db = sum_n dZ,  dU = s dY act(Z)
 //
-// A first pass bounds dZ's largest magnitude, which sets the power of two that its planes are scaled by; a second one stores it as
+// A first pass finds dZ's largest magnitude, which sets the power of two that its planes are scaled by; a second one stores it as
 // one f16 plane (f16 gradients) or two (f32 ones), which both products then read (plane_gemm.h), also writes dU and
-// leaves db's sums of up to 64 rows. f32 X and W are scanned with it and packed as two planes; f16 ones are read as they lie where their
+// leaves db's sums of up to 64 rows. Where dZ is large the first pass reads neither Z nor evaluates an activation: it bounds dZ by |s dY U| times
+// the largest slope. What is large where the activation is off makes that bound as loose as it likes, so the second pass finds
+// the true magnitude, and where the bound has cost the planes bits a third launch stores them again (else it returns at once: 4 us, where reading Z
+// for the bound as well took 20 of 588 and 28 of 332). f32 X and W are scanned with it and packed as two planes; f16 ones are read as they lie where their
 // rows are aligned. Up to 128 rows (64 in f16) dX reads W once, as it lies (linear_ce_few.h). Sums run in a fixed order. Bound by the
 // matrix cores: two products of 2 N D F operations; dZ's passes move 10 (f16) to 28 (f32) bytes an element.
 //
@@ -70,7 +73,9 @@ __device__ __forceinline__ f8 dz_of(const GradIn &g, const Line<T> &l, f8 &du) {
 
 struct ScanArgs {
     int zblocks, xblocks, wblocks;   // workgroups of each array, in this order
+    int exact;                       // dZ's own magnitudes, not bounds
     unsigned *maxes;                 // [3][kScans]
+    unsigned *top;                   // bits of dZ's largest magnitude, for the second pass to raise
 };
 template <class T>
 __device__ __forceinline__ unsigned max8(unsigned m, const T &v) {
@@ -78,20 +83,27 @@ __device__ __forceinline__ unsigned max8(unsigned m, const T &v) {
     for (int k = 0; k < 8; k++) m = max(m, pg::magnitude(__float_as_uint((float)v[k])));
     return m;
 }
-// A wave a stretch of 2048 values of a row. dZ's magnitude is bounded by that of s dY U times the largest slope: neither Z is read for it nor
-// an activation evaluated, and where the bound is loose by 2^n the planes lose n of the 29 (one plane) or 18 binades that they have to spare.
+// The larger of m and |v|; infinities and NaN are passed over: v + 0 v is NaN then, which fmaxf drops.
+__device__ __forceinline__ float max_finite(float m, float v) { return fmaxf(m, fabsf(fmaf(v, 0.0f, v))); }
+
+// A wave a stretch of 2048 values of a row, or of 512 where it evaluates dZ.
 template <class T>
 __global__ __launch_bounds__(256) void linear_grad_scan_kernel(GradIn g, ScanArgs a) {
     __shared__ unsigned red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, which = (int)blockIdx.x < a.zblocks ? 0 : (int)blockIdx.x < a.zblocks + a.xblocks ? 1 : 2;
     const int b = blockIdx.x - (which == 0 ? 0 : which == 1 ? a.zblocks : a.zblocks + a.xblocks), blocks = which == 0 ? a.zblocks : which == 1 ? a.xblocks : a.wblocks;
-    const int width = which == 0 ? g.F : g.D, segs = (width + 2047) / 2048;
+    const int width = which == 0 ? g.F : g.D, stretch = which == 0 && a.exact ? 512 : 2048, segs = (width + stretch - 1) / stretch;
     const long rows = which == 2 ? g.F : g.N;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.top = 0;
     unsigned m = 0;
     for (long q = (long)b * 4 + wave; q < rows * segs; q += (long)blocks * 4) {
         const long r = q / segs;
-        const int c0 = (int)(q - r * segs) * 2048 + lane * 8;
-        if (which == 0) {
+        const int c0 = (int)(q - r * segs) * stretch + lane * 8;
+        if (which == 0 && a.exact) {
+            if (c0 >= width) continue;
+            f8 du;
+            m = max8(m, dz_of<T>(g, load_line<T>(g, r, c0), du).v);
+        } else if (which == 0) {
             typename Raw8<T>::type dy[4] = {}, u[4] = {};
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -100,13 +112,16 @@ __global__ __launch_bounds__(256) void linear_grad_scan_kernel(GradIn g, ScanArg
                 if (g.U) u[k] = load_raw8((const T *)g.U + r * g.ldu, c0 + k * 512, width);
             }
             const float s = g.scale * slope_bound(g.act);
+            float top = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                float v[8];
+            for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = s * (float)dy[k][e] * (g.U ? (float)u[k][e] : 1.0f);
-                m = max8(m, v);
-            }
+                for (int e = 0; e < 8; e++) {
+                    const float v = s * (float)dy[k][e] * (g.U ? (float)u[k][e] : 1.0f);
+                    top = g.act == AH_ACT_NONE ? max_finite(top, v) : fmaxf(top, fabsf(v));   // (without an activation it is dZ)
+                }
+            // a bound past f32's range counts as its largest value: dZ may be finite, and the second pass will tell
+            m = max(m, __float_as_uint(fminf(top, 0x1.fffffep127f)));
         } else {
             const float *p = which == 1 ? (const float *)g.X + r * g.ldx : (const float *)g.W + r * g.ldw;
             raw8_f32 v[4] = {};
@@ -144,57 +159,75 @@ struct PackArgs {
     float *dbpart;             // [row block][F] or null
     int Np, Fp, Dp;
     int zblocks, zcols, zrows, rest;  // workgroups for dZ (zcols a block of zrows rows), and for X's and W's rows
-    int *exps;                 // [3]: exponents of dZ, X and W
+    int *exps;                 // [4]: exponents of dZ, X and W; dZ's from the bound
+    bool track;                // dZ's exponent is from a bound: its largest magnitude is wanted
 };
+// Binades by which dZ's largest magnitude may lie below 2^14: two planes hold 22 bits down to 2^-3, and they are to do so down to 2^-14 of the
+// largest. A bound over many entries is within two binades where their slopes differ, as the slopes of a layer's features do.
+constexpr int kSlack = 3;
+
+// dZ's block zb: zrows rows by 512 columns, a thread eight columns of every fourth row. AGAIN: dZ alone. Returns this thread's largest magnitude.
+template <class T, int P, bool AGAIN>
+__device__ __forceinline__ float pack_dz(const GradIn &g, const PackArgs &a, int zb, int e) {
+    __shared__ float red[3][64][8];
+    const int rb = zb / a.zcols, n = (zb - rb * a.zcols) * 512 + (threadIdx.x & 63) * 8, w = threadIdx.x >> 6;
+    constexpr int B = sizeof(T) == 2 ? 4 : 2;   // rows whose loads are in flight together
+    f8 col = {};
+    float top = 0.0f;
+    if (n < a.Fp) {
+        for (int k0 = w; k0 < a.zrows; k0 += 4 * B) {
+            Line<T> line[B] = {};
+#pragma unroll
+            for (int b = 0; b < B; b++) {
+                const int m = rb * a.zrows + k0 + 4 * b;
+                if (k0 + 4 * b < a.zrows && m < g.N && n < g.F) line[b] = load_line<T>(g, m, n);
+            }
+#pragma unroll
+            for (int b = 0; b < B; b++) {
+                if (k0 + 4 * b >= a.zrows) break;
+                const int m = rb * a.zrows + k0 + 4 * b;
+                f8 v = {}, du;
+                if (m < g.N && n < g.F) {
+                    v = dz_of<T>(g, line[b], du);
+                    if (!AGAIN && a.dU) store8((T *)a.dU + (long)m * a.lddu, n, g.F, du);
+#pragma unroll
+                    for (int c = 0; c < 8; c++) col.v[c] += v.v[c];
+#pragma unroll
+                    for (int c = 0; c < 8; c++) top = AGAIN ? 0.0f : max_finite(top, v.v[c]);
+                }
+                if (!a.dZ) continue;
+#pragma unroll
+                for (int c = 0; c < 8; c++) v.v[c] = n + c < g.F ? ldexpf(v.v[c], e) : 0.0f;
+                plane_store8<P>(a.dZ + pg::panel_at<P>(a.Np, m, n), v);
+            }
+        }
+    }
+    if (AGAIN || !a.dbpart) return top;
+    if (w > 0)
+#pragma unroll
+        for (int c = 0; c < 8; c++) red[w - 1][threadIdx.x & 63][c] = col.v[c];
+    __syncthreads();
+    if (w == 0)
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            if (n + c < g.F) a.dbpart[(long)rb * g.F + n + c] = col.v[c] + red[0][threadIdx.x][c] + red[1][threadIdx.x][c] + red[2][threadIdx.x][c];
+    return top;
+}
+
 // P: planes of dZ; PO: of X and W.
 template <class T, int P, int PO>
 __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArgs a, ScanArgs s) {
-    __shared__ float red[3][64][8];
     int e[3] = {};
     if (s.zblocks) e[0] = pg::plane_exp(join_maxes(s.maxes, s.zblocks));
     if (s.xblocks) e[1] = pg::plane_exp(join_maxes(s.maxes + kScans, s.xblocks));
     if (s.wblocks) e[2] = pg::plane_exp(join_maxes(s.maxes + 2 * kScans, s.wblocks));
-    if (blockIdx.x == 0 && threadIdx.x < 3) a.exps[threadIdx.x] = threadIdx.x == 0 ? e[0] : threadIdx.x == 1 ? e[1] : e[2];
-    if ((int)blockIdx.x < a.zblocks) {   // zrows rows by 512 columns: a thread has eight columns of every fourth row
+    if (blockIdx.x == 0 && threadIdx.x < 4) a.exps[threadIdx.x] = threadIdx.x % 3 == 0 ? e[0] : threadIdx.x == 1 ? e[1] : e[2];
+    if ((int)blockIdx.x < a.zblocks) {
         // the last rows first, which the scan has left in the caches (16384 x 1024 -> 4096, both passes and the products: 420 -> 414 us)
-        const int zb = a.zblocks - 1 - (int)blockIdx.x, rb = zb / a.zcols, n = (zb - rb * a.zcols) * 512 + (threadIdx.x & 63) * 8, w = threadIdx.x >> 6;
-        constexpr int B = sizeof(T) == 2 ? 4 : 2;   // rows whose loads are in flight together
-        f8 col = {};
-        if (n < a.Fp) {
-            for (int k0 = w; k0 < a.zrows; k0 += 4 * B) {
-                Line<T> line[B] = {};
-#pragma unroll
-                for (int b = 0; b < B; b++) {
-                    const int m = rb * a.zrows + k0 + 4 * b;
-                    if (k0 + 4 * b < a.zrows && m < g.N && n < g.F) line[b] = load_line<T>(g, m, n);
-                }
-#pragma unroll
-                for (int b = 0; b < B; b++) {
-                    if (k0 + 4 * b >= a.zrows) break;
-                    const int m = rb * a.zrows + k0 + 4 * b;
-                    f8 v = {}, du;
-                    if (m < g.N && n < g.F) {
-                        v = dz_of<T>(g, line[b], du);
-                        if (a.dU) store8((T *)a.dU + (long)m * a.lddu, n, g.F, du);
-#pragma unroll
-                        for (int c = 0; c < 8; c++) col.v[c] += v.v[c];
-                    }
-                    if (!a.dZ) continue;
-#pragma unroll
-                    for (int c = 0; c < 8; c++) v.v[c] = n + c < g.F ? ldexpf(v.v[c], e[0]) : 0.0f;
-                    plane_store8<P>(a.dZ + pg::panel_at<P>(a.Np, m, n), v);
-                }
-            }
-        }
-        if (!a.dbpart) return;
-        if (w > 0)
-#pragma unroll
-            for (int c = 0; c < 8; c++) red[w - 1][threadIdx.x & 63][c] = col.v[c];
-        __syncthreads();
-        if (w == 0)
-#pragma unroll
-            for (int c = 0; c < 8; c++)
-                if (n + c < g.F) a.dbpart[(long)rb * g.F + n + c] = col.v[c] + red[0][threadIdx.x][c] + red[1][threadIdx.x][c] + red[2][threadIdx.x][c];
+        unsigned top = __float_as_uint(pack_dz<T, P, false>(g, a, a.zblocks - 1 - (int)blockIdx.x, e[0]));
+        if (!a.track) return;
+        for (int o = 32; o >= 1; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
+        if ((threadIdx.x & 63) == 0 && top > __hip_atomic_load(s.top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(s.top, top);   // any order: the same
         return;
     }
     constexpr int ESZ = PO == 1 ? 2 : 4;
@@ -203,6 +236,15 @@ __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArg
         if (q < xrows) pg::pack_row<PO>(a.Xp, g.N, q, (const char *)g.X + q * g.ldx * ESZ, g.D, a.Dp, e[1]);
         else pg::pack_row<PO>(a.Wp, g.F, q - xrows, (const char *)g.W + (q - xrows) * g.ldw * ESZ, g.D, a.Dp, e[2]);
     }
+}
+
+// dZ's planes again, by its own magnitude, where the bound's exponent has cost them bits.
+template <class T, int P>
+__global__ __launch_bounds__(256) void linear_grad_again_kernel(GradIn g, PackArgs a, const unsigned *top) {
+    const int e = pg::plane_exp(*top);
+    if (*top == 0 || e <= a.exps[3] + kSlack) return;
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.exps[0] = e;
+    for (int zb = blockIdx.x; zb < a.zblocks; zb += gridDim.x) pack_dz<T, P, true>(g, a, zb, e);
 }
 
 // ── the products ───────────────────────────────────────────────────────────────
@@ -448,8 +490,9 @@ struct Layout {
     int P, PO;                 // planes of dZ; of X and W
     int Np, Fp, Dp, few, zrows;
     bool products, pack_x, pack_w;
+    bool exact, track;         // dZ's magnitudes are scanned for, or bounded and found by the second pass
     Cuts cuts;
-    int64_t exps, maxes, dbpart, dZ, Xp, Wp, sums, wsums, total;
+    int64_t exps, top, maxes, dbpart, dZ, Xp, Wp, sums, wsums, total;
 };
 
 pg::Work few_work(const ah_linear_grad_desc &d, const Layout &l) {
@@ -466,6 +509,8 @@ Layout layout(const ah_linear_grad_desc &d) {
     l.Dp = (d.D + 63) & ~63;
     l.products = d.dX || d.dW;
     l.zrows = block_rows(l.Np, l.Fp);
+    l.exact = d.act != AH_ACT_NONE && (int64_t)d.N * ((d.F + 511) / 512) <= 4 * kScans;   // (without an activation the bound is exact)
+    l.track = l.products && d.act != AH_ACT_NONE && !l.exact;
     if (d.dX && d.N <= (f16 ? kFewF16 : kFewF32) && d.D >= 8) l.few = d.N <= 16 ? 1 : d.N <= 64 ? 4 : 8;
     l.pack_x = d.dW && (!f16 || !rows_aligned(d.X, d.ldx, d.D));
     l.pack_w = d.dX && !l.few && (!f16 || !rows_aligned(d.W, d.ldw, d.D));
@@ -476,6 +521,7 @@ Layout layout(const ah_linear_grad_desc &d) {
         return o;
     };
     l.exps = take(16);
+    l.top = take(4);
     l.maxes = take(3 * kScans * 4);
     if (d.dbias) l.dbpart = take((int64_t)(l.Np / l.zrows) * d.F * 4);
     if (l.products) l.dZ = take((int64_t)l.Np * l.Fp * 2 * l.P);
@@ -553,12 +599,14 @@ template <class T, int P, int PO>
 void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     char *ws = (char *)d.ws;
     const GradIn g{d.N, d.D, d.F, d.act, d.scale, d.dY, d.Z, d.U, d.lddy, d.ldz, d.ldu, d.X, d.W, d.ldx, d.ldw};
-    const auto scans = [](int64_t rows, int64_t width) { return (int)std::min<int64_t>((rows * ((width + 2047) / 2048) + 3) / 4, kScans); };
+    const auto scans = [](int64_t rows, int64_t width, int stretch = 2048) { return (int)std::min<int64_t>((rows * ((width + stretch - 1) / stretch) + 3) / 4, kScans); };
     ScanArgs sc{};
-    sc.zblocks = l.products ? scans(d.N, d.F) : 0;
+    sc.exact = l.exact;
+    sc.zblocks = l.products ? scans(d.N, d.F, l.exact ? 512 : 2048) : 0;
     sc.xblocks = l.pack_x && PO == 2 ? scans(d.N, d.D) : 0;
     sc.wblocks = l.pack_w && PO == 2 ? scans(d.F, d.D) : 0;
     sc.maxes = (unsigned *)(ws + l.maxes);
+    sc.top = (unsigned *)(ws + l.top);
     if (l.products) hipLaunchKernelGGL(linear_grad_scan_kernel<T>, dim3((unsigned)(sc.zblocks + sc.xblocks + sc.wblocks)), dim3(256), 0, s, g, sc);
 
     PackArgs p{};
@@ -576,7 +624,9 @@ void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     p.zblocks = l.Np / l.zrows * p.zcols;
     p.rest = (int)std::min<int64_t>(((l.pack_x ? d.N : 0) + (int64_t)(l.pack_w ? d.F : 0) + 3) / 4, 4096);
     p.exps = (int *)(ws + l.exps);
+    p.track = l.track;
     hipLaunchKernelGGL((linear_grad_pack_kernel<T, P, PO>), dim3((unsigned)(p.zblocks + p.rest)), dim3(256), 0, s, g, p, sc);
+    if (l.track) hipLaunchKernelGGL((linear_grad_again_kernel<T, P>), dim3((unsigned)std::min(p.zblocks, 1024)), dim3(256), 0, s, g, p, sc.top);
     PairArgs a{};
     a.x.ea = a.w.ea = p.exps;
     a.x.out16 = a.w.out16 = d.grad_dtype == AH_F16;

@@ -1,0 +1,115 @@
+"""ah_linear and ah_linear_grad where values of one array differ in size by far more than a plane's bits (GPU). Bounds as derived in
+block_oracle.py, taken as they stand."""
+import numpy as np
+import pytest
+
+import block_oracle as O
+from anneal_amd import _lib as L
+from test_gpu_linear import IDS, TYPES, Case
+
+pytestmark = pytest.mark.gpu
+KINDS = [L.ACT_RELU, L.ACT_GELU, L.ACT_GELU_TANH, L.ACT_SILU]
+OFF = 11   # a feature that is off for every row
+BIG = {(L.AH_F32, L.AH_F32): 1e4, (L.AH_F16, L.AH_F16): 3e4, (L.AH_F16, L.AH_F32): 4e3}
+SMALL = {(L.AH_F32, L.AH_F32): 1e-3, (L.AH_F16, L.AH_F16): 1e-2, (L.AH_F16, L.AH_F32): 1e-2}
+
+
+def inactive(N, types, kind, z, factor=True, D=96, F=64):
+    """dY and U are large where the activation is off, and nowhere else."""
+    c = Case(N, D, F, dtype=types[0], grad_dtype=types[1], kind=kind, bias=False, factor=factor, res=False)
+    c.dY = (c.dY * SMALL[types]).astype(c.dY.dtype)
+    c.dY[:, OFF], c.Z[:, OFF] = BIG[types], z
+    if factor:
+        c.U[:, OFF] = BIG[types]
+    return c
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("N", [1, 30, 200, 4200])   # 4200: dZ is bounded first, and stored again where the bound is loose
+@pytest.mark.parametrize("factor", [True, False])
+def test_what_is_off_does_not_set_the_scale(dev, N, kind, types, factor):
+    """At z = -200 every slope but ReLU's is under 2^-280, in f32 as in f16 0: the gradients are those of a call whose dY is 0 there."""
+    c = inactive(N, types, kind, -200.0, factor)
+    got = c.backward(dev)
+    c.dY[:, OFF] = 0
+    O.compare(got, c.gradients())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("z", [-4.0, -9.0, -30.0])
+@pytest.mark.parametrize("N", [30, 200, 4200])
+def test_what_is_nearly_off(dev, N, z, kind, types):
+    c = inactive(N, types, kind, z)
+    O.compare(c.backward(dev), c.gradients())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("N", [30, 200, 4200])
+def test_one_entry_that_is_off(dev, N, types):
+    """One large entry under ReLU, in a row and a column whose other entries are live."""
+    c = Case(N, 96, 64, dtype=types[0], grad_dtype=types[1], kind=L.ACT_RELU, factor=False)
+    c.dY[5, 7], c.Z[5, 7] = 2.0 ** 30 if types[0] == L.AH_F32 else 6e4, -1.0
+    c.dY[np.arange(N) != 5] *= c.dY.dtype.type(2.0 ** -10)
+    O.compare(c.backward(dev), c.gradients())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("kind", [L.ACT_NONE, L.ACT_RELU, L.ACT_SILU])
+@pytest.mark.parametrize("apart", [20, 30])
+@pytest.mark.parametrize("N", [30, 200, 4200])
+def test_rows_far_apart(dev, N, apart, kind, types):
+    """Rows of dY 2^20 and 2^30 apart (f16: what its range has): what is under 2^-39 of the largest dZ may go."""
+    c = Case(N, 96, 64, dtype=types[0], grad_dtype=types[1], kind=kind, factor=False)
+    size = np.float32(2.0) ** -np.linspace(0, apart, N).astype(np.float32)[:, None]
+    c.dY = (c.dY.astype(np.float32) * size).astype(c.dY.dtype)
+    O.compare(c.backward(dev), c.gradients())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("N", [30, 200, 4200])
+def test_a_gradient_near_the_end_of_f32(dev, N, kind):
+    """dZ fits f32 where dY times the largest slope of the GELUs does not."""
+    c = Case(N, 96, 64, kind=kind, bias=False, factor=False, res=False, scale=1.0)
+    c.W = (c.W * 2.0 ** -6).astype(np.float32)
+    c.X = (c.X * 2.0 ** -20).astype(np.float32)
+    c.dY[3, 4], c.Z[3, 4] = 3.3e38, 0.25
+    O.compare(c.backward(dev), c.gradients())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [64.0, 2.0 ** -6])
+def test_the_largest_in_any_place(dev, size, kind, types):
+    """The largest dZ early and late, with larger ones that are off before it and after it, in more rows and columns than the scan's waves see
+    at once; and the same bits again."""
+    for at in (0, 701, 2999):
+        c = Case(3000, 8, 2100, dtype=types[0], grad_dtype=types[1], kind=kind, factor=False)
+        c.dY = (c.dY * 2.0 ** -8).astype(c.dY.dtype)
+        c.Z[at, 2050], c.dY[at, 2050] = 3.0, size
+        for off in (17, 1500, 2700):
+            c.Z[off, ::5], c.dY[off, ::5] = -200.0, 3e4
+        got, again = c.backward(dev), c.backward(dev)
+        for off in (17, 1500, 2700):
+            c.dY[off, ::5] = 0
+        O.compare(got, c.gradients())
+        for k in got:
+            np.testing.assert_array_equal(got[k], again[k], err_msg=k)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("bad", [np.nan, np.inf], ids=str)
+@pytest.mark.parametrize("kind", [L.ACT_NONE, L.ACT_RELU, L.ACT_GELU])
+@pytest.mark.parametrize("N", [30, 4200])
+def test_what_is_not_finite_does_not_set_the_scale(dev, N, kind, bad, types):
+    clean = Case(N, 96, 64, dtype=types[0], grad_dtype=types[1], kind=kind)
+    clean.dY = (clean.dY * clean.dY.dtype.type(2.0 ** -8)).astype(clean.dY.dtype)
+    c = Case(N, 96, 64, dtype=types[0], grad_dtype=types[1], kind=kind)
+    c.dY = clean.dY.copy()
+    c.dY[4, 9] = bad
+    got, want = c.backward(dev), clean.gradients()
+    rows, cols = np.arange(N) != 4, np.arange(64) != 9
+    O.compare({"dX": got["dX"][rows], "dW": got["dW"][cols], "dU": got["dU"][rows]},
+              {"dX": tuple(v[rows] for v in want["dX"]), "dW": tuple(v[cols] for v in want["dW"]), "dU": tuple(v[rows] for v in want["dU"])})
+    assert not np.isfinite(got["dX"][4]).any() and not np.isfinite(got["dW"][9]).any()

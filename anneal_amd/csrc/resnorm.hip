@@ -264,10 +264,11 @@ struct Runs {
 };
 
 // What a row's gradients need of its sums:
-//   t = dh + c1 q - c2 h - c0,  c1 = r_h,  c2 = r_h^3 mean(q h),  c0 = r_h mean(q)
-//   dY = r_y p - px y - p1,     px = r_y^3 mean(p y),  p1 = r_y mean(p),  p = a t,  a = scale g w_post
-// (y, h less their means my, mh; c0, p1 of layer norms alone). The sums of p come from those of t's terms, so that all are taken at once:
-//   sum p y = sum a y dh + c1 sum a y q - c2 sum a y h - c0 sum a y,  and sum p likewise
+//   t = dh + c1 (q - c2 h) - c0,  c1 = r_h,  c2 = r_h (r_h mean(q h)),  c0 = r_h mean(q)
+//   dY = r_y (p - px y) - p1,     px = r_y (r_y mean(p y)),  p1 = r_y mean(p),  p = a t,  a = scale g w_post
+// (y, h less their means my, mh; c0, p1 of layer norms alone). c2 h and px y are as large as q and p whatever the rows' size; r^3 leaves f32's range where
+// y or h is past 2^42 or, with a small eps, below 2^-42. The sums of p come from those of t's terms, so that all are taken at once:
+//   sum p y = sum a y dh + c1 (sum a y q - c2 sum a y h) - c0 sum a y,  and sum p likewise
 struct RowTerms {
     float my, mh, ry, c1, c2, c0, px, p1;
 };
@@ -301,15 +302,15 @@ __device__ __forceinline__ RowTerms terms_of(const ah_residual_norm_grad_desc &d
     if (post) x.ry = 1.0f / sqrtf(s[0] * n + d.eps);
     if (pre) {
         x.c1 = 1.0f / sqrtf(s[1] * n + d.eps);
-        x.c2 = x.c1 * x.c1 * (x.c1 * (s[2] * n));
+        x.c2 = x.c1 * (x.c1 * (s[2] * n));
     }
-    float py = s[3] + x.c1 * s[4] - x.c2 * s[5];
+    float py = s[3] + x.c1 * (s[4] - x.c2 * s[5]);
     if constexpr (LAYER) {
         if (d.pre == AH_NORM_LAYER) x.c0 = x.c1 * (s[6] * n);
         py -= x.c0 * s[11];
-        if (d.post == AH_NORM_LAYER) x.p1 = x.ry * n * (s[7] + x.c1 * s[8] - x.c2 * s[9] - x.c0 * s[10]);
+        if (d.post == AH_NORM_LAYER) x.p1 = x.ry * (n * (s[7] + x.c1 * (s[8] - x.c2 * s[9]) - x.c0 * s[10]));
     }
-    if (post) x.px = x.ry * x.ry * x.ry * (n * py);
+    if (post) x.px = x.ry * (x.ry * (n * py));
     return x;
 }
 template <int V>
@@ -430,7 +431,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR <= 64 ? 3 : 4) void resn
 #pragma unroll
             for (int k = 0; k < V; k++) {
                 tt.v[k] = dh.v[k];
-                if (pre) tt.v[k] += fmaf(-x.c2, h.v[k], x.c1 * q.v[k]) - x.c0;
+                if (pre) tt.v[k] += fmaf(x.c1, fmaf(-x.c2, h.v[k], q.v[k]), -x.c0);
                 sums.wpre.v[k] = fmaf(dO.v[k], x.c1 * h.v[k], sums.wpre.v[k]);
                 ty.v[k] = fmaf(tt.v[k], x.ry * y.v[k], ty.v[k]);
                 if constexpr (LAYER) ts.v[k] += tt.v[k];
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, TPR <= 64 ? 3 : 4) void resn
         if (d.dY && in) {
             const fN<V> gw = gain();
 #pragma unroll
-            for (int k = 0; k < V; k++) o.v[k] = fmaf(-x.px, y.v[k], x.ry * (gw.v[k] * tt.v[k])) - x.p1;
+            for (int k = 0; k < V; k++) o.v[k] = fmaf(x.ry, fmaf(-x.px, y.v[k], gw.v[k] * tt.v[k]), -x.p1);
             store_cols<T, V>((T *)d.dY + (long)r * d.lddy, c, D, o);
         }
         if (--left == 0 || r + 1 == b) {

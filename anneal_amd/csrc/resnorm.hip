@@ -75,15 +75,19 @@ __device__ __forceinline__ void row_sums(float (&s)[K], int &turn) {
     }
 }
 
+// A row whose mean square v (with eps) is past f32's range, or so small that the squares have lost bits, is scaled by a power of two before it is
+// squared again: |x| up to 2^128 to 2^52 at most, and from 2^-149 to below 2^-48 (where eps, below 2^-96 then, keeps its share) past 2^-59.
+__device__ __forceinline__ float rescale(float v) { return v < 0x1p-96f ? 0x1p90f : v < __builtin_inff() ? 1.0f : 0x1p-76f; }
+
 struct Stats {
-    float m, r;
+    float m, r, up;   // the norm is ((x - m) up) r
 };
 // Mean and inverse deviation of a row. each(f): f(c, a) for each of this thread's column groups. One pass for the sum, and one for layer
 // norms' squares about the mean.
 template <int TPR, class Each>
 __device__ __forceinline__ Stats stats1(int D, int kind, float eps, Each each, int &turn) {
     const float n = 1.0f / (float)D;
-    Stats S{};
+    Stats S{0.0f, 0.0f, 1.0f};
     float s[1] = {};
     if (kind == AH_NORM_LAYER) {
         each([&](int, const f8 &a) {
@@ -94,15 +98,22 @@ __device__ __forceinline__ Stats stats1(int D, int kind, float eps, Each each, i
         S.m = s[0] * n;
         s[0] = 0.0f;
     }
-    each([&](int c, const f8 &a) {
+    const auto square = [&] {
+        s[0] = 0.0f;
+        each([&](int c, const f8 &a) {
 #pragma unroll
-        for (int k = 0; k < kVec; k++) {
-            const float x = c + k < D ? a.v[k] - S.m : 0.0f;
-            s[0] = fmaf(x, x, s[0]);
-        }
-    });
-    row_sums<TPR>(s, turn);
-    S.r = 1.0f / sqrtf(s[0] * n + eps);
+            for (int k = 0; k < kVec; k++) {
+                const float x = c + k < D ? (a.v[k] - S.m) * S.up : 0.0f;
+                s[0] = fmaf(x, x, s[0]);
+            }
+        });
+        row_sums<TPR>(s, turn);
+        return fmaf(s[0], n, eps * S.up * S.up);
+    };
+    float v = square();
+    S.up = rescale(v);
+    if (S.up != 1.0f) v = square();
+    S.r = 1.0f / sqrtf(v);
     return S;
 }
 
@@ -149,13 +160,26 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR, G == 1 ? 8 : 4) void resnorm
 #pragma unroll
             for (int g = 0; g < G; g++) x[g] = less<V, true>(x[g], m, col(g), D);
         }
-        s[0] = 0.0f;
+        float up = 1.0f;
+        const auto square = [&] {
+            s[0] = 0.0f;
 #pragma unroll
-        for (int g = 0; g < G; g++)
+            for (int g = 0; g < G; g++)
 #pragma unroll
-            for (int k = 0; k < V; k++) s[0] = fmaf(x[g].v[k], x[g].v[k], s[0]);
-        row_sums<TPR>(s, turn);
-        const float r = 1.0f / sqrtf(s[0] * n + d.eps);
+                for (int k = 0; k < V; k++) s[0] = fmaf(x[g].v[k], x[g].v[k], s[0]);
+            row_sums<TPR>(s, turn);
+            return fmaf(s[0], n, d.eps * up * up);
+        };
+        float v = square();
+        up = rescale(v);
+        if (up != 1.0f) {   // the same in all of a row's threads
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int k = 0; k < V; k++) x[g].v[k] *= up;
+            v = square();
+        }
+        const float r = 1.0f / sqrtf(v);
 #pragma unroll
         for (int g = 0; g < G; g++) {
             const f8 ww = weights(w, g, 1.0f), bb = weights(b, g, 0.0f);
@@ -215,7 +239,7 @@ __global__ __launch_bounds__(kWideT) void resnorm_wide_kernel(ah_residual_norm_d
         const R *H = d.H ? (const R *)d.H + r * d.ldh : nullptr;
         const T *Y = d.Y ? (const T *)d.Y + r * d.ldy : nullptr;
         const T *G = d.gate ? (const T *)d.gate + (long)(d.rows_per_gate ? (int)r / d.rows_per_gate : 0) * d.ldgate : nullptr;
-        Stats P{0.0f, 1.0f}, Q{0.0f, 1.0f};
+        Stats P{0.0f, 1.0f, 1.0f}, Q{0.0f, 1.0f, 1.0f};
         if (d.post != AH_NORM_NONE) P = stats1<kWideT>(D, d.post, d.eps, [&](auto f) { groups([&](int c) { f(c, load8(Y, c, D)); }); }, turn);
         const auto sum_at = [&](int c) {
             f8 s = {};
@@ -224,7 +248,7 @@ __global__ __launch_bounds__(kWideT) void resnorm_wide_kernel(ah_residual_norm_d
                 if (d.post != AH_NORM_NONE) {
                     const f8 w = load8_or(pw, c, D, 1.0f), b = load8_or(pb, c, D, 0.0f);
 #pragma unroll
-                    for (int k = 0; k < kVec; k++) s.v[k] = fmaf((s.v[k] - P.m) * P.r, w.v[k], b.v[k]);
+                    for (int k = 0; k < kVec; k++) s.v[k] = fmaf((s.v[k] - P.m) * P.up * P.r, w.v[k], b.v[k]);
                 }
                 const f8 g = load8_or(G, c, D, 1.0f);
 #pragma unroll
@@ -244,7 +268,7 @@ __global__ __launch_bounds__(kWideT) void resnorm_wide_kernel(ah_residual_norm_d
             if (!d.O) return;
             const f8 w = load8_or(nw, c, D, 1.0f), b = load8_or(nb, c, D, 0.0f);
 #pragma unroll
-            for (int k = 0; k < kVec; k++) s.v[k] = fmaf((s.v[k] - Q.m) * Q.r, w.v[k], b.v[k]);
+            for (int k = 0; k < kVec; k++) s.v[k] = fmaf((s.v[k] - Q.m) * Q.up * Q.r, w.v[k], b.v[k]);
             store8((T *)d.O + r * d.ldo, c, D, s);
         });
     }
@@ -295,13 +319,15 @@ __device__ __forceinline__ void add_terms(float (&s)[kSums<LAYER>], const fN<V> 
         }
     }
 }
+// 1 / sqrt(v); NaN where v is past f32's range or below its normal numbers: not a gradient of 0.
+__device__ __forceinline__ float inverse(float v) { return v >= 0x1p-126f && v < __builtin_inff() ? 1.0f / sqrtf(v) : __builtin_nanf(""); }
 template <bool LAYER>
 __device__ __forceinline__ RowTerms terms_of(const ah_residual_norm_grad_desc &d, const float (&m)[2], const float (&s)[kSums<LAYER>], float n) {
     const bool pre = d.pre != AH_NORM_NONE, post = d.post != AH_NORM_NONE;
     RowTerms x{m[0], m[1], 1.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (post) x.ry = 1.0f / sqrtf(s[0] * n + d.eps);
+    if (post) x.ry = inverse(s[0] * n + d.eps);
     if (pre) {
-        x.c1 = 1.0f / sqrtf(s[1] * n + d.eps);
+        x.c1 = inverse(s[1] * n + d.eps);
         x.c2 = x.c1 * (x.c1 * (s[2] * n));
     }
     float py = s[3] + x.c1 * (s[4] - x.c2 * s[5]);

@@ -55,14 +55,15 @@ __device__ __forceinline__ Line<T> load_line(const GradIn &g, long n, int c) {
     if (g.U) l.u = load_raw8((const T *)g.U + n * g.ldu, c, g.F);
     return l;
 }
-// dZ and dU.
-template <class T>
+// dZ and dU; P: planes of dZ. One plane takes the activations' FAST forms: its dZ is rounded to f16 (db's terms with them: off by 2^-20, where
+// dY itself has f16's 2^-12).
+template <class T, int P>
 __device__ __forceinline__ f8 dz_of(const GradIn &g, const Line<T> &l, f8 &du) {
     f8 v;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
         float slope;
-        const float y = act_slope<sizeof(T) == 2>(g.act, (float)l.z[k], slope), t = g.scale * (float)l.dy[k];
+        const float y = act_slope<P == 1>(g.act, (float)l.z[k], slope), t = g.scale * (float)l.dy[k];
         v.v[k] = g.U ? t * slope * (float)l.u[k] : t * slope;
         du.v[k] = t * y;
     }
@@ -87,7 +88,7 @@ __device__ __forceinline__ unsigned max8(unsigned m, const T &v) {
 __device__ __forceinline__ float max_finite(float m, float v) { return fmaxf(m, fabsf(fmaf(v, 0.0f, v))); }
 
 // A wave a stretch of 2048 values of a row, or of 512 where it evaluates dZ.
-template <class T>
+template <class T, int P>
 __global__ __launch_bounds__(256) void linear_grad_scan_kernel(GradIn g, ScanArgs a) {
     __shared__ unsigned red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, which = (int)blockIdx.x < a.zblocks ? 0 : (int)blockIdx.x < a.zblocks + a.xblocks ? 1 : 2;
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(256) void linear_grad_scan_kernel(GradIn g, ScanArg
         if (which == 0 && a.exact) {
             if (c0 >= width) continue;
             f8 du;
-            m = max8(m, dz_of<T>(g, load_line<T>(g, r, c0), du).v);
+            m = max8(m, dz_of<T, P>(g, load_line<T>(g, r, c0), du).v);
         } else if (which == 0) {
             typename Raw8<T>::type dy[4] = {}, u[4] = {};
 #pragma unroll
@@ -188,7 +189,7 @@ __device__ __forceinline__ float pack_dz(const GradIn &g, const PackArgs &a, int
                 const int m = rb * a.zrows + k0 + 4 * b;
                 f8 v = {}, du;
                 if (m < g.N && n < g.F) {
-                    v = dz_of<T>(g, line[b], du);
+                    v = dz_of<T, P>(g, line[b], du);
                     if (!AGAIN && a.dU) store8((T *)a.dU + (long)m * a.lddu, n, g.F, du);
 #pragma unroll
                     for (int c = 0; c < 8; c++) col.v[c] += v.v[c];
@@ -607,7 +608,7 @@ void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     sc.wblocks = l.pack_w && PO == 2 ? scans(d.F, d.D) : 0;
     sc.maxes = (unsigned *)(ws + l.maxes);
     sc.top = (unsigned *)(ws + l.top);
-    if (l.products) hipLaunchKernelGGL(linear_grad_scan_kernel<T>, dim3((unsigned)(sc.zblocks + sc.xblocks + sc.wblocks)), dim3(256), 0, s, g, sc);
+    if (l.products) hipLaunchKernelGGL((linear_grad_scan_kernel<T, P>), dim3((unsigned)(sc.zblocks + sc.xblocks + sc.wblocks)), dim3(256), 0, s, g, sc);
 
     PackArgs p{};
     if (l.products) p.dZ = (half_t *)(ws + l.dZ);

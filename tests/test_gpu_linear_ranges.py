@@ -2,9 +2,11 @@
 block_oracle.py, taken as they stand."""
 import numpy as np
 import pytest
+from scipy.special import erfc
 
 import block_oracle as O
 from anneal_amd import _lib as L
+from block_oracle import U32
 from test_gpu_linear import IDS, TYPES, Case
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +115,33 @@ def test_what_is_not_finite_does_not_set_the_scale(dev, N, kind, bad, types):
     O.compare({"dX": got["dX"][rows], "dW": got["dW"][cols], "dU": got["dU"][rows]},
               {"dX": tuple(v[rows] for v in want["dX"]), "dW": tuple(v[cols] for v in want["dW"]), "dU": tuple(v[rows] for v in want["dU"])})
     assert not np.isfinite(got["dX"][4]).any() and not np.isfinite(got["dW"][9]).any()
+
+
+@pytest.mark.parametrize("kind", [L.ACT_GELU, L.ACT_GELU_TANH, L.ACT_SILU])
+@pytest.mark.parametrize("N", [1, 4200])
+def test_f32_gradients_of_f16_operands_have_f32_slopes(dev, N, kind):
+    """dbias of one live row is dZ itself. With e = 2^-24: e^x is off by 2^-22 of its value and 4 e |x| for its argument's roundings, 1 / (1 + e^x) by
+    2^-22 of its value, s (1 - s) by 2^-21 and erfc by 2^-21 of theirs, and the last product and sum by 2 e of the slope. e^x may be 0 below 2^-126, the
+    smallest normal f32: that times what it is multiplied with. (GELU's slope is p + z g with p from erfc: 1 + erf(z) is off by 2^-53 in f64, more than all
+    of it at z = -12.)"""
+    z = np.linspace(-12, 12, 4801).astype(np.float16)
+    c = Case(N, 1, len(z), dtype=L.AH_F16, kind=kind, bias=False, factor=False, res=False, scale=1.0)
+    c.dY[:], c.dY[0], c.Z[:] = 0, 1, z
+    got = c.backward(dev, want=("dbias",))["dbias"][0].astype(np.float64)
+    x, e = z.astype(np.float64), U32
+    _, slope = O.act(kind, x)
+    flushed = 2.0 ** -126
+    if kind == L.ACT_GELU:
+        p, g = 0.5 * erfc(-x / np.sqrt(2)), np.exp(-0.5 * x * x) / np.sqrt(2 * np.pi)
+        slope = p + x * g
+        flushed *= 1 + np.abs(x)
+        tol = 2 ** -21 * p + 2 * e * g * np.abs(x) + np.abs(x * g) * (e * x * x + 2 ** -21)
+    else:
+        a, b = (1.0, 0.0) if kind == L.ACT_SILU else (2 * O._C, 2 * O._C * 0.044715)
+        t = x * (a + b * x * x)
+        s, s1 = 1 / (1 + np.exp(-t)), np.exp(-np.abs(t)) / (1 + np.exp(-np.abs(t))) ** 2
+        arg = 4 * e * np.abs(t) if b else 0.0
+        flushed *= 1 + np.abs(x) * (a + 3 * b * x * x)
+        tol = np.abs(x) * s1 * (a + 3 * b * x * x) * (arg + 2 ** -21) + s1 * arg + 2 ** -22 * s
+    tol = tol + 2 * e * np.abs(slope) + flushed
+    assert np.all(np.abs(got - slope) <= tol), float(np.max(np.abs(got - slope) / tol))

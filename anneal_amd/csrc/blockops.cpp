@@ -38,12 +38,22 @@ int check_arrays(const char *fn, const Array *a, int n) {
     return AH_OK;
 }
 
+// Whether two arrays share a byte. Rows of one stride may lie side by side, as the halves of one [N, 2 F] array do; between rows of another
+// stride nothing else may lie.
+bool shared(const Array &a, const Array &b) {
+    if (!overlap(a.span(), b.span())) return false;
+    const int64_t ld = a.ld * a.esz;
+    if (ld != b.ld * b.esz) return true;
+    const int64_t by = (int64_t)((intptr_t)b.p - (intptr_t)a.p) % ld, at = by < 0 ? by + ld : by;   // where b's rows begin, from a's on
+    return at < a.cols * a.esz || at + b.cols * b.esz > ld;
+}
+
 // Outputs (the first n_out) against one another and the inputs. same[i]: the array that output i may be, or -1.
 int check_outputs(const char *fn, const Array *a, int n, int n_out, const int *same) {
     for (int i = 0; i < n_out; i++)
         for (int j = i + 1; j < n; j++) {
             if (same && same[i] == j && a[i].p == a[j].p && a[i].ld == a[j].ld) continue;
-            if (overlap(a[i].span(), a[j].span())) return set_error(AH_ERR_INVALID, "%s: %s overlaps %s", fn, a[i].name, a[j].name);
+            if (shared(a[i], a[j])) return set_error(AH_ERR_INVALID, "%s: %s overlaps %s", fn, a[i].name, a[j].name);
         }
     return AH_OK;
 }

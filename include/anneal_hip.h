@@ -414,6 +414,8 @@ int ah_muon_step(ah_device *dev, const ah_muon_desc *d);
 /* ── A residual block of a training step, and clipping before its update ──────
  * No counterpart in the reference (no activation but ReLU, no norm layer, no clipping). As above: asynchronous on the device stream,
  * nothing allocated, a workspace of the caller's (where there is one) that calls of one handle may share and graphs hold.
+ * An output shares no byte with another array of its call but where it says so; arrays of one row stride may lie side by side, as Z and U in
+ * the halves of one [N, 2 F] array.
  *
  * Linear layer with its epilogue. X [N,D], W [F,D], bias [F]; U, R, Y, Z [N,F]:
  *   Z = X W^T + bias,  Y = R + scale act(Z) U        (elementwise; bias, U, R may be null: 0, 1, 0)

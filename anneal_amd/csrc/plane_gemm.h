@@ -158,8 +158,9 @@ struct PFetch {
             }
         }
     }
-    // krem: k of the operand from the stage's first on, at least 1 (a stage wholly past them would be off by 2^32 bytes). Past them T = 1 reads the last k-row and T = 0 the stage's first chunk of the
-    // row (krem is then a multiple of a chunk's 8): the other operand is 0 there, and nothing behind the array is read.
+    // krem: k of the operand from the stage's first on, at least 1 (stages_of sees to it: at less the offset would be off by 2^32 bytes). Past them
+    // T = 1 reads the last k-row and T = 0 the stage's first chunk of the row (krem is then a multiple of a chunk's 8): the other operand is 0 there,
+    // and nothing behind the array is read.
     __device__ __forceinline__ void issue(int j, const char *base, long ld, int krem, uint32_t lds, int wave_u, int lane) const {
         uint32_t o = off[j];
         if (krem < BK) {
@@ -222,6 +223,13 @@ struct Tile {
     static_assert(SMEM <= 160 * 1024, "stages exceed the LDS");
 };
 
+// Of nk stages of bk from stage kt0 on, those that an operand of k has something of; the others' products are 0, and behind the operand there may
+// be nothing to read.
+__host__ __device__ __forceinline__ int stages_of(int k, int bk, int kt0, int nk) {
+    const int there = (k + bk - 1) / bk - kt0;
+    return there < nk ? there : nk;
+}
+
 struct Operand {
     const char *p;   // the array
     long ld;         // halves from a stored row to the next
@@ -262,6 +270,7 @@ __device__ __forceinline__ void contract(const Operand &A, const Operand &B, int
     for (int i = 0; i < FA; i++)
 #pragma unroll
         for (int j = 0; j < FB; j++) acc[i][j] = (floatx4){};
+    if constexpr (C::TB == 1 || C::PB == 1) nk = stages_of(B.k, BK, kt0, nk);   // (else B's panels have them all)
     if (nk <= 0) return;
 
     typename C::FetchA fa;

@@ -193,8 +193,9 @@ __device__ __forceinline__ float pack_dz(const GradIn &g, const PackArgs &a, int
                     if (!AGAIN && a.dU) store8((T *)a.dU + (long)m * a.lddu, n, g.F, du);
 #pragma unroll
                     for (int c = 0; c < 8; c++) col.v[c] += v.v[c];
+                    if (!AGAIN && a.track)
 #pragma unroll
-                    for (int c = 0; c < 8; c++) top = AGAIN ? 0.0f : max_finite(top, v.v[c]);
+                        for (int c = 0; c < 8; c++) top = max_finite(top, v.v[c]);
                 }
                 if (!a.dZ) continue;
 #pragma unroll

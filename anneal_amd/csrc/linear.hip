@@ -402,7 +402,7 @@ template <class T>
 void launch_few(const ProductArgs &a, const FewArgs &f, int few, hipStream_t s) {
     if (few == 1) launch_few<1, T>(a, f, s);
     else if (few == 4) launch_few<4, T>(a, f, s);
-    else launch_few<8, T>(a, f, s);
+    else if constexpr (sizeof(T) == 4) launch_few<8, T>(a, f, s);   // (f16 stops at 64 rows)
 }
 
 }  // namespace

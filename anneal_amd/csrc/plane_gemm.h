@@ -95,11 +95,11 @@ __device__ __forceinline__ void plane_store(half_t *p, floatx4 v) {
     *(h4 *)(p + 32) = lo;
 }
 
-// Power of two that brings the largest finite magnitude into [2^14, 2^15); 0 where there is none but 0.
+// Power of two that brings the largest finite magnitude into [2^14, 2^15), up to 2^163 for f32's smallest; 0 where there is none but 0.
 __device__ __forceinline__ int plane_exp(unsigned maxbits) {
     const float m = __uint_as_float(maxbits);
     if (!(m > 0.0f)) return 0;
-    return min(14 - ilogbf(m), 120);
+    return 14 - ilogbf(m);
 }
 // The bits of non-negative floats order as integers; 0 for infinities and NaN, which leave the others' scale alone.
 __device__ __forceinline__ unsigned magnitude(uint32_t bits) {

@@ -145,3 +145,26 @@ def test_f32_gradients_of_f16_operands_have_f32_slopes(dev, N, kind):
         tol = np.abs(x) * s1 * (a + 3 * b * x * x) * (arg + 2 ** -21) + s1 * arg + 2 ** -22 * s
     tol = tol + 2 * e * np.abs(slope) + flushed
     assert np.all(np.abs(got - slope) <= tol), float(np.max(np.abs(got - slope) / tol))
+
+
+@pytest.mark.parametrize("power", [-110, -126, -135])
+@pytest.mark.parametrize("which", ["X", "W", "rows of X", "rows of W"])
+def test_operands_near_the_beginning_of_f32(dev, which, power):
+    """f32 operands down to f32's subnormals beside large ones: their planes hold what they have."""
+    c = Case(200, 96, 64, kind=L.ACT_NONE, bias=False, factor=False, res=False, scale=1.0)
+    small, other = (c.X, c.W) if "X" in which else (c.W, c.X)
+    other *= np.float32(2.0 ** 100)
+    rows = slice(3, 20) if "rows" in which else slice(None)
+    small[rows] *= np.float32(2.0 ** power)
+    O.compare(c.forward(dev), c.expected())
+    if "rows" not in which:
+        c.dY *= np.float32(2.0 ** 20)
+        O.compare(c.backward(dev), c.gradients())
+
+
+@pytest.mark.parametrize("power", [-110, -126, -135])
+def test_gradients_near_the_beginning_of_f32(dev, power):
+    c = Case(200, 96, 64, kind=L.ACT_RELU, bias=False, factor=False, res=False, scale=1.0)
+    c.dY *= np.float32(2.0 ** power)
+    c.X, c.W = c.X * np.float32(2.0 ** 100), c.W * np.float32(2.0 ** 100)
+    O.compare(c.backward(dev), c.gradients())

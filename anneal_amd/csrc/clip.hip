@@ -139,15 +139,21 @@ __device__ __forceinline__ void norm_part(const Args &a, At at) {
     if (threadIdx.x == 0) a.part[blockIdx.x] = s;
 }
 
-// unscale c as a product of a power of two and an f32 that is not subnormal: a norm near f32's end leaves a factor of 2^-130.
-struct Factor {
-    float pre, m;
-    bool zero;
-    __device__ __forceinline__ Factor(double f, bool bad) : pre(f < 0x1p-62 ? 0x1p-64f : 1.0f), m((float)(f < 0x1p-62 ? f * 0x1p64 : f)), zero(bad) {}
-    __device__ __forceinline__ float of(float v) const { return zero ? 0.0f : v * pre * m; }
+// A value times unscale c, which is an f32 but where a norm near f32's end makes it less than f32's normal numbers: products in f64 have all of
+// f32's bits then.
+struct Single {
+    float f;
+    __device__ __forceinline__ float of(float v) const { return v * f; }
+};
+struct Double {
+    double f;
+    __device__ __forceinline__ float of(float v) const { return (float)((double)v * f); }
+};
+struct Zero {   // what is not finite is 0 too
+    __device__ __forceinline__ float of(float) const { return 0.0f; }
 };
 
-template <class T, class O>
+template <class T, class O, class Factor>
 __device__ __forceinline__ void scale_range(const T *p, O *q, long from, long to, Factor f) {
     typedef Vec<T> V;
     typedef O out __attribute__((ext_vector_type(V::N), aligned(sizeof(O))));
@@ -185,17 +191,22 @@ __device__ __forceinline__ void scale_part(const Args &a, At at) {
     const double norm = (double)a.unscale * sqrt(s), under = norm + (double)a.eps;
     const bool bad = !(s < __builtin_inf());
     const double c = bad ? 0.0 : (double)a.max_norm < under ? (double)a.max_norm / under : 1.0;
-    const Factor f(c * (double)a.unscale, bad);
+    const double f = c * (double)a.unscale;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         if (a.norm) *a.norm = (float)norm;
         if (a.coef) *a.coef = (float)c;
     }
-    walk<true>(a, at, [&](const Entry &e, long from, long to) {
-        if (!e.dst || (e.dst == e.src && f.pre * f.m == 1.0f)) return;
-        if (!e.half) scale_range((const float *)e.src, (float *)e.dst, from, to, f);
-        else if (e.half_out) scale_range((const half_t *)e.src, (half_t *)e.dst, from, to, f);
-        else scale_range((const half_t *)e.src, (float *)e.dst, from, to, f);
-    });
+    const auto scale = [&](auto factor, bool one) {
+        walk<true>(a, at, [&](const Entry &e, long from, long to) {
+            if (!e.dst || (e.dst == e.src && one)) return;
+            if (!e.half) scale_range((const float *)e.src, (float *)e.dst, from, to, factor);
+            else if (e.half_out) scale_range((const half_t *)e.src, (half_t *)e.dst, from, to, factor);
+            else scale_range((const half_t *)e.src, (float *)e.dst, from, to, factor);
+        });
+    };
+    if (bad) scale(Zero{}, false);
+    else if (f < 0x1p-126) scale(Double{f}, false);
+    else scale(Single{(float)f}, (float)f == 1.0f);
 }
 
 __global__ __launch_bounds__(256) void clip_norm_kernel(Args a) {

@@ -168,3 +168,48 @@ def test_gradients_near_the_beginning_of_f32(dev, power):
     c.dY *= np.float32(2.0 ** power)
     c.X, c.W = c.X * np.float32(2.0 ** 100), c.W * np.float32(2.0 ** 100)
     O.compare(c.backward(dev), c.gradients())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("kind", [L.ACT_RELU, L.ACT_GELU])
+def test_few_rows_of_many_features(dev, kind, types):
+    """Few rows, whose dX reads W as it lies, with more features than are scanned for dZ's magnitude."""
+    N, F = (60, 36000) if types[0] == L.AH_F16 else (100, 21504)
+    c = inactive(N, types, kind, -200.0, D=16, F=F)
+    got = c.backward(dev)
+    c.dY[:, OFF] = 0
+    O.compare(got, c.gradients())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("N", [200, 4200])
+def test_captured_with_other_gradients(dev, N, types):
+    """A captured call, replayed on gradients whose largest is live, off, and live again: what one replay found is nothing to the next."""
+    import ctypes as C
+    a, b = inactive(N, types, L.ACT_GELU, -200.0), inactive(N, types, L.ACT_GELU, -200.0)
+    a.dY[:, OFF] = 0
+    arrays = {k: dev.buffer(getattr(a, k), types[0]) for k in ("X", "W", "Z", "U", "dY")}
+    shapes = {"dX": (N, 96, types[1]), "dW": (64, 96, types[1]), "dbias": (1, 64, L.AH_F32), "dU": (N, 64, types[0])}
+    out = {k: dev.buffer(np.full(s[:2], np.nan), s[2]) for k, s in shapes.items()}
+    kw = dict(dtype=types[0], grad_dtype=types[1], N=N, D=96, F=64, act=a.kind, scale=a.scale, **arrays, **out)
+    ws = dev.buffer(dev.linear_grad_workspace(**kw) // 4 + 4)
+    g = C.c_void_p()
+    L.check(dev.lib.ah_graph_begin(dev.h))
+    dev.linear_grad(ws=ws, **kw)
+    L.check(dev.lib.ah_graph_end(dev.h, C.byref(g)))
+    want = {k: v for k, v in a.gradients().items()}   # of both: what is off adds nothing
+    first = None
+    for c in (a, b, a, b, b, a):
+        arrays["dY"].write(c.dY)
+        for k, s in shapes.items():
+            out[k].write(np.full(s[:2], np.nan).astype(O.NP[s[2]]))
+        L.check(dev.lib.ah_graph_replay(dev.h, g))
+        dev.sync()
+        got = {k: v.read().reshape(shapes[k][:2]) for k, v in out.items()}
+        O.compare(got, want)
+        first = first or got
+        for k in got if c is a else ():
+            np.testing.assert_array_equal(got[k], first[k], err_msg=k)
+        dev.linear_grad(ws=ws, **kw)   # eager between the replays
+    dev.sync()
+    dev.lib.ah_graph_destroy(g)

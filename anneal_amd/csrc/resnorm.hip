@@ -319,15 +319,17 @@ __device__ __forceinline__ void add_terms(float (&s)[kSums<LAYER>], const fN<V> 
         }
     }
 }
-// 1 / sqrt(v); NaN where v is past f32's range or below its normal numbers: not a gradient of 0.
-__device__ __forceinline__ float inverse(float v) { return v >= 0x1p-126f && v < __builtin_inff() ? 1.0f / sqrtf(v) : __builtin_nanf(""); }
+// 1 / sqrt(v) of a mean square with eps; NaN where squares are past f32's range, or below its normal numbers and not hidden by eps: not a gradient of 0.
+__device__ __forceinline__ float inverse(float v, float eps) {
+    return (v >= 0x1p-126f || v == eps) && v < __builtin_inff() ? 1.0f / sqrtf(v) : __builtin_nanf("");
+}
 template <bool LAYER>
 __device__ __forceinline__ RowTerms terms_of(const ah_residual_norm_grad_desc &d, const float (&m)[2], const float (&s)[kSums<LAYER>], float n) {
     const bool pre = d.pre != AH_NORM_NONE, post = d.post != AH_NORM_NONE;
     RowTerms x{m[0], m[1], 1.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (post) x.ry = inverse(s[0] * n + d.eps);
+    if (post) x.ry = inverse(s[0] * n + d.eps, d.eps);
     if (pre) {
-        x.c1 = inverse(s[1] * n + d.eps);
+        x.c1 = inverse(s[1] * n + d.eps, d.eps);
         x.c2 = x.c1 * (x.c1 * (s[2] * n));
     }
     float py = s[3] + x.c1 * (s[4] - x.c2 * s[5]);

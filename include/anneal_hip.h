@@ -488,7 +488,8 @@ int ah_linear_grad(ah_device *dev, const ah_linear_grad_desc *d);
  * post, pre: none, RMS x / sqrt(mean x^2 + eps) w, or layer (x - mean) / sqrt(var + eps) w + b; weights [D], may be null (1 and 0).
  * H null: no first term. Y null: no second one (gate and post then none). H_out or O may be null (O where pre is none); O is the norm of
  * H_out before its rounding. dtype (Y, O, gate, weights) AH_F32 or AH_F16; res_dtype (H, H_out) AH_F32, or AH_F16 where dtype is.
- * Computed in f32, rows of any finite size among them (a layer norm's as long as its sum is finite); H_out may be H. A row that is not finite leaves the others alone. N to 2^27, D to 2^20. No workspace. */
+ * Computed in f32, rows of any finite size among them (a layer norm's as long as its sum is finite); H_out may be H. A row that is not finite
+ * leaves the others alone. N to 2^27, D to 2^20. No workspace. */
 enum { AH_NORM_NONE = 0, AH_NORM_RMS = 1, AH_NORM_LAYER = 2 };
 typedef struct {
     int32_t dtype, res_dtype;
@@ -515,7 +516,8 @@ int ah_residual_norm(ah_device *dev, const ah_residual_norm_desc *d);
  * and the weights' gradients, sums over all rows. Null outputs are not computed. dgate is of dtype, the weights' gradients are
  * f32. Y is needed for dgate and where post is not none, H_out where pre is not none. Sums over rows run in a fixed order: results repeat
  * bit for bit. dH may be dH_out. A row's sums hold products of a gradient's entry with Y's and H_out's (less their means), gate and weights, in
- * f32: where those are past its range, so is the row, and where its mean square plus eps is (or is below 2^-126) it is NaN. */
+ * f32: where those are past its range, so is the row, and where its mean square plus eps is (or is below 2^-126 and not eps itself) it
+ * is NaN. */
 typedef struct {
     int32_t dtype, res_dtype;
     int32_t N, D;

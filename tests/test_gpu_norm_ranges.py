@@ -81,3 +81,14 @@ def test_gradients_past_the_range_are_not_zeros(dev, D, which, kind):
     rows = ("dH", "dY", "dgate")
     O.compare({k: got[k][keep] for k in rows}, {k: tuple(x[keep] for x in want[k]) for k in rows})
     assert np.isnan(got["dY"][3]).all() and (which == "Y" or np.isnan(got["dH"][3]).all())
+
+
+@pytest.mark.parametrize("kind", [RMS, LAYER])
+@pytest.mark.parametrize("D", [40, 1000, 9000])
+def test_gradients_of_zeros_under_a_tiny_eps(dev, D, kind):
+    """eps is a subnormal f32 and divides a row of zeros: its gradients are large and finite."""
+    c = Case(4, D, post=kind, pre=kind, gate=False, weights=False, eps=2.0 ** -130)
+    c.H[:], c.Y[:] = 0, 0
+    c.dH_out, c.dO = c.dH_out * np.float32(2.0 ** -20), c.dO * np.float32(2.0 ** -90)
+    O.compare(c.forward(dev), c.expected())
+    O.compare(c.backward(dev), c.gradients())

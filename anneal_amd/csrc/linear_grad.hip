@@ -27,6 +27,7 @@ namespace ah {
 namespace {
 
 constexpr int kScans = 1024;   // workgroups that look for an array's largest magnitude, at most
+constexpr int kTops = 256, kTopStep = 16;   // places, 64 bytes apart, for dZ's: at one place 2304 waves took 14 us
 // Rows of a block of dZ: 64, or fewer where those blocks would not fill the chip (300 x 1024 -> 1024 in 8 rather than 32: 29 -> 23 us).
 int block_rows(int Np, int Fp) {
     const int64_t blocks = (int64_t)(Np / 64) * ((Fp + 511) / 512);
@@ -74,9 +75,8 @@ __device__ __forceinline__ f8 dz_of(const GradIn &g, const Line<T> &l, f8 &du) {
 
 struct ScanArgs {
     int zblocks, xblocks, wblocks;   // workgroups of each array, in this order
-    int exact;                       // dZ's own magnitudes, not bounds
     unsigned *maxes;                 // [3][kScans]
-    unsigned *top;                   // bits of dZ's largest magnitude, for the second pass to raise
+    unsigned *tops;                  // [kTops * kTopStep]: bits of dZ's largest magnitudes, for the second pass to raise
 };
 template <class T>
 __device__ __forceinline__ unsigned max8(unsigned m, const T &v) {
@@ -87,42 +87,44 @@ __device__ __forceinline__ unsigned max8(unsigned m, const T &v) {
 // The larger of m and |v|; infinities and NaN are passed over: v + 0 v is NaN then, which fmaxf drops.
 __device__ __forceinline__ float max_finite(float m, float v) { return fmaxf(m, fabsf(fmaf(v, 0.0f, v))); }
 
-// A wave a stretch of 2048 values of a row, or of 512 where it evaluates dZ.
+// A wave a stretch of 2048 values of a row, or, P > 0, of 512 for dZ's own magnitudes in place of bounds (P: planes of dZ).
 template <class T, int P>
 __global__ __launch_bounds__(256) void linear_grad_scan_kernel(GradIn g, ScanArgs a) {
     __shared__ unsigned red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, which = (int)blockIdx.x < a.zblocks ? 0 : (int)blockIdx.x < a.zblocks + a.xblocks ? 1 : 2;
     const int b = blockIdx.x - (which == 0 ? 0 : which == 1 ? a.zblocks : a.zblocks + a.xblocks), blocks = which == 0 ? a.zblocks : which == 1 ? a.xblocks : a.wblocks;
-    const int width = which == 0 ? g.F : g.D, stretch = which == 0 && a.exact ? 512 : 2048, segs = (width + stretch - 1) / stretch;
+    const int width = which == 0 ? g.F : g.D, stretch = which == 0 && P ? 512 : 2048, segs = (width + stretch - 1) / stretch;
     const long rows = which == 2 ? g.F : g.N;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.top = 0;
+    if (blockIdx.x == 0 && threadIdx.x < kTops) a.tops[threadIdx.x * kTopStep] = 0;
     unsigned m = 0;
     for (long q = (long)b * 4 + wave; q < rows * segs; q += (long)blocks * 4) {
         const long r = q / segs;
         const int c0 = (int)(q - r * segs) * stretch + lane * 8;
-        if (which == 0 && a.exact) {
-            if (c0 >= width) continue;
-            f8 du;
-            m = max8(m, dz_of<T, P>(g, load_line<T>(g, r, c0), du).v);
-        } else if (which == 0) {
-            typename Raw8<T>::type dy[4] = {}, u[4] = {};
+        if (which == 0) {
+            if constexpr (P > 0) {
+                if (c0 >= width) continue;
+                f8 du;
+                m = max8(m, dz_of<T, P>(g, load_line<T>(g, r, c0), du).v);
+            } else {
+                typename Raw8<T>::type dy[4] = {}, u[4] = {};
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (c0 + k * 512 >= width) continue;
-                dy[k] = load_raw8((const T *)g.dY + r * g.lddy, c0 + k * 512, width);
-                if (g.U) u[k] = load_raw8((const T *)g.U + r * g.ldu, c0 + k * 512, width);
-            }
-            const float s = g.scale * slope_bound(g.act);
-            float top = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float v = s * (float)dy[k][e] * (g.U ? (float)u[k][e] : 1.0f);
-                    top = g.act == AH_ACT_NONE ? max_finite(top, v) : fmaxf(top, fabsf(v));   // (without an activation it is dZ)
+                for (int k = 0; k < 4; k++) {
+                    if (c0 + k * 512 >= width) continue;
+                    dy[k] = load_raw8((const T *)g.dY + r * g.lddy, c0 + k * 512, width);
+                    if (g.U) u[k] = load_raw8((const T *)g.U + r * g.ldu, c0 + k * 512, width);
                 }
-            // a bound past f32's range counts as its largest value: dZ may be finite, and the second pass will tell
-            m = max(m, __float_as_uint(fminf(top, 0x1.fffffep127f)));
+                const float s = g.scale * slope_bound(g.act);
+                float top = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float v = s * (float)dy[k][e] * (g.U ? (float)u[k][e] : 1.0f);
+                        top = g.act == AH_ACT_NONE ? max_finite(top, v) : fmaxf(top, fabsf(v));   // (without an activation it is dZ)
+                    }
+                // a bound past f32's range counts as its largest value: dZ may be finite, and the second pass will tell
+                m = max(m, __float_as_uint(fminf(top, 0x1.fffffep127f)));
+            }
         } else {
             const float *p = which == 1 ? (const float *)g.X + r * g.ldx : (const float *)g.W + r * g.ldw;
             raw8_f32 v[4] = {};
@@ -139,11 +141,11 @@ __global__ __launch_bounds__(256) void linear_grad_scan_kernel(GradIn g, ScanArg
     if (threadIdx.x == 0) a.maxes[which * kScans + b] = max(max(red[0], red[1]), max(red[2], red[3]));
 }
 
-// The largest of n workgroups' values; all 256 threads of a workgroup.
-__device__ __forceinline__ unsigned join_maxes(const unsigned *maxes, int n) {
+// The largest of n values `step` apart; all 256 threads of a workgroup.
+__device__ __forceinline__ unsigned join_maxes(const unsigned *maxes, int n, int step = 1) {
     __shared__ unsigned red[4];
     unsigned m = 0;
-    for (int i = threadIdx.x; i < n; i += 256) m = max(m, maxes[i]);
+    for (int i = threadIdx.x; i < n; i += 256) m = max(m, maxes[i * step]);
     for (int o = 32; o >= 1; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
@@ -229,7 +231,7 @@ __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArg
         unsigned top = __float_as_uint(pack_dz<T, P, false>(g, a, a.zblocks - 1 - (int)blockIdx.x, e[0]));
         if (!a.track) return;
         for (int o = 32; o >= 1; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
-        if ((threadIdx.x & 63) == 0 && top > __hip_atomic_load(s.top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(s.top, top);   // any order: the same
+        if ((threadIdx.x & 63) == 0) atomicMax(s.tops + (blockIdx.x * 4 + (threadIdx.x >> 6)) % kTops * kTopStep, top);   // in any order the same
         return;
     }
     constexpr int ESZ = PO == 1 ? 2 : 4;
@@ -242,9 +244,10 @@ __global__ __launch_bounds__(256) void linear_grad_pack_kernel(GradIn g, PackArg
 
 // dZ's planes again, by its own magnitude, where the bound's exponent has cost them bits.
 template <class T, int P>
-__global__ __launch_bounds__(256) void linear_grad_again_kernel(GradIn g, PackArgs a, const unsigned *top) {
-    const int e = pg::plane_exp(*top);
-    if (*top == 0 || e <= a.exps[3] + kSlack) return;
+__global__ __launch_bounds__(256) void linear_grad_again_kernel(GradIn g, PackArgs a, const unsigned *tops) {
+    const unsigned top = join_maxes(tops, kTops, kTopStep);
+    const int e = pg::plane_exp(top);
+    if (top == 0 || e <= a.exps[3] + kSlack) return;
     if (blockIdx.x == 0 && threadIdx.x == 0) a.exps[0] = e;
     for (int zb = blockIdx.x; zb < a.zblocks; zb += gridDim.x) pack_dz<T, P, true>(g, a, zb, e);
 }
@@ -494,7 +497,7 @@ struct Layout {
     bool products, pack_x, pack_w;
     bool exact, track;         // dZ's magnitudes are scanned for, or bounded and found by the second pass
     Cuts cuts;
-    int64_t exps, top, maxes, dbpart, dZ, Xp, Wp, sums, wsums, total;
+    int64_t exps, tops, maxes, dbpart, dZ, Xp, Wp, sums, wsums, total;
 };
 
 pg::Work few_work(const ah_linear_grad_desc &d, const Layout &l) {
@@ -511,7 +514,10 @@ Layout layout(const ah_linear_grad_desc &d) {
     l.Dp = (d.D + 63) & ~63;
     l.products = d.dX || d.dW;
     l.zrows = block_rows(l.Np, l.Fp);
-    l.exact = d.act != AH_ACT_NONE && (int64_t)d.N * ((d.F + 511) / 512) <= 4 * kScans;   // (without an activation the bound is exact)
+    // dZ itself is looked through where a wave has one stretch of it, or two whose slopes cost little (the third launch | that: f32, tanh GELU's and GELU's
+    // slopes in full, 1900 x 512 -> 2048 47.5 | 48.8 and 63.4 | 66.7 us; f16 SiLU 1100 rows 37.9 | 36.2). Without an activation the bound is exact.
+    const bool cheap = l.P == 1 || d.act == AH_ACT_RELU;
+    l.exact = d.act != AH_ACT_NONE && (int64_t)d.N * ((d.F + 511) / 512) <= (cheap ? 8 : 4) * kScans;
     l.track = l.products && d.act != AH_ACT_NONE && !l.exact;
     if (d.dX && d.N <= (f16 ? kFewF16 : kFewF32) && d.D >= 8) l.few = d.N <= 16 ? 1 : d.N <= 64 ? 4 : 8;
     l.pack_x = d.dW && (!f16 || !rows_aligned(d.X, d.ldx, d.D));
@@ -523,7 +529,7 @@ Layout layout(const ah_linear_grad_desc &d) {
         return o;
     };
     l.exps = take(16);
-    l.top = take(4);
+    l.tops = take(kTops * kTopStep * 4);
     l.maxes = take(3 * kScans * 4);
     if (d.dbias) l.dbpart = take((int64_t)(l.Np / l.zrows) * d.F * 4);
     if (l.products) l.dZ = take((int64_t)l.Np * l.Fp * 2 * l.P);
@@ -603,13 +609,16 @@ void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     const GradIn g{d.N, d.D, d.F, d.act, d.scale, d.dY, d.Z, d.U, d.lddy, d.ldz, d.ldu, d.X, d.W, d.ldx, d.ldw};
     const auto scans = [](int64_t rows, int64_t width, int stretch = 2048) { return (int)std::min<int64_t>((rows * ((width + stretch - 1) / stretch) + 3) / 4, kScans); };
     ScanArgs sc{};
-    sc.exact = l.exact;
     sc.zblocks = l.products ? scans(d.N, d.F, l.exact ? 512 : 2048) : 0;
     sc.xblocks = l.pack_x && PO == 2 ? scans(d.N, d.D) : 0;
     sc.wblocks = l.pack_w && PO == 2 ? scans(d.F, d.D) : 0;
     sc.maxes = (unsigned *)(ws + l.maxes);
-    sc.top = (unsigned *)(ws + l.top);
-    if (l.products) hipLaunchKernelGGL((linear_grad_scan_kernel<T, P>), dim3((unsigned)(sc.zblocks + sc.xblocks + sc.wblocks)), dim3(256), 0, s, g, sc);
+    sc.tops = (unsigned *)(ws + l.tops);
+    if (l.products) {
+        const dim3 grid((unsigned)(sc.zblocks + sc.xblocks + sc.wblocks));
+        if (l.exact) hipLaunchKernelGGL((linear_grad_scan_kernel<T, P>), grid, dim3(256), 0, s, g, sc);
+        else hipLaunchKernelGGL((linear_grad_scan_kernel<T, 0>), grid, dim3(256), 0, s, g, sc);
+    }
 
     PackArgs p{};
     if (l.products) p.dZ = (half_t *)(ws + l.dZ);
@@ -628,7 +637,7 @@ void run(const ah_linear_grad_desc &d, const Layout &l, hipStream_t s) {
     p.exps = (int *)(ws + l.exps);
     p.track = l.track;
     hipLaunchKernelGGL((linear_grad_pack_kernel<T, P, PO>), dim3((unsigned)(p.zblocks + p.rest)), dim3(256), 0, s, g, p, sc);
-    if (l.track) hipLaunchKernelGGL((linear_grad_again_kernel<T, P>), dim3((unsigned)std::min(p.zblocks, 1024)), dim3(256), 0, s, g, p, sc.top);
+    if (l.track) hipLaunchKernelGGL((linear_grad_again_kernel<T, P>), dim3((unsigned)std::min(p.zblocks, 1024)), dim3(256), 0, s, g, p, sc.tops);
     PairArgs a{};
     a.x.ea = a.w.ea = p.exps;
     a.x.out16 = a.w.out16 = d.grad_dtype == AH_F16;

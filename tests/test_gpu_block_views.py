@@ -41,7 +41,7 @@ class Beside:
 
 @pytest.mark.parametrize("types", TYPES, ids=IDS)
 @pytest.mark.parametrize("gap", [0, 1])
-@pytest.mark.parametrize("shape", [(1, 64, 96), (5, 40, 33), (40, 100, 65), (200, 72, 131), (4200, 16, 64)], ids=lambda s: "%dx%dx%d" % s)
+@pytest.mark.parametrize("shape", [(1, 64, 96), (5, 40, 33), (40, 100, 65), (200, 72, 131), (8400, 16, 64)], ids=lambda s: "%dx%dx%d" % s)
 def test_a_gated_unit_in_one_array(dev, shape, gap, types):
     """Z, U and Y side by side going forward; Z, U, dU and dY going back."""
     N, D, F = shape

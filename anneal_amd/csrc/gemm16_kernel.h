@@ -126,18 +126,23 @@ struct Fetch {
 
 // L2 prefetch of one operand's stage (k = k0 .. k0+63): the stage is R lines of 128 bytes (a
 // K-contiguous row holds 64 halves = one line; an MN-contiguous k-row of R halves holds R/64 lines).
-// Line i of the stage is touched by thread i (callers pass i < R, ragged rows clamped).
+// Line i of the stage is touched by thread i (callers pass i < R, ragged rows clamped), in four bytes: an MN-contiguous operand's
+// columns past its end fall on its last eight, so that the last k-row's four bytes end inside the array too.
+template <int R, int T>
+__host__ __device__ __forceinline__ long prefetch_offset(long ld, int r0, int rmax, int k0, int i) {
+    if constexpr (T == 0) {
+        const int row = r0 + i < rmax - 1 ? r0 + i : rmax - 1;
+        return ((long)row * ld + k0) * 2;
+    } else {
+        constexpr int LPR = R / 64;
+        const int at = r0 + (i % LPR) * 64, col = at < rmax - 8 ? at : rmax - 8;
+        return ((long)(k0 + i / LPR) * ld + col) * 2;
+    }
+}
 template <int R, int T>
 __device__ __forceinline__ void prefetch_stage(const char *base, long ld, int r0, int rmax, int k0, int i,
                                                const char *junk) {
-    if constexpr (T == 0) {
-        const int row = min(r0 + i, rmax - 1);
-        prefetch_line(base + ((long)row * ld + k0) * 2, junk);
-    } else {
-        constexpr int LPR = R / 64;
-        const int col = min(r0 + (i % LPR) * 64, rmax - 1);
-        prefetch_line(base + ((long)(k0 + i / LPR) * ld + col) * 2, junk);
-    }
+    prefetch_line(base + prefetch_offset<R, T>(ld, r0, rmax, k0, i), junk);
 }
 
 template <int R, int T, int BK>

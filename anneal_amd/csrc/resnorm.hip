@@ -12,7 +12,7 @@
 // row's loads in flight, and leaves its sums in the workspace, where a second launch adds them in the workers' order (f16, the same size: 178 us,
 // 4.6 TB/s; f32, 1999 x 1001 with layer norms: 23, latency). A run that begins or ends inside a gate's rows leaves that gate's part there too;
 // the sums of gates whose rows are all its own it writes itself. Rows that 1024 threads do not hold take two launches, the rows' terms and
-// then the columns (4000 x 12000 f16: 234 us, 4000 x 6000 f32 with layer norms 218; one launch with fewer threads' registers spilled 280).
+// then the columns (4000 x 12000 f16: 239 us, 4000 x 6000 f32 with layer norms 217; one launch with fewer threads' registers spilled 280).
 #include "resnorm.h"
 
 #include <algorithm>
@@ -621,7 +621,7 @@ struct Plan {
 Plan plan_of(const ah_residual_norm_grad_desc &d) {
     Plan p{};
     // Eight columns a thread where its registers hold them and the next row's; four for f32 streams and for layer norms' sums. Rows past
-    // 1024 threads' columns take two launches (4000 x 12000 f16 234 us; 410 by several readings of whole rows).
+    // 1024 threads' columns take two launches (4000 x 12000 f16 239 us; 410 by several readings of whole rows).
     const int cols = d.res_dtype == AH_F32 || has_layer(d) ? 4 : kVec;
     p.tpr = d.D > 1024 * cols ? 0 : threads_of(d.D, cols);
     Runs &u = p.u;
